@@ -553,6 +553,43 @@ int trnblas_hip_trsm(int dtype, int64_t n, int64_t nrhs, int upper, int unit, do
                      int64_t ldb_c, void* X, int64_t ldx_r, int64_t ldx_c, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/*
+ * Products over ragged groups of rows (rows sorted by expert). No counterpart
+ * in the reference.
+ *
+ * offsets: device int32 (offsets64 == 0) or int64 [groups + 1], nondecreasing:
+ * group g is rows offsets[g] .. offsets[g + 1] - 1. They are read on the device
+ * only (the call never waits for them); each is clamped to [0, rows], so bad
+ * ones give wrong rows but no access outside the operands.
+ * dtype: TRNBLAS_F32, TRNBLAS_BF16 or TRNBLAS_F16, the element type of A and B;
+ * C and D have it too, or are fp32 for out_f32 != 0. Sums are fp32, with one
+ * rounding at the end. All matrices are row-major with any leading dimension
+ * and alignment; 16-byte aligned operands whose leading dimensions, strides and
+ * K (N where B is N-contiguous; M and N for grouped_rank_k) are multiples of 16
+ * bytes run faster. D must not overlap A or B; it may be C itself.
+ *
+ * grouped_gemm:   D[r] = alpha A[r] op(B[g]) + beta C[r] for the rows r of
+ * group g, D[r] = beta C[r] (zeros when beta == 0) for rows of no group.
+ * A is rows x K; B[g] starts at B + g * strideB (elements): K x N, or N x K for
+ * transB != 0.
+ */
+int trnblas_hip_grouped_gemm(int dtype, int out_f32, int transB, int64_t groups, int64_t rows,
+                             int64_t N, int64_t K, double alpha, const void* A, int64_t lda,
+                             const void* B, int64_t ldb, int64_t strideB, const void* offsets,
+                             int offsets64, double beta, const void* C, int64_t ldc, void* D,
+                             int64_t ldd, void* stream);
+
+/*
+ * grouped_rank_k: D[g] = alpha A_g^T B_g + beta C[g] (M x N each), A_g and B_g
+ * the rows of group g of A (rows x M) and B (rows x N): the gradient of
+ * grouped_gemm to its B. A group without rows gives beta C[g].
+ */
+int trnblas_hip_grouped_rank_k(int dtype, int out_f32, int64_t groups, int64_t rows, int64_t M,
+                               int64_t N, double alpha, const void* A, int64_t lda, const void* B,
+                               int64_t ldb, const void* offsets, int offsets64, double beta,
+                               const void* C, int64_t ldc, int64_t strideC, void* D, int64_t ldd,
+                               int64_t strideD, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,266 @@
+"""grouped_gemm / grouped_rank_k on the GPU against 64-bit products, at sizes, layouts and group shapes where they can go
+wrong. The bound is `oracle.grouped.excess`'s."""
+
+import pytest
+import torch
+
+import trnblas_amd as tb
+from oracle import grouped as og
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+DTYPES = [F32, BF16, F16]
+
+
+def _randn(g, *shape, dtype=F32):
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+def _split(rows, sizes, lead=0):
+    """Offsets of groups of `sizes` rows after `lead` rows of no group."""
+    o = [lead]
+    for s in sizes:
+        o.append(o[-1] + s)
+    assert o[-1] <= rows
+    return torch.tensor(o, dtype=torch.int32)
+
+
+# (rows, sizes of the groups, rows before the first): one row, empty groups, tiles that end inside, rows of no group
+GROUPS = {
+    "one": (1, [1], 0),
+    "one_of_many": (1, [0] * 37 + [1] + [0] * 26, 0),
+    "token": (6, [0, 1, 0, 2, 0, 0, 1, 1, 0, 1], 0),
+    "gaps": (77, [0, 9, 0, 40, 3], 11),
+    "all_gap": (19, [0, 0, 0], 7),
+    "small": (150, [17, 33, 1, 64, 35], 0),
+    "many": (300, [(3 * i) % 5 for i in range(140)], 2),
+    "uneven": (700, [513, 0, 2, 185], 0),
+    "single": (400, [400], 0),
+}
+# (K, N): below and across the tiles of 16, 32, 64, 128 and 256, multiples of 16 bytes and not
+SIZES = [(1, 1), (7, 5), (33, 70), (64, 128), (100, 61), (136, 264), (264, 136), (512, 520), (515, 257), (1032, 384)]
+
+
+@pytest.mark.parametrize("shape", list(GROUPS))
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_grouped_gemm(dev, shape, dtype):
+    rows, sizes, lead = GROUPS[shape]
+    off = _split(rows, sizes, lead)
+    for i, (K, N) in enumerate(SIZES):
+        for transB in (False, True):
+            g = torch.Generator().manual_seed(100 * i + transB)
+            A = _randn(g, rows, K, dtype=dtype)
+            B = _randn(g, len(sizes), *((N, K) if transB else (K, N)), dtype=dtype)
+            D = tb.grouped_gemm(1.0, A.to(dev), B.to(dev), off.to(dev), transB=transB)
+            ref, den = og.grouped_gemm(1.0, A, B, off, transB=transB)
+            assert D.dtype == dtype and og.excess(D, ref, den, K) <= 1, (K, N, transB)
+
+
+@pytest.mark.parametrize("shape", ["one", "token", "gaps", "small", "uneven", "single"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_grouped_rank_k(dev, shape, dtype):
+    rows, sizes, lead = GROUPS[shape]
+    off = _split(rows, sizes, lead)
+    for i, (M, N) in enumerate([(1, 1), (5, 7), (70, 33), (128, 64), (136, 264), (264, 512), (257, 515)]):
+        g = torch.Generator().manual_seed(i)
+        A, B = _randn(g, rows, M, dtype=dtype), _randn(g, rows, N, dtype=dtype)
+        for out in {dtype, F32}:
+            D = tb.grouped_rank_k(1.0, A.to(dev), B.to(dev), off.to(dev), dtype=out)
+            ref, den = og.grouped_rank_k(1.0, A, B, off)
+            assert D.dtype == out and og.excess(D, ref, den, rows) <= 1, (M, N, out)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_fp32_products_keep_the_fp32_gate(dev, dtype):
+    # same-sign operands: the worst case of a running sum; fp32 is held to 1e-6 |A||B| as `gemm` is
+    g = torch.Generator().manual_seed(5)
+    A, B = torch.rand(300, 4100, generator=g).to(dtype), torch.rand(2, 4100, 260, generator=g).to(dtype)
+    off = _split(300, [130, 170])
+    D = tb.grouped_gemm(1.0, A.to(dev), B.to(dev), off.to(dev), dtype=F32)
+    ref, den = og.grouped_gemm(1.0, A, B, off)
+    assert float(((D.double().cpu() - ref).abs() / den).max()) <= (1e-6 if dtype == F32 else 4100 * 2.0**-23)
+    A, B = torch.rand(4100, 136, generator=g).to(dtype), torch.rand(4100, 260, generator=g).to(dtype)
+    off = _split(4100, [4000, 100])
+    D = tb.grouped_rank_k(1.0, A.to(dev), B.to(dev), off.to(dev), dtype=F32)
+    ref, den = og.grouped_rank_k(1.0, A, B, off)
+    assert float(((D.double().cpu() - ref).abs() / den).max()) <= (1e-6 if dtype == F32 else 4000 * 2.0**-23)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N", [(64, 128), (100, 61), (264, 256)])
+def test_alpha_beta_and_result_type(dev, dtype, K, N):
+    rows, sizes, lead = GROUPS["gaps"]
+    off = _split(rows, sizes, lead).to(torch.int64)
+    g = torch.Generator().manual_seed(2)
+    A, B = _randn(g, rows, K, dtype=dtype), _randn(g, len(sizes), K, N, dtype=dtype)
+    for out in {dtype, F32}:
+        for C in (_randn(g, rows, N, dtype=out), _randn(g, N, dtype=out), _randn(g, rows, 2 * N + 1, dtype=out)[:, 1 : N + 1]):
+            D = tb.grouped_gemm(-1.5, A.to(dev), B.to(dev), off.to(dev), 0.25, C.to(dev), dtype=out)
+            ref, den = og.grouped_gemm(-1.5, A, B, off, 0.25, C)
+            assert og.excess(D, ref, den, K) <= 1
+        W = _randn(g, rows, N, dtype=dtype)
+        C = _randn(g, len(sizes), K, N, dtype=out)
+        D = tb.grouped_rank_k(-1.5, A.to(dev), W.to(dev), off.to(dev), 1.0, C.to(dev), dtype=out)
+        ref, den = og.grouped_rank_k(-1.5, A, W, off, 1.0, C)
+        assert og.excess(D, ref, den, rows) <= 1
+
+
+def test_nan_in_c_is_not_read_without_beta(dev):
+    A, B, off = torch.ones(40, 64, device=dev), torch.ones(2, 64, 32, device=dev), _split(40, [10, 20]).to(dev)
+    C = torch.full((40, 32), float("nan"), device=dev)
+    D = tb.grouped_gemm(1.0, A, B, off, 0.0, C)
+    assert torch.equal(D[:30], torch.full((30, 32), 64.0, device=dev)) and not D[30:].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_of_other_groups_stay_out(dev, dtype):
+    # infinities and NaN in rows of no group, in rows of other groups and in their matrices, and past the ends of padded
+    # rows: none of them reaches a result
+    for K, N in ((40, 72), (61, 33), (256, 256)):
+        g = torch.Generator().manual_seed(3)
+        off = _split(60, [9, 21, 0, 5], 10)
+        Ap, Bp = _randn(g, 60, K + 8, dtype=dtype), _randn(g, 4, K, N + 8, dtype=dtype)
+        W = _randn(g, 60, N, dtype=dtype)
+        bad = Ap.clone(), Bp.clone(), W.clone()
+        bad[0][:10], bad[0][19:40], bad[0][45:], bad[0][:, K:] = (float(x) for x in ("inf", "nan", "nan", "inf"))
+        bad[1][1:3], bad[1][:, :, N:] = float("nan"), float("inf")
+        bad[2][:10], bad[2][19:40], bad[2][45:] = float("nan"), float("inf"), float("nan")
+        A, B, W = Ap.to(dev), Bp.to(dev), W.to(dev)
+        Ab, Bb, Wb = (x.to(dev) for x in bad)
+        want = tb.grouped_gemm(1.0, A[:, :K], B[:, :, :N], off.to(dev))
+        got = tb.grouped_gemm(1.0, Ab[:, :K], Bb[:, :, :N], off.to(dev))
+        for a, b in ((10, 19), (40, 45)):
+            assert torch.equal(got[a:b], want[a:b]) and want[a:b].isfinite().all()
+        assert not got[:10].any() and not got[45:].any()
+        want = tb.grouped_rank_k(1.0, A[:, :K], W, off.to(dev))
+        got = tb.grouped_rank_k(1.0, Ab[:, :K], Wb, off.to(dev))
+        for i in (0, 2, 3):
+            assert torch.equal(got[i], want[i]) and want[i].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N", [(64, 128), (100, 61), (520, 264)])
+def test_layouts(dev, dtype, K, N):
+    rows, sizes = 150, [17, 33, 1, 64, 35]
+    off = _split(rows, sizes)
+    g = torch.Generator().manual_seed(4)
+    A, B = _randn(g, rows, K, dtype=dtype), _randn(g, 5, K, N, dtype=dtype)
+    ref, den = og.grouped_gemm(1.0, A, B, off)
+    Ad, Bd, od = A.to(dev), B.to(dev), off.to(dev)
+
+    def inside(X, before, after):  # X inside a larger buffer: another leading dimension and another alignment
+        P = torch.full((*X.shape[:-1], X.shape[-1] + before + after), float("nan"), dtype=dtype, device=dev)
+        P[..., before : before + X.shape[-1]] = X
+        return P[..., before : before + X.shape[-1]]
+
+    views = {
+        "wide": (inside(Ad, 0, 8), inside(Bd, 0, 16)),
+        "shifted": (inside(Ad, 1, 2), inside(Bd, 3, 0)),
+        "aligned_shift": (inside(Ad, 8, 8), inside(Bd, 16, 8)),
+        "transposed_a": (Ad.mT.contiguous().mT, Bd),
+        "transposed_b": (Ad, Bd.mT.contiguous().mT),
+        "groups_apart": (Ad, torch.stack([Bd, Bd * 0 + float("nan")], 1)[:, 0]),
+        "rows_apart": (torch.stack([Ad, Ad * 0 + float("nan")], 1)[:, 0], Bd),
+    }
+    for name, (a, b) in views.items():
+        D = tb.grouped_gemm(1.0, a, b, od)
+        assert og.excess(D, ref, den, K) <= 1, name
+    one = B[2].to(dev).expand(5, K, N)
+    D = tb.grouped_gemm(1.0, Ad, one, od)
+    assert og.excess(D, *og.grouped_gemm(1.0, A, B[2].expand(5, K, N), off), K) <= 1
+    W = _randn(g, rows, N, dtype=dtype)
+    ref, den = og.grouped_rank_k(1.0, A, W, off)
+    for a, w in ((inside(Ad, 1, 2), inside(W.to(dev), 0, 3)), (inside(Ad, 8, 8), inside(W.to(dev), 8, 0))):
+        assert og.excess(tb.grouped_rank_k(1.0, a, w, od), ref, den, rows) <= 1
+
+
+def test_offsets_outside_the_rows_are_clamped(dev):
+    g = torch.Generator().manual_seed(6)
+    A, B = _randn(g, 50, 32), _randn(g, 3, 32, 16)
+    want = tb.grouped_gemm(1.0, A.to(dev), B.to(dev), torch.tensor([0, 20, 20, 50], device=dev))
+    for dt, big in ((torch.int32, 2**31 - 1), (torch.int64, 2**40)):
+        off = torch.tensor([-big, 20, 20, big], dtype=dt, device=dev)
+        assert torch.equal(tb.grouped_gemm(1.0, A.to(dev), B.to(dev), off), want)
+    # decreasing offsets: any values, but nothing outside the operands is touched
+    off = torch.tensor([40, 10, 60, 0], dtype=torch.int32, device=dev)
+    assert tb.grouped_gemm(1.0, A.to(dev), B.to(dev), off).shape == (50, 16)
+    assert tb.grouped_rank_k(1.0, A.to(dev), A.to(dev), off).shape == (3, 32, 32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients(dev, dtype):
+    rows, sizes, lead = GROUPS["gaps"]
+    off = _split(rows, sizes, lead)
+    g = torch.Generator().manual_seed(7)
+    for transB in (False, True):
+        K, N = 72, 136
+        A = _randn(g, rows, K, dtype=dtype)
+        B = _randn(g, len(sizes), *((N, K) if transB else (K, N)), dtype=dtype)
+        dD = _randn(g, rows, N, dtype=dtype)
+        a, b = A.to(dev).requires_grad_(), B.to(dev).requires_grad_()
+        D = tb.grouped_gemm(1.0, a, b, off.to(dev), transB=transB)
+        dA, dB = torch.autograd.grad(D, (a, b), dD.to(dev))
+        assert og.excess(D, *og.grouped_gemm(1.0, A, B, off, transB=transB), K) <= 1
+        assert og.excess(dA, *og.grouped_gemm(1.0, dD, B, off, transB=not transB), N) <= 1
+        want = og.grouped_rank_k(1.0, dD, A, off) if transB else og.grouped_rank_k(1.0, A, dD, off)
+        assert og.excess(dB, *want, rows) <= 1 and dB.shape == B.shape
+
+
+def test_other_stream(dev):
+    g = torch.Generator().manual_seed(8)
+    A, B, off = _randn(g, 90, 64).to(dev), _randn(g, 3, 64, 48).to(dev), _split(90, [30, 1, 59]).to(dev)
+    want = tb.grouped_gemm(1.0, A, B, off)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        big = torch.randn(2048, 2048, device=dev)
+        for _ in range(4):
+            big = big @ big * 1e-3  # keeps the stream busy: a launch elsewhere would read A too early
+        A2 = A + 0 * big[0, 0].nan_to_num(0.0, 0.0, 0.0)
+        got = tb.grouped_gemm(1.0, A2, B, off)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,K,N", [(BF16, 128, 256), (F16, 61, 33), (F32, 64, 48)])
+def test_captured_graph_serves_any_routing(dev, dtype, K, N):
+    g = torch.Generator().manual_seed(9)
+    A, B, W = (_randn(g, *s, dtype=dtype).to(dev) for s in ((96, K), (6, K, N), (96, N)))
+    off = _split(96, [16] * 6).to(dev)
+
+    def both():
+        return tb.grouped_gemm(1.0, A, B, off), tb.grouped_rank_k(1.0, A, W, off)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        both()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        D, P = both()
+    for sizes in ([16] * 6, [0, 0, 96, 0, 0, 0], [1, 2, 3, 4, 5, 6], [40, 0, 40, 0, 1, 0]):
+        off.copy_(_split(96, sizes))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = both()
+        torch.cuda.synchronize()
+        assert torch.equal(D, want[0]) and torch.equal(P, want[1])
+
+
+def test_long_rows_pass_32_bit_offsets(dev):
+    # rows whose byte offsets pass 2^32, and a B whose groups lie 2^32 bytes apart
+    ld = 1 << 20
+    A = torch.empty(2200, ld, dtype=BF16, device=dev)[:, :64]
+    B = torch.empty(3, ld, 1024, dtype=BF16, device=dev)[:, :64, :72]
+    g = torch.Generator().manual_seed(10)
+    Ah, Bh = _randn(g, 2200, 64, dtype=BF16), _randn(g, 3, 64, 72, dtype=BF16)
+    A.copy_(Ah)
+    B.copy_(Bh)
+    off = _split(2200, [2100, 0, 100])
+    D = tb.grouped_gemm(1.0, A, B, off.to(dev))
+    assert og.excess(D, *og.grouped_gemm(1.0, Ah, Bh, off), 64) <= 1
+    W = _randn(g, 2200, 40, dtype=BF16)
+    P = tb.grouped_rank_k(1.0, A, W.to(dev), off.to(dev))
+    assert og.excess(P, *og.grouped_rank_k(1.0, Ah, W, off), 2100) <= 1

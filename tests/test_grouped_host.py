@@ -1,0 +1,107 @@
+"""grouped_gemm / grouped_rank_k on host tensors: values, gradients against differences, refusals."""
+
+import pytest
+import torch
+
+import trnblas_amd as tb
+from oracle import grouped as og
+
+
+def _offsets(*o, dtype=torch.int32):
+    return torch.tensor(o, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("transB", [False, True])
+def test_values(dtype, transB):
+    g = torch.Generator().manual_seed(0)
+    A = torch.randn(20, 9, generator=g).to(dtype)
+    B = torch.randn(4, *((5, 9) if transB else (9, 5)), generator=g).to(dtype)
+    C = torch.randn(20, 5, generator=g).to(dtype)
+    off = _offsets(1, 4, 4, 17, 18)  # rows 0, 18, 19 of no group, group 1 empty
+    D = tb.grouped_gemm(1.5, A, B, off, 0.5, C, transB=transB)
+    ref, den = og.grouped_gemm(1.5, A, B, off, 0.5, C, transB)
+    assert D.dtype == dtype and og.excess(D, ref, den, 9) <= 1
+    W = torch.randn(20, 5, generator=g).to(dtype)
+    P = tb.grouped_rank_k(2.0, A, W, off, dtype=torch.float32)
+    ref, den = og.grouped_rank_k(2.0, A, W, off)
+    assert P.dtype == torch.float32 and og.excess(P, ref, den, 20) <= 1
+    assert not P[1].any()
+
+
+def test_gradients_against_differences():
+    g = torch.Generator().manual_seed(1)
+    off = _offsets(0, 3, 3, 6, dtype=torch.int64)
+    A, B, C = (torch.randn(s, generator=g, dtype=torch.float64, requires_grad=True) for s in ((7, 4), (3, 4, 5), (7, 5)))
+    W = torch.randn(7, 5, generator=g, dtype=torch.float64, requires_grad=True)
+    row = torch.randn(5, generator=g, dtype=torch.float64, requires_grad=True)
+    assert torch.autograd.gradcheck(lambda a, b, c: tb.grouped_gemm(0.7, a, b, off, 0.3, c), (A, B, C))
+    # C broadcast over the rows, B given transposed, and a view of one matrix for all groups
+    assert torch.autograd.gradcheck(
+        lambda a, b, c: tb.grouped_gemm(0.7, a, b.mT.contiguous(), off, 0.3, c, transB=True), (A, B, row)
+    )
+    one = torch.randn(4, 5, generator=g, dtype=torch.float64, requires_grad=True)
+    assert torch.autograd.gradcheck(lambda a, b: tb.grouped_gemm(1.0, a, b.expand(3, 4, 5), off), (A, one))
+    acc = torch.randn(3, 4, 5, generator=g, dtype=torch.float64, requires_grad=True)
+    assert torch.autograd.gradcheck(lambda a, w, c: tb.grouped_rank_k(0.7, a, w, off, 1.0, c), (A, W, acc))
+    assert torch.autograd.gradgradcheck(lambda a, b: tb.grouped_gemm(0.7, a, b, off), (A, B))
+
+
+def test_sizes_of_zero():
+    off = _offsets(0, 0, 0)
+    assert tb.grouped_gemm(1.0, torch.zeros(0, 4), torch.zeros(2, 4, 3), off).shape == (0, 3)
+    D = tb.grouped_gemm(1.0, torch.zeros(5, 0), torch.zeros(2, 0, 3), _offsets(0, 2, 5))
+    assert D.shape == (5, 3) and not D.any()
+    assert tb.grouped_rank_k(1.0, torch.zeros(0, 4), torch.zeros(0, 3), off).shape == (2, 4, 3)
+    assert tb.grouped_gemm(1.0, torch.zeros(3, 4), torch.zeros(0, 4, 3), _offsets(0)).shape == (3, 3)
+
+
+def test_refusals():
+    A, B, off = torch.zeros(6, 4), torch.zeros(2, 4, 3), _offsets(0, 2, 6)
+    with pytest.raises(ValueError, match="inner dimensions"):
+        tb.grouped_gemm(1.0, A, B, off, transB=True)
+    with pytest.raises(ValueError, match="need 3 offsets"):
+        tb.grouped_gemm(1.0, A, B, _offsets(0, 6))
+    with pytest.raises(TypeError, match="int32 or int64"):
+        tb.grouped_gemm(1.0, A, B, off.float())
+    with pytest.raises(ValueError, match="1-D"):
+        tb.grouped_gemm(1.0, A, B, [0, 2, 6])
+    with pytest.raises(TypeError, match="mixed dtypes"):
+        tb.grouped_gemm(1.0, A.bfloat16(), B, off)
+    with pytest.raises(TypeError, match="floating"):
+        tb.grouped_gemm(1.0, A.int(), B.int(), off)
+    with pytest.raises(ValueError, match="3-D"):
+        tb.grouped_gemm(1.0, A, B[0], off)
+    with pytest.raises(ValueError, match="needs C"):
+        tb.grouped_gemm(1.0, A, B, off, beta=1.0)
+    with pytest.raises(ValueError, match="broadcast"):
+        tb.grouped_gemm(1.0, A, B, off, 1.0, torch.zeros(5, 3))
+    with pytest.raises(TypeError, match="C is"):
+        tb.grouped_gemm(1.0, A, B, off, 1.0, torch.zeros(6, 3).double())
+    with pytest.raises(TypeError, match="result dtype"):
+        tb.grouped_gemm(1.0, A, B, off, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="rows"):
+        tb.grouped_rank_k(1.0, A, torch.zeros(5, 3), off)
+    with pytest.raises(ValueError, match="transB"):
+        tb.grouped_gemm(1.0, A, B, off, transB="x")
+
+
+def test_c_abi_refusals():
+    from trnblas_amd.hip import _lib
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    lib = _lib.load()
+
+    def gemm(dtype=0, groups=2, rows=6, n=3, k=4, lda=4, ldb=3, off=4096, beta=0.0, c=None, ldd=3):
+        # the pointers are never dereferenced: every call fails its argument checks
+        return lib.trnblas_hip_grouped_gemm(dtype, 0, 0, groups, rows, n, k, 1.0, 4096, lda, 4096, ldb, 12, off, 0, beta, c,
+                                            3, 4096, ldd, None)  # fmt: skip
+
+    for bad, word in ((dict(dtype=7), b"dtype"), (dict(rows=-1), b"sizes"), (dict(groups=1 << 24), b"sizes"),
+                      (dict(lda=3), b"leading"), (dict(ldd=2), b"leading"), (dict(off=None), b"offsets"),
+                      (dict(off=4098), b"offsets"), (dict(beta=1.0), b"without C"), (dict(k=1 << 31), b"sizes")):  # fmt: skip
+        assert gemm(**bad) == _lib.E_ARG and word in lib.trnblas_hip_last_error(), bad
+    assert gemm(rows=0) == 0  # nothing to do
+    rc = lib.trnblas_hip_grouped_rank_k(1, 0, 2, 6, 4, 3, 1.0, 4096, 3, 4096, 3, 4096, 0, 0.0, None, 3, 0, 4096, 3, 12, None)
+    assert rc == _lib.E_ARG and b"leading" in lib.trnblas_hip_last_error()

@@ -13,6 +13,7 @@ __version__ = "0.1.0"
 
 from . import hip  # noqa: F401
 from . import ozaki  # noqa: F401
+from .grouped import grouped_gemm, grouped_rank_k
 from .hip import get_autotune, get_backend, get_cores, set_autotune, set_backend, set_cores
 from .level3 import batched_gemm, gemm, gemm_fp64, metric_inv_half, syrk, trsm
 
@@ -32,6 +33,8 @@ __all__ = [
     "syrk",
     "trsm",
     "metric_inv_half",
+    "grouped_gemm",
+    "grouped_rank_k",
     "HAS_HIP",
     "HAS_NKI",
     "set_backend",

@@ -53,7 +53,7 @@ static inline bool planned(const GemmArgs& g, const char* kernel) {
 // 6.1e-7 / 4.2e-7 / 3.6e-7, at 1.094 / 1.057 / 1.046 ms. Hence L grows with
 // K. 16-bit operands keep L >= 128 (two of their 64-wide k-tiles: the DMA
 // kernel folds after an even number of k-tiles).
-static inline int chain_length(int64_t K, int elem_bytes) {
+__host__ __device__ static inline int chain_length(int64_t K, int elem_bytes) {
   const int L = K <= 1024 ? 64 : K <= 4096 ? 128 : K < 16384 ? 256 : K < 65536 ? 512 : 1024;
   return elem_bytes == 2 && L < 128 ? 128 : L;
 }

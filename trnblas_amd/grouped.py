@@ -1,0 +1,170 @@
+"""Products over ragged groups of rows: `grouped_gemm` and `grouped_rank_k`.
+
+Rows sorted by expert, each expert with its own matrix, as many rows per
+expert as a router gave it. No counterpart in the reference; signatures and
+result semantics follow `gemm` (a fresh result, C never written, alpha / beta
+fused). Both are differentiable, and each other's gradients:
+
+    D = grouped_gemm(A, B)     dA = grouped_gemm(dD, B^T)   dB = grouped_rank_k(A, dD)
+    D = grouped_rank_k(A, B)   dA = grouped_gemm(B, dD^T)   dB = grouped_gemm(A, dD)
+
+`offsets` (int32 or int64, groups + 1 entries, nondecreasing) gives group g the
+rows offsets[g] .. offsets[g + 1] - 1; groups may be empty, and rows before
+the first or after the last group belong to none. On a ROCm GPU the offsets are
+read by the kernel: no call waits for them, so a captured graph serves any
+routing. Entries outside [0, R] are clamped; decreasing ones give unspecified
+rows (never an access outside the operands).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ._flags import trans_flag
+from .hip import dispatch as _d
+
+__all__ = ["grouped_gemm", "grouped_rank_k"]
+
+
+def _check_offsets(what: str, offsets, like: torch.Tensor, groups: int | None = None) -> int:
+    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 1:
+        raise ValueError(f"{what}: offsets must be a 1-D tensor of groups + 1 row numbers")
+    if offsets.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: offsets must be int32 or int64, got {offsets.dtype}")
+    if offsets.device != like.device:
+        raise ValueError(f"{what}: offsets on {offsets.device}, operands on {like.device}")
+    if groups is not None and offsets.shape[0] != groups + 1:
+        raise ValueError(f"{what}: {groups} groups need {groups + 1} offsets, got {offsets.shape[0]}")
+    return offsets.shape[0] - 1
+
+
+def _check_result(what: str, shape, dtype, beta, C, operand: torch.Tensor, types=None) -> torch.dtype:
+    """The result's dtype; C's shape, dtype and device checked against it."""
+    out = operand.dtype if dtype is None else dtype
+    if out not in (types or (operand.dtype, torch.float32)):
+        raise TypeError(f"{what}: result dtype {out} for {operand.dtype} operands (theirs or float32)")
+    if beta != 0.0:
+        if C is None:
+            raise ValueError(f"{what}: beta != 0 needs C")
+        if C.dtype != out:
+            raise TypeError(f"{what}: C is {C.dtype}, the result {out}")
+        if C.device != operand.device:
+            raise ValueError(f"{what}: C on {C.device}, operands on {operand.device}")
+        if C.dim() > len(shape) or any(c not in (1, s) for c, s in zip(C.shape[::-1], shape[::-1])):
+            raise ValueError(f"{what}: C {tuple(C.shape)} does not broadcast to {tuple(shape)}")
+    return out
+
+
+def _check_operands(what: str, A, B, dims) -> None:
+    for name, X, dim in (("A", A, dims[0]), ("B", B, dims[1])):
+        if not isinstance(X, torch.Tensor) or X.dim() != dim:
+            raise ValueError(f"{what}: {name} must be a {dim}-D tensor")
+        if not X.is_floating_point():
+            raise TypeError(f"{what}: {name} must be a real floating tensor, got {X.dtype}")
+    if A.dtype != B.dtype:
+        raise TypeError(f"{what}: mixed dtypes {A.dtype}, {B.dtype}")
+    if A.device != B.device:
+        raise ValueError(f"{what}: operands on different devices: {A.device} and {B.device}")
+
+
+class _GroupedGemm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, alpha, A, B, offsets, beta, C, out_dtype):
+        ctx.save_for_backward(A, B, offsets)
+        ctx.alpha, ctx.beta = alpha, beta
+        return _d.grouped_gemm(alpha, A, B, offsets, beta, C, out_dtype)
+
+    @staticmethod
+    def backward(ctx, dD):
+        A, B, offsets = ctx.saved_tensors
+        dA = dB = dC = None
+        if ctx.needs_input_grad[5]:
+            dC = ctx.beta * dD
+        # an fp32 result of 16-bit operands: its gradient meets them in their type
+        dD = dD.to(A.dtype)
+        if ctx.needs_input_grad[1]:
+            dA = _GroupedGemm.apply(ctx.alpha, dD, B.mT, offsets, 0.0, None, A.dtype)
+        if ctx.needs_input_grad[2]:
+            if B.stride(1) == 1 and B.stride(2) > 1:  # B is a transposed view: so is its gradient
+                dB = _GroupedRankK.apply(ctx.alpha, dD, A, offsets, 0.0, None, B.dtype).mT
+            else:
+                dB = _GroupedRankK.apply(ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
+        return None, dA, dB, None, None, dC, None
+
+
+class _GroupedRankK(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, alpha, A, B, offsets, beta, C, out_dtype):
+        ctx.save_for_backward(A, B, offsets)
+        ctx.alpha, ctx.beta = alpha, beta
+        return _d.grouped_rank_k(alpha, A, B, offsets, beta, C, out_dtype)
+
+    @staticmethod
+    def backward(ctx, dD):
+        A, B, offsets = ctx.saved_tensors
+        dA = dB = dC = None
+        if ctx.needs_input_grad[5]:
+            dC = ctx.beta * dD
+        dD = dD.to(A.dtype)
+        if ctx.needs_input_grad[1]:
+            dA = _GroupedGemm.apply(ctx.alpha, B, dD.mT, offsets, 0.0, None, A.dtype)
+        if ctx.needs_input_grad[2]:
+            dB = _GroupedGemm.apply(ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
+        return None, dA, dB, None, None, dC, None
+
+
+def grouped_gemm(
+    alpha: float,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    offsets: torch.Tensor,
+    beta: float = 0.0,
+    C: torch.Tensor | None = None,
+    transB: bool = False,
+    dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """D[r] = alpha * A[r] @ op(B[g]) + beta * C[r] for the rows r of group g.
+
+    A (R, K), B (G, K, N), or (G, N, K) with transB; D (R, N) in the operands'
+    dtype, or `dtype` float32 (16-bit operands are summed in fp32 either way).
+    Rows of no group come out as beta * C[r]. A C that broadcasts to (R, N) is
+    taken as in `gemm`. One launch on the GPU, whatever the group sizes.
+    """
+    _check_operands("grouped_gemm", A, B, (2, 3))
+    b = B.mT if trans_flag(transB, "transB") else B
+    _check_offsets("grouped_gemm", offsets, A, b.shape[0])
+    if A.shape[1] != b.shape[1]:
+        raise ValueError(f"grouped_gemm: inner dimensions differ: A {tuple(A.shape)}, op(B) {tuple(b.shape)}")
+    shape = (A.shape[0], b.shape[2])
+    out = _check_result("grouped_gemm", shape, dtype, beta, C, A)
+    c = C.expand(shape) if beta != 0.0 else None
+    if _d._wants_grad(A, B, *(() if c is None else (c,))):
+        return _GroupedGemm.apply(alpha, A, b, offsets, beta, c, out)
+    return _d.grouped_gemm(alpha, A, b, offsets, beta, c, out)
+
+
+def grouped_rank_k(
+    alpha: float,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    offsets: torch.Tensor,
+    beta: float = 0.0,
+    C: torch.Tensor | None = None,
+    dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """D[g] = alpha * A_g^T @ B_g + beta * C[g], A_g and B_g the rows of group g.
+
+    A (R, M), B (R, N); D (G, M, N) in the operands' dtype, or `dtype` float32
+    (with beta = 1 the gradient of earlier calls is added to in fp32). A group
+    without rows gives beta * C[g].
+    """
+    _check_operands("grouped_rank_k", A, B, (2, 2))
+    groups = _check_offsets("grouped_rank_k", offsets, A)
+    if A.shape[0] != B.shape[0]:
+        raise ValueError(f"grouped_rank_k: A has {A.shape[0]} rows, B {B.shape[0]}")
+    shape = (groups, A.shape[1], B.shape[1])
+    out = _check_result("grouped_rank_k", shape, dtype, beta, C, A)
+    c = C.expand(shape) if beta != 0.0 else None
+    if _d._wants_grad(A, B, *(() if c is None else (c,))):
+        return _GroupedRankK.apply(alpha, A, B, offsets, beta, c, out)
+    return _d.grouped_rank_k(alpha, A, B, offsets, beta, c, out)

@@ -19,7 +19,7 @@ import torch  # noqa: F401  (loads torch's HIP runtime before the library)
 _PKG = Path(__file__).resolve().parent.parent
 LIB_PATH = Path(os.environ.get("TRNBLAS_HIP_LIB", _PKG / "lib" / "libtrnblas_hip.so"))
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 F32, BF16, F16, F64 = 0, 1, 2, 3
 DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
@@ -151,6 +151,16 @@ SIGNATURES = {
         [_c_int, _c_i64, _c_i64, _c_int, _c_int, _c_dbl]
         + [_c_ptr, _c_i64, _c_i64] * 3
         + [_c_ptr, _c_size, _c_ptr],
+    ),
+    "trnblas_hip_grouped_gemm": (
+        _c_int,
+        [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_ptr, _c_i64]
+        + [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr],
+    ),
+    "trnblas_hip_grouped_rank_k": (
+        _c_int,
+        [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64]
+        + [_c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr],
     ),
     "trnblas_hip_dgemm": (
         _c_int,

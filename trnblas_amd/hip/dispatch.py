@@ -1303,3 +1303,70 @@ def get_native_ops() -> dict:
 
         _native_ops = _native.OPS
     return _native_ops
+
+
+# ── products over ragged groups of rows (no counterpart in the reference) ─────
+#
+# Device operands of a kernel dtype run the HIP kernels under `auto` and `hip`;
+# anything else is computed by torch where the data is, group by group (which
+# reads the offsets on the host).
+
+
+def _group_rows(offsets: torch.Tensor, rows: int):
+    """(group, first row, row after the last) of each group that has rows."""
+    o = [min(max(int(x), 0), rows) for x in offsets.tolist()]
+    for g, (a, b) in enumerate(zip(o, o[1:])):
+        if b > a:
+            yield g, a, b
+
+
+def _sum_dtype(dtype: torch.dtype) -> torch.dtype:
+    """16-bit operands are multiplied and summed in fp32, as the kernels do."""
+    return torch.float32 if dtype in (torch.bfloat16, torch.float16) else dtype
+
+
+def _scaled_sum(P: torch.Tensor, alpha: float, beta: float, C, out_dtype: torch.dtype) -> torch.Tensor:
+    D = alpha * P if alpha != 1.0 else P
+    return (D + beta * C.to(P.dtype) if beta != 0.0 else D).to(out_dtype)
+
+
+def _grouped_on_hip(op: str, *operands: torch.Tensor) -> bool:
+    if not _use_hip() or not _on_gpu(*operands):
+        return False
+    if operands[0].dtype not in _GEMM_KERNEL_DTYPES:
+        _no_kernel_for_dtype(op, *operands)
+        return False
+    return True
+
+
+def grouped_gemm(alpha, A, B, offsets, beta, C, out_dtype) -> torch.Tensor:
+    """alpha * A[r] @ B[g] + beta * C[r]; see `trnblas_amd.grouped_gemm` (which
+    checks the arguments; B here is op(B), C has the result's shape)."""
+    if _grouped_on_hip("grouped_gemm", A, B):
+        from . import grouped_kernels
+
+        try:
+            return grouped_kernels.grouped_gemm(A, B, offsets, alpha, beta, C, out_dtype)
+        except Exception as exc:  # noqa: BLE001
+            _kernel_failed(exc)
+    dt = _sum_dtype(A.dtype)
+    P = torch.zeros((A.shape[0], B.shape[2]), dtype=dt, device=A.device)
+    for g, a, b in _group_rows(offsets, A.shape[0]):
+        P[a:b] = A[a:b].to(dt) @ B[g].to(dt)
+    return _scaled_sum(P, alpha, beta, C, out_dtype)
+
+
+def grouped_rank_k(alpha, A, B, offsets, beta, C, out_dtype) -> torch.Tensor:
+    """alpha * A_g^T @ B_g + beta * C[g]; see `trnblas_amd.grouped_rank_k`."""
+    if _grouped_on_hip("grouped_rank_k", A, B):
+        from . import grouped_kernels
+
+        try:
+            return grouped_kernels.grouped_rank_k(A, B, offsets, alpha, beta, C, out_dtype)
+        except Exception as exc:  # noqa: BLE001
+            _kernel_failed(exc)
+    dt = _sum_dtype(A.dtype)
+    P = torch.zeros((offsets.shape[0] - 1, A.shape[1], B.shape[1]), dtype=dt, device=A.device)
+    for g, a, b in _group_rows(offsets, A.shape[0]):
+        P[g] = A[a:b].to(dt).mT @ B[a:b].to(dt)
+    return _scaled_sum(P, alpha, beta, C, out_dtype)
