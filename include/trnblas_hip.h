@@ -590,6 +590,45 @@ int trnblas_hip_grouped_rank_k(int dtype, int out_f32, int64_t groups, int64_t r
                                const void* C, int64_t ldc, int64_t strideC, void* D, int64_t ldd,
                                int64_t strideD, void* stream);
 
+/*
+ * Microscaled 4-bit floats (e2m1 codes with one power-of-two scale per 32
+ * values along K). No counterpart in the reference.
+ *
+ * A matrix of R rows by K is two buffers, 16-byte aligned:
+ *  - codes: R rows of Kp / 2 bytes (Kp = K rounded up to 32), two codes per
+ *    byte, the even value low; 0 .. 7 are 0, .5, 1, 1.5, 2, 3, 4, 6 and 8 .. 15
+ *    their negatives; values K .. Kp - 1 are zero;
+ *  - scales: chunks of 256 bytes, one per 16 rows by 512 values, ceil(K / 512)
+ *    chunks along K, ceil(R / 16) rows of chunks: byte 64 (b % 4) + 4 r + b / 4
+ *    of a chunk is e + 127 of its row r, block b (a value is code x 2^e); 255:
+ *    the block is NaN. Bytes of rows and blocks outside the matrix are not 255.
+ * A batch of matrices has them back to back.
+ *
+ * mx_quantize: e = floor(log2(largest magnitude)) - 2, at least -127; codes
+ * rounded to nearest even and saturated at 6; a block with an infinity or a NaN
+ * gets scale byte 255. X (R x K, element (r, k) at r * sr + k * sk, matrix b at
+ * b * sx; elements, >= 0) is TRNBLAS_F32, TRNBLAS_BF16 or TRNBLAS_F16.
+ */
+int trnblas_hip_mx_quantize(int dtype, int64_t R, int64_t K, const void* X, int64_t sr, int64_t sk,
+                            int64_t sx, void* codes, void* scales, int64_t batch, void* stream);
+
+/* The values of such a matrix, in D's type `dtype` (rounded to nearest even). */
+int trnblas_hip_mx_dequantize(int dtype, int64_t R, int64_t K, const void* codes,
+                              const void* scales, void* D, int64_t ldd, int64_t strideD,
+                              int64_t batch, void* stream);
+
+/*
+ * D[r] = alpha A[r] B[g]^T + beta C[r] for the rows r of group g (D[r] =
+ * beta C[r] for rows of no group): A rows x K, B groups matrices of N x K, both
+ * microscaled; products exact, sums fp32. C and D (rows x N) have the type
+ * out_dtype. offsets as in trnblas_hip_grouped_gemm; NULL (groups == 1): one
+ * matrix for all rows.
+ */
+int trnblas_hip_mx_gemm(int out_dtype, int64_t groups, int64_t rows, int64_t N, int64_t K,
+                        double alpha, const void* A, const void* A_scales, const void* B,
+                        const void* B_scales, const void* offsets, int offsets64, double beta,
+                        const void* C, int64_t ldc, void* D, int64_t ldd, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

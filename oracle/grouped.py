@@ -3,6 +3,29 @@
 import torch
 
 
+def split(rows, sizes, lead=0):
+    """Offsets of groups of `sizes` rows after `lead` rows of no group."""
+    o = [lead]
+    for s in sizes:
+        o.append(o[-1] + s)
+    assert o[-1] <= rows
+    return torch.tensor(o, dtype=torch.int32)
+
+
+# (rows, sizes of the groups, rows before the first): one row, empty groups, tiles that end inside, rows of no group
+GROUPS = {
+    "one": (1, [1], 0),
+    "one_of_many": (1, [0] * 37 + [1] + [0] * 26, 0),
+    "token": (6, [0, 1, 0, 2, 0, 0, 1, 1, 0, 1], 0),
+    "gaps": (77, [0, 9, 0, 40, 3], 11),
+    "all_gap": (19, [0, 0, 0], 7),
+    "small": (150, [17, 33, 1, 64, 35], 0),
+    "many": (300, [(3 * i) % 5 for i in range(140)], 2),
+    "uneven": (700, [513, 0, 2, 185], 0),
+    "single": (400, [400], 0),
+}
+
+
 def rows_of(offsets, rows):
     o = [min(max(int(x), 0), rows) for x in offsets.tolist()]
     return [(g, a, b) for g, (a, b) in enumerate(zip(o, o[1:])) if b > a]

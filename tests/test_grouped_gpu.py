@@ -6,6 +6,8 @@ import torch
 
 import trnblas_amd as tb
 from oracle import grouped as og
+from oracle.grouped import GROUPS
+from oracle.grouped import split as _split
 
 pytestmark = pytest.mark.gpu
 
@@ -17,27 +19,6 @@ def _randn(g, *shape, dtype=F32):
     return torch.randn(*shape, generator=g).to(dtype)
 
 
-def _split(rows, sizes, lead=0):
-    """Offsets of groups of `sizes` rows after `lead` rows of no group."""
-    o = [lead]
-    for s in sizes:
-        o.append(o[-1] + s)
-    assert o[-1] <= rows
-    return torch.tensor(o, dtype=torch.int32)
-
-
-# (rows, sizes of the groups, rows before the first): one row, empty groups, tiles that end inside, rows of no group
-GROUPS = {
-    "one": (1, [1], 0),
-    "one_of_many": (1, [0] * 37 + [1] + [0] * 26, 0),
-    "token": (6, [0, 1, 0, 2, 0, 0, 1, 1, 0, 1], 0),
-    "gaps": (77, [0, 9, 0, 40, 3], 11),
-    "all_gap": (19, [0, 0, 0], 7),
-    "small": (150, [17, 33, 1, 64, 35], 0),
-    "many": (300, [(3 * i) % 5 for i in range(140)], 2),
-    "uneven": (700, [513, 0, 2, 185], 0),
-    "single": (400, [400], 0),
-}
 # (K, N): below and across the tiles of 16, 32, 64, 128 and 256, multiples of 16 bytes and not
 SIZES = [(1, 1), (7, 5), (33, 70), (64, 128), (100, 61), (136, 264), (264, 136), (512, 520), (515, 257), (1032, 384)]
 

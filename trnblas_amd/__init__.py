@@ -16,6 +16,7 @@ from . import ozaki  # noqa: F401
 from .grouped import grouped_gemm, grouped_rank_k
 from .hip import get_autotune, get_backend, get_cores, set_autotune, set_backend, set_cores
 from .level3 import batched_gemm, gemm, gemm_fp64, metric_inv_half, syrk, trsm
+from .mx import MXMatrix, mx_dequantize, mx_gemm, mx_grouped_gemm, mx_quantize
 
 nki = hip  # the reference's subpackage name
 
@@ -35,6 +36,11 @@ __all__ = [
     "metric_inv_half",
     "grouped_gemm",
     "grouped_rank_k",
+    "MXMatrix",
+    "mx_quantize",
+    "mx_dequantize",
+    "mx_gemm",
+    "mx_grouped_gemm",
     "HAS_HIP",
     "HAS_NKI",
     "set_backend",

@@ -162,6 +162,19 @@ SIGNATURES = {
         [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64]
         + [_c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr],
     ),
+    "trnblas_hip_mx_quantize": (
+        _c_int,
+        [_c_int, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_ptr],
+    ),
+    "trnblas_hip_mx_dequantize": (
+        _c_int,
+        [_c_int, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr],
+    ),
+    "trnblas_hip_mx_gemm": (
+        _c_int,
+        [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_ptr, _c_ptr, _c_ptr, _c_ptr]
+        + [_c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr],
+    ),
     "trnblas_hip_dgemm": (
         _c_int,
         [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_dbl]

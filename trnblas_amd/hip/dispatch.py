@@ -1370,3 +1370,17 @@ def grouped_rank_k(alpha, A, B, offsets, beta, C, out_dtype) -> torch.Tensor:
     for g, a, b in _group_rows(offsets, A.shape[0]):
         P[g] = A[a:b].to(dt).mT @ B[a:b].to(dt)
     return _scaled_sum(P, alpha, beta, C, out_dtype)
+
+
+# ── microscaled 4-bit floats (no counterpart in the reference) ────────────────
+
+
+def mx_on_hip(*operands: torch.Tensor) -> bool:
+    """Whether the kernels serve these operands: float ones of a kernel dtype,
+    codes and scales always."""
+    if not _use_hip() or not _on_gpu(*operands):
+        return False
+    bad = [t for t in operands if t.is_floating_point() and t.dtype not in _GEMM_KERNEL_DTYPES]
+    if bad:
+        _no_kernel_for_dtype("mx", *bad)
+    return not bad

@@ -1,4 +1,4 @@
-"""Tensor-level wrappers of the grouped products' C ABI, in the manner of
+"""Tensor-level wrappers of the grouped and the microscaled 4-bit products' C ABI, in the manner of
 `kernels.py`: device tensors in, a fresh output on their device, launched on
 torch's current stream. The group offsets stay on the device: no call waits
 for the GPU.
@@ -86,5 +86,63 @@ def grouped_rank_k(
         G, R, M, N, float(alpha), ptr(a), lda, ptr(b), ldb, ptr(o), o64, float(beta) if c is not None else 0.0,
         ptr(c), max(c.stride(1), N) if c is not None else N, c.stride(0) if c is not None and G > 1 else 0,
         ptr(D), max(N, 1), M * N, stream_of(dev),
+    )  # fmt: skip
+    return D
+
+
+def mx_buffers(shape, dev) -> tuple[torch.Tensor, torch.Tensor]:
+    """Fresh (codes, scales) buffers of a matrix (..., R, K); see
+    include/trnblas_hip.h for their layout."""
+    *lead, R, K = shape
+    codes = torch.empty((*lead, R, -(-K // 32) * 16), dtype=torch.uint8, device=dev)
+    return codes, torch.empty((*lead, -(-R // 16), -(-K // 512), 256), dtype=torch.uint8, device=dev)
+
+
+def mx_quantize(X: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of X (R, K) or (batch, R, K), any strides."""
+    dev = _require_device(X)
+    codes, scales = mx_buffers(X.shape, dev)
+    if any(s < 0 for s in X.stride()):
+        X = X.contiguous()
+    batch, sx = (X.shape[0], X.stride(0)) if X.dim() == 3 else (1, 0)
+    R, K = X.shape[-2:]
+    _probed_call(
+        "mx_quantize", "trnblas_hip_mx_quantize", _lib.DTYPE_CODES[X.dtype], R, K, ptr(X), X.stride(-2), X.stride(-1),
+        sx, ptr(codes), ptr(scales), batch, stream_of(dev),
+    )  # fmt: skip
+    return codes, scales
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int, dtype: torch.dtype) -> torch.Tensor:
+    dev = _require_device(codes, scales)
+    *lead, R, _ = codes.shape
+    D = torch.empty((*lead, R, K), dtype=dtype, device=dev)
+    _probed_call(
+        "mx_dequantize", "trnblas_hip_mx_dequantize", _lib.DTYPE_CODES[dtype], R, K, ptr(codes), ptr(scales), ptr(D),
+        max(K, 1), R * K, lead[0] if lead else 1, stream_of(dev),
+    )  # fmt: skip
+    return D
+
+
+def mx_gemm(
+    a: tuple[torch.Tensor, torch.Tensor],
+    b: tuple[torch.Tensor, torch.Tensor],
+    K: int,
+    out_dtype: torch.dtype,
+    offsets: torch.Tensor | None = None,
+    alpha: float = 1.0,
+    beta: float = 0.0,
+    C: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """alpha * A[r] @ B[g]^T + beta * C[r] of (codes, scales) pairs: A (R, K),
+    B (N, K), or (G, N, K) with offsets (G + 1)."""
+    dev = _require_device(*a, *b, *(() if C is None else (C,)), *(() if offsets is None else (offsets,)))
+    R, N = a[0].shape[0], b[0].shape[-2]
+    o, o64 = (None, 0) if offsets is None else offsets_of(offsets)
+    D, c = _output_like(C, beta, (R, N), out_dtype, dev)
+    _probed_call(
+        "mx_gemm", "trnblas_hip_mx_gemm", _lib.DTYPE_CODES[out_dtype], 1 if offsets is None else b[0].shape[0], R, N, K,
+        float(alpha), ptr(a[0]), ptr(a[1]), ptr(b[0]), ptr(b[1]), ptr(o), o64, float(beta) if c is not None else 0.0,
+        ptr(c), max(c.stride(0), N) if c is not None else N, ptr(D), max(N, 1), stream_of(dev),
     )  # fmt: skip
     return D
