@@ -64,4 +64,4 @@ def excess(D, ref, den, k):
     tiny = {torch.float32: 2.0**-149, torch.bfloat16: 2.0**-133, torch.float16: 2.0**-25}[D.dtype]
     bound = (k + 2) * 2.0**-23 * den
     bound = bound + u * (ref.abs() + bound) + tiny
-    return float(((D.double().cpu() - ref).abs() / bound).max()) if D.numel() else 0.0
+    return float(((D.detach().double().cpu() - ref).abs() / bound).max()) if D.numel() else 0.0

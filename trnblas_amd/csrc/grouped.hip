@@ -9,88 +9,11 @@
 
 #include "gemm.hpp"
 #include "grouped.hpp"
+#include "grouped_plan.hpp"
+#include "ring.hpp"
+#include "rows.hpp"
 
 namespace trnblas {
-
-// The tile of a workgroup: where its operand panels start, how many rows of
-// each are inside, the k range, and where the output goes.
-struct TileJob {
-  const char *A, *B;  // panel corners at k = 0
-  int rows_a, rows_b, K;
-  int64_t m;  // first output row
-  int n;      // first output column
-  const void* C;
-  void* D;
-};
-
-// RK: ragged k (grouped_rank_k), else ragged rows.
-template <typename T, int BM, int BN, bool BKC, bool RK>
-__device__ __forceinline__ bool tile_job(const GroupedArgs& g, TileJob& j) {
-  const int64_t es = sizeof(T), eo = g.out32 ? 4 : es;
-  if constexpr (RK) {
-    const int t = xcd_remap(blockIdx.x, gridDim.x);
-    const int per = g.tiles_m * g.tiles_n, grp = t / per;
-    int tm, tn;
-    grouped_tile(t - grp * per, g.tiles_m, g.tiles_n, 8, tm, tn);
-    const int start = boundary(g, grp + 1), end = max(boundary(g, grp + 2), start);
-    j.m = tm * BM;
-    j.n = tn * BN;
-    j.K = end - start;
-    j.A = static_cast<const char*>(g.A) + (start * g.lda + j.m) * es;
-    j.B = static_cast<const char*>(g.B) + (start * g.ldb + j.n) * es;
-    j.rows_a = min(BM, g.M - (int)j.m);
-    j.C = static_cast<const char*>(g.C) + (g.C ? grp * g.sC * eo : 0);
-    j.D = static_cast<char*>(g.D) + grp * g.sD * eo;
-  } else {
-    Segment s;
-    if (!ragged_tile<BM>(g, blockIdx.x, 8, s)) return false;
-    const bool of_group = s.group >= 0 && s.group < g.groups;
-    j.m = s.row;
-    j.n = s.tn * BN;
-    j.K = of_group ? g.K : 0;
-    j.A = static_cast<const char*>(g.A) + s.row * g.lda * es;
-    j.B = static_cast<const char*>(g.B) + (of_group ? s.group * g.sB + (BKC ? j.n * g.ldb : j.n) : 0) * es;
-    j.rows_a = min(BM, s.end - s.row);
-    j.C = g.C;
-    j.D = g.D;
-  }
-  j.rows_b = min(BN, g.N - j.n);
-  return true;
-}
-
-// The 16-byte group of an operand at (row, k): `n` of its EV values are inside.
-typedef i32x4 __attribute__((aligned(2))) i32x4_at2;
-typedef i32x4 __attribute__((aligned(4))) i32x4_at4;
-
-template <typename T>
-__device__ __forceinline__ i32x4 load_any(const char* p, int n) {
-  constexpr int EV = 16 / sizeof(T);
-  using loose = std::conditional_t<sizeof(T) == 2, i32x4_at2, i32x4_at4>;
-  if (n >= EV) return *reinterpret_cast<const loose*>(p);
-  union {
-    T e[EV];
-    i32x4 v;
-  } u;
-  u.v = i32x4{0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < EV; ++i)
-    if (i < n) u.e[i] = reinterpret_cast<const T*>(p)[i];
-  return u.v;
-}
-
-template <int FM, int FN, typename O>
-__device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& j, const f32x4 (&acc)[FM][FN], int m0,
-                                           int n0, int lane) {
-#pragma unroll
-  for (int a = 0; a < FM; ++a) {
-    const int m = m0 + 16 * a + (lane & 15);
-    if (m < j.rows_a) {
-#pragma unroll
-      for (int b = 0; b < FN; ++b)
-        store_quad<O>(g, static_cast<const O*>(j.C), static_cast<O*>(j.D), j.m + m, j.n + n0 + 16 * b + 4 * (lane >> 4), acc[a][b]);
-    }
-  }
-}
 
 // Operands of any alignment and any strides: the panels go through registers.
 // 256 threads on a 64 x 64 tile, each wave 32 x 32; the loads of k-tile t + 1 are
@@ -109,19 +32,29 @@ __global__ __launch_bounds__(256) void grouped_any_kernel(GroupedArgs g) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m0 = 32 * (wave & 1), n0 = 32 * (wave >> 1);
-  int ra, ka, rb, kb;
-  PA::where(tid, ra, ka);
-  PB::where(tid, rb, kb);
-  const char* pa = j.A + (RK ? (int64_t)ka * g.lda + ra : (int64_t)ra * g.lda + ka) * ES;
-  const char* pb = j.B + (BKC ? (int64_t)rb * g.ldb + kb : (int64_t)kb * g.ldb + rb) * ES;
+  int ra[2], ka[2], rb[2], kb[2];
+  const char *pa[2], *pb[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    PA::where(tid + 256 * h, ra[h], ka[h]);
+    PB::where(tid + 256 * h, rb[h], kb[h]);
+    pa[h] = j.A + (RK ? (int64_t)ka[h] * g.lda + ra[h] : (int64_t)ra[h] * g.lda + ka[h]) * ES;
+    pb[h] = j.B + (BKC ? (int64_t)rb[h] * g.ldb + kb[h] : (int64_t)kb[h] * g.ldb + rb[h]) * ES;
+  }
   const int64_t step_a = (RK ? BK * g.lda : BK) * ES, step_b = (BKC ? BK : BK * g.ldb) * ES;
   const int nk = (j.K + BK - 1) / BK;
-  i32x4 va, vb;
+  i32x4 va[2], vb[2];
   auto load = [&](int kt) __attribute__((always_inline)) {
     const int left = j.K - kt * BK;
-    va = load_any<T>(pa + kt * step_a, RK ? (ka < left ? j.rows_a - ra : 0) : (ra < j.rows_a ? left - ka : 0));
-    vb = load_any<T>(pb + kt * step_b, BKC ? (rb < j.rows_b ? left - kb : 0) : (kb < left ? j.rows_b - rb : 0));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      va[h] = load_any<T>(pa[h] + kt * step_a, RK ? (ka[h] < left ? j.rows_a - ra[h] : 0) : (ra[h] < j.rows_a ? left - ka[h] : 0));
+      vb[h] = load_any<T>(pb[h] + kt * step_b, BKC ? (rb[h] < j.rows_b ? left - kb[h] : 0) : (kb[h] < left ? j.rows_b - rb[h] : 0));
+    }
   };
+  uint32_t oa[PA::NV], ob[PB::NV];
+  PA::lane_offsets(m0, lane, oa);
+  PB::lane_offsets(n0, lane, ob);
   f32x4 acc[FM][FN], sum[FM][FN];
 #pragma unroll
   for (int a = 0; a < FM; ++a)
@@ -132,20 +65,31 @@ __global__ __launch_bounds__(256) void grouped_any_kernel(GroupedArgs g) {
   if (nk > 0) load(0);
   for (int kt = 0; kt < nk; ++kt) {
     char* st = lds[kt & 1];
-    *reinterpret_cast<i32x4*>(st + 16 * tid) = va;
-    *reinterpret_cast<i32x4*>(st + PA::BYTES + 16 * tid) = vb;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      *reinterpret_cast<i32x4*>(st + 16 * (tid + 256 * h)) = va[h];
+      *reinterpret_cast<i32x4*>(st + PA::BYTES + 16 * (tid + 256 * h)) = vb[h];
+    }
     // one barrier per k-tile: stage t's readers are past it before t + 2 is stored
     __syncthreads();
     if (kt + 1 < nk) load(kt + 1);
-    i32x4 fa[FM], fb[FN];
+    const char *qa[PA::NV], *qb[PB::NV];
 #pragma unroll
-    for (int a = 0; a < FM; ++a) fa[a] = PA::frag(st, m0 + 16 * a, lane);
+    for (int i = 0; i < PA::NV; ++i) qa[i] = st + oa[i];
 #pragma unroll
-    for (int b = 0; b < FN; ++b) fb[b] = PB::frag(st + PA::BYTES, n0 + 16 * b, lane);
+    for (int i = 0; i < PB::NV; ++i) qb[i] = st + PA::BYTES + ob[i];
 #pragma unroll
-    for (int b = 0; b < FN; ++b)
+    for (int h = 0; h < 2; ++h) {
+      i32x4 fa[FM], fb[FN];
 #pragma unroll
-      for (int a = 0; a < FM; ++a) mma_tile<T>(acc[a][b], fb[b], fa[a]);
+      for (int a = 0; a < FM; ++a) fa[a] = PA::frag(qa, a, h);
+#pragma unroll
+      for (int b = 0; b < FN; ++b) fb[b] = PB::frag(qb, b, h);
+#pragma unroll
+      for (int b = 0; b < FN; ++b)
+#pragma unroll
+        for (int a = 0; a < FM; ++a) mma_tile<T>(acc[a][b], fb[b], fa[a]);
+    }
     if (FOLD && --chain == 0) {
 #pragma unroll
       for (int a = 0; a < FM; ++a)
@@ -195,14 +139,82 @@ static int run_any(GroupedArgs g, hipStream_t s) {
   return check_launch(what);
 }
 
+// Operands that LDS DMA reads in place: see ring.hpp. Its 32-bit offsets reach
+// over one panel of a K-contiguous operand and one k-tile of the other kind.
+template <typename T>
+static bool dma_ready(const GroupedArgs& g, bool bkc, bool rk) {
+  const int64_t es = sizeof(T), far = INT32_MAX - 1024;
+  auto whole = [&](const void* p, int64_t ld, int64_t st, int64_t ext) {
+    return (uintptr_t)p % 16 == 0 && ld * es % 16 == 0 && st * es % 16 == 0 && ext * es % 16 == 0;
+  };
+  const int64_t ra = rk ? 128 / es : 256, rb = bkc ? 256 : 128 / es;
+  return whole(g.A, g.lda, 0, rk ? g.M : g.K) && whole(g.B, g.ldb, g.sB, bkc ? g.K : g.N) && (!rk || g.rows < far) &&
+         ra * g.lda * es < far && rb * g.ldb * es < far;
+}
+
+template <typename T, int FM, int FN, bool BKC, bool RK>
+static int run_ring(GroupedArgs g, hipStream_t s) {
+  constexpr int BM = 32 * FM, BN = 32 * FN;
+  const char* what = RK ? kRankK : kGemm;
+  g.tiles_m = (g.M + BM - 1) / BM;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  unsigned grid;
+  const int64_t rows = RK ? (int64_t)g.groups * g.tiles_m : row_tiles(g.rows, g.groups, BM);
+  if (int rc = grid_of(rows * g.tiles_n, what, &grid)) return rc;
+  if (!RK) grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
+  hipLaunchKernelGGL((ring_kernel<T, FM, FN, BKC, RK>), dim3(grid), dim3(256), 0, s, g, MxScales{});
+  return check_launch(what);
+}
+
+template <typename T, int MF, int NF, int KS, bool BKC>
+static int run_rows(GroupedArgs g, hipStream_t s) {
+  constexpr int BN = 128 * NF / KS;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  unsigned grid;
+  if (int rc = grid_of(row_tiles(g.rows, g.groups, 16 * MF) * g.tiles_n, kGemm, &grid)) return rc;
+  grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
+  hipLaunchKernelGGL((rows_kernel<T, MF, NF, KS, BKC>), dim3(grid), dim3(512), 0, s, g, MxScales{});
+  return check_launch(kGemm);
+}
+
+template <typename T, int MF, bool BKC>
+static int run_rows_split(int ks, const GroupedArgs& g, hipStream_t s) {
+  constexpr int NF = BKC ? 1 : 4;
+  return ks == 8   ? run_rows<T, MF, NF, 8, BKC>(g, s)
+         : ks == 4 ? run_rows<T, MF, NF, 4, BKC>(g, s)
+         : ks == 2 ? run_rows<T, MF, NF, 2, BKC>(g, s)
+                   : run_rows<T, MF, NF, 1, BKC>(g, s);
+}
+
+// ring: index of kRing16. fp32 always takes the 64 x 128 tiles: three workgroups
+// per CU hide its longer MFMAs' steps best (8 groups of 128 rows, 2048 x 4096: 217 us
+// against 220 on 128 x 128 and 267 on grouped_any_kernel).
+template <typename T, bool BKC, bool RK>
+static int run_ring_choice(int ring, const GroupedArgs& g, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (ring == 0) return run_ring<T, 8, 8, BKC, RK>(g, s);
+    if (ring == 1) return run_ring<T, 4, 4, BKC, RK>(g, s);
+  }
+  return run_ring<T, 2, 4, BKC, RK>(g, s);
+}
+
+template <typename T, bool BKC>
+static int run_grouped(const GroupedArgs& g, hipStream_t s) {
+  const bool ready = dma_ready<T>(g, BKC, false);
+  const GroupedChoice c = choose_grouped(kRing16, g.rows, g.groups, g.N, g.K, (double)g.K * sizeof(T), sizeof(T), BKC);
+  if (c.ring < 0) return c.mf == 1 ? run_rows_split<T, 1, BKC>(c.ks, g, s) : run_rows_split<T, 2, BKC>(c.ks, g, s);
+  return ready ? run_ring_choice<T, BKC, false>(c.ring, g, s) : run_any<T, BKC, false>(g, s);
+}
+
 template <typename T>
 static int run_gemm(const GroupedArgs& g, bool bkc, hipStream_t s) {
-  return bkc ? run_any<T, true, false>(g, s) : run_any<T, false, false>(g, s);
+  return bkc ? run_grouped<T, true>(g, s) : run_grouped<T, false>(g, s);
 }
 
 template <typename T>
 static int run_rank_k(const GroupedArgs& g, hipStream_t s) {
-  return run_any<T, false, true>(g, s);
+  if (!dma_ready<T>(g, false, true)) return run_any<T, false, true>(g, s);
+  return run_ring_choice<T, false, true>(choose_rank_k(g.groups, g.M, g.N, (double)g.rows / g.groups * sizeof(T) / 128.0), g, s);
 }
 
 static bool quads(const GroupedArgs& g, int dtype) {

@@ -27,6 +27,7 @@ struct GroupedArgs {
   int M, N, K;       // ragged rows: M unused; ragged k: K unused
   int tiles_m, tiles_n;
   float alpha, beta;
+  int out_f16;  // D and C are fp16 (products of 4-bit floats; else bf16 or fp32)
   int out32;  // D and C are fp32 whatever the operands are
   int vec4;   // D and C take 4-element accesses (aligned, ld % 4 == 0)
 };
@@ -54,13 +55,15 @@ struct Segment {
   int tn;          // column tile
 };
 
-// Inclusive sum over the lanes of the wave.
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+// Inclusive sum over the lanes of the wave, by DPP: lanes 1, 2, 4 and 8 back in
+// each row of 16, then the rows' last lanes broadcast to the rows after them.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
   return v;
 }
 
@@ -79,7 +82,7 @@ __device__ __forceinline__ bool ragged_tile(const GroupedArgs& g, int bid, int b
     const int i = base + lane;
     st = boundary(g, i);
     en = max(boundary(g, i + 1), st);
-    incl = wave_scan(i < nseg ? (en - st + BM - 1) / BM : 0, lane);
+    incl = wave_scan(i < nseg ? (en - st + BM - 1) / BM : 0);
     total += __builtin_amdgcn_readlane(incl, 63);
   }
   const int ntile = total * g.tiles_n;
@@ -96,7 +99,7 @@ __device__ __forceinline__ bool ragged_tile(const GroupedArgs& g, int bid, int b
       const int j = base + lane;
       st = boundary(g, j);
       en = max(boundary(g, j + 1), st);
-      incl = wave_scan(j < nseg ? (en - st + BM - 1) / BM : 0, lane);
+      incl = wave_scan(j < nseg ? (en - st + BM - 1) / BM : 0);
       const int sum = __builtin_amdgcn_readlane(incl, 63);
       if (tm < before + sum || base + 64 >= nseg) {
         tm -= before;
@@ -126,60 +129,79 @@ __device__ __forceinline__ s16x4 lds_transpose(const void* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(const_cast<void*>(p)));
 }
 
-// LDS panel of ROWS rows (of M or N) by one k-tile of 64 bytes per row.
-// KC: the operand's rows are K-contiguous; row r takes 64 bytes, its 16-byte
-// group q in slot q ^ ((r / 4) % 4), so that the 16 lanes of a quarter wave,
-// which read the same group of 16 rows, cover all banks. Otherwise rows of k
-// with ROWS values each; 16-byte group q of row k sits in slot q ^ swz(k): the
-// transposing reads of 16 lanes take four rows of k at the same columns (16-bit
-// types), the four quarters of a wave rows k, k + 4, k + 8, k + 12 (fp32).
+// LDS panel of ROWS rows (of M or N) by one k-tile of 128 bytes per row, two
+// MFMA steps of 64 bytes.
+// KC: the operand's rows are K-contiguous; row r takes 128 bytes, its 16-byte
+// group q in slot q ^ ((r / 2) % 8). A 16-byte LDS read serves lanes 0-3, 12-15 and
+// 20-27 together, then 4-11, 16-19 and 28-31 (and the same of the upper half):
+// each such set then covers all banks. (64 bytes per row and k-tile cost 10 %:
+// the L2 serves 128-byte lines.) Otherwise rows of k with ROWS values each; 16-byte
+// group q of row k sits in slot q ^ swz(k): the transposing reads of 32 lanes take
+// rows k .. k + 3 and k + 8 .. k + 11 at the same columns (16-bit types), the four
+// quarters of a wave rows k, k + 4, k + 8, k + 12 (fp32).
 template <typename T, int ROWS, bool KC>
 struct Panel {
-  static constexpr int ES = sizeof(T), EV = 16 / ES, BK = 64 / ES, BYTES = ROWS * 64;
+  static constexpr int ES = sizeof(T), EV = 16 / ES, BK = 128 / ES, BYTES = ROWS * 128;
   static constexpr int GPR = ROWS / EV;  // groups per row of k
   static __device__ __forceinline__ int swz(int k) {
     if constexpr (ES == 4) return 4 * ((k >> 2) & 3);
-    return ROWS >= 128 ? 4 * (k & 3) : 4 * ((k >> 1) & 1);
+    return (ROWS >= 128 ? 4 * (k & 3) : 4 * ((k >> 1) & 1)) + 2 * ((k >> 3) & 1);
   }
   // which values 16-byte group `i` of the panel (in LDS order) holds
   static __device__ __forceinline__ void where(int i, int& row, int& k) {
     if constexpr (KC) {
-      row = i >> 2;
-      k = EV * ((i & 3) ^ ((row >> 2) & 3));
+      row = i >> 3;
+      k = EV * ((i & 7) ^ ((row >> 1) & 7));
     } else {
       k = i / GPR;
       row = EV * ((i % GPR) ^ swz(k));
     }
   }
-  // MFMA operand of rows row0 .. row0 + 15: lane l holds row l % 16, 16 bytes
-  // of k from group l / 16.
-  static __device__ __forceinline__ i32x4 frag(const char* p, int row0, int lane) {
+  // MFMA operand i of a wave whose rows start at row0 (a multiple of 64, or of
+  // 32 with fewer than five operands), step s: rows row0 + 16 i .. + 15, lane l with
+  // row l % 16 and 16 bytes of k from group 4 s + l / 16. The swizzles make its LDS
+  // offset a constant plus one of NV offsets of the lane.
+  static constexpr int NV = KC ? 2 : ES == 4 ? 4 : 8;
+  static __device__ __forceinline__ void lane_offsets(int row0, int lane, uint32_t (&v)[NV]) {
     const int li = lane & 15, lg = lane >> 4;
     if constexpr (KC) {
-      const int r = row0 + li;
-      return *reinterpret_cast<const i32x4*>(p + r * 64 + 16 * (lg ^ ((r >> 2) & 3)));
+#pragma unroll
+      for (int s = 0; s < 2; ++s) v[s] = (row0 + li) * 128 + 16 * ((4 * s + lg) ^ (li >> 1));
     } else if constexpr (ES == 4) {
-      const int c = row0 + li;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = 4 * lg * (ROWS * 4) + 16 * (((row0 >> 2) + 4 * i + (li >> 2)) ^ (4 * lg)) + 4 * (li & 3);
+    } else {
+      const int k = 8 * lg + (li >> 2);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = k * (ROWS * 2) + 16 * (((row0 >> 3) + 2 * i + ((li & 3) >> 1)) ^ swz(k)) + 8 * (li & 1);
+    }
+  }
+  // p: the panel plus lane_offsets'
+  static __device__ __forceinline__ i32x4 frag(const char* const (&p)[NV], int i, int s) {
+    if constexpr (KC) {
+      return *reinterpret_cast<const i32x4*>(p[s] + 2048 * i);
+    } else if constexpr (ES == 4) {
       i32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        v[e] = *reinterpret_cast<const int*>(p + (4 * lg + e) * (ROWS * 4) + 16 * ((c >> 2) ^ (4 * lg)) + 4 * (c & 3));
+        v[e] = *reinterpret_cast<const int*>(p[i & 3] + (16 * s + e) * (ROWS * 4) + 256 * (i >> 2));
       return v;
     } else {
-      const int k = 8 * lg + (li >> 2), c = row0 + 4 * (li & 3);
-      const char* s = p + k * (ROWS * 2) + 16 * ((c >> 3) ^ swz(k)) + 2 * (c & 4);
+      const char* q = p[i & 7] + 256 * (i >> 3) + 32 * s * (ROWS * 2);
       union {
         s16x4 h[2];
         i32x4 v;
       } u;
-      u.h[0] = lds_transpose(s);
-      u.h[1] = lds_transpose(s + 4 * (ROWS * 2));
+      u.h[0] = lds_transpose(q);
+      u.h[1] = lds_transpose(q + 4 * (ROWS * 2));
       return u.v;
     }
   }
 };
 
-// acc += one k-tile of (rows n of b) x (rows m of a): lane l holds column
+// acc += one MFMA step of (rows n of b) x (rows m of a): lane l holds column
 // m = l % 16 and rows n = 4 (l / 16) + r, so four consecutive n of one m.
 template <typename T>
 __device__ __forceinline__ void mma_tile(f32x4& acc, const i32x4& b, const i32x4& a) {
@@ -220,6 +242,69 @@ __device__ __forceinline__ void store_quad(const GroupedArgs& g, const O* C, O* 
         if (g.beta != 0.0f) v[u] = __builtin_fmaf(g.beta, (float)c[u], v[u]);
         d[u] = (O)v[u];
       }
+  }
+}
+
+// The tile of a workgroup: where its operand panels start, how many rows of
+// each are inside, the k range, and where the output goes.
+struct TileJob {
+  const char *A, *B;  // panel corners at k = 0
+  int rows_a, rows_b, K;
+  int group;
+  int64_t m;  // first output row
+  int n;      // first output column
+  const void* C;
+  void* D;
+};
+
+// RK: ragged k (grouped_rank_k), else ragged rows.
+template <typename T, int BM, int BN, bool BKC, bool RK>
+__device__ __forceinline__ bool tile_job(const GroupedArgs& g, TileJob& j) {
+  const int64_t es = sizeof(T), eo = g.out32 ? 4 : es;
+  if constexpr (RK) {
+    const int t = xcd_remap(blockIdx.x, gridDim.x);
+    const int per = g.tiles_m * g.tiles_n, grp = t / per;
+    int tm, tn;
+    grouped_tile(t - grp * per, g.tiles_m, g.tiles_n, 8, tm, tn);
+    const int start = boundary(g, grp + 1), end = max(boundary(g, grp + 2), start);
+    j.group = grp;
+    j.m = tm * BM;
+    j.n = tn * BN;
+    j.K = end - start;
+    j.A = static_cast<const char*>(g.A) + (start * g.lda + j.m) * es;
+    j.B = static_cast<const char*>(g.B) + (start * g.ldb + j.n) * es;
+    j.rows_a = min(BM, g.M - (int)j.m);
+    j.C = static_cast<const char*>(g.C) + (g.C ? grp * g.sC * eo : 0);
+    j.D = static_cast<char*>(g.D) + grp * g.sD * eo;
+  } else {
+    Segment s;
+    if (!ragged_tile<BM>(g, blockIdx.x, 8, s)) return false;
+    const bool of_group = s.group >= 0 && s.group < g.groups;
+    j.group = s.group;
+    j.m = s.row;
+    j.n = s.tn * BN;
+    j.K = of_group ? g.K : 0;
+    j.A = static_cast<const char*>(g.A) + s.row * g.lda * es;
+    j.B = static_cast<const char*>(g.B) + (of_group ? s.group * g.sB + (BKC ? j.n * g.ldb : j.n) : 0) * es;
+    j.rows_a = min(BM, s.end - s.row);
+    j.C = g.C;
+    j.D = g.D;
+  }
+  j.rows_b = min(BN, g.N - j.n);
+  return true;
+}
+
+template <int FM, int FN, typename O>
+__device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& j, const f32x4 (&acc)[FM][FN], int m0,
+                                           int n0, int lane) {
+#pragma unroll
+  for (int a = 0; a < FM; ++a) {
+    const int m = m0 + 16 * a + (lane & 15);
+    if (m < j.rows_a) {
+#pragma unroll
+      for (int b = 0; b < FN; ++b)
+        store_quad<O>(g, static_cast<const O*>(j.C), static_cast<O*>(j.D), j.m + m, j.n + n0 + 16 * b + 4 * (lane >> 4), acc[a][b]);
+    }
   }
 }
 

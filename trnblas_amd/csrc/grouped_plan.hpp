@@ -1,0 +1,88 @@
+// Which kernel a grouped product runs on: from its sizes, types and alignment
+// only (the group sizes are on the device), by estimated times.
+#pragma once
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.hpp"
+
+namespace trnblas {
+
+// Times of the ring kernels (us), fitted to a sweep of 1, 8 and 64 groups of 1 ..
+// 2048 rows over matrices of 1024 x 1024, 2048 x 4096 and 4096 x 1536 (bf16 / fp4,
+// weights from HBM; within 25 % but for the smallest): a tile takes `start` and, per
+// k-tile, from `alone` (an empty GPU) to `full` (all slots taken).
+struct RingCost {
+  int fm, fn;      // MFMA blocks of a wave: tile 32 fm x 32 fn
+  int per_cu;      // workgroups of a CU
+  double start, alone, full;
+};
+constexpr RingCost kRing16[] = {{8, 8, 1, 10.0, 0.95, 1.5}, {4, 4, 2, 4.0, 0.38, 1.12}, {2, 4, 3, 4.0, 0.36, 1.06}};
+constexpr RingCost kRing4[] = {{8, 8, 1, 11.0, 1.2, 1.6}, {4, 4, 2, 6.0, 0.5, 1.12}, {2, 4, 3, 6.0, 0.41, 1.1}};
+
+inline double ring_time(const RingCost& c, double tiles, double k_tiles) {
+  const double t = tiles / (c.per_cu * device_cus());
+  // one workgroup per CU runs in whole rounds; several drift apart
+  const double rounds = t <= 1.0 ? 1.0 : c.per_cu == 1 ? std::ceil(t) : t + 0.3;
+  return rounds * (c.start + k_tiles * (c.alone + (c.full - c.alone) * std::min(1.0, t)));
+}
+
+// Row tiles of BM rows that `rows` rows in `groups` groups are likely to take: each
+// group that has any rows ends in a tile half full.
+inline double likely_row_tiles(double rows, double groups, int bm) {
+  if (groups <= 1) return std::ceil(rows / bm);
+  const double g = std::min(groups, rows);
+  return std::max(g, rows / bm + 0.5 * g);
+}
+
+struct GroupedChoice {
+  int ring;    // index into kRing16 / kRing4, or -1: rows_kernel
+  int mf, ks;  // rows_kernel: row blocks, waves along K
+};
+
+// grouped_gemm and mx_gemm. row_bytes: of A along K; elem: bytes per value of B.
+inline GroupedChoice choose_grouped(const RingCost (&ring)[3], double rows, double groups, double N, double K, double row_bytes,
+                                    double elem, bool kc) {
+  const double g = std::min(groups, rows), weights = g * K * N * elem, nk = std::ceil(row_bytes / 128.0);
+  GroupedChoice best{-1, 1, 8};
+  // Few rows: rows_kernel reads the weights once per 16 mf rows at about 4.5 TB/s
+  // (two row blocks of a K-contiguous B: 3.2), its waves splitting K; the rings
+  // need a tile per CU to read as fast: 8 groups of one row, 4096 x 1536: 20.5 us
+  // against 38.4 (96 tiles); 64 groups of one: 90 and 81.
+  double time = 1e30;
+  if (rows <= 64.0 * g) {
+    best.mf = rows <= 8.0 * g ? 1 : 2;
+    const double again = likely_row_tiles(rows, groups, 16 * best.mf) / g;
+    time = 4.5 + row_bytes / 8192.0 + weights * again / (best.mf == 2 && kc ? 3.2e6 : 4.5e6);
+    // the fewest waves along K that leave two workgroups per CU
+    while (best.ks > 1 && again * g * std::ceil(N * (best.ks / 2) / (kc ? 128.0 : 512.0)) >= 2.0 * device_cus()) best.ks /= 2;
+  }
+  for (int i = 0; i < 3; ++i) {
+    const RingCost& c = ring[i];
+    const double t = std::max(3.0 + weights / 4.6e6,
+                              ring_time(c, likely_row_tiles(rows, groups, 32 * c.fm) * std::ceil(N / (32 * c.fn)), nk));
+    if (t < time * (i == 2 ? 0.97 : 1.0)) {
+      time = t;
+      best.ring = i;
+    }
+  }
+  return best;
+}
+
+// grouped_rank_k: groups x (M x N), k_tiles of the average group.
+inline int choose_rank_k(double groups, double M, double N, double k_tiles) {
+  int best = 0;
+  double time = 1e30;
+  for (int i = 0; i < 3; ++i) {
+    const RingCost& c = kRing16[i];
+    const double t = ring_time(c, groups * std::ceil(M / (32 * c.fm)) * std::ceil(N / (32 * c.fn)), k_tiles + 0.5);
+    if (t < time * (i == 2 ? 0.97 : 1.0)) {
+      time = t;
+      best = i;
+    }
+  }
+  return best;
+}
+
+}  // namespace trnblas

@@ -13,13 +13,11 @@
 //    64 lanes read 256 bytes in a row.
 #include <algorithm>
 
-#include "grouped.hpp"
+#include "grouped_plan.hpp"
+#include "ring.hpp"
+#include "rows.hpp"
 
 namespace trnblas {
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-constexpr int kChunk = 256;  // bytes of scales per 16 rows x 512 values
 
 static const char* kQuantize = "trnblas_hip_mx_quantize";
 static const char* kDequantize = "trnblas_hip_mx_dequantize";
@@ -158,98 +156,49 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(DequantArgs g) {
   }
 }
 
-// acc += (16 rows n) x (16 rows m) over 128 values of K; byte J of each scale
-// dword. Lane l holds column m = l % 16 and rows n = 4 (l / 16) + r.
-template <int J>
-__device__ __forceinline__ void mma_mx(f32x4& acc, const i32x4& n, const i32x4& m, int sn, int sm) {
-  const i32x8 a = {n[0], n[1], n[2], n[3], 0, 0, 0, 0}, b = {m[0], m[1], m[2], m[3], 0, 0, 0, 0};
-  acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, J, sn, J, sm);
-}
-
-struct MxArgs {
-  GroupedArgs g;  // A, B: codes; lda, ldb: bytes per row; sB: bytes per matrix
-  const uint8_t* sa;
-  const uint8_t* sb;
-  int chunks;       // of scales along K, the same for A and B
-  int64_t sb_step;  // bytes of scales per matrix of B
-};
-
-// 64 x 64 tiles, each wave 32 x 32, its fragments straight from memory.
-template <typename O>
-__global__ __launch_bounds__(256) void mx_any_kernel(MxArgs x) {
-  const GroupedArgs& g = x.g;
-  Segment s;
-  if (!ragged_tile<64>(g, blockIdx.x, 8, s)) return;
-  const bool of_group = s.group >= 0 && s.group < g.groups;
-  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m0 = s.row + 32 * (wave & 1), n0 = s.tn * 64 + 32 * (wave >> 1);
-  const int nk = of_group ? (int)((g.lda + 63) / 64) : 0;  // 64-byte k-tiles
-  const uint8_t *pa[2], *pb[2];
-  const uint32_t *qa[2], *qb[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    // rows past the segment or the matrix repeat its last one: not stored
-    const int64_t m = min(m0 + 16 * i + li, s.end - 1), n = min(n0 + 16 * i + li, g.N - 1);
-    pa[i] = static_cast<const uint8_t*>(g.A) + m * g.lda + 16 * lg;
-    pb[i] = static_cast<const uint8_t*>(g.B) + s.group * g.sB + n * g.ldb + 16 * lg;
-    qa[i] = reinterpret_cast<const uint32_t*>(x.sa + (m >> 4) * x.chunks * kChunk + 64 * lg + 4 * (m & 15));
-    qb[i] = reinterpret_cast<const uint32_t*>(x.sb + s.group * x.sb_step + (n >> 4) * x.chunks * kChunk + 64 * lg + 4 * (n & 15));
-  }
-  f32x4 acc[2][2];
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  auto tile = [&](int kt, auto j, const int (&sa)[2], const int (&sb)[2]) __attribute__((always_inline)) {
-    if (kt >= nk) return;
-    i32x4 fa[2], fb[2];
-    const bool in = 64 * kt + 16 * lg < (int)g.lda;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      fa[i] = fb[i] = i32x4{0, 0, 0, 0};
-      if (in) {
-        fa[i] = *reinterpret_cast<const i32x4*>(pa[i] + 64 * kt);
-        fb[i] = *reinterpret_cast<const i32x4*>(pb[i] + 64 * kt);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int a = 0; a < 2; ++a) mma_mx<decltype(j)::value>(acc[a][b], fb[b], fa[a], sb[b], sa[a]);
-  };
-  for (int c = 0; 4 * c < nk; ++c) {
-    int sa[2], sb[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      sa[i] = qa[i][c * (kChunk / 4)];
-      sb[i] = qb[i][c * (kChunk / 4)];
-    }
-    tile(4 * c, std::integral_constant<int, 0>{}, sa, sb);
-    tile(4 * c + 1, std::integral_constant<int, 1>{}, sa, sb);
-    tile(4 * c + 2, std::integral_constant<int, 2>{}, sa, sb);
-    tile(4 * c + 3, std::integral_constant<int, 3>{}, sa, sb);
-  }
-#pragma unroll
-  for (int a = 0; a < 2; ++a) {
-    const int m = m0 + 16 * a + li;
-    if (m < s.end) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-        store_quad<O>(g, static_cast<const O*>(g.C), static_cast<O*>(g.D), m, n0 + 16 * b + 4 * lg, acc[a][b]);
-    }
-  }
-}
-
-template <typename O>
-static int run_mx(MxArgs x, hipStream_t s) {
-  GroupedArgs& g = x.g;
-  g.tiles_n = (g.N + 63) / 64;
-  const int64_t tiles = (g.rows / 64 + std::min<int64_t>(g.groups + 2, g.rows)) * g.tiles_n;
+static int mx_grid(const GroupedArgs& g, int bm, unsigned* grid) {
+  const int64_t tiles = (g.rows / bm + std::min<int64_t>(g.groups + 2, g.rows)) * g.tiles_n;
   TRNBLAS_CHECK_ARG(tiles < ((int64_t)1 << 31) - 8, "%s: too many tiles", kMxGemm);
-  const unsigned grid = (unsigned)((tiles + kNumXcd - 1) / kNumXcd * kNumXcd);
-  hipLaunchKernelGGL(mx_any_kernel<O>, dim3(grid), dim3(256), 0, s, x);
+  *grid = (unsigned)((tiles + kNumXcd - 1) / kNumXcd * kNumXcd);
+  return TRNBLAS_OK;
+}
+
+template <int FM, int FN>
+static int run_ring(GroupedArgs g, const MxScales& x, hipStream_t s) {
+  constexpr int BM = 32 * FM, BN = 32 * FN;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  unsigned grid;
+  if (int rc = mx_grid(g, BM, &grid)) return rc;
+  hipLaunchKernelGGL((ring_kernel<fp4x2, FM, FN, true, false>), dim3(grid), dim3(256), 0, s, g, x);
   return check_launch(kMxGemm);
+}
+
+template <int MF, int NF, int KS>
+static int run_rows(GroupedArgs g, const MxScales& x, hipStream_t s) {
+  constexpr int BN = 128 * NF / KS;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  unsigned grid;
+  if (int rc = mx_grid(g, 16 * MF, &grid)) return rc;
+  hipLaunchKernelGGL((rows_kernel<fp4x2, MF, NF, KS, true>), dim3(grid), dim3(512), 0, s, g, x);
+  return check_launch(kMxGemm);
+}
+
+template <int MF>
+static int run_rows_split(int ks, const GroupedArgs& g, const MxScales& x, hipStream_t s) {
+  return ks == 8   ? run_rows<MF, 1, 8>(g, x, s)
+         : ks == 4 ? run_rows<MF, 1, 4>(g, x, s)
+         : ks == 2 ? run_rows<MF, 1, 2>(g, x, s)
+                   : run_rows<MF, 1, 1>(g, x, s);
+}
+
+static int run_mx(const GroupedArgs& g, const MxScales& x, hipStream_t s) {
+  const GroupedChoice c = choose_grouped(kRing4, g.rows, g.groups, g.N, g.K, g.K, 17.0 / 16.0, true);
+  switch (c.ring) {
+    case 0: return run_ring<8, 8>(g, x, s);
+    case 1: return run_ring<4, 4>(g, x, s);
+    case 2: return run_ring<2, 4>(g, x, s);
+    default: return c.mf == 1 ? run_rows_split<1>(c.ks, g, x, s) : run_rows_split<2>(c.ks, g, x, s);
+  }
 }
 
 static int check_layout(const char* what, int64_t R, int64_t K, int64_t batch) {
@@ -342,29 +291,28 @@ extern "C" int trnblas_hip_mx_gemm(int out_dtype, int64_t groups, int64_t rows, 
   TRNBLAS_CHECK_ARG(ldd >= N && (beta == 0.0 || ldc >= N), "%s: bad leading dimension", kMxGemm);
   if (rows == 0 || N == 0) return TRNBLAS_OK;
   TRNBLAS_CHECK_ARG(D != nullptr && (K == 0 || groups == 0 || (A && A_scales && B && B_scales)), "%s: null operand", kMxGemm);
+  // a panel's codes and a tile's scales within 32-bit offsets
+  TRNBLAS_CHECK_ARG(K < 8 << 20, "%s: K %lld too large", kMxGemm, (long long)K);
   for (const void* p : {A, A_scales, B, B_scales})
     TRNBLAS_CHECK_ARG((uintptr_t)p % 16 == 0, "%s: codes and scales must be 16-byte aligned", kMxGemm);
-  MxArgs x{};
-  GroupedArgs& g = x.g;
+  GroupedArgs g{};
+  MxScales x{};
   g.A = A, g.B = B;
   g.lda = g.ldb = (K + 31) / 32 * 16;
   g.sB = N * g.ldb;
-  x.sa = static_cast<const uint8_t*>(A_scales);
-  x.sb = static_cast<const uint8_t*>(B_scales);
+  x.a = static_cast<const uint8_t*>(A_scales);
+  x.b = static_cast<const uint8_t*>(B_scales);
   x.chunks = (int)((K + 511) / 512);
-  x.sb_step = (N + 15) / 16 * x.chunks * kChunk;
+  x.b_step = (N + 15) / 16 * x.chunks * kChunk;
   g.offsets = offsets;
   g.offsets64 = offsets64 != 0;
-  g.groups = (int)groups, g.rows = (int)rows, g.N = (int)N, g.K = (int)K;
+  g.groups = (int)groups, g.rows = (int)rows, g.N = (int)N, g.K = (int)g.lda;  // bytes of codes along K
   g.alpha = (float)alpha, g.beta = (float)beta;
   g.C = beta != 0.0 ? C : nullptr, g.ldc = ldc;
   g.D = D, g.ldd = ldd;
-  const int eo = out_dtype == TRNBLAS_F32 ? 4 : 2;
+  g.out32 = out_dtype == TRNBLAS_F32, g.out_f16 = out_dtype == TRNBLAS_F16;
+  const int eo = g.out32 ? 4 : 2;
   g.vec4 = (uintptr_t)D % (4 * eo) == 0 && ldd % 4 == 0 && (g.C == nullptr || ((uintptr_t)C % (4 * eo) == 0 && ldc % 4 == 0));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (out_dtype) {
-    case TRNBLAS_F32: return run_mx<float>(x, s);
-    case TRNBLAS_BF16: return run_mx<__bf16>(x, s);
-    default: return run_mx<_Float16>(x, s);
-  }
+  return run_mx(g, x, s);
 }
