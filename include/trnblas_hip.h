@@ -629,6 +629,19 @@ int trnblas_hip_mx_gemm(int out_dtype, int64_t groups, int64_t rows, int64_t N, 
                         const void* B_scales, const void* offsets, int offsets64, double beta,
                         const void* C, int64_t ldc, void* D, int64_t ldd, void* stream);
 
+/*
+ * mx_gemm with an A that is quantised on the way (as mx_quantize does it): A is
+ * rows x K values of `dtype`, element (r, k) at r * sr + k * sk. workspace: as
+ * many bytes as mx_gemm_from_workspace says, 16-byte aligned, not shared by
+ * calls that can overlap; few rows of a K-contiguous A do not use it.
+ */
+size_t trnblas_hip_mx_gemm_from_workspace(int64_t rows, int64_t K);
+int trnblas_hip_mx_gemm_from(int dtype, int out_dtype, int64_t groups, int64_t rows, int64_t N,
+                             int64_t K, double alpha, const void* A, int64_t sr, int64_t sk,
+                             const void* B, const void* B_scales, const void* offsets,
+                             int offsets64, double beta, const void* C, int64_t ldc, void* D,
+                             int64_t ldd, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

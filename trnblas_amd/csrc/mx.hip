@@ -34,27 +34,6 @@ struct QuantArgs {
   int vec;  // 16-byte loads (K-contiguous: every row starts on 16 bytes)
 };
 
-// Scale byte of a block whose largest magnitude has these bits (as fp32):
-// floor(log2) - 2 so that it lands in [4, 8), not below 2^-127; infinities and
-// NaN give 255.
-__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
-  const uint32_t e = top >> 23;
-  return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
-}
-// 2^-(byte - 127)
-__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __builtin_bit_cast(float, (254u - byte) << 23); }
-
-// Eight values times inv (exact but for results far below 0.25) to eight
-// codes: the conversion rounds to nearest even and saturates at 6.
-__device__ __forceinline__ uint32_t codes8(const float (&v)[8], float inv) {
-  uint32_t c = 0;
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0] * inv, v[1] * inv, 1.0f, 0);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2] * inv, v[3] * inv, 1.0f, 1);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4] * inv, v[5] * inv, 1.0f, 2);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6] * inv, v[7] * inv, 1.0f, 3);
-  return c;
-}
-
 // Rows by K, 16 rows x 512 values per workgroup of 256 threads: a wave takes
 // four rows, a lane eight values of each, four lanes a block.
 template <typename T>
@@ -105,6 +84,49 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(QuantArgs g) {
     uint8_t* scales = g.scales + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kChunk;
     reinterpret_cast<uint32_t*>(scales)[tid] = sc[tid];
   }
+}
+
+// K by rows (a row's values are sk apart, rows next to each other): 64 rows x 128
+// values per workgroup, a wave one block of 32 of each row, a lane one row, so
+// that its loads are 64 neighbouring values; the codes go out through LDS, 64 bytes
+// per row. 8192 x 8192 bf16: see the row-contiguous kernel, which reads as fast.
+template <typename T>
+__global__ __launch_bounds__(256) void mx_quantize_columns_kernel(QuantArgs g) {
+  __shared__ __attribute__((aligned(16))) char sc[64 * 80];  // 16 bytes between rows
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tiles_k = g.chunks * 4;
+  const int tr = blockIdx.x / tiles_k, tk = blockIdx.x - tr * tiles_k;
+  const int r = tr * 64 + lane, b = tk * 4 + wave, k = 32 * b;
+  const int left = r < g.R ? g.K - k : 0;
+  const T* p = static_cast<const T*>(g.X) + blockIdx.y * g.sx + r * g.sr + k * g.sk;
+  float v[4][8];
+  if (left >= 32) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e / 8][e % 8] = (float)p[e * g.sk];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e / 8][e % 8] = e < left ? (float)p[e * g.sk] : 0.0f;
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) top = max(top, __builtin_bit_cast(uint32_t, v[e / 8][e % 8]) & 0x7fffffffu);
+  const uint32_t byte = scale_byte(top);
+  i32x4 c = {0, 0, 0, 0};
+  if (byte != 255) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c[q] = (int)codes8(v[q], inverse_scale(byte));
+  }
+  *reinterpret_cast<i32x4*>(sc + 80 * lane + 16 * wave) = c;
+  const int row_blocks = (g.R + 15) / 16;
+  if (r < 16 * row_blocks) {
+    uint8_t* scales = g.scales + (((int64_t)blockIdx.y * row_blocks + (r >> 4)) * g.chunks + (b >> 4)) * kChunk;
+    scales[64 * (b & 3) + 4 * (r & 15) + ((b >> 2) & 3)] = (uint8_t)byte;
+  }
+  __syncthreads();
+  const int row = tr * 64 + threadIdx.x / 4, off = 64 * tk + 16 * (threadIdx.x & 3);
+  if (row < g.R && off < g.row_bytes)
+    *reinterpret_cast<i32x4*>(g.codes + ((int64_t)blockIdx.y * g.R + row) * g.row_bytes + off) =
+        *reinterpret_cast<const i32x4*>(sc + 80 * (threadIdx.x / 4) + 16 * (threadIdx.x & 3));
 }
 
 struct DequantArgs {
@@ -173,26 +195,30 @@ static int run_ring(GroupedArgs g, const MxScales& x, hipStream_t s) {
   return check_launch(kMxGemm);
 }
 
-template <int MF, int NF, int KS>
+template <int MF, int KS, typename X>
 static int run_rows(GroupedArgs g, const MxScales& x, hipStream_t s) {
-  constexpr int BN = 128 * NF / KS;
+  constexpr int BN = 128 / KS;
   g.tiles_n = (g.N + BN - 1) / BN;
   unsigned grid;
   if (int rc = mx_grid(g, 16 * MF, &grid)) return rc;
-  hipLaunchKernelGGL((rows_kernel<fp4x2, MF, NF, KS, true>), dim3(grid), dim3(512), 0, s, g, x);
+  hipLaunchKernelGGL((rows_kernel<fp4x2, MF, 1, KS, true, X>), dim3(grid), dim3(512), 0, s, g, x);
   return check_launch(kMxGemm);
 }
 
-template <int MF>
+template <int MF, typename X = void>
 static int run_rows_split(int ks, const GroupedArgs& g, const MxScales& x, hipStream_t s) {
-  return ks == 8   ? run_rows<MF, 1, 8>(g, x, s)
-         : ks == 4 ? run_rows<MF, 1, 4>(g, x, s)
-         : ks == 2 ? run_rows<MF, 1, 2>(g, x, s)
-                   : run_rows<MF, 1, 1>(g, x, s);
+  return ks == 8   ? run_rows<MF, 8, X>(g, x, s)
+         : ks == 4 ? run_rows<MF, 4, X>(g, x, s)
+         : ks == 2 ? run_rows<MF, 2, X>(g, x, s)
+                   : run_rows<MF, 1, X>(g, x, s);
+}
+
+static GroupedChoice choose_mx(const GroupedArgs& g) {
+  return choose_grouped(kRing4, g.rows, g.groups, g.N, g.K, g.K, 17.0 / 16.0, true);
 }
 
 static int run_mx(const GroupedArgs& g, const MxScales& x, hipStream_t s) {
-  const GroupedChoice c = choose_grouped(kRing4, g.rows, g.groups, g.N, g.K, g.K, 17.0 / 16.0, true);
+  const GroupedChoice c = choose_mx(g);
   switch (c.ring) {
     case 0: return run_ring<8, 8>(g, x, s);
     case 1: return run_ring<4, 4>(g, x, s);
@@ -240,6 +266,17 @@ extern "C" int trnblas_hip_mx_quantize(int dtype, int64_t R, int64_t K, const vo
   g.scales = static_cast<uint8_t*>(scales);
   g.vec = sk == 1 && (uintptr_t)X % 16 == 0 && sr * es % 16 == 0 && sx * es % 16 == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (sr == 1 && sk > 1 && R >= 16) {
+    const int64_t tiles = (R + 63) / 64 * 4 * g.chunks;
+    TRNBLAS_CHECK_ARG(tiles < (int64_t)1 << 31, "%s: matrix too large (%lld x %lld)", kQuantize, (long long)R, (long long)K);
+    const dim3 by_columns((unsigned)tiles, (unsigned)batch);
+    switch (dtype) {
+      case TRNBLAS_F32: hipLaunchKernelGGL(mx_quantize_columns_kernel<float>, by_columns, dim3(256), 0, s, g); break;
+      case TRNBLAS_BF16: hipLaunchKernelGGL(mx_quantize_columns_kernel<__bf16>, by_columns, dim3(256), 0, s, g); break;
+      default: hipLaunchKernelGGL(mx_quantize_columns_kernel<_Float16>, by_columns, dim3(256), 0, s, g); break;
+    }
+    return check_launch(kQuantize);
+  }
   switch (dtype) {
     case TRNBLAS_F32: hipLaunchKernelGGL(mx_quantize_kernel<float>, grid, dim3(256), 0, s, g); break;
     case TRNBLAS_BF16: hipLaunchKernelGGL(mx_quantize_kernel<__bf16>, grid, dim3(256), 0, s, g); break;
@@ -276,13 +313,14 @@ extern "C" int trnblas_hip_mx_dequantize(int dtype, int64_t R, int64_t K, const 
   return check_launch(kDequantize);
 }
 
-extern "C" int trnblas_hip_mx_gemm(int out_dtype, int64_t groups, int64_t rows, int64_t N, int64_t K, double alpha,
-                                   const void* A, const void* A_scales, const void* B, const void* B_scales,
-                                   const void* offsets, int offsets64, double beta, const void* C, int64_t ldc, void* D,
-                                   int64_t ldd, void* stream) {
+// The checks and arguments that both products share; K in values.
+static int mx_args(GroupedArgs& g, MxScales& x, int out_dtype, int64_t groups, int64_t rows, int64_t N, int64_t K, double alpha,
+                   const void* B, const void* B_scales, const void* offsets, int offsets64, double beta, const void* C, int64_t ldc,
+                   void* D, int64_t ldd) {
   TRNBLAS_CHECK_ARG(out_dtype == TRNBLAS_F32 || out_dtype == TRNBLAS_BF16 || out_dtype == TRNBLAS_F16, "%s: bad dtype %d", kMxGemm, out_dtype);
+  // K: a panel's codes and a tile's scales lie within 32-bit offsets
   TRNBLAS_CHECK_ARG(groups >= 0 && groups < (1 << 24) && rows >= 0 && rows < INT32_MAX - 1024 && N >= 0 &&
-                        N < INT32_MAX - 1024 && K >= 0 && K < INT32_MAX - 1024,
+                        N < INT32_MAX - 1024 && K >= 0 && K < 8 << 20,
                     "%s: bad sizes (groups %lld, rows %lld, N %lld, K %lld)", kMxGemm, (long long)groups, (long long)rows,
                     (long long)N, (long long)K);
   TRNBLAS_CHECK_ARG(offsets != nullptr ? (uintptr_t)offsets % (offsets64 ? 8 : 4) == 0 : groups == 1,
@@ -290,17 +328,11 @@ extern "C" int trnblas_hip_mx_gemm(int out_dtype, int64_t groups, int64_t rows, 
   TRNBLAS_CHECK_ARG(beta == 0.0 || C != nullptr, "%s: beta != 0 without C", kMxGemm);
   TRNBLAS_CHECK_ARG(ldd >= N && (beta == 0.0 || ldc >= N), "%s: bad leading dimension", kMxGemm);
   if (rows == 0 || N == 0) return TRNBLAS_OK;
-  TRNBLAS_CHECK_ARG(D != nullptr && (K == 0 || groups == 0 || (A && A_scales && B && B_scales)), "%s: null operand", kMxGemm);
-  // a panel's codes and a tile's scales within 32-bit offsets
-  TRNBLAS_CHECK_ARG(K < 8 << 20, "%s: K %lld too large", kMxGemm, (long long)K);
-  for (const void* p : {A, A_scales, B, B_scales})
-    TRNBLAS_CHECK_ARG((uintptr_t)p % 16 == 0, "%s: codes and scales must be 16-byte aligned", kMxGemm);
-  GroupedArgs g{};
-  MxScales x{};
-  g.A = A, g.B = B;
+  TRNBLAS_CHECK_ARG(D != nullptr && (K == 0 || groups == 0 || (B && B_scales)), "%s: null operand", kMxGemm);
+  TRNBLAS_CHECK_ARG((uintptr_t)B % 16 == 0 && (uintptr_t)B_scales % 16 == 0, "%s: codes and scales must be 16-byte aligned", kMxGemm);
+  g.B = B;
   g.lda = g.ldb = (K + 31) / 32 * 16;
   g.sB = N * g.ldb;
-  x.a = static_cast<const uint8_t*>(A_scales);
   x.b = static_cast<const uint8_t*>(B_scales);
   x.chunks = (int)((K + 511) / 512);
   x.b_step = (N + 15) / 16 * x.chunks * kChunk;
@@ -313,6 +345,66 @@ extern "C" int trnblas_hip_mx_gemm(int out_dtype, int64_t groups, int64_t rows, 
   g.out32 = out_dtype == TRNBLAS_F32, g.out_f16 = out_dtype == TRNBLAS_F16;
   const int eo = g.out32 ? 4 : 2;
   g.vec4 = (uintptr_t)D % (4 * eo) == 0 && ldd % 4 == 0 && (g.C == nullptr || ((uintptr_t)C % (4 * eo) == 0 && ldc % 4 == 0));
+  return TRNBLAS_OK;
+}
+
+static size_t codes_bytes(int64_t rows, int64_t K) { return (size_t)(rows * ((K + 31) / 32 * 16)); }
+static size_t scales_bytes(int64_t rows, int64_t K) { return (size_t)((rows + 15) / 16 * ((K + 511) / 512) * kChunk); }
+
+extern "C" int trnblas_hip_mx_gemm(int out_dtype, int64_t groups, int64_t rows, int64_t N, int64_t K, double alpha,
+                                   const void* A, const void* A_scales, const void* B, const void* B_scales,
+                                   const void* offsets, int offsets64, double beta, const void* C, int64_t ldc, void* D,
+                                   int64_t ldd, void* stream) {
+  GroupedArgs g{};
+  MxScales x{};
+  if (int rc = mx_args(g, x, out_dtype, groups, rows, N, K, alpha, B, B_scales, offsets, offsets64, beta, C, ldc, D, ldd)) return rc;
+  if (rows == 0 || N == 0) return TRNBLAS_OK;
+  TRNBLAS_CHECK_ARG(K == 0 || groups == 0 || (A && A_scales), "%s: null operand", kMxGemm);
+  TRNBLAS_CHECK_ARG((uintptr_t)A % 16 == 0 && (uintptr_t)A_scales % 16 == 0, "%s: codes and scales must be 16-byte aligned", kMxGemm);
+  g.A = A;
+  x.a = static_cast<const uint8_t*>(A_scales);
+  return run_mx(g, x, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t trnblas_hip_mx_gemm_from_workspace(int64_t rows, int64_t K) {
+  if (rows <= 0 || K <= 0) return 0;
+  return (codes_bytes(rows, K) + 255) / 256 * 256 + scales_bytes(rows, K);
+}
+
+extern "C" int trnblas_hip_mx_gemm_from(int dtype, int out_dtype, int64_t groups, int64_t rows, int64_t N, int64_t K, double alpha,
+                                        const void* A, int64_t sr, int64_t sk, const void* B, const void* B_scales,
+                                        const void* offsets, int offsets64, double beta, const void* C, int64_t ldc, void* D,
+                                        int64_t ldd, void* workspace, size_t workspace_bytes, void* stream) {
+  GroupedArgs g{};
+  MxScales x{};
+  TRNBLAS_CHECK_ARG(dtype == TRNBLAS_F32 || dtype == TRNBLAS_BF16 || dtype == TRNBLAS_F16, "%s: bad dtype %d", kMxGemm, dtype);
+  TRNBLAS_CHECK_ARG(sr >= 0 && sk >= 0, "%s: negative stride", kMxGemm);
+  if (int rc = mx_args(g, x, out_dtype, groups, rows, N, K, alpha, B, B_scales, offsets, offsets64, beta, C, ldc, D, ldd)) return rc;
+  if (rows == 0 || N == 0) return TRNBLAS_OK;
+  TRNBLAS_CHECK_ARG(K == 0 || groups == 0 || A, "%s: null operand", kMxGemm);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  const GroupedChoice c = choose_mx(g);
+  if (c.ring < 0 && c.mf == 1 && sk == 1 && std::min<int64_t>(rows, 16) * K <= kInPlace) {
+    const int es = dtype == TRNBLAS_F32 ? 4 : 2;
+    x.x = A, x.ldx = sr, x.kx = (int)K;
+    x.vec = (uintptr_t)A % 16 == 0 && (sr * es % 16 == 0 || rows == 1);
+    switch (dtype) {
+      case TRNBLAS_F32: return run_rows_split<1, float>(c.ks, g, x, s);
+      case TRNBLAS_BF16: return run_rows_split<1, __bf16>(c.ks, g, x, s);
+      default: return run_rows_split<1, _Float16>(c.ks, g, x, s);
+    }
+  }
+  if (K > 0 && groups > 0) {
+    const size_t need = trnblas_hip_mx_gemm_from_workspace(rows, K);
+    if (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0) {
+      set_error("%s: workspace of %zu bytes, 16-byte aligned, needed (got %zu)", kMxGemm, need, workspace_bytes);
+      return TRNBLAS_E_WORKSPACE;
+    }
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    uint8_t* scales = codes + (codes_bytes(rows, K) + 255) / 256 * 256;
+    if (int rc = trnblas_hip_mx_quantize(dtype, rows, K, A, sr, sk, 0, codes, scales, 1, stream)) return rc;
+    g.A = codes;
+    x.a = scales;
+  }
   return run_mx(g, x, s);
 }

@@ -30,6 +30,10 @@ constexpr int kChunk = 256;  // bytes of scales per 16 rows x 512 values (mx.hip
 struct MxScales {
   const uint8_t* a;
   const uint8_t* b;
+  const void* x;    // rows_kernel: A before quantisation, kx values per row,
+  int64_t ldx;      // leading dimension ldx
+  int kx;
+  int vec;          // its rows start on 16 bytes
   int chunks;       // along K, the same for A and B
   int64_t b_step;   // bytes per matrix of B
 };

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "gemm.hpp"
+#include "mx_block.hpp"
 #include "ring.hpp"
 
 namespace trnblas {
@@ -87,6 +88,52 @@ struct ColumnStep {
   }
 };
 
+constexpr int kInPlace = 32768;
+
+// Quantises nr rows of x.x from row `row` on into LDS, one block of 32 values per
+// thread at a time: rows of g.lda bytes of codes, 16 bytes apart, and scale
+// dwords (row, chunk of 512 values, quarter q: the blocks 4 h + q, h = 0 .. 3).
+template <typename X>
+__device__ __forceinline__ void quantize_rows(const GroupedArgs& g, const MxScales& x, int row, int nr, char* codes, char* scales) {
+  const int blocks = x.chunks * 16, have = (int)g.lda / 16;
+  for (int i = threadIdx.x; i < nr * blocks; i += 512) {
+    const int r = i / blocks, b = i - r * blocks;
+    uint32_t byte = 0;
+    if (b < have) {
+      const X* p = static_cast<const X*>(x.x) + (row + r) * x.ldx + 32 * b;
+      const int left = x.kx - 32 * b;
+      float v[4][8];
+      if (x.vec && left >= 32) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          union {
+            i32x4 w[sizeof(X) / 2];
+            X e[8];
+          } u;
+#pragma unroll
+          for (int h = 0; h < (int)sizeof(X) / 2; ++h) u.w[h] = reinterpret_cast<const i32x4*>(p + 8 * q)[h];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[q][e] = (float)u.e[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e / 8][e % 8] = e < left ? (float)p[e] : 0.0f;
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) top = max(top, __builtin_bit_cast(uint32_t, v[e / 8][e % 8]) & 0x7fffffffu);
+      byte = scale_byte(top);
+      i32x4 c = {0, 0, 0, 0};
+      if (byte != 255) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) c[q] = (int)codes8(v[q], inverse_scale(byte));
+      }
+      *reinterpret_cast<i32x4*>(codes + r * ((int)g.lda + 16) + 16 * b) = c;
+    }
+    scales[r * x.chunks * 16 + (b >> 4) * 16 + 4 * (b & 3) + ((b >> 2) & 3)] = (char)byte;
+  }
+}
+
 // Tiles of 16 MF rows by BN columns. KS of the eight waves split K between them
 // (chunks of CH bytes per row, chunk c to wave c % KS) and add their sums through
 // LDS in wave order; 8 / KS such sets take 16 NF columns each. What bounds it is
@@ -96,13 +143,18 @@ struct ColumnStep {
 // K-contiguous B: one row of 64 bytes per lane quad and step. Column-contiguous B: NF
 // = 4, whole 128-byte lines of 16-bit values. Rows of A past the segment repeat
 // its last one (not stored). fp32: the sums restart every 512 values of k per wave.
-template <typename T, int MF, int NF, int KS, bool BKC>
+//
+// X (4-bit floats only): A comes as values of that type, at most kInPlace in the
+// tile's rows; the workgroup quantises them into LDS behind its first loads of B,
+// which saves a launch of its own (one row of 8192 by 8192^2: 5 us).
+template <typename T, int MF, int NF, int KS, bool BKC, typename X = void>
 __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
   constexpr bool MX = std::is_same_v<T, fp4x2>, FOLD = std::is_same_v<T, float>;
   constexpr int ES = sizeof(T), EV = 16 / ES, BM = 16 * MF, BW = 16 * NF, BN = 8 / KS * BW;
   constexpr int STEPS = rows_steps<T>, CH = 64 * STEPS, CK = CH / ES;  // a chunk: bytes, values of k
   constexpr int U = rows_ahead<T>(MF, NF);
   static_assert(BKC || NF == 4, "four columns of a lane");
+  constexpr bool QUANT = !std::is_void_v<X>;
   __shared__ __attribute__((aligned(16))) f32x4 part[8][BM * BW / 4];
   Segment s;
   if (!ragged_tile<BM>(g, blockIdx.x, 8, s)) return;
@@ -112,14 +164,23 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
   const int kw = wave % KS, set = wave / KS;
   const int n0 = s.tn * BN + set * BW, K = of_group && n0 < g.N ? g.K : 0;
   const int grp = of_group ? s.group : 0;
+  // quantised rows: codes, 16 bytes between rows (LDS banks); then scale dwords by row, chunk and quarter
+  __shared__ __attribute__((aligned(16))) char qlds[QUANT ? kInPlace / 2 + kInPlace / 32 + 64 * BM : 16];
+  [[maybe_unused]] const int nr = min(s.end - s.row, BM);
   const char* pa[MF];
   const char* pb[BKC ? NF : 1];
   [[maybe_unused]] const uint8_t *qa[MF], *qb[NF];
 #pragma unroll
   for (int a = 0; a < MF; ++a) {
-    const int64_t m = min(s.row + 16 * a + li, s.end - 1);
-    pa[a] = static_cast<const char*>(g.A) + m * g.lda * ES + 16 * lg;
-    if constexpr (MX) qa[a] = x.a + (m >> 4) * x.chunks * kChunk + 64 * lg + 4 * (m & 15);
+    if constexpr (QUANT) {
+      const int r = min(16 * a + li, nr - 1);
+      pa[a] = qlds + r * ((int)g.lda + 16) + 16 * lg;
+      qa[a] = reinterpret_cast<const uint8_t*>(qlds) + nr * ((int)g.lda + 16) + r * x.chunks * 16 + 4 * lg;
+    } else {
+      const int64_t m = min(s.row + 16 * a + li, s.end - 1);
+      pa[a] = static_cast<const char*>(g.A) + m * g.lda * ES + 16 * lg;
+      if constexpr (MX) qa[a] = x.a + (m >> 4) * x.chunks * kChunk + 64 * lg + 4 * (m & 15);
+    }
   }
   if constexpr (BKC) {
 #pragma unroll
@@ -147,11 +208,17 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
       acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if constexpr (FOLD) sum[a][b] = acc[a][b];
     }
-  auto load = [&](Chunk& v, int c) __attribute__((always_inline)) {
+  auto load_a = [&](Chunk& v, int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < MF; ++a) {
+#pragma unroll
+      for (int h = 0; h < STEPS; ++h) v.a[a][h] = load16<T>(pa[a] + (int64_t)c * CH + 64 * h);
+      if constexpr (MX) v.sa[a] = *reinterpret_cast<const int*>(qa[a] + (int64_t)c * (QUANT ? 16 : kChunk));
+    }
+  };
+  auto load_b = [&](Chunk& v, int c) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < STEPS; ++h) {
-#pragma unroll
-      for (int a = 0; a < MF; ++a) v.a[a][h] = load16<T>(pa[a] + (int64_t)c * CH + 64 * h);
       if constexpr (BKC) {
 #pragma unroll
         for (int b = 0; b < NF; ++b) v.b[b][h] = load16<T>(pb[b] + (int64_t)c * CH + 64 * h);
@@ -162,6 +229,10 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
         else
           v.c[h].load_any(p, g.ldb, EV, g.N - n0 - 4 * li);
       }
+    }
+    if constexpr (MX) {
+#pragma unroll
+      for (int b = 0; b < NF; ++b) v.sb[b] = *reinterpret_cast<const int*>(qb[b] + (int64_t)c * kChunk);
     }
   };
   // the last, partial chunk
@@ -178,11 +249,9 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
         v.c[h].load_any(pb[0] + (int64_t)(STEPS * c + h) * kstep, g.ldb, left, g.N - n0 - 4 * li);
       }
     }
-  };
-  auto scales = [&](Chunk& v, int c) __attribute__((always_inline)) {
     if constexpr (MX) {
 #pragma unroll
-      for (int a = 0; a < MF; ++a) v.sa[a] = *reinterpret_cast<const int*>(qa[a] + (int64_t)c * kChunk);
+      for (int a = 0; a < MF; ++a) v.sa[a] = *reinterpret_cast<const int*>(qa[a] + (int64_t)c * (QUANT ? 16 : kChunk));
 #pragma unroll
       for (int b = 0; b < NF; ++b) v.sb[b] = *reinterpret_cast<const int*>(qb[b] + (int64_t)c * kChunk);
     }
@@ -212,16 +281,20 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
   };
   const int nc = K / CK;
   int chain = 0;
+  auto batch = [&](int c, auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c + KS * u < nc) f(w[u], c + KS * u);
+  };
+  if constexpr (QUANT) {
+    batch(kw, load_b);
+    quantize_rows<X>(g, x, s.row, of_group ? nr : 0, qlds, qlds + nr * ((int)g.lda + 16));
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
   for (int c = kw; c < nc; c += KS * U) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c + KS * u < nc) {
-        load(w[u], c + KS * u);
-        scales(w[u], c + KS * u);
-      }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c + KS * u < nc) multiply(w[u]);
+    if (!QUANT || c != kw) batch(c, load_b);
+    batch(c, load_a);
+    batch(c, [&](const Chunk& v, int) __attribute__((always_inline)) { multiply(v); });
     if constexpr (FOLD) {
       if ((chain += U) >= 512 / CK) {
         chain = 0;
@@ -237,7 +310,6 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
   }
   if (kw == nc % KS && nc * CK < K) {
     load_last(w[0], nc);
-    scales(w[0], nc);
     multiply(w[0]);
   }
   // operand j of a column-contiguous B holds columns 4 li + j, so its register r is column 4 (4 lg + r) + j

@@ -26,6 +26,33 @@ from .hip import dispatch as _d
 __all__ = ["grouped_gemm", "grouped_rank_k"]
 
 
+_kernels = None
+
+
+def _gk():
+    global _kernels
+    if _kernels is None:
+        from .hip import grouped_kernels
+
+        _kernels = grouped_kernels
+    return _kernels
+
+
+def _fast_call(A, B, offsets) -> bool:
+    """Tensors on the GPU, no gradient, and the kernels serve: the call may take the short way."""
+    return (
+        type(A) in _PLAIN
+        and type(B) in _PLAIN
+        and type(offsets) is torch.Tensor
+        and A.is_cuda
+        and not ((A.requires_grad or B.requires_grad) and torch.is_grad_enabled())
+        and _d._use_hip()
+    )
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
 def _check_offsets(what: str, offsets, like: torch.Tensor, groups: int | None = None) -> int:
     if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 1:
         raise ValueError(f"{what}: offsets must be a 1-D tensor of groups + 1 row numbers")
@@ -130,6 +157,13 @@ def grouped_gemm(
     Rows of no group come out as beta * C[r]. A C that broadcasts to (R, N) is
     taken as in `gemm`. One launch on the GPU, whatever the group sizes.
     """
+    if beta == 0.0 and _fast_call(A, B, offsets) and type(transB) is bool:
+        try:
+            D = _gk().grouped_gemm_fast(alpha, A, B, offsets, transB, dtype)
+            if D is not None:
+                return D
+        except _d.HipKernelError as exc:
+            _d._kernel_failed(exc)
     _check_operands("grouped_gemm", A, B, (2, 3))
     b = B.mT if trans_flag(transB, "transB") else B
     _check_offsets("grouped_gemm", offsets, A, b.shape[0])
@@ -158,6 +192,13 @@ def grouped_rank_k(
     (with beta = 1 the gradient of earlier calls is added to in fp32). A group
     without rows gives beta * C[g].
     """
+    if beta == 0.0 and _fast_call(A, B, offsets):
+        try:
+            D = _gk().grouped_rank_k_fast(alpha, A, B, offsets, dtype)
+            if D is not None:
+                return D
+        except _d.HipKernelError as exc:
+            _d._kernel_failed(exc)
     _check_operands("grouped_rank_k", A, B, (2, 2))
     groups = _check_offsets("grouped_rank_k", offsets, A)
     if A.shape[0] != B.shape[0]:

@@ -175,6 +175,12 @@ SIGNATURES = {
         [_c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_ptr, _c_ptr, _c_ptr, _c_ptr]
         + [_c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr],
     ),
+    "trnblas_hip_mx_gemm_from_workspace": (_c_size, [_c_i64, _c_i64]),
+    "trnblas_hip_mx_gemm_from": (
+        _c_int,
+        [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_ptr, _c_i64, _c_i64, _c_ptr]
+        + [_c_ptr, _c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_size, _c_ptr],
+    ),
     "trnblas_hip_dgemm": (
         _c_int,
         [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_dbl]

@@ -10,6 +10,7 @@ import torch
 
 from . import _lib
 from ._lib import ptr, stream_of
+from . import kernels as _kernels
 from .kernels import _batched_layout, _probed_call, _require_device
 
 
@@ -114,14 +115,45 @@ def mx_quantize(X: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int, dtype: torch.dtype) -> torch.Tensor:
-    dev = _require_device(codes, scales)
     *lead, R, _ = codes.shape
-    D = torch.empty((*lead, R, K), dtype=dtype, device=dev)
+    D = codes.new_empty((*lead, R, K), dtype=dtype)
     _probed_call(
         "mx_dequantize", "trnblas_hip_mx_dequantize", _lib.DTYPE_CODES[dtype], R, K, ptr(codes), ptr(scales), ptr(D),
-        max(K, 1), R * K, lead[0] if lead else 1, stream_of(dev),
+        max(K, 1), R * K, lead[0] if lead else 1, stream_of(codes.device),
     )  # fmt: skip
     return D
+
+
+def mx_gemm_from(
+    A: torch.Tensor,
+    b: tuple[torch.Tensor, torch.Tensor],
+    out_dtype: torch.dtype,
+    offsets: torch.Tensor | None = None,
+    alpha: float = 1.0,
+    beta: float = 0.0,
+    C: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """`mx_gemm` of a float A (R, K), quantised on the way (in the same call)."""
+    dev = _require_device(A, *b, *(() if C is None else (C,)), *(() if offsets is None else (offsets,)))
+    if any(s < 0 for s in A.stride()):
+        A = A.contiguous()
+    R, K = A.shape
+    N = b[0].shape[-2]
+    o, o64 = (None, 0) if offsets is None else offsets_of(offsets)
+    D, c = _output_like(C, beta, (R, N), out_dtype, dev)
+    ws = torch.empty(_from_workspace(R, K), dtype=torch.uint8, device=dev)
+    _probed_call(
+        "mx_gemm", "trnblas_hip_mx_gemm_from", _lib.DTYPE_CODES[A.dtype], _lib.DTYPE_CODES[out_dtype],
+        1 if offsets is None else b[0].shape[0], R, N, K, float(alpha), ptr(A), A.stride(0), A.stride(1), ptr(b[0]), ptr(b[1]),
+        ptr(o), o64, float(beta) if c is not None else 0.0, ptr(c), max(c.stride(0), N) if c is not None else N, ptr(D),
+        max(N, 1), ptr(ws), ws.numel(), stream_of(dev),
+    )  # fmt: skip
+    return D
+
+
+def _from_workspace(R: int, K: int) -> int:
+    """trnblas_hip_mx_gemm_from_workspace (the same formula; a library call costs more)."""
+    return -(-R * -(-K // 32) * 16 // 256) * 256 + -(-R // 16) * -(-K // 512) * 256
 
 
 def mx_gemm(
@@ -146,3 +178,131 @@ def mx_gemm(
         ptr(c), max(c.stride(0), N) if c is not None else N, ptr(D), max(N, 1), stream_of(dev),
     )  # fmt: skip
     return D
+
+
+# ── the common calls without the general path's checks, one by one ────────────
+#
+# A call with few rows takes as long on the host as on the GPU (the general path
+# 12 us, these 8). Each returns None where anything is out of the ordinary: the
+# general path then reports it or deals with it.
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_fns: dict = {}
+_INTS = (torch.int32, torch.int64)
+
+
+def _fn(name: str):
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(_lib.load(), name)
+    return f
+
+
+def _checked(name: str, rc: int) -> None:
+    if rc < 0:
+        msg = _lib.load().trnblas_hip_last_error()
+        raise _lib.HipKernelError(name, rc, msg.decode() if msg else "")
+
+
+def grouped_gemm_fast(alpha, A, B, offsets, transB, out_dtype):
+    code = _lib.DTYPE_CODES.get(A.dtype)
+    if code is None or B.dtype is not A.dtype or _kernels._launch_probe is not None or A.dim() != 2 or B.dim() != 3:
+        return None
+    R, K = A.shape
+    lda, s1 = A.stride()
+    G, b0, b1 = B.shape
+    sb, t0, t1 = B.stride()
+    k, N = (b1, b0) if transB else (b0, b1)
+    dev = A.get_device()
+    if (
+        k != K or s1 != 1 or lda < K or t1 != 1 or t0 < b1 or sb < 0 or N == 0 or dev < 0
+        or B.get_device() != dev or offsets.get_device() != dev or offsets.dtype not in _INTS
+        or offsets.shape != (G + 1,) or offsets.stride() != (1,)
+    ):  # fmt: skip
+        return None
+    if out_dtype is not None and out_dtype is not A.dtype and out_dtype is not torch.float32:
+        return None
+    D = A.new_empty((R, N), dtype=out_dtype)
+    rc = _fn("trnblas_hip_grouped_gemm")(
+        code, D.dtype is torch.float32, transB, G, R, N, K, alpha, A.data_ptr(), lda, B.data_ptr(), t0, sb,
+        offsets.data_ptr(), offsets.dtype is torch.int64, 0.0, None, N, D.data_ptr(), N, _raw_stream(dev),
+    )  # fmt: skip
+    _checked("trnblas_hip_grouped_gemm", rc)
+    return D
+
+
+def mx_gemm_fast(alpha, A, b, offsets, out_dtype):
+    """b: (codes, scales) of the quantised operand."""
+    code = _lib.DTYPE_CODES.get(A.dtype)
+    out = code if out_dtype is None else _lib.DTYPE_CODES.get(out_dtype)
+    if code is None or out is None or _kernels._launch_probe is not None or A.dim() != 2:
+        return None
+    codes, scales = b
+    R, K = A.shape
+    sr, sk = A.stride()
+    dev = A.get_device()
+    N = codes.shape[-2]
+    if dev < 0 or codes.get_device() != dev or sr < 0 or sk < 0 or N == 0:
+        return None
+    G, o, o64 = 1, None, False
+    if offsets is not None:
+        G = codes.shape[0]
+        if (
+            offsets.get_device() != dev or offsets.dtype not in _INTS or offsets.shape != (G + 1,) or offsets.stride() != (1,)
+        ):  # fmt: skip
+            return None
+        o, o64 = offsets.data_ptr(), offsets.dtype is torch.int64
+    D = A.new_empty((R, N), dtype=out_dtype)
+    n = _from_workspace(R, K)
+    ws = codes.new_empty(n)
+    rc = _fn("trnblas_hip_mx_gemm_from")(
+        code, out, G, R, N, K, alpha, A.data_ptr(), sr, sk, codes.data_ptr(), scales.data_ptr(), o, o64, 0.0, None, N,
+        D.data_ptr(), N, ws.data_ptr(), n, _raw_stream(dev),
+    )  # fmt: skip
+    _checked("trnblas_hip_mx_gemm_from", rc)
+    return D
+
+
+def grouped_rank_k_fast(alpha, A, B, offsets, out_dtype):
+    code = _lib.DTYPE_CODES.get(A.dtype)
+    if code is None or B.dtype is not A.dtype or _kernels._launch_probe is not None or A.dim() != 2 or B.dim() != 2:
+        return None
+    R, M = A.shape
+    R2, N = B.shape
+    lda, s1 = A.stride()
+    ldb, t1 = B.stride()
+    dev = A.get_device()
+    if (
+        R2 != R or s1 != 1 or lda < M or t1 != 1 or ldb < N or M == 0 or N == 0 or dev < 0 or B.get_device() != dev
+        or offsets.get_device() != dev or offsets.dtype not in _INTS or offsets.dim() != 1 or offsets.stride() != (1,)
+    ):  # fmt: skip
+        return None
+    if out_dtype is not None and out_dtype is not A.dtype and out_dtype is not torch.float32:
+        return None
+    G = offsets.shape[0] - 1
+    D = A.new_empty((G, M, N), dtype=out_dtype)
+    rc = _fn("trnblas_hip_grouped_rank_k")(
+        code, D.dtype is torch.float32, G, R, M, N, alpha, A.data_ptr(), lda, B.data_ptr(), ldb, offsets.data_ptr(),
+        offsets.dtype is torch.int64, 0.0, None, N, 0, D.data_ptr(), N, M * N, _raw_stream(dev),
+    )  # fmt: skip
+    _checked("trnblas_hip_grouped_rank_k", rc)
+    return D
+
+
+def mx_quantize_fast(X):
+    """(codes, scales) of X (R, K), or None."""
+    code = _lib.DTYPE_CODES.get(X.dtype)
+    dev = X.get_device()
+    if code is None or dev < 0 or X.dim() != 2 or _kernels._launch_probe is not None:
+        return None
+    R, K = X.shape
+    sr, sk = X.stride()
+    if sr < 0 or sk < 0:
+        return None
+    codes = X.new_empty((R, -(-K // 32) * 16), dtype=torch.uint8)
+    scales = X.new_empty((-(-R // 16), -(-K // 512), 256), dtype=torch.uint8)
+    rc = _fn("trnblas_hip_mx_quantize")(
+        code, R, K, X.data_ptr(), sr, sk, 0, codes.data_ptr(), scales.data_ptr(), 1, _raw_stream(dev)
+    )
+    _checked("trnblas_hip_mx_quantize", rc)
+    return codes, scales

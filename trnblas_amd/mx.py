@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from ._flags import trans_flag
-from .grouped import _check_offsets, _check_result
+from .grouped import _check_offsets, _check_result, _gk
 from .hip import dispatch as _d
 
 __all__ = ["MXMatrix", "mx_quantize", "mx_dequantize", "mx_gemm", "mx_grouped_gemm"]
@@ -56,6 +56,13 @@ class MXMatrix:
         codes, scales = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
                          for t in (codes, scales))  # fmt: skip
         self.codes, self.scales, self.shape = codes, scales, shape
+
+    @classmethod
+    def _of(cls, codes: torch.Tensor, scales: torch.Tensor, shape) -> MXMatrix:
+        """From buffers that this package laid out itself."""
+        Q = object.__new__(cls)
+        Q.codes, Q.scales, Q.shape = codes, scales, torch.Size(shape)
+        return Q
 
     @classmethod
     def from_parts(cls, codes: torch.Tensor, block_scales: torch.Tensor, K: int) -> MXMatrix:
@@ -151,10 +158,11 @@ def mx_quantize(X: torch.Tensor, trans: bool = False) -> MXMatrix:
     if trans_flag(trans):
         X = X.mT
     if _d.mx_on_hip(X):
-        from .hip import grouped_kernels
-
         try:
-            return MXMatrix(*grouped_kernels.mx_quantize(X), X.shape)
+            parts = _gk().mx_quantize_fast(X)
+            if parts is not None:
+                return MXMatrix._of(*parts, X.shape)
+            return MXMatrix._of(*_gk().mx_quantize(X), X.shape)
         except Exception as exc:  # noqa: BLE001
             _d._kernel_failed(exc)
     return _quantize_torch(X)
@@ -168,10 +176,8 @@ def mx_dequantize(Q: MXMatrix, dtype: torch.dtype = torch.float32) -> torch.Tens
     if dtype not in _FLOATS:
         raise TypeError(f"mx_dequantize: dtype {dtype} (float32, bfloat16 or float16)")
     if _d.mx_on_hip(Q.codes):
-        from .hip import grouped_kernels
-
         try:
-            return grouped_kernels.mx_dequantize(Q.codes, Q.scales, Q.shape[-1], dtype)
+            return _gk().mx_dequantize(Q.codes, Q.scales, Q.shape[-1], dtype)
         except Exception as exc:  # noqa: BLE001
             _d._kernel_failed(exc)
     return _dequantize_torch(Q, dtype)
@@ -179,6 +185,17 @@ def mx_dequantize(Q: MXMatrix, dtype: torch.dtype = torch.float32) -> torch.Tens
 
 def _product(what: str, alpha, A, B, offsets, beta, C, dtype) -> torch.Tensor:
     dims = 2 if offsets is None else 3
+    if (
+        beta == 0.0 and type(A) is torch.Tensor and A.is_cuda and type(B) is MXMatrix and len(B.shape) == dims
+        and A.dim() == 2 and A.shape[1] == B.shape[-1] and (offsets is None or type(offsets) is torch.Tensor)
+        and not (A.requires_grad and torch.is_grad_enabled()) and _d._use_hip()
+    ):  # fmt: skip
+        try:  # the short way; None: something is out of the ordinary
+            D = _gk().mx_gemm_fast(alpha, A, (B.codes, B.scales), offsets, dtype)
+            if D is not None:
+                return D
+        except _d.HipKernelError as exc:
+            _d._kernel_failed(exc)
     if not isinstance(B, MXMatrix) or len(B.shape) != dims:
         raise ValueError(f"{what}: B must be an MXMatrix of {dims} dimensions (see mx_quantize)")
     if isinstance(A, torch.Tensor):
@@ -207,11 +224,11 @@ def _product(what: str, alpha, A, B, offsets, beta, C, dtype) -> torch.Tensor:
         raise NotImplementedError(f"{what}: no gradient (detach C, or use no_grad)")
     c = C.expand(shape) if beta != 0.0 else None
     if _d.mx_on_hip(codes, B.codes):
-        from .hip import grouped_kernels
-
         try:
-            a = (A.codes, A.scales) if isinstance(A, MXMatrix) else grouped_kernels.mx_quantize(A)
-            return grouped_kernels.mx_gemm(a, (B.codes, B.scales), A.shape[1], out, offsets, alpha, beta, c)
+            b = (B.codes, B.scales)
+            if isinstance(A, MXMatrix):
+                return _gk().mx_gemm((A.codes, A.scales), b, A.shape[1], out, offsets, alpha, beta, c)
+            return _gk().mx_gemm_from(A, b, out, offsets, alpha, beta, c)
         except Exception as exc:  # noqa: BLE001
             _d._kernel_failed(exc)
     a = _dequantize_torch(A if isinstance(A, MXMatrix) else _quantize_torch(A), torch.float32)
