@@ -566,7 +566,10 @@ int trnblas_hip_trsm(int dtype, int64_t n, int64_t nrhs, int upper, int unit, do
  * rounding at the end. All matrices are row-major with any leading dimension
  * and alignment; 16-byte aligned operands whose leading dimensions, strides and
  * K (N where B is N-contiguous; M and N for grouped_rank_k) are multiples of 16
- * bytes run faster. D must not overlap A or B; it may be C itself.
+ * bytes run faster. padded != 0: every row of A and B (16-byte aligned, as
+ * trnblas_hip_pack_k leaves them) is followed by zeros up to a multiple of 16 bytes
+ * that may be read; the extents then need not be multiples. D must not overlap A
+ * or B; it may be C itself.
  *
  * grouped_gemm:   D[r] = alpha A[r] op(B[g]) + beta C[r] for the rows r of
  * group g, D[r] = beta C[r] (zeros when beta == 0) for rows of no group.
@@ -577,7 +580,7 @@ int trnblas_hip_grouped_gemm(int dtype, int out_f32, int transB, int64_t groups,
                              int64_t N, int64_t K, double alpha, const void* A, int64_t lda,
                              const void* B, int64_t ldb, int64_t strideB, const void* offsets,
                              int offsets64, double beta, const void* C, int64_t ldc, void* D,
-                             int64_t ldd, void* stream);
+                             int64_t ldd, int padded, void* stream);
 
 /*
  * grouped_rank_k: D[g] = alpha A_g^T B_g + beta C[g] (M x N each), A_g and B_g
@@ -588,7 +591,7 @@ int trnblas_hip_grouped_rank_k(int dtype, int out_f32, int64_t groups, int64_t r
                                int64_t N, double alpha, const void* A, int64_t lda, const void* B,
                                int64_t ldb, const void* offsets, int offsets64, double beta,
                                const void* C, int64_t ldc, int64_t strideC, void* D, int64_t ldd,
-                               int64_t strideD, void* stream);
+                               int64_t strideD, int padded, void* stream);
 
 /*
  * Microscaled 4-bit floats (e2m1 codes with one power-of-two scale per 32

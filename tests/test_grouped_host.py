@@ -96,12 +96,12 @@ def test_c_abi_refusals():
     def gemm(dtype=0, groups=2, rows=6, n=3, k=4, lda=4, ldb=3, off=4096, beta=0.0, c=None, ldd=3):
         # the pointers are never dereferenced: every call fails its argument checks
         return lib.trnblas_hip_grouped_gemm(dtype, 0, 0, groups, rows, n, k, 1.0, 4096, lda, 4096, ldb, 12, off, 0, beta, c,
-                                            3, 4096, ldd, None)  # fmt: skip
+                                            3, 4096, ldd, 0, None)  # fmt: skip
 
     for bad, word in ((dict(dtype=7), b"dtype"), (dict(rows=-1), b"sizes"), (dict(groups=1 << 24), b"sizes"),
                       (dict(lda=3), b"leading"), (dict(ldd=2), b"leading"), (dict(off=None), b"offsets"),
                       (dict(off=4098), b"offsets"), (dict(beta=1.0), b"without C"), (dict(k=1 << 31), b"sizes")):  # fmt: skip
         assert gemm(**bad) == _lib.E_ARG and word in lib.trnblas_hip_last_error(), bad
     assert gemm(rows=0) == 0  # nothing to do
-    rc = lib.trnblas_hip_grouped_rank_k(1, 0, 2, 6, 4, 3, 1.0, 4096, 3, 4096, 3, 4096, 0, 0.0, None, 3, 0, 4096, 3, 12, None)
+    rc = lib.trnblas_hip_grouped_rank_k(1, 0, 2, 6, 4, 3, 1.0, 4096, 3, 4096, 3, 4096, 0, 0.0, None, 3, 0, 4096, 3, 12, 0, None)
     assert rc == _lib.E_ARG and b"leading" in lib.trnblas_hip_last_error()

@@ -16,63 +16,71 @@
 namespace trnblas {
 
 // Operands of any alignment and any strides: the panels go through registers.
-// 256 threads on a 64 x 64 tile, each wave 32 x 32; the loads of k-tile t + 1 are
-// in flight behind the MFMAs of t. fp32 sums restart every chain_length(K)
-// values of k (gemm.hpp).
+// 256 threads on a 64 x 64 tile, each wave 32 x 32; the loads of k-tile t + 2 are in
+// flight behind the MFMAs of t. fp32 sums restart every chain_length(K) values of k
+// (gemm.hpp). Bound by the loads of rows that start anywhere (16 bytes two bytes past
+// a word take several times as long; the five words around them, shifted, longer
+// still): bf16 4093 rows in 8 groups by 1023 x 2047 77 us (223 TFLOP/s; transposed
+// 101), fp32 4093 by 2047^2 395 us (87); larger products are packed first.
 template <typename T, bool BKC, bool RK>
-__global__ __launch_bounds__(256) void grouped_any_kernel(GroupedArgs g) {
-  constexpr int BM = 64, BN = 64, FM = 2, FN = 2;
+__global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
+  constexpr int FM = 2, FN = 2, BM = 32 * FM, BN = 32 * FN, AHEAD = 2;
   using PA = Panel<T, BM, !RK>;
   using PB = Panel<T, BN, BKC>;
-  constexpr int BK = PA::BK, EV = PA::EV, ES = sizeof(T);
+  constexpr int BK = PA::BK, ES = sizeof(T), HA = PA::BYTES / 4096, HB = PB::BYTES / 4096;
   constexpr bool FOLD = std::is_same_v<T, float>;
   __shared__ __attribute__((aligned(16))) char lds[2][PA::BYTES + PB::BYTES];
   TileJob j;
   if (!tile_job<T, BM, BN, BKC, RK>(g, j)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int m0 = 32 * (wave & 1), n0 = 32 * (wave >> 1);
-  int ra[2], ka[2], rb[2], kb[2];
-  const char *pa[2], *pb[2];
+  const int m0 = 16 * FM * (wave & 1), n0 = 16 * FN * (wave >> 1);
+  int ra[HA], ka[HA], rb[HB], kb[HB];
+  const char *pa[HA], *pb[HB];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < HA; ++h) {
     PA::where(tid + 256 * h, ra[h], ka[h]);
-    PB::where(tid + 256 * h, rb[h], kb[h]);
     pa[h] = j.A + (RK ? (int64_t)ka[h] * g.lda + ra[h] : (int64_t)ra[h] * g.lda + ka[h]) * ES;
+  }
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    PB::where(tid + 256 * h, rb[h], kb[h]);
     pb[h] = j.B + (BKC ? (int64_t)rb[h] * g.ldb + kb[h] : (int64_t)kb[h] * g.ldb + rb[h]) * ES;
   }
   const int64_t step_a = (RK ? BK * g.lda : BK) * ES, step_b = (BKC ? BK : BK * g.ldb) * ES;
   const int nk = (j.K + BK - 1) / BK;
-  i32x4 va[2], vb[2];
-  auto load = [&](int kt) __attribute__((always_inline)) {
+  i32x4 va[AHEAD][HA], vb[AHEAD][HB];
+  auto load = [&](int kt, int set) __attribute__((always_inline)) {
     const int left = j.K - kt * BK;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      va[h] = load_any<T>(pa[h] + kt * step_a, RK ? (ka[h] < left ? j.rows_a - ra[h] : 0) : (ra[h] < j.rows_a ? left - ka[h] : 0));
-      vb[h] = load_any<T>(pb[h] + kt * step_b, BKC ? (rb[h] < j.rows_b ? left - kb[h] : 0) : (kb[h] < left ? j.rows_b - rb[h] : 0));
-    }
+    for (int h = 0; h < HA; ++h)
+      va[set][h] = load_any<T>(pa[h] + kt * step_a, RK ? (ka[h] < left ? j.rows_a - ra[h] : 0) : (ra[h] < j.rows_a ? left - ka[h] : 0));
+#pragma unroll
+    for (int h = 0; h < HB; ++h)
+      vb[set][h] = load_any<T>(pb[h] + kt * step_b, BKC ? (rb[h] < j.rows_b ? left - kb[h] : 0) : (kb[h] < left ? j.rows_b - rb[h] : 0));
   };
   uint32_t oa[PA::NV], ob[PB::NV];
   PA::lane_offsets(m0, lane, oa);
   PB::lane_offsets(n0, lane, ob);
-  f32x4 acc[FM][FN], sum[FM][FN];
+  f32x4 acc[FM][FN], sum[FOLD ? FM : 1][FOLD ? FN : 1];
 #pragma unroll
   for (int a = 0; a < FM; ++a)
 #pragma unroll
-    for (int b = 0; b < FN; ++b) acc[a][b] = sum[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int b = 0; b < FN; ++b) {
+      acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (FOLD) sum[a][b] = acc[a][b];
+    }
   const int span = chain_length(j.K, ES) / BK;
   int chain = span;
-  if (nk > 0) load(0);
-  for (int kt = 0; kt < nk; ++kt) {
+  auto k_tile = [&](int kt, int set) __attribute__((always_inline)) {
     char* st = lds[kt & 1];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      *reinterpret_cast<i32x4*>(st + 16 * (tid + 256 * h)) = va[h];
-      *reinterpret_cast<i32x4*>(st + PA::BYTES + 16 * (tid + 256 * h)) = vb[h];
-    }
+    for (int h = 0; h < HA; ++h) *reinterpret_cast<i32x4*>(st + 16 * (tid + 256 * h)) = va[set][h];
+#pragma unroll
+    for (int h = 0; h < HB; ++h) *reinterpret_cast<i32x4*>(st + PA::BYTES + 16 * (tid + 256 * h)) = vb[set][h];
     // one barrier per k-tile: stage t's readers are past it before t + 2 is stored
-    __syncthreads();
-    if (kt + 1 < nk) load(kt + 1);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kt + AHEAD < nk) load(kt + AHEAD, set);
     const char *qa[PA::NV], *qb[PB::NV];
 #pragma unroll
     for (int i = 0; i < PA::NV; ++i) qa[i] = st + oa[i];
@@ -90,18 +98,27 @@ __global__ __launch_bounds__(256) void grouped_any_kernel(GroupedArgs g) {
 #pragma unroll
         for (int a = 0; a < FM; ++a) mma_tile<T>(acc[a][b], fb[b], fa[a]);
     }
-    if (FOLD && --chain == 0) {
+    if constexpr (FOLD) {
+      if (--chain == 0) {
 #pragma unroll
-      for (int a = 0; a < FM; ++a)
+        for (int a = 0; a < FM; ++a)
 #pragma unroll
-        for (int b = 0; b < FN; ++b) {
-          sum[a][b] += acc[a][b];
-          acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-      chain = span;
+          for (int b = 0; b < FN; ++b) {
+            sum[a][b] += acc[a][b];
+            acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          }
+        chain = span;
+      }
     }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (i < nk) load(i, i);
+  for (int kt = 0; kt < nk; kt += AHEAD) {
+    k_tile(kt, 0);
+    if (kt + 1 < nk) k_tile(kt + 1, 1);
   }
-  if (FOLD) {
+  if constexpr (FOLD) {
 #pragma unroll
     for (int a = 0; a < FM; ++a)
 #pragma unroll
@@ -127,11 +144,12 @@ static int grid_of(int64_t tiles, const char* what, unsigned* grid) {
 
 template <typename T, bool BKC, bool RK>
 static int run_any(GroupedArgs g, hipStream_t s) {
+  constexpr int BM = 64;
   const char* what = RK ? kRankK : kGemm;
-  g.tiles_m = (g.M + 63) / 64;
-  g.tiles_n = (g.N + 63) / 64;
+  g.tiles_m = (g.M + BM - 1) / BM;
+  g.tiles_n = (g.N + BM - 1) / BM;
   unsigned grid;
-  const int64_t rows = RK ? (int64_t)g.groups * g.tiles_m : row_tiles(g.rows, g.groups, 64);
+  const int64_t rows = RK ? (int64_t)g.groups * g.tiles_m : row_tiles(g.rows, g.groups, BM);
   if (int rc = grid_of(rows * g.tiles_n, what, &grid)) return rc;
   // whole rounds of the XCDs: a grid that is a bound on the tiles reaches the last one of each
   if (!RK) grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
@@ -139,13 +157,15 @@ static int run_any(GroupedArgs g, hipStream_t s) {
   return check_launch(what);
 }
 
-// Operands that LDS DMA reads in place: see ring.hpp. Its 32-bit offsets reach
-// over one panel of a K-contiguous operand and one k-tile of the other kind.
+// Operands that LDS DMA reads in place: see ring.hpp. Whole groups of 16 bytes
+// lie inside the operands, or (g.padded) are zeros past their ends. Its 32-bit
+// offsets reach over one panel of a K-contiguous operand and one k-tile of the
+// other kind.
 template <typename T>
 static bool dma_ready(const GroupedArgs& g, bool bkc, bool rk) {
   const int64_t es = sizeof(T), far = INT32_MAX - 1024;
   auto whole = [&](const void* p, int64_t ld, int64_t st, int64_t ext) {
-    return (uintptr_t)p % 16 == 0 && ld * es % 16 == 0 && st * es % 16 == 0 && ext * es % 16 == 0;
+    return (uintptr_t)p % 16 == 0 && ld * es % 16 == 0 && st * es % 16 == 0 && (g.padded || ext * es % 16 == 0);
   };
   const int64_t ra = rk ? 128 / es : 256, rb = bkc ? 256 : 128 / es;
   return whole(g.A, g.lda, 0, rk ? g.M : g.K) && whole(g.B, g.ldb, g.sB, bkc ? g.K : g.N) && (!rk || g.rows < far) &&
@@ -227,12 +247,13 @@ static bool quads(const GroupedArgs& g, int dtype) {
 
 // checks and fields that both entry points share
 static int common_args(const char* what, GroupedArgs& g, int dtype, int out_f32, int64_t groups, int64_t rows, double alpha,
-                       double beta, const void* offsets, int offsets64, const void* C) {
+                       double beta, const void* offsets, int offsets64, const void* C, int padded) {
   TRNBLAS_CHECK_ARG(dtype == TRNBLAS_F32 || dtype == TRNBLAS_BF16 || dtype == TRNBLAS_F16, "%s: bad dtype %d", what, dtype);
   TRNBLAS_CHECK_ARG(groups >= 0 && groups < (1 << 24) && rows >= 0 && rows < INT32_MAX - 1024,
                     "%s: bad sizes (groups %lld, rows %lld)", what, (long long)groups, (long long)rows);
   TRNBLAS_CHECK_ARG(offsets != nullptr && (uintptr_t)offsets % (offsets64 ? 8 : 4) == 0, "%s: offsets missing or misaligned", what);
   TRNBLAS_CHECK_ARG(beta == 0.0 || C != nullptr, "%s: beta != 0 without C", what);
+  g.padded = padded != 0;
   g.offsets = offsets;
   g.offsets64 = offsets64 != 0;
   g.groups = (int)groups;
@@ -250,9 +271,9 @@ using namespace trnblas;
 extern "C" int trnblas_hip_grouped_gemm(int dtype, int out_f32, int transB, int64_t groups, int64_t rows, int64_t N, int64_t K,
                                         double alpha, const void* A, int64_t lda, const void* B, int64_t ldb, int64_t strideB,
                                         const void* offsets, int offsets64, double beta, const void* C, int64_t ldc, void* D,
-                                        int64_t ldd, void* stream) {
+                                        int64_t ldd, int padded, void* stream) {
   GroupedArgs g{};
-  if (int rc = common_args(kGemm, g, dtype, out_f32, groups, rows, alpha, beta, offsets, offsets64, C)) return rc;
+  if (int rc = common_args(kGemm, g, dtype, out_f32, groups, rows, alpha, beta, offsets, offsets64, C, padded)) return rc;
   TRNBLAS_CHECK_ARG(N >= 0 && N < INT32_MAX - 1024 && K >= 0 && K < INT32_MAX - 1024, "%s: bad sizes (N %lld, K %lld)", kGemm,
                     (long long)N, (long long)K);
   TRNBLAS_CHECK_ARG(lda >= K && ldb >= (transB ? K : N) && ldd >= N && (beta == 0.0 || ldc >= N) && strideB >= 0,
@@ -276,9 +297,9 @@ extern "C" int trnblas_hip_grouped_gemm(int dtype, int out_f32, int transB, int6
 extern "C" int trnblas_hip_grouped_rank_k(int dtype, int out_f32, int64_t groups, int64_t rows, int64_t M, int64_t N, double alpha,
                                           const void* A, int64_t lda, const void* B, int64_t ldb, const void* offsets,
                                           int offsets64, double beta, const void* C, int64_t ldc, int64_t strideC, void* D,
-                                          int64_t ldd, int64_t strideD, void* stream) {
+                                          int64_t ldd, int64_t strideD, int padded, void* stream) {
   GroupedArgs g{};
-  if (int rc = common_args(kRankK, g, dtype, out_f32, groups, rows, alpha, beta, offsets, offsets64, C)) return rc;
+  if (int rc = common_args(kRankK, g, dtype, out_f32, groups, rows, alpha, beta, offsets, offsets64, C, padded)) return rc;
   TRNBLAS_CHECK_ARG(M >= 0 && M < INT32_MAX - 1024 && N >= 0 && N < INT32_MAX - 1024, "%s: bad sizes (M %lld, N %lld)", kRankK,
                     (long long)M, (long long)N);
   TRNBLAS_CHECK_ARG(lda >= M && ldb >= N && ldd >= N && (beta == 0.0 || ldc >= N) && strideC >= 0 && strideD >= 0,

@@ -155,12 +155,13 @@ SIGNATURES = {
     "trnblas_hip_grouped_gemm": (
         _c_int,
         [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_ptr, _c_i64]
-        + [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr],
+        + [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_int]
+        + [_c_ptr],
     ),
     "trnblas_hip_grouped_rank_k": (
         _c_int,
         [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64]
-        + [_c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr],
+        + [_c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_int, _c_ptr],
     ),
     "trnblas_hip_mx_quantize": (
         _c_int,

@@ -11,7 +11,7 @@ import torch
 from . import _lib
 from ._lib import ptr, stream_of
 from . import kernels as _kernels
-from .kernels import _batched_layout, _probed_call, _require_device
+from .kernels import _batched_layout, _pack_k, _probed_call, _require_device
 
 
 def row_major(X: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -37,6 +37,31 @@ def _output_like(C: torch.Tensor | None, beta: float, shape, dtype, dev):
     return D, c if (c.stride(-1) == 1 or n <= 1) and (c.stride(-2) >= n or shape[-2] <= 1) else c.contiguous()
 
 
+# Operands that LDS DMA cannot read in place (base, leading dimension or extent no
+# multiple of 16 bytes) are copied first, their rows padded with zeros, where the
+# copies cost less than grouped_any_kernel's loads: both read and write at about 4 TB/s
+# and start in 4 us each; the kernel makes 300 TFLOP/s (rank_k 230; fp32 90) of such operands,
+# the ring kernels 800 (fp32 120) of copied ones. bf16 16383 rows in 8 groups, 2047 x
+# 4095: 763 us in place. Products of few flops per byte stay in place.
+_PACK_SAVES = {  # us per multiply-add
+    ("gemm", 2): 2 * (1 / 300e6 - 1 / 800e6), ("rank_k", 2): 2 * (1 / 230e6 - 1 / 800e6),
+    ("gemm", 4): 2 * (1 / 90e6 - 1 / 120e6), ("rank_k", 4): 2 * (1 / 90e6 - 1 / 120e6),
+}  # fmt: skip
+
+
+def _ready(p: int, ld: int, stride: int, ext: int, ev: int) -> bool:
+    return p % 16 == 0 and ld % ev == 0 and stride % ev == 0 and ext % ev == 0
+
+
+def _pack_pays(op: str, es: int, macs: int, copied: int) -> bool:
+    """copied: elements of the operands that are not ready."""
+    return macs * _PACK_SAVES[op, es] > 8 + 2 * copied * es / 4e6
+
+
+def _up(n: int, ev: int) -> int:
+    return -(-n // ev) * ev
+
+
 def grouped_gemm(
     A: torch.Tensor,
     B: torch.Tensor,
@@ -53,12 +78,22 @@ def grouped_gemm(
     G, _, N = B.shape
     a, lda = row_major(A)
     b, tb, ldb, sb = _batched_layout(B)
+    ev, padded = 16 // A.element_size(), False
+    a_ok = _ready(a.data_ptr(), lda, 0, K, ev)
+    b_ok = _ready(b.data_ptr(), ldb, sb, K if tb else N, ev)
+    if not (a_ok and b_ok):
+        padded = _pack_pays("gemm", A.element_size(), R * K * N, (not a_ok) * R * K + (not b_ok) * G * K * N)
+    if padded and not a_ok:
+        a, lda = _pack_k(A, _up(K, ev)), _up(K, ev)
+    if padded and not b_ok:
+        b = _pack_k(B.mT if tb else B, _up(K if tb else N, ev))
+        ldb, sb = b.stride(1), b.stride(0)
     o, o64 = offsets_of(offsets)
     D, c = _output_like(C, beta, (R, N), out_dtype or A.dtype, dev)
     _probed_call(
         "grouped_gemm", "trnblas_hip_grouped_gemm", _lib.DTYPE_CODES[A.dtype], int(D.dtype == torch.float32), int(tb),
         G, R, N, K, float(alpha), ptr(a), lda, ptr(b), ldb, sb, ptr(o), o64, float(beta) if c is not None else 0.0,
-        ptr(c), max(c.stride(0), N) if c is not None else N, ptr(D), max(N, 1), stream_of(dev),
+        ptr(c), max(c.stride(0), N) if c is not None else N, ptr(D), max(N, 1), int(padded), stream_of(dev),
     )  # fmt: skip
     return D
 
@@ -80,13 +115,21 @@ def grouped_rank_k(
     G = offsets.shape[0] - 1
     a, lda = row_major(A)
     b, ldb = row_major(B)
+    ev, padded = 16 // A.element_size(), False
+    a_ok, b_ok = _ready(a.data_ptr(), lda, 0, M, ev), _ready(b.data_ptr(), ldb, 0, N, ev)
+    if not (a_ok and b_ok):
+        padded = _pack_pays("rank_k", A.element_size(), R * M * N, (not a_ok) * R * M + (not b_ok) * R * N)
+    if padded and not a_ok:
+        a, lda = _pack_k(A, _up(M, ev)), _up(M, ev)
+    if padded and not b_ok:
+        b, ldb = _pack_k(B, _up(N, ev)), _up(N, ev)
     o, o64 = offsets_of(offsets)
     D, c = _output_like(C, beta, (G, M, N), out_dtype or A.dtype, dev)
     _probed_call(
         "grouped_rank_k", "trnblas_hip_grouped_rank_k", _lib.DTYPE_CODES[A.dtype], int(D.dtype == torch.float32),
         G, R, M, N, float(alpha), ptr(a), lda, ptr(b), ldb, ptr(o), o64, float(beta) if c is not None else 0.0,
         ptr(c), max(c.stride(1), N) if c is not None else N, c.stride(0) if c is not None and G > 1 else 0,
-        ptr(D), max(N, 1), M * N, stream_of(dev),
+        ptr(D), max(N, 1), M * N, int(padded), stream_of(dev),
     )  # fmt: skip
     return D
 
@@ -186,6 +229,7 @@ def mx_gemm(
 # 12 us, these 8). Each returns None where anything is out of the ordinary: the
 # general path then reports it or deals with it.
 
+_PACK_LOOK = 1 << 30  # multiply-adds below which no packing pays
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _fns: dict = {}
 _INTS = (torch.int32, torch.int64)
@@ -222,10 +266,15 @@ def grouped_gemm_fast(alpha, A, B, offsets, transB, out_dtype):
         return None
     if out_dtype is not None and out_dtype is not A.dtype and out_dtype is not torch.float32:
         return None
+    pa, pb = A.data_ptr(), B.data_ptr()
+    ev = 4 if code == 0 else 8
+    if (pa | pb) % 16 or (lda | t0 | sb | K | b1) % ev:
+        if R * K * N > _PACK_LOOK:
+            return None  # the general path may pack
     D = A.new_empty((R, N), dtype=out_dtype)
     rc = _fn("trnblas_hip_grouped_gemm")(
-        code, D.dtype is torch.float32, transB, G, R, N, K, alpha, A.data_ptr(), lda, B.data_ptr(), t0, sb,
-        offsets.data_ptr(), offsets.dtype is torch.int64, 0.0, None, N, D.data_ptr(), N, _raw_stream(dev),
+        code, D.dtype is torch.float32, transB, G, R, N, K, alpha, pa, lda, pb, t0, sb,
+        offsets.data_ptr(), offsets.dtype is torch.int64, 0.0, None, N, D.data_ptr(), N, 0, _raw_stream(dev),
     )  # fmt: skip
     _checked("trnblas_hip_grouped_gemm", rc)
     return D
@@ -279,11 +328,15 @@ def grouped_rank_k_fast(alpha, A, B, offsets, out_dtype):
         return None
     if out_dtype is not None and out_dtype is not A.dtype and out_dtype is not torch.float32:
         return None
+    ev = 4 if code == 0 else 8
+    if (A.data_ptr() | B.data_ptr()) % 16 or (lda | ldb | M | N) % ev:
+        if R * M * N > _PACK_LOOK:
+            return None
     G = offsets.shape[0] - 1
     D = A.new_empty((G, M, N), dtype=out_dtype)
     rc = _fn("trnblas_hip_grouped_rank_k")(
         code, D.dtype is torch.float32, G, R, M, N, alpha, A.data_ptr(), lda, B.data_ptr(), ldb, offsets.data_ptr(),
-        offsets.dtype is torch.int64, 0.0, None, N, 0, D.data_ptr(), N, M * N, _raw_stream(dev),
+        offsets.dtype is torch.int64, 0.0, None, N, 0, D.data_ptr(), N, M * N, 0, _raw_stream(dev),
     )  # fmt: skip
     _checked("trnblas_hip_grouped_rank_k", rc)
     return D
