@@ -124,10 +124,13 @@ __global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
 #pragma unroll
       for (int b = 0; b < FN; ++b) acc[a][b] += sum[a][b];
   }
+  static_assert(4 * kStoreLds<FN> <= sizeof(lds));
+  char* own = lds[0] + wave * kStoreLds<FN>;
+  __syncthreads();  // the other waves' reads
   if (g.out32)
-    store_wave<FM, FN, float>(g, j, acc, m0, n0, lane);
+    store_wave<FM, FN, float>(g, j, acc, m0, n0, lane, own);
   else
-    store_wave<FM, FN, T>(g, j, acc, m0, n0, lane);
+    store_wave<FM, FN, T>(g, j, acc, m0, n0, lane, own);
 }
 
 static const char* kGemm = "trnblas_hip_grouped_gemm";
@@ -137,7 +140,7 @@ static const char* kRankK = "trnblas_hip_grouped_rank_k";
 static int64_t row_tiles(int64_t rows, int64_t groups, int bm) { return rows / bm + std::min(groups + 2, rows); }
 
 static int grid_of(int64_t tiles, const char* what, unsigned* grid) {
-  TRNBLAS_CHECK_ARG(tiles < (int64_t)1 << 31, "%s: too many tiles", what);
+  TRNBLAS_CHECK_ARG(tiles < ((int64_t)1 << 31) - 4096, "%s: too many tiles", what);
   *grid = (unsigned)tiles;
   return TRNBLAS_OK;
 }
@@ -151,8 +154,8 @@ static int run_any(GroupedArgs g, hipStream_t s) {
   unsigned grid;
   const int64_t rows = RK ? (int64_t)g.groups * g.tiles_m : row_tiles(g.rows, g.groups, BM);
   if (int rc = grid_of(rows * g.tiles_n, what, &grid)) return rc;
-  // whole rounds of the XCDs: a grid that is a bound on the tiles reaches the last one of each
-  if (!RK) grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
+  // whole rounds of the XCDs, so that each one's last tile is reached
+  grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
   hipLaunchKernelGGL((grouped_any_kernel<T, BKC, RK>), dim3(grid), dim3(256), 0, s, g);
   return check_launch(what);
 }
@@ -180,8 +183,7 @@ static int run_ring(GroupedArgs g, hipStream_t s) {
   g.tiles_n = (g.N + BN - 1) / BN;
   unsigned grid;
   const int64_t rows = RK ? (int64_t)g.groups * g.tiles_m : row_tiles(g.rows, g.groups, BM);
-  if (int rc = grid_of(rows * g.tiles_n, what, &grid)) return rc;
-  if (!RK) grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
+  if (int rc = grid_of(ring_grid<FM, FN>(g, rows * g.tiles_n), what, &grid)) return rc;
   hipLaunchKernelGGL((ring_kernel<T, FM, FN, BKC, RK>), dim3(grid), dim3(256), 0, s, g, MxScales{});
   return check_launch(what);
 }

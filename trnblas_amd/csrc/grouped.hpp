@@ -26,6 +26,7 @@ struct GroupedArgs {
   int groups, rows;  // rows of the ragged operand(s)
   int M, N, K;       // ragged rows: M unused; ragged k: K unused
   int tiles_m, tiles_n;
+  int slots;  // workgroups that run at a time (tiles of one workgroup per CU)
   float alpha, beta;
   int out_f16;  // D and C are fp16 (products of 4-bit floats; else bf16 or fp32)
   int out32;  // D and C are fp32 whatever the operands are
@@ -54,7 +55,32 @@ struct Segment {
   int start, end;  // its rows
   int row;         // first row of this tile
   int tn;          // column tile
+  int quarter;     // of the tile, or -1
 };
+
+// Tile of workgroup `bid` among `tiles`; false when there is none left. Workgroups
+// go to the XCDs round-robin: each XCD walks one contiguous range of the tiles.
+// SPLIT (one workgroup per CU, g.slots of them): tiles that would not fill a last
+// round are cut into quarters, one workgroup each, unless they fill three quarters
+// of it: a quarter takes about a third of a tile's time.
+template <bool SPLIT>
+__device__ __forceinline__ bool tile_of(const GroupedArgs& g, int bid, int tiles, int& tile, int& quarter) {
+  auto range = [](int b, int n, int& t) __attribute__((always_inline)) {
+    const int q = n / kNumXcd, r = n % kNumXcd, x = b % kNumXcd, i = b / kNumXcd;
+    t = x * q + min(x, r) + i;
+    return i < q + (x < r);
+  };
+  quarter = -1;
+  if constexpr (!SPLIT) return range(bid, tiles, tile);
+  int whole = tiles / g.slots * g.slots, cut = tiles - whole;
+  if (4 * cut > 3 * g.slots) whole = tiles, cut = 0;
+  const int first = (whole + kNumXcd - 1) / kNumXcd * kNumXcd;  // workgroups up to here take whole tiles
+  if (bid < first) return range(bid, whole, tile);
+  if (!range(bid - first, 4 * cut, tile)) return false;
+  quarter = tile & 3;
+  tile = whole + (tile >> 2);
+  return true;
+}
 
 // Inclusive sum over the lanes of the wave, by DPP: lanes 1, 2, 4 and 8 back in
 // each row of 16, then the rows' last lanes broadcast to the rows after them.
@@ -68,13 +94,11 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// Tile of workgroup `bid` among ragged rows cut into tiles of BM rows per
-// segment and g.tiles_n column tiles; false when there is none left. The
-// number of tiles is known on the device only: the grid is a bound, and each
-// wave counts the tiles of 64 segments at a time (one load and a scan).
-// Workgroups go to the XCDs round-robin: each XCD walks one contiguous range
-// of the tiles that are really there, in bands of `band` row tiles by columns.
-template <int BM>
+// tile_of among ragged rows cut into tiles of BM rows per segment and g.tiles_n
+// column tiles, walked in bands of `band` row tiles by columns. The number of
+// tiles is known on the device only: the grid is a bound, and each wave counts the
+// tiles of 64 segments at a time (one load and a scan).
+template <int BM, bool SPLIT = false>
 __device__ __forceinline__ bool ragged_tile(const GroupedArgs& g, int bid, int band, Segment& s) {
   const int lane = threadIdx.x & 63;
   const int nseg = g.groups + 2;
@@ -86,12 +110,8 @@ __device__ __forceinline__ bool ragged_tile(const GroupedArgs& g, int bid, int b
     incl = wave_scan(i < nseg ? (en - st + BM - 1) / BM : 0);
     total += __builtin_amdgcn_readlane(incl, 63);
   }
-  const int ntile = total * g.tiles_n;
-  const int q = ntile / kNumXcd, r = ntile % kNumXcd;
-  const int x = bid % kNumXcd, i = bid / kNumXcd;
-  if (i >= q + (x < r)) return false;
-  const int t = x * q + min(x, r) + i;
-  int tm, tn;
+  int t, tm, tn;
+  if (!tile_of<SPLIT>(g, bid, total * g.tiles_n, t, s.quarter)) return false;
   grouped_tile(t, total, g.tiles_n, band, tm, tn);
   s.tn = tn;
   if (nseg > 64) {  // walk the segments again up to the one that holds tm
@@ -251,7 +271,7 @@ __device__ __forceinline__ void store_quad(const GroupedArgs& g, const O* C, O* 
 struct TileJob {
   const char *A, *B;  // panel corners at k = 0
   int rows_a, rows_b, K;
-  int group;
+  int group, quarter;
   int64_t m;  // first output row
   int n;      // first output column
   const void* C;
@@ -259,13 +279,14 @@ struct TileJob {
 };
 
 // RK: ragged k (grouped_rank_k), else ragged rows.
-template <typename T, int BM, int BN, bool BKC, bool RK>
+template <typename T, int BM, int BN, bool BKC, bool RK, bool SPLIT = false>
 __device__ __forceinline__ bool tile_job(const GroupedArgs& g, TileJob& j) {
   const int64_t es = sizeof(T), eo = g.out32 ? 4 : es;
   if constexpr (RK) {
-    const int t = xcd_remap(blockIdx.x, gridDim.x);
-    const int per = g.tiles_m * g.tiles_n, grp = t / per;
-    int tm, tn;
+    const int per = g.tiles_m * g.tiles_n;
+    int t, tm, tn;
+    if (!tile_of<SPLIT>(g, blockIdx.x, g.groups * per, t, j.quarter)) return false;
+    const int grp = t / per;
     grouped_tile(t - grp * per, g.tiles_m, g.tiles_n, 8, tm, tn);
     const int start = boundary(g, grp + 1), end = max(boundary(g, grp + 2), start);
     j.group = grp;
@@ -279,7 +300,8 @@ __device__ __forceinline__ bool tile_job(const GroupedArgs& g, TileJob& j) {
     j.D = static_cast<char*>(g.D) + grp * g.sD * eo;
   } else {
     Segment s;
-    if (!ragged_tile<BM>(g, blockIdx.x, 8, s)) return false;
+    if (!ragged_tile<BM, SPLIT>(g, blockIdx.x, 8, s)) return false;
+    j.quarter = s.quarter;
     const bool of_group = s.group >= 0 && s.group < g.groups;
     j.group = s.group;
     j.m = s.row;
@@ -292,6 +314,17 @@ __device__ __forceinline__ bool tile_job(const GroupedArgs& g, TileJob& j) {
     j.D = g.D;
   }
   j.rows_b = min(BN, g.N - j.n);
+  if constexpr (SPLIT) {
+    if (j.quarter >= 0) {
+      const int m = BM / 2 * (j.quarter & 1), n = BN / 2 * (j.quarter >> 1);
+      j.rows_a = min(BM / 2, j.rows_a - m);
+      j.rows_b = min(BN / 2, j.rows_b - n);
+      if (j.rows_a <= 0 || j.rows_b <= 0) return false;
+      j.m += m, j.n += n;
+      j.A += (RK ? m : m * g.lda) * es;
+      j.B += (BKC ? n * g.ldb : n) * es;
+    }
+  }
   return true;
 }
 
@@ -299,21 +332,26 @@ __device__ __forceinline__ bool tile_job(const GroupedArgs& g, TileJob& j) {
 // Whole quads (aligned, N a multiple of 4): all of C's quads of a block row are
 // under way before the first is used, the next row's behind this row's stores (one
 // quad at a time, each waiting for its C, the accumulated fp32 gradients of 24 groups
-// took 186 us). Quads outside repeat the last one inside.
+// took 186 us). Quads outside repeat the last one inside. Rows that start anywhere:
+// a block row goes through LDS (kStoreLds bytes of the wave's own, no longer used by
+// others), so that neighbouring lanes store neighbouring values (four separate
+// stores of each lane's quad: 16383 x 4095 bf16 took 120 us longer).
+template <int FN>
+constexpr int kStoreLds = 16 * (16 * FN + 4) * 4;
 template <int FM, int FN, typename O>
 __device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& j, const f32x4 (&acc)[FM][FN], int m0,
-                                           int n0, int lane) {
+                                           int n0, int lane, char* lds) {
   typedef O o4 __attribute__((ext_vector_type(4)));
   const O* C = static_cast<const O*>(j.C);
   O* D = static_cast<O*>(j.D);
   const int li = lane & 15, n = j.n + n0 + 4 * (lane >> 4);
+  // the sum of a block, read here: the compiler would scale all of them before the branches
+  auto take = [&](int a, int b) __attribute__((always_inline)) {
+    f32x4 v = acc[a][b];
+    asm volatile("" : "+v"(v));
+    return v;
+  };
   if (g.vec4 && (g.N & 3) == 0) {
-    // the sum of a block, read here: the compiler would scale all of them before the branches
-    auto take = [&](int a, int b) __attribute__((always_inline)) {
-      f32x4 v = acc[a][b];
-      asm volatile("" : "+v"(v));
-      return v;
-    };
     auto store = [&](int a, auto value) __attribute__((always_inline)) {
       const int m = m0 + 16 * a + li;
       O* d = D + (j.m + m) * g.ldd + n;
@@ -348,17 +386,23 @@ __device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& 
     }
     return;
   }
+  constexpr int W = 16 * FN, LD = W + 4;
+  float* buf = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int a = 0; a < FM; ++a) {
-    const int m = m0 + 16 * a + li;
-    if (m < j.rows_a) {
 #pragma unroll
-      for (int b = 0; b < FN; ++b) {
-        f32x4 v = acc[a][b];
-        asm volatile("" : "+v"(v));
-        store_quad<O>(g, C, D, j.m + m, n + 16 * b, v);
+    for (int b = 0; b < FN; ++b) *reinterpret_cast<f32x4*>(buf + li * LD + 16 * b + 4 * (lane >> 4)) = take(a, b) * g.alpha;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int h = 0; h < W / 4; ++h) {
+      const int e = 64 * h + lane, r = e / W, c = e % W, m = m0 + 16 * a + r, col = j.n + n0 + c;
+      float v = buf[r * LD + c];
+      if (m < j.rows_a && col < g.N) {
+        if (g.beta != 0.0f) v = __builtin_fmaf(g.beta, (float)C[(j.m + m) * g.ldc + col], v);
+        D[(j.m + m) * g.ldd + col] = (O)v;
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 

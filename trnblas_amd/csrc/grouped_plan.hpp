@@ -23,8 +23,10 @@ constexpr RingCost kRing4[] = {{8, 8, 1, 11.0, 1.2, 1.6}, {4, 4, 2, 6.0, 0.5, 1.
 
 inline double ring_time(const RingCost& c, double tiles, double k_tiles) {
   const double t = tiles / (c.per_cu * device_cus());
-  // one workgroup per CU runs in whole rounds; several drift apart
-  const double rounds = t <= 1.0 ? 1.0 : c.per_cu == 1 ? std::ceil(t) : t + 0.3;
+  // several workgroups of a CU drift apart; one runs in whole rounds, what is left of the last cut into quarters (tile_of)
+  const double part = t - std::floor(t);
+  const double rounds = c.per_cu > 1 ? std::max(1.0, t <= 1.0 ? 1.0 : t + 0.3)
+                                     : std::floor(t) + (part > 0.75 ? 1.0 : 0.36 * std::ceil(4.0 * part));
   return rounds * (c.start + k_tiles * (c.alone + (c.full - c.alone) * std::min(1.0, t)));
 }
 

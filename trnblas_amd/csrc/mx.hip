@@ -175,9 +175,13 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(DequantArgs g) {
   }
 }
 
-static int mx_grid(const GroupedArgs& g, int bm, unsigned* grid) {
-  const int64_t tiles = (g.rows / bm + std::min<int64_t>(g.groups + 2, g.rows)) * g.tiles_n;
-  TRNBLAS_CHECK_ARG(tiles < ((int64_t)1 << 31) - 8, "%s: too many tiles", kMxGemm);
+// Bound on the tiles of bm rows (see ragged_tile).
+static int64_t mx_tiles(const GroupedArgs& g, int bm) {
+  return (g.rows / bm + std::min<int64_t>(g.groups + 2, g.rows)) * g.tiles_n;
+}
+
+static int mx_grid(int64_t tiles, unsigned* grid) {
+  TRNBLAS_CHECK_ARG(tiles < ((int64_t)1 << 31) - 4096, "%s: too many tiles", kMxGemm);
   *grid = (unsigned)((tiles + kNumXcd - 1) / kNumXcd * kNumXcd);
   return TRNBLAS_OK;
 }
@@ -187,7 +191,7 @@ static int run_ring(GroupedArgs g, const MxScales& x, hipStream_t s) {
   constexpr int BM = 32 * FM, BN = 32 * FN;
   g.tiles_n = (g.N + BN - 1) / BN;
   unsigned grid;
-  if (int rc = mx_grid(g, BM, &grid)) return rc;
+  if (int rc = mx_grid(ring_grid<FM, FN>(g, mx_tiles(g, BM)), &grid)) return rc;
   hipLaunchKernelGGL((ring_kernel<fp4x2, FM, FN, true, false>), dim3(grid), dim3(256), 0, s, g, x);
   return check_launch(kMxGemm);
 }
@@ -197,7 +201,7 @@ static int run_rows(GroupedArgs g, const MxScales& x, hipStream_t s) {
   constexpr int BN = 128 / KS;
   g.tiles_n = (g.N + BN - 1) / BN;
   unsigned grid;
-  if (int rc = mx_grid(g, 16 * MF, &grid)) return rc;
+  if (int rc = mx_grid(mx_tiles(g, 16 * MF), &grid)) return rc;
   hipLaunchKernelGGL((rows_kernel<fp4x2, MF, 1, KS, true, X>), dim3(grid), dim3(512), 0, s, g, x);
   return check_launch(kMxGemm);
 }

@@ -145,22 +145,27 @@ struct PanelDma {
 // Scales (fp4x2): a dword per row and block-of-four serves four steps. They come
 // by DMA too, whole chunks, two groups of four steps ahead, into a ring of two: a group is in registers before its slot is filled again.
 // The rows of a tile start anywhere in a chunk, so A's take one chunk more.
+// The sizes of a tile's LDS.
+template <typename T, int FM, int FN>
+struct RingLds {
+  static constexpr int BM = 32 * FM, BN = 32 * FN, NS = 2, STAGE = 128 * (BM + BN);
+  static constexpr int SA = BM / 64 + 1, SB = BN / 64;  // scale DMAs of a group: four chunks each
+  static constexpr int SGROUP = std::is_same_v<T, fp4x2> ? 1024 * (SA + SB) : 0, SRING = 2;
+  static constexpr int BYTES = NS * STAGE + SRING * SGROUP;
+};
+
 template <typename T, int FM, int FN, bool BKC, bool RK>
-__global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(GroupedArgs g, MxScales x) {
+__device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& x, const TileJob& j, char* lds) {
   constexpr bool MX = std::is_same_v<T, fp4x2>, FOLD = std::is_same_v<T, float>;
-  constexpr int WAVES = 4, BM = 32 * FM, BN = 32 * FN, NS = 2;
+  using L = RingLds<T, FM, FN>;
+  constexpr int WAVES = 4, BM = L::BM, BN = L::BN, NS = L::NS, SA = L::SA, SB = L::SB, SGROUP = L::SGROUP, SRING = L::SRING;
   using DA = PanelDma<T, BM, !RK, WAVES>;
   using DB = PanelDma<T, BN, BKC, WAVES>;
   using PA = typename DA::P;
   using PB = typename DB::P;
-  constexpr int STAGE = PA::BYTES + PB::BYTES;
-  constexpr int ND = DA::NB + DB::NB;                              // DMAs per wave and k-tile, besides scales
-  constexpr int SA = BM / 64 + 1, SB = BN / 64;                    // scale DMAs of a group: four chunks each
-  constexpr int SGROUP = MX ? 1024 * (SA + SB) : 0, SRING = 2;
-  static_assert(SA + SB <= 16, "one scale DMA per wave and step");
-  __shared__ __attribute__((aligned(16))) char lds[NS * STAGE + SRING * SGROUP];
-  TileJob j;
-  if (!tile_job<T, BM, BN, BKC, RK>(g, j)) return;
+  constexpr int STAGE = L::STAGE;
+  constexpr int ND = DA::NB + DB::NB;  // DMAs per wave and k-tile, besides scales
+  static_assert(STAGE == PA::BYTES + PB::BYTES && SA + SB <= 16, "one scale DMA per wave and step");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m0 = (wave & 1) * (16 * FM), n0 = (wave >> 1) * (16 * FN);
@@ -170,9 +175,6 @@ __global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(Groupe
   DB db;
   da.init(j.A, g.lda, j.rows_a, wave, lane);
   db.init(j.B, g.ldb, j.rows_b, wave, lane);
-  uint32_t oa[PA::NV], ob[PB::NV];
-  PA::lane_offsets(m0, lane, oa);
-  PB::lane_offsets(n0, lane, ob);
   i32x4 ra, rb;
   uint32_t sta, stb;  // LDS offsets of the wave's blocks in the stage that takes the DMA
   // k-tile kt is the next to move, into stage kt % NS
@@ -243,12 +245,22 @@ __global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(Groupe
   };
   i32x4 fa[2][FM], fb[2][FN];
   const char *pa[PA::NV], *pb[PB::NV];
+  {
+    uint32_t oa[PA::NV], ob[PB::NV];
+    PA::lane_offsets(m0, lane, oa);
+    PB::lane_offsets(n0, lane, ob);
+#pragma unroll
+    for (int i = 0; i < PA::NV; ++i) pa[i] = lds + oa[i];
+#pragma unroll
+    for (int i = 0; i < PB::NV; ++i) pb[i] = lds + PA::BYTES + ob[i];
+  }
+  // the reads go on to the stage of k-tile kt
   auto read_from = [&](int kt) __attribute__((always_inline)) {
-    const char* st = lds + (uint32_t)kt % NS * STAGE;
+    const int d = kt & 1 ? STAGE : -STAGE;
 #pragma unroll
-    for (int i = 0; i < PA::NV; ++i) pa[i] = st + oa[i];
+    for (int i = 0; i < PA::NV; ++i) pa[i] += d;
 #pragma unroll
-    for (int i = 0; i < PB::NV; ++i) pb[i] = st + PA::BYTES + ob[i];
+    for (int i = 0; i < PB::NV; ++i) pb[i] += d;
   };
   auto read = [&](int i, int set) __attribute__((always_inline)) {
     if (i < FN)
@@ -322,7 +334,6 @@ __global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(Groupe
     }
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(ND) : "memory");
     read_scales(0);
-    read_from(0);
 #pragma unroll
     for (int i = 0; i < FN + FM; ++i) read(i, 0);
     if constexpr (FOLD) chain = span = 2 * chain_length(j.K, 4) / PA::BK;
@@ -340,12 +351,38 @@ __global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(Groupe
       for (int b = 0; b < FN; ++b) acc[a][b] += sum[a][b];
   }
   using O = std::conditional_t<MX, __bf16, T>;
+  static_assert(4 * kStoreLds<FN> <= L::BYTES);
+  char* own = lds + wave * kStoreLds<FN>;
+  if (!(g.vec4 && (g.N & 3) == 0)) __syncthreads();  // the other waves' reads
   if (g.out32)
-    store_wave<FM, FN, float>(g, j, acc, m0, n0, lane);
+    store_wave<FM, FN, float>(g, j, acc, m0, n0, lane, own);
   else if (MX && g.out_f16)
-    store_wave<FM, FN, _Float16>(g, j, acc, m0, n0, lane);
+    store_wave<FM, FN, _Float16>(g, j, acc, m0, n0, lane, own);
   else
-    store_wave<FM, FN, O>(g, j, acc, m0, n0, lane);
+    store_wave<FM, FN, O>(g, j, acc, m0, n0, lane, own);
+}
+
+template <typename T, int FM, int FN, bool BKC, bool RK>
+__global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(GroupedArgs g, MxScales x) {
+  constexpr bool SPLIT = FM * FN == 64;  // one workgroup per CU: see tile_of
+  __shared__ __attribute__((aligned(16))) char lds[RingLds<T, FM, FN>::BYTES];
+  TileJob j;
+  if (!tile_job<T, 32 * FM, 32 * FN, BKC, RK, SPLIT>(g, j)) return;
+  if constexpr (SPLIT) {
+    if (j.quarter >= 0) {
+      ring_tile<T, FM / 2, FN / 2, BKC, RK>(g, x, j, lds);
+      return;
+    }
+  }
+  ring_tile<T, FM, FN, BKC, RK>(g, x, j, lds);
+}
+
+// Workgroups of such a launch over `tiles` tiles (or at most so many), SPLIT's
+// quarters included.
+template <int FM, int FN>
+static int64_t ring_grid(GroupedArgs& g, int64_t tiles) {
+  g.slots = device_cus();
+  return (tiles + (FM * FN == 64 ? 9 * g.slots / 4 + 2 * kNumXcd : 0) + kNumXcd - 1) / kNumXcd * kNumXcd;
 }
 
 }  // namespace trnblas
