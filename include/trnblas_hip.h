@@ -645,6 +645,15 @@ int trnblas_hip_mx_gemm_from(int dtype, int out_dtype, int64_t groups, int64_t r
                              int offsets64, double beta, const void* C, int64_t ldc, void* D,
                              int64_t ldd, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * The name of the kernel that trnblas_hip_grouped_gemm (op 0), grouped_rank_k (op 1;
+ * M x N per group) or mx_gemm (op 2; dtype and transB unused) launches for
+ * back-to-back 16-byte aligned operands of these sizes, or NULL with the last error
+ * set. Launches nothing and needs no GPU (256 CUs are assumed without one).
+ */
+const char* trnblas_hip_grouped_plan(int op, int dtype, int transB, int64_t groups, int64_t rows,
+                                     int64_t M, int64_t N, int64_t K);
+
 #ifdef __cplusplus
 }
 #endif

@@ -65,3 +65,19 @@ def excess(D, ref, den, k):
     bound = (k + 2) * 2.0**-23 * den
     bound = bound + u * (ref.abs() + bound) + tiny
     return float(((D.detach().double().cpu() - ref).abs() / bound).max()) if D.numel() else 0.0
+
+
+def plan(op, dtype, transB, groups, rows, M, N, K):
+    from trnblas_amd.hip import _lib
+
+    return _lib.load().trnblas_hip_grouped_plan(op, _lib.DTYPE_CODES[dtype], transB, groups, rows, M, N, K).decode()
+
+
+def uneven(groups, rows, seed):
+    """Offsets of `groups` uneven groups, one of them empty where there are several, some rows of no group."""
+    g = torch.Generator().manual_seed(seed)
+    w = torch.rand(groups, generator=g) + 0.2
+    if groups > 2:
+        w[1] = 0
+    sizes = (w / w.sum() * (rows - 3)).long()
+    return split(rows, sizes.tolist(), 2)

@@ -7,7 +7,9 @@ import torch
 import trnblas_amd as tb
 from oracle import grouped as og
 from oracle.grouped import GROUPS
+from oracle.grouped import plan as _plan
 from oracle.grouped import split as _split
+from oracle.grouped import uneven as _uneven
 
 pytestmark = pytest.mark.gpu
 
@@ -245,3 +247,90 @@ def test_long_rows_pass_32_bit_offsets(dev):
     W = _randn(g, 2200, 40, dtype=BF16)
     P = tb.grouped_rank_k(1.0, A, W.to(dev), off.to(dev))
     assert og.excess(P, *og.grouped_rank_k(1.0, Ah, W, off), 2100) <= 1
+
+
+# Sizes that reach each kernel: (groups, rows, K, N). 256 x 256 tiles with whole rounds and a last one in quarters, with
+# ragged ends of rows, columns and K, K of fewer values than a k-tile, and an odd number of k-tiles.
+REACH = {
+    "ring_kernel 256 x 256": [(3, 5200, 520, 2312), (1, 7000, 1160, 2568)],
+    "ring_kernel 128 x 128": [(5, 20000, 2056, 1032), (3, 2600, 1032, 1288), (5, 9000, 40, 2304)],
+    "ring_kernel 64 x 128": [(8, 1500, 264, 1032), (8, 900, 520, 264), (3, 500, 72, 1032)],
+    "rows_kernel": [(8, 8, 1032, 520), (5, 60, 264, 136)],
+}
+
+
+def _excess_gpu(D, ref, den, k):
+    return og.excess(D.cpu(), ref.cpu(), den.cpu(), k)
+
+
+@pytest.mark.parametrize("kernel", list(REACH))
+@pytest.mark.parametrize("transB", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_each_kernel_of_grouped_gemm(dev, dtype, transB, kernel):
+    for i, (G, R, K, N) in enumerate(REACH[kernel]):
+        if dtype != F32:
+            assert _plan(0, dtype, transB, G, R, 0, N, K) == kernel
+        g = torch.Generator(device=dev).manual_seed(i)
+        off = _uneven(G, R, i)
+        A = torch.randn(R, K, generator=g, device=dev).to(dtype)
+        B = torch.randn(G, *((N, K) if transB else (K, N)), generator=g, device=dev).to(dtype)
+        C = torch.randn(R, N, generator=g, device=dev).to(dtype)
+        for beta in (0.0, 0.5):
+            D = tb.grouped_gemm(1.0, A, B, off.to(dev), beta, C, transB=transB)
+            ref = beta * C.double()
+            den = ref.abs()
+            for j, a, b in og.rows_of(off, R):
+                W = (B[j].T if transB else B[j]).double().contiguous()
+                ref[a:b] += A[a:b].double() @ W
+                den[a:b] += A[a:b].double().abs() @ W.abs()
+            assert _excess_gpu(D, ref, den, K) <= 1, (G, R, K, N, beta)
+
+
+RANK_K = {  # (groups, rows, M, N)
+    "ring_kernel 256 x 256": [(3, 9000, 2056, 2312)],
+    "ring_kernel 128 x 128": [(8, 4100, 2056, 1032), (3, 2600, 1032, 1288)],
+    "ring_kernel 64 x 128": [(8, 900, 264, 1032)],
+}
+
+
+@pytest.mark.parametrize("kernel", list(RANK_K))
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_each_kernel_of_grouped_rank_k(dev, dtype, kernel):
+    for i, (G, R, M, N) in enumerate(RANK_K[kernel]):
+        if dtype != F32:
+            assert _plan(1, dtype, 0, G, R, M, N, 0) == kernel
+        g = torch.Generator(device=dev).manual_seed(i)
+        off = _uneven(G, R, i)
+        A = torch.randn(R, M, generator=g, device=dev).to(dtype)
+        B = torch.randn(R, N, generator=g, device=dev).to(dtype)
+        C = torch.randn(G, M, N, generator=g, device=dev)
+        ref, den = torch.zeros(2, G, M, N, dtype=torch.float64, device=dev)
+        for j, a, b in og.rows_of(off, R):
+            left = A[a:b].double().T.contiguous()
+            ref[j], den[j] = left @ B[a:b].double(), left.abs() @ B[a:b].double().abs()
+        assert _excess_gpu(tb.grouped_rank_k(1.0, A, B, off.to(dev)), ref, den, R) <= 1, (G, R, M, N)
+        D = tb.grouped_rank_k(1.0, A, B, off.to(dev), 1.0, C, dtype=F32)
+        assert _excess_gpu(D, ref + C.double(), den + C.double().abs(), R) <= 1, (G, R, M, N)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_operands(dev, dtype):
+    # large operands that start or end anywhere are copied first; the results are those of aligned ones
+    G, R, K, N = 3, 4099, 1021, 2043
+    for transB in (False, True):
+        g = torch.Generator(device=dev).manual_seed(1)
+        off = _uneven(G, R, 1)
+        A = torch.randn(R, K + 3, generator=g, device=dev).to(dtype)[:, 1:-2]
+        B = torch.randn(G, *((N, K) if transB else (K, N)), generator=g, device=dev).to(dtype)
+        D = tb.grouped_gemm(1.0, A, B, off.to(dev), transB=transB)
+        dB = tb.grouped_rank_k(1.0, A, D, off.to(dev))
+        ref, den = torch.zeros(2, R, N, dtype=torch.float64, device=dev)
+        for j, a, b in og.rows_of(off, R):
+            W = (B[j].T if transB else B[j]).double().contiguous()
+            ref[a:b], den[a:b] = A[a:b].double() @ W, A[a:b].double().abs() @ W.abs()
+        assert _excess_gpu(D, ref, den, K) <= 1
+        ref, den = torch.zeros(2, G, K, N, dtype=torch.float64, device=dev)
+        for j, a, b in og.rows_of(off, R):
+            left = A[a:b].double().T.contiguous()
+            ref[j], den[j] = left @ D[a:b].double(), left.abs() @ D[a:b].double().abs()
+        assert _excess_gpu(dB, ref, den, R) <= 1

@@ -6,7 +6,7 @@ import torch
 import trnblas_amd as tb
 from oracle import grouped as og
 from oracle import mx as om
-from oracle.grouped import GROUPS
+from oracle.grouped import GROUPS, plan, uneven
 from oracle.grouped import split as _split
 from oracle.mx import wide as _wide
 
@@ -166,3 +166,46 @@ def test_scales_far_apart(dev):
                 assert 0 <= D[i, j] <= 2.0**-126
             else:
                 assert D[i, j] == (want[i, j] if want[i, j] < 2.0**128 else float("inf")), (i, j)
+
+
+MX_REACH = {
+    "ring_kernel 256 x 256": [(3, 5200, 520, 2312), (1, 7000, 1160, 2568)],
+    "ring_kernel 128 x 128": [(5, 20000, 2056, 1032)],
+    "ring_kernel 64 x 128": [(3, 2600, 1032, 1288), (8, 1500, 264, 1032), (8, 900, 520, 264), (3, 700, 1030, 520)],
+    "rows_kernel": [(8, 8, 4100, 520), (2, 20, 1030, 136)],
+}
+
+
+@pytest.mark.parametrize("kernel", list(MX_REACH))
+def test_each_kernel(dev, kernel):
+    for i, (G, R, K, N) in enumerate(MX_REACH[kernel]):
+        assert plan(2, BF16, 1, G, R, 0, N, K) == kernel
+        g = torch.Generator(device=dev).manual_seed(i)
+        off = uneven(G, R, i)
+        A = torch.randn(R, K, generator=g, device=dev) * torch.exp2(torch.arange(R, device=dev) % 7)[:, None]
+        E = tb.mx_quantize(torch.randn(G, N, K, generator=g, device=dev))
+        a, w = tb.mx_quantize(A).dequantize().double(), E.dequantize().double()
+        ref, den = torch.zeros(2, R, N, dtype=torch.float64, device=dev)
+        for j, p, q in og.rows_of(off, R):
+            W = w[j].T.contiguous()
+            ref[p:q], den[p:q] = a[p:q] @ W, a[p:q].abs() @ W.abs()
+        for out in (F32, F16 if kernel != "rows_kernel" else BF16):
+            for x in (A, tb.mx_quantize(A)):
+                D = tb.mx_grouped_gemm(1.0, x, E, off.to(dev), dtype=out)
+                assert og.excess(D.cpu(), ref.cpu(), den.cpu(), K) <= 1, (G, R, K, N, out)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K", [(1, 8192), (1, 8191), (3, 10900), (4, 8192), (16, 2048), (16, 2050), (15, 33)])
+def test_few_rows_quantised_in_place(dev, dtype, M, K):
+    g = torch.Generator().manual_seed(M)
+    A, W = _wide(g, M, K + 2, dtype=dtype)[:, 1:-1], torch.randn(200, K, generator=g)
+    A[0, K // 2] = 0.0
+    ref, den = om.product(1.0, om.quantize(A)[0], om.quantize(W)[0])
+    Q = tb.mx_quantize(W.to(dev))
+    for x in (A.to(dev), A.contiguous().to(dev)):
+        assert og.excess(tb.mx_gemm(1.0, x, Q, dtype=F32), ref, den, K) <= 1
+    A = A.clone()
+    A[M - 1, K - 1] = float("inf")
+    D = tb.mx_gemm(1.0, A.to(dev), Q, dtype=F32)
+    assert D[M - 1].isnan().all() and D[: M - 1].isfinite().all()

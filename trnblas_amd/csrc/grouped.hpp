@@ -406,4 +406,11 @@ __device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& 
   }
 }
 
+// The launches for one element type (grouped_run.hpp); bkc: B's columns are
+// K-contiguous.
+template <typename T>
+int grouped_gemm_run(const GroupedArgs& g, bool bkc, hipStream_t s);
+template <typename T>
+int grouped_rank_k_run(const GroupedArgs& g, hipStream_t s);
+
 }  // namespace trnblas

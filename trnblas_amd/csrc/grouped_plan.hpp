@@ -9,24 +9,27 @@
 
 namespace trnblas {
 
-// Times of the ring kernels (us), fitted to a sweep of 1, 8 and 64 groups of 1 ..
-// 2048 rows over matrices of 1024 x 1024, 2048 x 4096 and 4096 x 1536 (bf16 / fp4,
-// weights from HBM; within 25 % but for the smallest): a tile takes `start` and, per
-// k-tile, from `alone` (an empty GPU) to `full` (all slots taken).
+// Times of the ring kernels (us), fitted to sweeps of 1 .. 64 groups and 1 .. 16384
+// rows over matrices of 512 x 512 .. 2048 x 4096 (bf16 / fp4): a tile takes `start`
+// and, per k-tile, from `alone` (an empty GPU) to `full` (all slots taken). Of 228
+// sizes, each run on all three, the choice is the fastest within 10 % at all but 12,
+// and within 30 % at all. 256 rows, 4096 x 1024: 27.3, 27.4 and 21.4 us (64 x 128 has
+// the most tiles); 4096 rows: 62, 51 and 55; 16384 rows, 2048 x 4096: 225, 256, 316.
 struct RingCost {
   int fm, fn;      // MFMA blocks of a wave: tile 32 fm x 32 fn
   int per_cu;      // workgroups of a CU
   double start, alone, full;
 };
-constexpr RingCost kRing16[] = {{8, 8, 1, 10.0, 0.95, 1.5}, {4, 4, 2, 4.0, 0.38, 1.12}, {2, 4, 3, 4.0, 0.36, 1.06}};
-constexpr RingCost kRing4[] = {{8, 8, 1, 11.0, 1.2, 1.6}, {4, 4, 2, 6.0, 0.5, 1.12}, {2, 4, 3, 6.0, 0.41, 1.1}};
+constexpr RingCost kRing16[] = {{8, 8, 1, 10.0, 0.95, 1.5}, {4, 4, 2, 4.0, 0.38, 1.12}, {2, 4, 3, 3.3, 0.36, 1.08}};
+constexpr RingCost kRing4[] = {{8, 8, 1, 11.0, 1.2, 1.6}, {4, 4, 2, 5.5, 0.5, 1.12}, {2, 4, 3, 5.0, 0.41, 1.12}};
 
 inline double ring_time(const RingCost& c, double tiles, double k_tiles) {
   const double t = tiles / (c.per_cu * device_cus());
   // several workgroups of a CU drift apart; one runs in whole rounds, what is left of the last cut into quarters (tile_of)
   const double part = t - std::floor(t);
+  if (c.per_cu == 1 && t <= 0.75) return 1e30;  // nothing but quarters: the 128 x 128 kernel's tiles, one per CU
   const double rounds = c.per_cu > 1 ? std::max(1.0, t <= 1.0 ? 1.0 : t + 0.3)
-                                     : std::floor(t) + (part > 0.75 ? 1.0 : 0.36 * std::ceil(4.0 * part));
+                                     : std::floor(t) + (part > 0.75 ? 1.0 : 0.45 * std::ceil(4.0 * part));
   return rounds * (c.start + k_tiles * (c.alone + (c.full - c.alone) * std::min(1.0, t)));
 }
 
@@ -64,7 +67,7 @@ inline GroupedChoice choose_grouped(const RingCost (&ring)[3], double rows, doub
     const RingCost& c = ring[i];
     const double t = std::max(3.0 + weights / 4.6e6,
                               ring_time(c, likely_row_tiles(rows, groups, 32 * c.fm) * std::ceil(N / (32 * c.fn)), nk));
-    if (t < time * (i == 2 ? 0.97 : 1.0)) {
+    if (t < time) {
       time = t;
       best.ring = i;
     }
@@ -79,7 +82,7 @@ inline int choose_rank_k(double groups, double M, double N, double k_tiles) {
   for (int i = 0; i < 3; ++i) {
     const RingCost& c = kRing16[i];
     const double t = ring_time(c, groups * std::ceil(M / (32 * c.fm)) * std::ceil(N / (32 * c.fn)), k_tiles + 0.5);
-    if (t < time * (i == 2 ? 0.97 : 1.0)) {
+    if (t < time) {
       time = t;
       best = i;
     }

@@ -1,0 +1,240 @@
+// The launches of the grouped products for one element type, and their kernel for
+// operands of any alignment; grouped_f32.hip, grouped_bf16.hip and grouped_f16.hip
+// compile them side by side.
+#pragma once
+
+#include <algorithm>
+
+#include "gemm.hpp"
+#include "grouped.hpp"
+#include "grouped_plan.hpp"
+#include "ring.hpp"
+#include "rows.hpp"
+
+namespace trnblas {
+
+// Operands of any alignment and any strides: the panels go through registers.
+// 256 threads on a 64 x 64 tile, each wave 32 x 32; the loads of k-tile t + 2 are in
+// flight behind the MFMAs of t. fp32 sums restart every chain_length(K) values of k
+// (gemm.hpp). Bound by the loads of rows that start anywhere (16 bytes two bytes past
+// a word take several times as long; the five words around them, shifted, longer
+// still): bf16 4093 rows in 8 groups by 1023 x 2047 77 us (223 TFLOP/s; transposed
+// 101), fp32 4093 by 2047^2 395 us (87); larger products are packed first.
+template <typename T, bool BKC, bool RK>
+__global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
+  constexpr int FM = 2, FN = 2, BM = 32 * FM, BN = 32 * FN, AHEAD = 2;
+  using PA = Panel<T, BM, !RK>;
+  using PB = Panel<T, BN, BKC>;
+  constexpr int BK = PA::BK, ES = sizeof(T), HA = PA::BYTES / 4096, HB = PB::BYTES / 4096;
+  constexpr bool FOLD = std::is_same_v<T, float>;
+  __shared__ __attribute__((aligned(16))) char lds[2][PA::BYTES + PB::BYTES];
+  TileJob j;
+  if (!tile_job<T, BM, BN, BKC, RK>(g, j)) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m0 = 16 * FM * (wave & 1), n0 = 16 * FN * (wave >> 1);
+  int ra[HA], ka[HA], rb[HB], kb[HB];
+  const char *pa[HA], *pb[HB];
+#pragma unroll
+  for (int h = 0; h < HA; ++h) {
+    PA::where(tid + 256 * h, ra[h], ka[h]);
+    pa[h] = j.A + (RK ? (int64_t)ka[h] * g.lda + ra[h] : (int64_t)ra[h] * g.lda + ka[h]) * ES;
+  }
+#pragma unroll
+  for (int h = 0; h < HB; ++h) {
+    PB::where(tid + 256 * h, rb[h], kb[h]);
+    pb[h] = j.B + (BKC ? (int64_t)rb[h] * g.ldb + kb[h] : (int64_t)kb[h] * g.ldb + rb[h]) * ES;
+  }
+  const int64_t step_a = (RK ? BK * g.lda : BK) * ES, step_b = (BKC ? BK : BK * g.ldb) * ES;
+  const int nk = (j.K + BK - 1) / BK;
+  i32x4 va[AHEAD][HA], vb[AHEAD][HB];
+  auto load = [&](int kt, int set) __attribute__((always_inline)) {
+    const int left = j.K - kt * BK;
+#pragma unroll
+    for (int h = 0; h < HA; ++h)
+      va[set][h] = load_any<T>(pa[h] + kt * step_a, RK ? (ka[h] < left ? j.rows_a - ra[h] : 0) : (ra[h] < j.rows_a ? left - ka[h] : 0));
+#pragma unroll
+    for (int h = 0; h < HB; ++h)
+      vb[set][h] = load_any<T>(pb[h] + kt * step_b, BKC ? (rb[h] < j.rows_b ? left - kb[h] : 0) : (kb[h] < left ? j.rows_b - rb[h] : 0));
+  };
+  uint32_t oa[PA::NV], ob[PB::NV];
+  PA::lane_offsets(m0, lane, oa);
+  PB::lane_offsets(n0, lane, ob);
+  f32x4 acc[FM][FN], sum[FOLD ? FM : 1][FOLD ? FN : 1];
+#pragma unroll
+  for (int a = 0; a < FM; ++a)
+#pragma unroll
+    for (int b = 0; b < FN; ++b) {
+      acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (FOLD) sum[a][b] = acc[a][b];
+    }
+  const int span = chain_length(j.K, ES) / BK;
+  int chain = span;
+  auto k_tile = [&](int kt, int set) __attribute__((always_inline)) {
+    char* st = lds[kt & 1];
+#pragma unroll
+    for (int h = 0; h < HA; ++h) *reinterpret_cast<i32x4*>(st + 16 * (tid + 256 * h)) = va[set][h];
+#pragma unroll
+    for (int h = 0; h < HB; ++h) *reinterpret_cast<i32x4*>(st + PA::BYTES + 16 * (tid + 256 * h)) = vb[set][h];
+    // one barrier per k-tile: stage t's readers are past it before t + 2 is stored
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kt + AHEAD < nk) load(kt + AHEAD, set);
+    const char *qa[PA::NV], *qb[PB::NV];
+#pragma unroll
+    for (int i = 0; i < PA::NV; ++i) qa[i] = st + oa[i];
+#pragma unroll
+    for (int i = 0; i < PB::NV; ++i) qb[i] = st + PA::BYTES + ob[i];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      i32x4 fa[FM], fb[FN];
+#pragma unroll
+      for (int a = 0; a < FM; ++a) fa[a] = PA::frag(qa, a, h);
+#pragma unroll
+      for (int b = 0; b < FN; ++b) fb[b] = PB::frag(qb, b, h);
+#pragma unroll
+      for (int b = 0; b < FN; ++b)
+#pragma unroll
+        for (int a = 0; a < FM; ++a) mma_tile<T>(acc[a][b], fb[b], fa[a]);
+    }
+    if constexpr (FOLD) {
+      if (--chain == 0) {
+#pragma unroll
+        for (int a = 0; a < FM; ++a)
+#pragma unroll
+          for (int b = 0; b < FN; ++b) {
+            sum[a][b] += acc[a][b];
+            acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          }
+        chain = span;
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (i < nk) load(i, i);
+  for (int kt = 0; kt < nk; kt += AHEAD) {
+    k_tile(kt, 0);
+    if (kt + 1 < nk) k_tile(kt + 1, 1);
+  }
+  if constexpr (FOLD) {
+#pragma unroll
+    for (int a = 0; a < FM; ++a)
+#pragma unroll
+      for (int b = 0; b < FN; ++b) acc[a][b] += sum[a][b];
+  }
+  static_assert(4 * kStoreLds<FN> <= sizeof(lds));
+  char* own = lds[0] + wave * kStoreLds<FN>;
+  __syncthreads();  // the other waves' reads
+  if (g.out32)
+    store_wave<FM, FN, float>(g, j, acc, m0, n0, lane, own);
+  else
+    store_wave<FM, FN, T>(g, j, acc, m0, n0, lane, own);
+}
+
+static const char* const kGemm = "trnblas_hip_grouped_gemm";
+static const char* const kRankK = "trnblas_hip_grouped_rank_k";
+
+// Bound on the row tiles of `rows` rows in `groups` groups and the two gaps.
+static int64_t row_tiles(int64_t rows, int64_t groups, int bm) { return rows / bm + std::min(groups + 2, rows); }
+
+static int grid_of(int64_t tiles, const char* what, unsigned* grid) {
+  TRNBLAS_CHECK_ARG(tiles < ((int64_t)1 << 31) - 4096, "%s: too many tiles", what);
+  *grid = (unsigned)tiles;
+  return TRNBLAS_OK;
+}
+
+template <typename T, bool BKC, bool RK>
+static int run_any(GroupedArgs g, hipStream_t s) {
+  constexpr int BM = 64;
+  const char* what = RK ? kRankK : kGemm;
+  g.tiles_m = (g.M + BM - 1) / BM;
+  g.tiles_n = (g.N + BM - 1) / BM;
+  unsigned grid;
+  const int64_t rows = RK ? (int64_t)g.groups * g.tiles_m : row_tiles(g.rows, g.groups, BM);
+  if (int rc = grid_of(rows * g.tiles_n, what, &grid)) return rc;
+  // whole rounds of the XCDs, so that each one's last tile is reached
+  grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
+  hipLaunchKernelGGL((grouped_any_kernel<T, BKC, RK>), dim3(grid), dim3(256), 0, s, g);
+  return check_launch(what);
+}
+
+// Operands that LDS DMA reads in place: see ring.hpp. Whole groups of 16 bytes
+// lie inside the operands, or (g.padded) are zeros past their ends. Its 32-bit
+// offsets reach over one panel of a K-contiguous operand and one k-tile of the
+// other kind.
+template <typename T>
+static bool dma_ready(const GroupedArgs& g, bool bkc, bool rk) {
+  const int64_t es = sizeof(T), far = INT32_MAX - 1024;
+  auto whole = [&](const void* p, int64_t ld, int64_t st, int64_t ext) {
+    return (uintptr_t)p % 16 == 0 && ld * es % 16 == 0 && st * es % 16 == 0 && (g.padded || ext * es % 16 == 0);
+  };
+  const int64_t ra = rk ? 128 / es : 256, rb = bkc ? 256 : 128 / es;
+  return whole(g.A, g.lda, 0, rk ? g.M : g.K) && whole(g.B, g.ldb, g.sB, bkc ? g.K : g.N) && (!rk || g.rows < far) &&
+         ra * g.lda * es < far && rb * g.ldb * es < far;
+}
+
+template <typename T, int FM, int FN, bool BKC, bool RK>
+static int run_ring(GroupedArgs g, hipStream_t s) {
+  constexpr int BM = 32 * FM, BN = 32 * FN;
+  const char* what = RK ? kRankK : kGemm;
+  g.tiles_m = (g.M + BM - 1) / BM;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  unsigned grid;
+  const int64_t rows = RK ? (int64_t)g.groups * g.tiles_m : row_tiles(g.rows, g.groups, BM);
+  if (int rc = grid_of(ring_grid<FM, FN>(g, rows * g.tiles_n), what, &grid)) return rc;
+  hipLaunchKernelGGL((ring_kernel<T, FM, FN, BKC, RK>), dim3(grid), dim3(256), 0, s, g, MxScales{});
+  return check_launch(what);
+}
+
+template <typename T, int MF, int NF, int KS, bool BKC>
+static int run_rows(GroupedArgs g, hipStream_t s) {
+  constexpr int BN = 128 * NF / KS;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  unsigned grid;
+  if (int rc = grid_of(row_tiles(g.rows, g.groups, 16 * MF) * g.tiles_n, kGemm, &grid)) return rc;
+  grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
+  hipLaunchKernelGGL((rows_kernel<T, MF, NF, KS, BKC>), dim3(grid), dim3(512), 0, s, g, MxScales{});
+  return check_launch(kGemm);
+}
+
+template <typename T, int MF, bool BKC>
+static int run_rows_split(int ks, const GroupedArgs& g, hipStream_t s) {
+  constexpr int NF = BKC ? 1 : 4;
+  return ks == 8   ? run_rows<T, MF, NF, 8, BKC>(g, s)
+         : ks == 4 ? run_rows<T, MF, NF, 4, BKC>(g, s)
+         : ks == 2 ? run_rows<T, MF, NF, 2, BKC>(g, s)
+                   : run_rows<T, MF, NF, 1, BKC>(g, s);
+}
+
+// ring: index of kRing16. fp32 always takes the 64 x 128 tiles: three workgroups
+// per CU hide its longer MFMAs' steps best (8 groups of 128 rows, 2048 x 4096: 217 us
+// against 220 on 128 x 128 and 267 on grouped_any_kernel).
+template <typename T, bool BKC, bool RK>
+static int run_ring_choice(int ring, const GroupedArgs& g, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (ring == 0) return run_ring<T, 8, 8, BKC, RK>(g, s);
+    if (ring == 1) return run_ring<T, 4, 4, BKC, RK>(g, s);
+  }
+  return run_ring<T, 2, 4, BKC, RK>(g, s);
+}
+
+template <typename T, bool BKC>
+static int run_grouped(const GroupedArgs& g, hipStream_t s) {
+  const bool ready = dma_ready<T>(g, BKC, false);
+  const GroupedChoice c = choose_grouped(kRing16, g.rows, g.groups, g.N, g.K, (double)g.K * sizeof(T), sizeof(T), BKC);
+  if (c.ring < 0) return c.mf == 1 ? run_rows_split<T, 1, BKC>(c.ks, g, s) : run_rows_split<T, 2, BKC>(c.ks, g, s);
+  return ready ? run_ring_choice<T, BKC, false>(c.ring, g, s) : run_any<T, BKC, false>(g, s);
+}
+
+template <typename T>
+int grouped_gemm_run(const GroupedArgs& g, bool bkc, hipStream_t s) {
+  return bkc ? run_grouped<T, true>(g, s) : run_grouped<T, false>(g, s);
+}
+
+template <typename T>
+int grouped_rank_k_run(const GroupedArgs& g, hipStream_t s) {
+  if (!dma_ready<T>(g, false, true)) return run_any<T, false, true>(g, s);
+  return run_ring_choice<T, false, true>(choose_rank_k(g.groups, g.M, g.N, (double)g.rows / g.groups * sizeof(T) / 128.0), g, s);
+}
+
+}  // namespace trnblas

@@ -182,6 +182,7 @@ SIGNATURES = {
         [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_dbl, _c_ptr, _c_i64, _c_i64, _c_ptr]
         + [_c_ptr, _c_ptr, _c_int, _c_dbl, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_size, _c_ptr],
     ),
+    "trnblas_hip_grouped_plan": (ctypes.c_char_p, [_c_int, _c_int, _c_int] + [_c_i64] * 5),
     "trnblas_hip_dgemm": (
         _c_int,
         [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_dbl]
