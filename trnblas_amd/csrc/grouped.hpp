@@ -362,6 +362,34 @@ __device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& 
       }
       __builtin_amdgcn_sched_barrier(0);  // a row's registers at a time
     };
+    // 16-bit rows that start on 16 bytes: lanes 16 apart exchange halves of two
+    // blocks, so that a lane stores 16 bytes and a row 64 at a time (8 and 32: 8192 x
+    // 2048 x 8192 237 us, now 223; 8191 x 2056 x 4104 of 4-bit values 88, now 82)
+    if constexpr (sizeof(O) == 2) {
+      if (g.beta == 0.0f && (((uint64_t)D / 2 | (uint64_t)g.ldd | (uint64_t)g.N) & 7) == 0) {
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        auto pack = [&](int a, int b) __attribute__((always_inline)) {
+          const f32x4 v = take(a, b) * g.alpha;
+          return __builtin_bit_cast(i32x2, o4{(O)v[0], (O)v[1], (O)v[2], (O)v[3]});
+        };
+        const int lg = lane >> 4, col = j.n + n0 + 16 * (lg & 1) + 8 * (lg >> 1);
+#pragma unroll
+        for (int a = 0; a < FM; ++a) {
+          const int m = m0 + 16 * a + li;
+          O* d = D + (j.m + m) * g.ldd + col;
+#pragma unroll
+          for (int b = 0; b < FN; b += 2) {
+            const i32x2 x = pack(a, b), y = pack(a, b + 1);
+            const auto p = __builtin_amdgcn_permlane16_swap(x[0], y[0], false, false);
+            const auto q = __builtin_amdgcn_permlane16_swap(x[1], y[1], false, false);
+            if (m < j.rows_a && col + 16 * b < g.N)
+              *reinterpret_cast<i32x4*>(d + 16 * b) = i32x4{(int)p[0], (int)q[0], (int)p[1], (int)q[1]};
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        return;
+      }
+    }
     if (g.beta == 0.0f) {
 #pragma unroll
       for (int a = 0; a < FM; ++a) store(a, [&](int p, int b) __attribute__((always_inline)) { return take(p, b) * g.alpha; });
