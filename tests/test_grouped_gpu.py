@@ -334,3 +334,27 @@ def test_packed_operands(dev, dtype):
             left = A[a:b].double().T.contiguous()
             ref[j], den[j] = left @ D[a:b].double(), left.abs() @ D[a:b].double().abs()
         assert _excess_gpu(dB, ref, den, R) <= 1
+
+
+def _amid_nans(x, left):
+    """x as a view of a larger buffer of NaNs, its rows starting anywhere."""
+    buf = torch.full((*x.shape[:-2], x.shape[-2] + 2, x.shape[-1] + left + 3), float("nan"), dtype=x.dtype, device=x.device)
+    view = buf[..., 1:-1, left : left + x.shape[-1]]
+    return view.copy_(x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N", [(1, 3), (3, 4), (4, 7), (5, 8), (7, 9), (8, 65), (9, 1), (31, 66), (33, 5), (64, 129), (65, 71)])
+def test_extents_near_16_bytes_amid_nans(dev, dtype, K, N):
+    # rows shorter than, equal to and just past 16 bytes; nothing from outside an operand reaches a sum
+    G, R = 2, 213
+    g = torch.Generator(device=dev).manual_seed(K)
+    off = torch.tensor([1, 70, 211])
+    A = torch.randn(R, K, generator=g, device=dev).to(dtype)
+    dD = torch.randn(R, N, generator=g, device=dev).to(dtype)
+    for transB in (False, True):
+        B = torch.randn(G, *((N, K) if transB else (K, N)), generator=g, device=dev).to(dtype)
+        D = tb.grouped_gemm(1.0, _amid_nans(A, 1), _amid_nans(B, 3), off.to(dev), transB=transB)
+        assert og.excess(D.cpu(), *og.grouped_gemm(1.0, A.cpu(), (B.mT if transB else B).cpu(), off), K) <= 1
+    P = tb.grouped_rank_k(1.0, _amid_nans(A, 1), _amid_nans(dD, 3), off.to(dev))
+    assert og.excess(P.cpu(), *og.grouped_rank_k(1.0, A.cpu(), dD.cpu(), off), R) <= 1

@@ -13,16 +13,107 @@
 
 namespace trnblas {
 
+// 16 bytes of values ending at a row's end, loaded in the place of n values that start
+// that much later: moved down, zeros behind them (n <= 0: zeros).
+template <typename T>
+__device__ __forceinline__ i32x4 end_of_row(i32x4 v, int n) {
+  constexpr int EV = 16 / sizeof(T);
+  const int s = (EV - n) * (int)sizeof(T);  // bytes
+  if (s & 8) v = i32x4{v[2], v[3], 0, 0};
+  if (s & 4) v = i32x4{v[1], v[2], v[3], 0};
+  if constexpr (sizeof(T) == 2) {
+    if (s & 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (int)__builtin_amdgcn_alignbit(i < 3 ? v[i + 1] : 0, v[i], 16);
+    }
+  }
+  return n > 0 ? v : i32x4{0, 0, 0, 0};
+}
+
+// One operand's loads of a k-tile, 16 bytes per lane and 256 groups, in Panel's order:
+// with no branch, so that those of two k-tiles stay under way. Of a group that passes
+// its row's end the row's last 16 bytes are loaded and moved down behind a uniform
+// branch (put); what lies outside is loaded from some place inside and stored as zeros
+// (rows of a K-contiguous operand past the tile's end: as they are, their sums are not
+// stored). TINY: rows shorter than 16 bytes, one value at a time.
+template <typename T, int ROWS, bool KC, bool TINY>
+struct Loads {
+  using P = Panel<T, ROWS, KC>;
+  static constexpr int ES = sizeof(T), EV = 16 / ES, BK = P::BK, H = P::BYTES / 4096;
+  const char* p[H];   // KC: the row's start; else the group's of the first k-tile
+  const char* first;  // the first row's first values
+  int64_t step;       // bytes per k-tile
+  int K, at, inside;  // KC: the group's k; else its first k (16-byte groups h: k_of), values inside
+  int slot;
+  bool edge;          // the tile passes the rows' end
+
+  // base: the panel's corner, `before` values after its row's start
+  __device__ __forceinline__ Loads(const char* base, int64_t before, int64_t ld, int rows, int k, int tid) : K(k) {
+    first = base - before * ES;
+    slot = 16 * tid;
+    edge = !KC && rows < ROWS;
+    step = (KC ? BK : BK * ld) * ES;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      int r, q;
+      P::where(tid + 256 * h, r, q);  // the same q (KC) or r for all h
+      if constexpr (KC) {
+        at = q;
+        inside = r < rows;
+        p[h] = base + (TINY ? r : min(r, rows - 1)) * ld * ES;
+        if constexpr (TINY) inside = rows;
+      } else {
+        if (h == 0) at = q;
+        inside = rows - r;
+        p[h] = (TINY || inside >= EV ? base + r * ES : inside > 0 ? base + (rows - EV) * ES : first) + q * ld * ES;
+      }
+    }
+  }
+  static __device__ __forceinline__ int k_of(int h) { return h * (256 / P::GPR); }
+  __device__ __forceinline__ void load(int kt, i32x4 (&v)[H]) const {
+    const int left = K - kt * BK;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      if constexpr (TINY && KC)
+        v[h] = load_any<T>(p[h] + kt * step + at * ES, (slot >> 7) + 32 * h < inside ? left - at : 0);
+      else if constexpr (TINY)
+        v[h] = load_any<T>(p[h] + kt * step, at + k_of(h) < left ? inside : 0);
+      else if constexpr (KC)
+        v[h] = load16<T>(p[h] + (int64_t)min(kt * BK + at, K - EV) * ES);
+      else
+        v[h] = load16<T>(at + k_of(h) < left ? p[h] + kt * step : first);
+    }
+  }
+  __device__ __forceinline__ void put(char* st, int kt, i32x4 (&v)[H]) const {
+    const int left = K - kt * BK;
+    if (!TINY && (left < BK || edge)) {
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const int n = KC ? left - at : at + k_of(h) < left ? inside : 0;
+        v[h] = n < EV ? end_of_row<T>(v[h], n) : v[h];
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < H; ++h) *reinterpret_cast<i32x4*>(st + slot + 4096 * h) = v[h];
+  }
+};
+
 // Operands of any alignment and any strides: the panels go through registers.
 // 256 threads on a 64 x 64 tile, each wave 32 x 32; the loads of k-tile t + 2 are in
 // flight behind the MFMAs of t. fp32 sums restart every chain_length(K) values of k
-// (gemm.hpp). Bound by the loads of rows that start anywhere (16 bytes two bytes past
-// a word take several times as long; the five words around them, shifted, longer
-// still): bf16 4093 rows in 8 groups by 1023 x 2047 77 us (223 TFLOP/s; transposed
-// 101), fp32 4093 by 2047^2 395 us (87); larger products are packed first.
-template <typename T, bool BKC, bool RK>
+// (gemm.hpp). fp32 gemm takes 32 x 64: its MFMAs are eight times as long, so that the
+// last round's idle CUs cost more than the smaller tile's loads (1501 rows in 6 groups
+// by 515 x 771: 360 tiles 31 us, 720 tiles 27; 4093 by 2047^2 385 and 393). 16-bit:
+// bound by the loads of rows that start anywhere (16 bytes two bytes past a word take
+// several times as long; the five words around them, shifted, longer still): bf16 4093
+// rows in 8 groups by 1023 x 2047 61 us (281 TFLOP/s), 16383 by 2047 x 4095 678 (405);
+// 512 rows in 16 groups by 1023 x 2047 21 us, 64 when each load was a branch whose
+// merge waited for all loads. Larger products are packed first.
+template <typename T, bool RK>
+constexpr int any_fm = std::is_same_v<T, float> && !RK ? 1 : 2;
+template <typename T, bool BKC, bool RK, bool TINY>
 __global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
-  constexpr int FM = 2, FN = 2, BM = 32 * FM, BN = 32 * FN, AHEAD = 2;
+  constexpr int FM = any_fm<T, RK>, FN = 2, BM = 32 * FM, BN = 32 * FN, AHEAD = 2;
   using PA = Panel<T, BM, !RK>;
   using PB = Panel<T, BN, BKC>;
   constexpr int BK = PA::BK, ES = sizeof(T), HA = PA::BYTES / 4096, HB = PB::BYTES / 4096;
@@ -33,30 +124,10 @@ __global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m0 = 16 * FM * (wave & 1), n0 = 16 * FN * (wave >> 1);
-  int ra[HA], ka[HA], rb[HB], kb[HB];
-  const char *pa[HA], *pb[HB];
-#pragma unroll
-  for (int h = 0; h < HA; ++h) {
-    PA::where(tid + 256 * h, ra[h], ka[h]);
-    pa[h] = j.A + (RK ? (int64_t)ka[h] * g.lda + ra[h] : (int64_t)ra[h] * g.lda + ka[h]) * ES;
-  }
-#pragma unroll
-  for (int h = 0; h < HB; ++h) {
-    PB::where(tid + 256 * h, rb[h], kb[h]);
-    pb[h] = j.B + (BKC ? (int64_t)rb[h] * g.ldb + kb[h] : (int64_t)kb[h] * g.ldb + rb[h]) * ES;
-  }
-  const int64_t step_a = (RK ? BK * g.lda : BK) * ES, step_b = (BKC ? BK : BK * g.ldb) * ES;
   const int nk = (j.K + BK - 1) / BK;
+  Loads<T, BM, !RK, TINY> la(j.A, RK ? j.m : 0, g.lda, j.rows_a, j.K, tid);
+  Loads<T, BN, BKC, TINY> lb(j.B, BKC ? 0 : j.n, g.ldb, j.rows_b, j.K, tid);
   i32x4 va[AHEAD][HA], vb[AHEAD][HB];
-  auto load = [&](int kt, int set) __attribute__((always_inline)) {
-    const int left = j.K - kt * BK;
-#pragma unroll
-    for (int h = 0; h < HA; ++h)
-      va[set][h] = load_any<T>(pa[h] + kt * step_a, RK ? (ka[h] < left ? j.rows_a - ra[h] : 0) : (ra[h] < j.rows_a ? left - ka[h] : 0));
-#pragma unroll
-    for (int h = 0; h < HB; ++h)
-      vb[set][h] = load_any<T>(pb[h] + kt * step_b, BKC ? (rb[h] < j.rows_b ? left - kb[h] : 0) : (kb[h] < left ? j.rows_b - rb[h] : 0));
-  };
   uint32_t oa[PA::NV], ob[PB::NV];
   PA::lane_offsets(m0, lane, oa);
   PB::lane_offsets(n0, lane, ob);
@@ -72,13 +143,12 @@ __global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
   int chain = span;
   auto k_tile = [&](int kt, int set) __attribute__((always_inline)) {
     char* st = lds[kt & 1];
-#pragma unroll
-    for (int h = 0; h < HA; ++h) *reinterpret_cast<i32x4*>(st + 16 * (tid + 256 * h)) = va[set][h];
-#pragma unroll
-    for (int h = 0; h < HB; ++h) *reinterpret_cast<i32x4*>(st + PA::BYTES + 16 * (tid + 256 * h)) = vb[set][h];
+    la.put(st, kt, va[set]);
+    lb.put(st + PA::BYTES, kt, vb[set]);
     // one barrier per k-tile: stage t's readers are past it before t + 2 is stored
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (kt + AHEAD < nk) load(kt + AHEAD, set);
+    la.load(min(kt + AHEAD, nk - 1), va[set]);  // past the end again the last, unused
+    lb.load(min(kt + AHEAD, nk - 1), vb[set]);
     const char *qa[PA::NV], *qb[PB::NV];
 #pragma unroll
     for (int i = 0; i < PA::NV; ++i) qa[i] = st + oa[i];
@@ -91,10 +161,21 @@ __global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
       for (int a = 0; a < FM; ++a) fa[a] = PA::frag(qa, a, h);
 #pragma unroll
       for (int b = 0; b < FN; ++b) fb[b] = PB::frag(qb, b, h);
+      if constexpr (FOLD) {  // four products per sum: the sums in turn
 #pragma unroll
-      for (int b = 0; b < FN; ++b)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int a = 0; a < FM; ++a) mma_tile<T>(acc[a][b], fb[b], fa[a]);
+          for (int b = 0; b < FN; ++b)
+#pragma unroll
+            for (int a = 0; a < FM; ++a)
+              acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, fb[b])[e], __builtin_bit_cast(f32x4, fa[a])[e],
+                                                               acc[a][b], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int b = 0; b < FN; ++b)
+#pragma unroll
+          for (int a = 0; a < FM; ++a) mma_tile<T>(acc[a][b], fb[b], fa[a]);
+      }
     }
     if constexpr (FOLD) {
       if (--chain == 0) {
@@ -109,12 +190,18 @@ __global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
       }
     }
   };
+  if (nk > 0) {
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i)
-    if (i < nk) load(i, i);
-  for (int kt = 0; kt < nk; kt += AHEAD) {
-    k_tile(kt, 0);
-    if (kt + 1 < nk) k_tile(kt + 1, 1);
+    for (int i = 0; i < AHEAD; ++i) {
+      la.load(min(i, nk - 1), va[i]);
+      lb.load(min(i, nk - 1), vb[i]);
+    }
+    int kt = 0;
+    for (; kt + 1 < nk; kt += 2) {
+      k_tile(kt, 0);
+      k_tile(kt + 1, 1);
+    }
+    if (kt < nk) k_tile(kt, 0);
   }
   if constexpr (FOLD) {
 #pragma unroll
@@ -145,16 +232,19 @@ static int grid_of(int64_t tiles, const char* what, unsigned* grid) {
 
 template <typename T, bool BKC, bool RK>
 static int run_any(GroupedArgs g, hipStream_t s) {
-  constexpr int BM = 64;
+  constexpr int BM = 32 * any_fm<T, RK>;
   const char* what = RK ? kRankK : kGemm;
   g.tiles_m = (g.M + BM - 1) / BM;
-  g.tiles_n = (g.N + BM - 1) / BM;
+  g.tiles_n = (g.N + 63) / 64;
   unsigned grid;
   const int64_t rows = RK ? (int64_t)g.groups * g.tiles_m : row_tiles(g.rows, g.groups, BM);
   if (int rc = grid_of(rows * g.tiles_n, what, &grid)) return rc;
   // whole rounds of the XCDs, so that each one's last tile is reached
   grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
-  hipLaunchKernelGGL((grouped_any_kernel<T, BKC, RK>), dim3(grid), dim3(256), 0, s, g);
+  constexpr int EV = 16 / sizeof(T);
+  const bool tiny = (RK ? g.M : g.K) < EV || (BKC ? g.K : g.N) < EV;
+  hipLaunchKernelGGL((tiny ? grouped_any_kernel<T, BKC, RK, true> : grouped_any_kernel<T, BKC, RK, false>), dim3(grid), dim3(256), 0,
+                     s, g);
   return check_launch(what);
 }
 

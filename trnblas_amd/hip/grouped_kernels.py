@@ -40,12 +40,12 @@ def _output_like(C: torch.Tensor | None, beta: float, shape, dtype, dev):
 # Operands that LDS DMA cannot read in place (base, leading dimension or extent no
 # multiple of 16 bytes) are copied first, their rows padded with zeros, where the
 # copies cost less than grouped_any_kernel's loads: both read and write at about 4 TB/s
-# and start in 4 us each; the kernel makes 300 TFLOP/s (rank_k 230; fp32 90) of such operands,
-# the ring kernels 800 (fp32 120) of copied ones. bf16 16383 rows in 8 groups, 2047 x
-# 4095: 763 us in place. Products of few flops per byte stay in place.
+# and start in 4 us each; the kernel makes 400 TFLOP/s (rank_k 310; fp32 90) of such operands,
+# the ring kernels 800 (fp32 115) of copied ones. bf16 16383 rows in 8 groups, 2047 x
+# 4095: 678 us in place, 450 packed; 4093 rows, 1023 x 2047: 61 and 64. Products of few flops per byte stay in place.
 _PACK_SAVES = {  # us per multiply-add
-    ("gemm", 2): 2 * (1 / 300e6 - 1 / 800e6), ("rank_k", 2): 2 * (1 / 230e6 - 1 / 800e6),
-    ("gemm", 4): 2 * (1 / 90e6 - 1 / 120e6), ("rank_k", 4): 2 * (1 / 90e6 - 1 / 120e6),
+    ("gemm", 2): 2 * (1 / 400e6 - 1 / 800e6), ("rank_k", 2): 2 * (1 / 310e6 - 1 / 800e6),
+    ("gemm", 4): 2 * (1 / 90e6 - 1 / 115e6), ("rank_k", 4): 2 * (1 / 90e6 - 1 / 115e6),
 }  # fmt: skip
 
 
