@@ -358,3 +358,22 @@ def test_extents_near_16_bytes_amid_nans(dev, dtype, K, N):
         assert og.excess(D.cpu(), *og.grouped_gemm(1.0, A.cpu(), (B.mT if transB else B).cpu(), off), K) <= 1
     P = tb.grouped_rank_k(1.0, _amid_nans(A, 1), _amid_nans(dD, 3), off.to(dev))
     assert og.excess(P.cpu(), *og.grouped_rank_k(1.0, A.cpu(), dD.cpu(), off), R) <= 1
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("G", [4, 8, 16])  # 4, 2 and 1 waves of a workgroup along K
+def test_few_rows_of_large_matrices(dev, dtype, G):
+    K, N = 2056, 4104
+    R = G + 3
+    assert _plan(0, dtype, 1, G, R, 0, N, K) == "rows_kernel"
+    g = torch.Generator(device=dev).manual_seed(G)
+    off = torch.arange(G + 1) + 1
+    off[2:] += 1
+    A = torch.randn(R, K, generator=g, device=dev).to(dtype)
+    B = torch.randn(G, N, K, generator=g, device=dev).to(dtype)
+    D = tb.grouped_gemm(1.0, A, B, off.to(dev), transB=True)
+    ref, den = torch.zeros(2, R, N, dtype=torch.float64, device=dev)
+    for j, a, b in og.rows_of(off, R):
+        W = B[j].double().T.contiguous()
+        ref[a:b], den[a:b] = A[a:b].double() @ W, A[a:b].double().abs() @ W.abs()
+    assert _excess_gpu(D, ref, den, K) <= 1

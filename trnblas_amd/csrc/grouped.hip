@@ -106,10 +106,7 @@ extern "C" const char* trnblas_hip_grouped_plan(int op, int dtype, int transB, i
     set_error("trnblas_hip_grouped_plan: bad arguments");
     return nullptr;
   }
-  if (op < 2 && (first * es % 16 != 0 || second * es % 16 != 0)) {
-    if (op == 0 && choose_grouped(kRing16, rows, groups, N, K, (double)K * es, es, transB != 0).ring < 0) return "rows_kernel";
-    return "grouped_any_kernel";
-  }
+  if (op < 2 && (first * es % 16 != 0 || second * es % 16 != 0)) return "grouped_any_kernel";
   int ring;
   if (op == 1)
     ring = choose_rank_k(groups, M, N, (double)rows / groups * es / 128.0);

@@ -53,8 +53,9 @@ inline GroupedChoice choose_grouped(const RingCost (&ring)[3], double rows, doub
   GroupedChoice best{-1, 1, 8};
   // Few rows: rows_kernel reads the weights once per 16 mf rows at about 4.5 TB/s
   // (two row blocks of a K-contiguous B: 3.2), its waves splitting K; the rings
-  // need a tile per CU to read as fast: 8 groups of one row, 4096 x 1536: 20.5 us
-  // against 38.4 (96 tiles); 64 groups of one: 90 and 81.
+  // need a tile per CU to read as fast, and read K-contiguous values at 3.9 TB/s. 8
+  // groups of one row, 4096 x 1536: 19 us, the rings 27 (96 tiles); 16 groups of one,
+  // 2048 x 4096, K-contiguous 58 and 73, otherwise 60 and 54.
   double time = 1e30;
   if (rows <= 64.0 * g) {
     best.mf = rows <= 8.0 * g ? 1 : 2;
@@ -65,7 +66,7 @@ inline GroupedChoice choose_grouped(const RingCost (&ring)[3], double rows, doub
   }
   for (int i = 0; i < 3; ++i) {
     const RingCost& c = ring[i];
-    const double t = std::max(3.0 + weights / 4.6e6,
+    const double t = std::max(3.0 + weights / (kc && elem >= 2 ? 3.9e6 : 4.6e6),
                               ring_time(c, likely_row_tiles(rows, groups, 32 * c.fm) * std::ceil(N / (32 * c.fn)), nk));
     // bound by the weights alike: the smaller tiles keep more loads under way (32
     // groups of 32 rows, 4096 x 1024 of 4-bit values: 37.0, 18.6 and 17.0 us)

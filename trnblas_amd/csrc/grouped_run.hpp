@@ -13,6 +13,23 @@
 
 namespace trnblas {
 
+// 16 bytes of values at any alignment, only the first n of them inside (n <= 0: none);
+// the rest zeros.
+template <typename T>
+__device__ __forceinline__ i32x4 load_any(const char* p, int n) {
+  constexpr int EV = 16 / sizeof(T);
+  if (n >= EV) return load16<T>(p);
+  union {
+    T e[EV];
+    i32x4 v;
+  } u;
+  u.v = i32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < EV; ++i)
+    if (i < n) u.e[i] = reinterpret_cast<const T*>(p)[i];
+  return u.v;
+}
+
 // 16 bytes of values ending at a row's end, loaded in the place of n values that start
 // that much later: moved down, zeros behind them (n <= 0: zeros).
 template <typename T>
@@ -287,13 +304,17 @@ static int run_rows(GroupedArgs g, hipStream_t s) {
   return check_launch(kGemm);
 }
 
+// Fewer than eight waves along K only where choose_grouped comes to it: one block of
+// rows, K-contiguous (else the rings have enough tiles before).
 template <typename T, int MF, bool BKC>
 static int run_rows_split(int ks, const GroupedArgs& g, hipStream_t s) {
   constexpr int NF = BKC ? 1 : 4;
-  return ks == 8   ? run_rows<T, MF, NF, 8, BKC>(g, s)
-         : ks == 4 ? run_rows<T, MF, NF, 4, BKC>(g, s)
-         : ks == 2 ? run_rows<T, MF, NF, 2, BKC>(g, s)
-                   : run_rows<T, MF, NF, 1, BKC>(g, s);
+  if constexpr (MF == 1 && BKC) {
+    if (ks == 4) return run_rows<T, MF, NF, 4, BKC>(g, s);
+    if (ks == 2) return run_rows<T, MF, NF, 2, BKC>(g, s);
+    if (ks == 1) return run_rows<T, MF, NF, 1, BKC>(g, s);
+  }
+  return run_rows<T, MF, NF, 8, BKC>(g, s);
 }
 
 // ring: index of kRing16. fp32 always takes the 64 x 128 tiles: three workgroups
@@ -310,10 +331,10 @@ static int run_ring_choice(int ring, const GroupedArgs& g, hipStream_t s) {
 
 template <typename T, bool BKC>
 static int run_grouped(const GroupedArgs& g, hipStream_t s) {
-  const bool ready = dma_ready<T>(g, BKC, false);
+  if (!dma_ready<T>(g, BKC, false)) return run_any<T, BKC, false>(g, s);
   const GroupedChoice c = choose_grouped(kRing16, g.rows, g.groups, g.N, g.K, (double)g.K * sizeof(T), sizeof(T), BKC);
   if (c.ring < 0) return c.mf == 1 ? run_rows_split<T, 1, BKC>(c.ks, g, s) : run_rows_split<T, 2, BKC>(c.ks, g, s);
-  return ready ? run_ring_choice<T, BKC, false>(c.ring, g, s) : run_any<T, BKC, false>(g, s);
+  return run_ring_choice<T, BKC, false>(c.ring, g, s);
 }
 
 template <typename T>

@@ -10,29 +10,12 @@ namespace trnblas {
 
 typedef i32x4 __attribute__((aligned(2))) i32x4_at2;
 typedef i32x4 __attribute__((aligned(4))) i32x4_at4;
-typedef unsigned int u32x2_at2 __attribute__((ext_vector_type(2), aligned(2)));
 
 // 16 bytes at any alignment of T.
 template <typename T>
 __device__ __forceinline__ i32x4 load16(const char* p) {
   using loose = std::conditional_t<sizeof(T) == 1, i32x4, std::conditional_t<sizeof(T) == 2, i32x4_at2, i32x4_at4>>;
   return *reinterpret_cast<const loose*>(p);
-}
-
-// The same with only its first n values inside (n <= 0: none); the rest zeros.
-template <typename T>
-__device__ __forceinline__ i32x4 load_any(const char* p, int n) {
-  constexpr int EV = 16 / sizeof(T);
-  if (n >= EV) return load16<T>(p);
-  union {
-    T e[EV];
-    i32x4 v;
-  } u;
-  u.v = i32x4{0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < EV; ++i)
-    if (i < n) u.e[i] = reinterpret_cast<const T*>(p)[i];
-  return u.v;
 }
 
 // Steps of a chunk, and chunks that a wave loads before it multiplies.
@@ -51,29 +34,14 @@ struct ColumnStep {
   static constexpr int ES = sizeof(T), KR = 16 / ES;  // k rows of a lane
   using word = std::conditional_t<ES == 2, u32x2, i32x4>;
   word w[KR];
-  // p: B at (k of the lane's first row, its first column); rows, cols: inside
+  // p: B at (k of the lane's first row, its first column); rows of k inside
   __device__ __forceinline__ void load(const char* p, int64_t ld) {
 #pragma unroll
-    for (int e = 0; e < KR; ++e) {
-      if constexpr (ES == 2)
-        w[e] = *reinterpret_cast<const u32x2_at2*>(p + e * ld * ES);
-      else
-        w[e] = *reinterpret_cast<const i32x4_at4*>(p + e * ld * ES);
-    }
+    for (int e = 0; e < KR; ++e) w[e] = *reinterpret_cast<const word*>(p + e * ld * ES);
   }
-  __device__ __forceinline__ void load_any(const char* p, int64_t ld, int rows, int cols) {
+  __device__ __forceinline__ void load_last(const char* p, int64_t ld, int rows) {
 #pragma unroll
-    for (int e = 0; e < KR; ++e) {
-      union {
-        T e[4];
-        word v;
-      } u;
-      u.v = word{};
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (e < rows && c < cols) u.e[c] = reinterpret_cast<const T*>(p + e * ld * ES)[c];
-      w[e] = u.v;
-    }
+    for (int e = 0; e < KR; ++e) w[e] = e < rows ? *reinterpret_cast<const word*>(p + e * ld * ES) : word{};
   }
   __device__ __forceinline__ i32x4 operand(int j) const {
     i32x4 v;
@@ -139,10 +107,14 @@ __device__ __forceinline__ void quantize_rows(const GroupedArgs& g, const MxScal
 // LDS in wave order; 8 / KS such sets take 16 NF columns each. What bounds it is
 // reading B: each wave has U chunks of loads in flight before it multiplies, no
 // LDS and no barrier in the loop; KS is chosen so that a wave has U chunks or
-// more, or the GPU enough workgroups (rows_split).
+// more, or the GPU enough workgroups (choose_grouped).
 // K-contiguous B: one row of 64 bytes per lane quad and step. Column-contiguous B: NF
-// = 4, whole 128-byte lines of 16-bit values. Rows of A past the segment repeat
-// its last one (not stored). fp32: the sums restart every 512 values of k per wave.
+// = 4, whole 128-byte lines of 16-bit values. Rows of A past the segment and columns past
+// N repeat the last ones (not stored). Operands as for the ring kernels: groups of 16
+// bytes along a row lie inside it, or in its padding, or outside as a whole (operands
+// that start anywhere: 8 groups of a row, 4095 x 1535, 69 us here with a branch per
+// load, 33 on grouped_any_kernel). One row of bf16 by 4096 x 1536 9 us, 16 groups of a
+// row by 2048 x 4096 58 us (4.6 TB/s); 4-bit 8192^2 and one row 9.4 (3.8). fp32: the sums restart every 512 values of k per wave.
 //
 // X (4-bit floats only): A comes as values of that type, at most kInPlace in the
 // tile's rows; the workgroup quantises them into LDS behind its first loads of B,
@@ -190,9 +162,8 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
       if constexpr (MX) qb[b] = x.b + grp * x.b_step + (n >> 4) * x.chunks * kChunk + 64 * lg + 4 * (n & 15);
     }
   } else {
-    pb[0] = static_cast<const char*>(g.B) + (grp * g.sB + (int64_t)(EV * lg) * g.ldb + n0 + 4 * li) * ES;
+    pb[0] = static_cast<const char*>(g.B) + (grp * g.sB + (int64_t)(EV * lg) * g.ldb + min(n0 + 4 * li, ((g.N + 3) & ~3) - 4)) * ES;
   }
-  const bool whole = BKC || n0 + BW <= g.N;  // all columns of a column-contiguous tile inside
   const int64_t kstep = (BKC ? 64 : 64 / ES * g.ldb * ES);  // bytes of B per step
   struct Chunk {
     i32x4 a[MF][STEPS];
@@ -223,11 +194,7 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
 #pragma unroll
         for (int b = 0; b < NF; ++b) v.b[b][h] = load16<T>(pb[b] + (int64_t)c * CH + 64 * h);
       } else {
-        const char* p = pb[0] + (int64_t)(STEPS * c + h) * kstep;
-        if (whole)
-          v.c[h].load(p, g.ldb);
-        else
-          v.c[h].load_any(p, g.ldb, EV, g.N - n0 - 4 * li);
+        v.c[h].load(pb[0] + (int64_t)(STEPS * c + h) * kstep, g.ldb);
       }
     }
     if constexpr (MX) {
@@ -241,12 +208,12 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
     for (int h = 0; h < STEPS; ++h) {
       const int left = K - c * CK - (64 / ES) * h - EV * lg;  // values of k from this lane's group on
 #pragma unroll
-      for (int a = 0; a < MF; ++a) v.a[a][h] = load_any<T>(pa[a] + (int64_t)c * CH + 64 * h, left);
+      for (int a = 0; a < MF; ++a) v.a[a][h] = left > 0 ? load16<T>(pa[a] + (int64_t)c * CH + 64 * h) : i32x4{0, 0, 0, 0};
       if constexpr (BKC) {
 #pragma unroll
-        for (int b = 0; b < NF; ++b) v.b[b][h] = load_any<T>(pb[b] + (int64_t)c * CH + 64 * h, left);
+        for (int b = 0; b < NF; ++b) v.b[b][h] = left > 0 ? load16<T>(pb[b] + (int64_t)c * CH + 64 * h) : i32x4{0, 0, 0, 0};
       } else {
-        v.c[h].load_any(pb[0] + (int64_t)(STEPS * c + h) * kstep, g.ldb, left, g.N - n0 - 4 * li);
+        v.c[h].load_last(pb[0] + (int64_t)(STEPS * c + h) * kstep, g.ldb, left);
       }
     }
     if constexpr (MX) {
