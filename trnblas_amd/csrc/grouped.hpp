@@ -58,6 +58,12 @@ struct Segment {
   int quarter;     // of the tile, or -1
 };
 
+// Tiles that SPLIT (see tile_of) leaves whole.
+__device__ __forceinline__ int whole_tiles(const GroupedArgs& g, int tiles) {
+  const int whole = tiles / g.slots * g.slots;
+  return 4 * (tiles - whole) > 3 * g.slots ? tiles : whole;
+}
+
 // Tile of workgroup `bid` among `tiles`; false when there is none left. Workgroups
 // go to the XCDs round-robin: each XCD walks one contiguous range of the tiles.
 // SPLIT (one workgroup per CU, g.slots of them): tiles that would not fill a last
@@ -72,8 +78,7 @@ __device__ __forceinline__ bool tile_of(const GroupedArgs& g, int bid, int tiles
   };
   quarter = -1;
   if constexpr (!SPLIT) return range(bid, tiles, tile);
-  int whole = tiles / g.slots * g.slots, cut = tiles - whole;
-  if (4 * cut > 3 * g.slots) whole = tiles, cut = 0;
+  const int whole = whole_tiles(g, tiles), cut = tiles - whole;
   const int first = (whole + kNumXcd - 1) / kNumXcd * kNumXcd;  // workgroups up to here take whole tiles
   if (bid < first) return range(bid, whole, tile);
   if (!range(bid - first, 4 * cut, tile)) return false;
@@ -286,8 +291,16 @@ __device__ __forceinline__ bool tile_job(const GroupedArgs& g, TileJob& j) {
     const int per = g.tiles_m * g.tiles_n;
     int t, tm, tn;
     if (!tile_of<SPLIT>(g, blockIdx.x, g.groups * per, t, j.quarter)) return false;
-    const int grp = t / per;
-    grouped_tile(t - grp * per, g.tiles_m, g.tiles_n, 8, tm, tn);
+    // the groups' numbers of rows differ: each XCD takes an eighth of every group's tiles
+    int grp = t / per, in = t - grp * per;
+    const int tiles = g.groups * per, whole = SPLIT ? whole_tiles(g, tiles) : tiles;
+    if (per % kNumXcd == 0 && whole % kNumXcd == 0) {
+      const int first = t < whole ? 0 : whole, each = ((t < whole ? whole : tiles) - first) / kNumXcd, share = per / kNumXcd;
+      const int x = (t - first) / each, i = first / kNumXcd + (t - first) - x * each;
+      grp = i / share;
+      in = x * share + i - grp * share;
+    }
+    grouped_tile(in, g.tiles_m, g.tiles_n, 8, tm, tn);
     const int start = boundary(g, grp + 1), end = max(boundary(g, grp + 2), start);
     j.group = grp;
     j.m = tm * BM;
