@@ -359,3 +359,17 @@ def mx_quantize_fast(X):
     )
     _checked("trnblas_hip_mx_quantize", rc)
     return codes, scales
+
+
+def mx_dequantize_fast(codes, scales, K, dtype):
+    """The values of one matrix, or None."""
+    dev = codes.get_device()
+    if dev < 0 or codes.dim() != 2 or _kernels._launch_probe is not None:
+        return None
+    R = codes.shape[0]
+    D = codes.new_empty((R, K), dtype=dtype)
+    rc = _fn("trnblas_hip_mx_dequantize")(
+        _lib.DTYPE_CODES[dtype], R, K, codes.data_ptr(), scales.data_ptr(), D.data_ptr(), K or 1, R * K, 1, _raw_stream(dev)
+    )
+    _checked("trnblas_hip_mx_dequantize", rc)
+    return D

@@ -152,7 +152,8 @@ def mx_quantize(X: torch.Tensor, trans: bool = False) -> MXMatrix:
         raise ValueError("mx_quantize: X must be a 2-D or 3-D tensor")
     if not X.is_floating_point():
         raise TypeError(f"mx_quantize: X must be a real floating tensor, got {X.dtype}")
-    X = X.detach()
+    if X.requires_grad:
+        X = X.detach()
     if X.dtype not in _FLOATS:
         X = X.float()
     if trans_flag(trans):
@@ -177,7 +178,8 @@ def mx_dequantize(Q: MXMatrix, dtype: torch.dtype = torch.float32) -> torch.Tens
         raise TypeError(f"mx_dequantize: dtype {dtype} (float32, bfloat16 or float16)")
     if _d.mx_on_hip(Q.codes):
         try:
-            return _gk().mx_dequantize(Q.codes, Q.scales, Q.shape[-1], dtype)
+            D = _gk().mx_dequantize_fast(Q.codes, Q.scales, Q.shape[-1], dtype)
+            return _gk().mx_dequantize(Q.codes, Q.scales, Q.shape[-1], dtype) if D is None else D
         except Exception as exc:  # noqa: BLE001
             _d._kernel_failed(exc)
     return _dequantize_torch(Q, dtype)
