@@ -94,12 +94,41 @@ def _check_operands(what: str, A, B, dims) -> None:
         raise ValueError(f"{what}: operands on different devices: {A.device} and {B.device}")
 
 
+def _gemm(alpha, A, B, offsets, beta, C, out_dtype):
+    """The product for the autograd functions, B as in _d.grouped_gemm: the short way where it serves."""
+    if beta == 0.0 and A.is_cuda and _d._use_hip():
+        kc = B.stride(2) != 1 and B.stride(1) == 1
+        try:
+            D = _gk().grouped_gemm_fast(alpha, A, B.mT if kc else B, offsets, kc, out_dtype)
+            if D is not None:
+                return D
+        except _d.HipKernelError as exc:
+            _d._kernel_failed(exc)
+    return _d.grouped_gemm(alpha, A, B, offsets, beta, C, out_dtype)
+
+
+def _rank_k(alpha, A, B, offsets, beta, C, out_dtype):
+    if beta == 0.0 and A.is_cuda and _d._use_hip():
+        try:
+            D = _gk().grouped_rank_k_fast(alpha, A, B, offsets, out_dtype)
+            if D is not None:
+                return D
+        except _d.HipKernelError as exc:
+            _d._kernel_failed(exc)
+    return _d.grouped_rank_k(alpha, A, B, offsets, beta, C, out_dtype)
+
+
+def _differentiable(function, product, *args):
+    """A product of a backward pass, itself differentiable only where that is asked for."""
+    return function.apply(*args) if torch.is_grad_enabled() else product(*args)
+
+
 class _GroupedGemm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, alpha, A, B, offsets, beta, C, out_dtype):
         ctx.save_for_backward(A, B, offsets)
         ctx.alpha, ctx.beta = alpha, beta
-        return _d.grouped_gemm(alpha, A, B, offsets, beta, C, out_dtype)
+        return _gemm(alpha, A, B, offsets, beta, C, out_dtype)
 
     @staticmethod
     def backward(ctx, dD):
@@ -110,12 +139,12 @@ class _GroupedGemm(torch.autograd.Function):
         # an fp32 result of 16-bit operands: its gradient meets them in their type
         dD = dD.to(A.dtype)
         if ctx.needs_input_grad[1]:
-            dA = _GroupedGemm.apply(ctx.alpha, dD, B.mT, offsets, 0.0, None, A.dtype)
+            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, dD, B.mT, offsets, 0.0, None, A.dtype)
         if ctx.needs_input_grad[2]:
             if B.stride(1) == 1 and B.stride(2) > 1:  # B is a transposed view: so is its gradient
-                dB = _GroupedRankK.apply(ctx.alpha, dD, A, offsets, 0.0, None, B.dtype).mT
+                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, dD, A, offsets, 0.0, None, B.dtype).mT
             else:
-                dB = _GroupedRankK.apply(ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
+                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
         return None, dA, dB, None, None, dC, None
 
 
@@ -124,7 +153,7 @@ class _GroupedRankK(torch.autograd.Function):
     def forward(ctx, alpha, A, B, offsets, beta, C, out_dtype):
         ctx.save_for_backward(A, B, offsets)
         ctx.alpha, ctx.beta = alpha, beta
-        return _d.grouped_rank_k(alpha, A, B, offsets, beta, C, out_dtype)
+        return _rank_k(alpha, A, B, offsets, beta, C, out_dtype)
 
     @staticmethod
     def backward(ctx, dD):
@@ -134,9 +163,9 @@ class _GroupedRankK(torch.autograd.Function):
             dC = ctx.beta * dD
         dD = dD.to(A.dtype)
         if ctx.needs_input_grad[1]:
-            dA = _GroupedGemm.apply(ctx.alpha, B, dD.mT, offsets, 0.0, None, A.dtype)
+            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, B, dD.mT, offsets, 0.0, None, A.dtype)
         if ctx.needs_input_grad[2]:
-            dB = _GroupedGemm.apply(ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
+            dB = _differentiable(_GroupedGemm, _gemm, ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
         return None, dA, dB, None, None, dC, None
 
 
