@@ -115,5 +115,6 @@ extern "C" const char* trnblas_hip_grouped_plan(int op, int dtype, int transB, i
   else
     ring = choose_grouped(kRing16, rows, groups, N, K, (double)K * es, es, transB != 0).ring;
   if (ring < 0) return "rows_kernel";
+  if (op == 0 && dtype == TRNBLAS_F32 && f32_small_tiles(rows, groups, N)) return "grouped_any_kernel";
   return kRingNames[op < 2 && dtype == TRNBLAS_F32 ? 2 : ring];
 }

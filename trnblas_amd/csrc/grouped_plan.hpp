@@ -78,6 +78,14 @@ inline GroupedChoice choose_grouped(const RingCost (&ring)[3], double rows, doub
   return best;
 }
 
+// fp32 (its MFMAs take eight times as long): below two 64 x 128 tiles per CU the 32 x
+// 64 ones of grouped_any_kernel spread better, aligned or not. 300 rows in 4 groups by
+// 2048 x 1024 35 us, the rings 72; 2000 in 8 by 1024^2 60 and 72; 4096 in 8 by 2048^2
+// (1088 tiles) 370 and 310.
+inline bool f32_small_tiles(double rows, double groups, double N) {
+  return likely_row_tiles(rows, groups, 64) * std::ceil(N / 128) < 2.0 * device_cus();
+}
+
 // grouped_rank_k: groups x (M x N), k_tiles of the average group.
 inline int choose_rank_k(double groups, double M, double N, double k_tiles) {
   int best = 0;

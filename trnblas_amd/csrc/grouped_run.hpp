@@ -317,9 +317,9 @@ static int run_rows_split(int ks, const GroupedArgs& g, hipStream_t s) {
   return run_rows<T, MF, NF, 8, BKC>(g, s);
 }
 
-// ring: index of kRing16. fp32 always takes the 64 x 128 tiles: three workgroups
-// per CU hide its longer MFMAs' steps best (8 groups of 128 rows, 2048 x 4096: 217 us
-// against 220 on 128 x 128 and 267 on grouped_any_kernel).
+// ring: index of kRing16. fp32 takes the 64 x 128 tiles: three workgroups per CU hide
+// its longer MFMAs' steps best (8 groups of 128 rows, 2048 x 4096: 217 us, 220 on 128 x
+// 128), or 32 x 64 ones (f32_small_tiles).
 template <typename T, bool BKC, bool RK>
 static int run_ring_choice(int ring, const GroupedArgs& g, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
@@ -334,6 +334,7 @@ static int run_grouped(const GroupedArgs& g, hipStream_t s) {
   if (!dma_ready<T>(g, BKC, false)) return run_any<T, BKC, false>(g, s);
   const GroupedChoice c = choose_grouped(kRing16, g.rows, g.groups, g.N, g.K, (double)g.K * sizeof(T), sizeof(T), BKC);
   if (c.ring < 0) return c.mf == 1 ? run_rows_split<T, 1, BKC>(c.ks, g, s) : run_rows_split<T, 2, BKC>(c.ks, g, s);
+  if (std::is_same_v<T, float> && f32_small_tiles(g.rows, g.groups, g.N)) return run_any<T, BKC, false>(g, s);
   return run_ring_choice<T, BKC, false>(c.ring, g, s);
 }
 
