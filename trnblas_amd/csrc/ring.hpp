@@ -67,19 +67,21 @@ __device__ __forceinline__ void lds_dma(const i32x4& rsrc, uint32_t lds, uint32_
                : "memory", "m0", "scc");
 }
 
-// acc += (rows n) x (rows m) over one k-tile of a 16 x 16 block; fp4x2: with the
-// low byte of each scale dword. Lane l holds column m = l % 16 and rows n = 4 (l
+// acc += (rows n) x (rows m) over one k-tile of a 16 x 16 block; fp4x2: with byte
+// BYTE of each scale dword. Lane l holds column m = l % 16 and rows n = 4 (l
 // / 16) + r. Inline asm with the sum in accumulation registers: left to choose,
 // the compiler moves the 64 blocks of a wave through four of them. Volatile, so
 // that the LDS reads and DMAs written between MFMAs stay there. The hazards that
 // the compiler cannot see: a block's next MFMA comes at least FM FN - 1 MFMAs
-// later, and the epilogue waits (settle).
-template <typename T>
+// later, the epilogue waits (settle), and no vector instruction writes an operand
+// within two wait states: operands and scales are as LDS reads leave them, the
+// scale's byte is the instruction's to pick, and a step begins with the wait.
+template <typename T, int BYTE>
 __device__ __forceinline__ void mma_block(f32x4& acc, const i32x4& n, const i32x4& m, int sn, int sm) {
   if constexpr (std::is_same_v<T, fp4x2>)
-    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%5,0] op_sel_hi:[%6,%6,0] cbsz:4 blgp:4"
                  : "+a"(acc)
-                 : "v"(n), "v"(m), "v"(sn), "v"(sm));
+                 : "v"(n), "v"(m), "v"(sn), "v"(sm), "n"(BYTE & 1), "n"(BYTE >> 1));
   else if constexpr (std::is_same_v<T, __bf16>)
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(n), "v"(m));
   else if constexpr (std::is_same_v<T, _Float16>)
@@ -278,14 +280,15 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
       fa[set][i - FN] = PA::frag(pa, i - FN, set);
   };
   [[maybe_unused]] int span = 0, chain = 0;
-  // step s of k-tile kt: the MFMAs of register set s, reads of the other set
-  auto step = [&](int kt, auto sc) __attribute__((always_inline)) {
-    constexpr int s = decltype(sc)::value;
+  // step s of k-tile kt (an odd one: ODD; fp4x2 only): the MFMAs of register set s, reads of the other set
+  auto step = [&](int kt, auto oddc, auto sc) __attribute__((always_inline)) {
+    constexpr int s = decltype(sc)::value, ODD = decltype(oddc)::value;
     constexpr int MM = FM * FN, HALF = MM / 2;
     constexpr int R0 = s ? HALF : 0, RW = MM * 3 / 8;           // MFMAs behind which the reads go
     constexpr int DW = MM * 5 / 4;                              // and the DMAs, from HALF of step 0
     constexpr int SENT = (MM * ND + DW - 1) / DW;               // DMAs sent when step 1 waits
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this step's fragments
+    asm volatile("s_nop 1");             // registers that the compiler moved where paths meet
     each<MM>([&](auto ic) __attribute__((always_inline)) {
       constexpr int i = decltype(ic)::value, a = i % FM, b = i / FM, t = s * MM + i - HALF;
       if constexpr (i == HALF) {
@@ -298,9 +301,7 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
           read_from(kt + 1);
         }
       }
-      mma_block<T>(acc[a][b], fb[s][b], fa[s][a], MX ? qb[b] : 0, MX ? qa[a] : 0);
-      if constexpr (MX && b == FN - 1) qa[a] = (int)((uint32_t)qa[a] >> 8);
-      if constexpr (MX && a == FM - 1) qb[b] = (int)((uint32_t)qb[b] >> 8);
+      mma_block<T, 2 * ODD + s>(acc[a][b], fb[s][b], fa[s][a], MX ? qb[b] : 0, MX ? qa[a] : 0);
       each<ND>([&](auto uc) __attribute__((always_inline)) {
         if constexpr (t >= 0 && decltype(uc)::value * DW / ND == t) dma(uc);
       });
@@ -309,10 +310,10 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
         if (R0 + r * RW / (FM + FN) == i) read(r, s ^ 1);
     });
     if constexpr (MX && s == 1) {
-      const int i = 8 * (kt & 1) + wave;
+      const int i = 8 * ODD + wave;
       if (i < SA + SB) scale_dma((kt >> 1) + 2, i);
       if (i + 4 < SA + SB) scale_dma((kt >> 1) + 2, i + 4);
-      if (kt & 1) read_scales((kt >> 1) + 1);
+      if constexpr (ODD) read_scales((kt >> 1) + 1);
     }
     if constexpr (FOLD) {
       if (--chain == 0) {
@@ -346,9 +347,23 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
 #pragma unroll
     for (int i = 0; i < FN + FM; ++i) read(i, 0);
     if constexpr (FOLD) chain = span = 2 * chain_length(j.K, 4) / PA::BK;
-    for (int kt = 0; kt < nk; ++kt) {
-      step(kt, std::integral_constant<int, 0>{});
-      step(kt, std::integral_constant<int, 1>{});
+    constexpr std::integral_constant<int, 0> zero{};
+    constexpr std::integral_constant<int, 1> one{};
+    if constexpr (MX) {
+      // two k-tiles at a time: the four bytes of a scale dword
+      for (int kt = 0; kt < nk; kt += 2) {
+        step(kt, zero, zero);
+        step(kt, zero, one);
+        if (kt + 1 < nk) {
+          step(kt + 1, one, zero);
+          step(kt + 1, one, one);
+        }
+      }
+    } else {
+      for (int kt = 0; kt < nk; ++kt) {
+        step(kt, zero, zero);
+        step(kt, zero, one);
+      }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA into the LDS of the next workgroup
     if constexpr (!FOLD) settle(acc);
