@@ -377,3 +377,27 @@ def test_few_rows_of_large_matrices(dev, dtype, G):
         W = B[j].double().T.contiguous()
         ref[a:b], den[a:b] = A[a:b].double() @ W, A[a:b].double().abs() @ W.abs()
     assert _excess_gpu(D, ref, den, K) <= 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_forward_mode_tangents(dev, dtype):
+    from torch.autograd import forward_ad as fwd
+
+    rows, sizes, lead = GROUPS["gaps"]
+    off = _split(rows, sizes, lead)
+    g = torch.Generator().manual_seed(11)
+    A, B, W = (_randn(g, *s, dtype=dtype) for s in ((rows, 72), (len(sizes), 72, 40), (rows, 40)))
+    tA, tB, tW = (_randn(g, *x.shape, dtype=dtype) for x in (A, B, W))
+    with fwd.dual_level():
+        dual = lambda x, t: fwd.make_dual(x.to(dev), t.to(dev))
+        D = fwd.unpack_dual(tb.grouped_gemm(1.0, dual(A, tA), dual(B, tB), off.to(dev)))
+        P = fwd.unpack_dual(tb.grouped_rank_k(1.0, dual(A, tA), dual(W, tW), off.to(dev)))
+        one = fwd.unpack_dual(tb.grouped_gemm(1.0, A.to(dev), dual(B, tB), off.to(dev)))
+        M = fwd.unpack_dual(tb.gemm(1.0, dual(A, tA), dual(B, tB).select(0, 1)))
+    a, b = og.grouped_gemm(1.0, tA, B, off), og.grouped_gemm(1.0, A, tB, off)
+    assert og.excess(D.primal, *og.grouped_gemm(1.0, A, B, off), 72) <= 1
+    assert og.excess(D.tangent, a[0] + b[0], a[1] + b[1], 2 * 72) <= 1
+    assert og.excess(one.tangent, *b, 72) <= 1
+    a, b = og.grouped_rank_k(1.0, tA, W, off), og.grouped_rank_k(1.0, A, tW, off)
+    assert og.excess(P.tangent, a[0] + b[0], a[1] + b[1], 2 * rows) <= 1
+    assert M.tangent is not None

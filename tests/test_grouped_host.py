@@ -47,6 +47,44 @@ def test_gradients_against_differences():
     assert torch.autograd.gradgradcheck(lambda a, b: tb.grouped_gemm(0.7, a, b, off), (A, B))
 
 
+def _products(off):
+    return (
+        lambda a, b, c, w, s: tb.grouped_gemm(0.7, a, b, off, 0.3, c),
+        lambda a, b, c, w, s: tb.grouped_gemm(0.7, a, b.mT.contiguous(), off, 0.3, c, transB=True),
+        lambda a, b, c, w, s: tb.grouped_rank_k(0.7, a, w, off, 0.5, s),
+    )
+
+
+def test_tangents_against_differences():
+    g = torch.Generator().manual_seed(3)
+    off = _offsets(0, 3, 3, 6)
+    args = tuple(torch.randn(s, generator=g, dtype=torch.float64, requires_grad=True)
+                 for s in ((7, 4), (3, 4, 5), (7, 5), (7, 5), (3, 4, 5)))  # fmt: skip
+    for f in _products(off):
+        used = lambda *x, f=f: f(*x) + 0.0 * sum(v.sum() for v in x)
+        assert torch.autograd.gradcheck(used, args, check_forward_ad=True, check_backward_ad=False)
+        assert torch.autograd.gradgradcheck(used, args, check_fwd_over_rev=True, check_rev_over_rev=False, check_undefined_grad=False)
+
+
+def test_tangents_of_each_operand_alone():
+    from torch.autograd import forward_ad as fwd
+
+    g = torch.Generator().manual_seed(4)
+    off = _offsets(1, 3, 3, 6)
+    X = [torch.randn(s, generator=g, dtype=torch.float64) for s in ((7, 4), (3, 4, 5), (7, 5), (7, 5), (3, 4, 5))]
+    T = [torch.randn(x.shape, generator=g, dtype=torch.float64) for x in X]
+    for f in _products(off):
+        for i in range(5):
+            step = lambda h: f(*(x + h * t if i == j else x for j, (x, t) in enumerate(zip(X, T))))
+            with fwd.dual_level():
+                got = fwd.unpack_dual(f(*(fwd.make_dual(x, t) if i == j else x for j, (x, t) in enumerate(zip(X, T)))))
+                got = got.tangent
+            # the products are linear in each operand: a difference is exact but for rounding
+            assert (got is None) == torch.equal(step(1.0), step(-1.0))
+            if got is not None:
+                assert torch.allclose(got, (step(1.0) - step(-1.0)) / 2, rtol=0, atol=1e-13)
+
+
 def test_sizes_of_zero():
     off = _offsets(0, 0, 0)
     assert tb.grouped_gemm(1.0, torch.zeros(0, 4), torch.zeros(2, 4, 3), off).shape == (0, 3)

@@ -209,3 +209,13 @@ def test_few_rows_quantised_in_place(dev, dtype, M, K):
     A[M - 1, K - 1] = float("inf")
     D = tb.mx_gemm(1.0, A.to(dev), Q, dtype=F32)
     assert D[M - 1].isnan().all() and D[: M - 1].isfinite().all()
+
+
+def test_tangents_are_refused(dev):
+    from torch.autograd import forward_ad as fwd
+
+    A, W = torch.ones(4, 64, device=dev), tb.mx_quantize(torch.ones(3, 64, device=dev))
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            tb.mx_gemm(1.0, fwd.make_dual(A, A), W)
+        assert torch.equal(tb.mx_gemm(1.0, A, W), torch.full((4, 3), 64.0, device=dev))

@@ -108,6 +108,20 @@ def test_refusals():
         tb.MXMatrix.from_parts(W.codes, torch.zeros(3, 3, dtype=torch.uint8), 64)
 
 
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad as fwd
+
+    A, C = torch.ones(4, 64), torch.ones(4, 3)
+    W, E, off = tb.mx_quantize(torch.ones(3, 64)), tb.mx_quantize(torch.ones(2, 3, 64)), torch.tensor([0, 1, 4])
+    with fwd.dual_level():
+        dual, c = fwd.make_dual(A, A), fwd.make_dual(C, C)
+        for call in (lambda: tb.mx_gemm(1.0, dual, W), lambda: tb.mx_grouped_gemm(1.0, dual, E, off),
+                     lambda: tb.mx_gemm(1.0, A, W, 1.0, c), lambda: tb.mx_grouped_gemm(1.0, A, E, off, 1.0, c)):  # fmt: skip
+            with pytest.raises(NotImplementedError, match="no gradient"):
+                call()
+        assert torch.equal(tb.mx_gemm(1.0, A, W), torch.full((4, 3), 64.0))
+
+
 def test_c_abi_refusals():
     from trnblas_amd.hip import _lib
 

@@ -8,6 +8,8 @@ fused). Both are differentiable, and each other's gradients:
     D = grouped_gemm(A, B)     dA = grouped_gemm(dD, B^T)   dB = grouped_rank_k(A, dD)
     D = grouped_rank_k(A, B)   dA = grouped_gemm(B, dD^T)   dB = grouped_gemm(A, dD)
 
+and in forward mode, with tangents tA, tB and tC, tD = alpha (tA B + A tB) + beta tC.
+
 `offsets` (int32 or int64, groups + 1 entries, nondecreasing) gives group g the
 rows offsets[g] .. offsets[g + 1] - 1; groups may be empty, and rows before
 the first or after the last group belong to none. On a ROCm GPU the offsets are
@@ -46,6 +48,7 @@ def _fast_call(A, B, offsets) -> bool:
         and type(offsets) is torch.Tensor
         and A.is_cuda
         and not ((A.requires_grad or B.requires_grad) and torch.is_grad_enabled())
+        and not _d._forward_mode()
         and _d._use_hip()
     )
 
@@ -120,15 +123,36 @@ def _rank_k(alpha, A, B, offsets, beta, C, out_dtype):
 
 def _differentiable(function, product, *args):
     """A product of a backward pass, itself differentiable only where that is asked for."""
-    return function.apply(*args) if torch.is_grad_enabled() else product(*args)
+    return function.apply(*args) if torch.is_grad_enabled() or _d._forward_mode() else product(*args)
+
+
+def _tangent(ctx, product, tA, tB, tC):
+    """The tangent of a product, summed in fp32 at least and rounded once."""
+    A, B, offsets = ctx.saved_for_forward
+    wide = torch.promote_types(ctx.out_dtype, torch.float32)
+    t = None if tC is None else ctx.beta * tC.to(wide)
+    for a, b in ((tA, B), (A, tB)):
+        if a is not None and b is not None:
+            t = product(ctx.alpha, a, b, offsets, 0.0 if t is None else 1.0, t, wide)
+    return t.to(ctx.out_dtype)
+
+
+def _save(ctx, alpha, A, B, offsets, beta, out_dtype):
+    ctx.save_for_backward(A, B, offsets)
+    if _d._forward_mode():
+        ctx.save_for_forward(A, B, offsets)
+    ctx.alpha, ctx.beta, ctx.out_dtype = alpha, beta, out_dtype
 
 
 class _GroupedGemm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, alpha, A, B, offsets, beta, C, out_dtype):
-        ctx.save_for_backward(A, B, offsets)
-        ctx.alpha, ctx.beta = alpha, beta
+        _save(ctx, alpha, A, B, offsets, beta, out_dtype)
         return _gemm(alpha, A, B, offsets, beta, C, out_dtype)
+
+    @staticmethod
+    def jvp(ctx, _alpha, tA, tB, _offsets, _beta, tC, _out_dtype):
+        return _tangent(ctx, _gemm, tA, tB, tC)
 
     @staticmethod
     def backward(ctx, dD):
@@ -151,9 +175,12 @@ class _GroupedGemm(torch.autograd.Function):
 class _GroupedRankK(torch.autograd.Function):
     @staticmethod
     def forward(ctx, alpha, A, B, offsets, beta, C, out_dtype):
-        ctx.save_for_backward(A, B, offsets)
-        ctx.alpha, ctx.beta = alpha, beta
+        _save(ctx, alpha, A, B, offsets, beta, out_dtype)
         return _rank_k(alpha, A, B, offsets, beta, C, out_dtype)
+
+    @staticmethod
+    def jvp(ctx, _alpha, tA, tB, _offsets, _beta, tC, _out_dtype):
+        return _tangent(ctx, _rank_k, tA, tB, tC)
 
     @staticmethod
     def backward(ctx, dD):

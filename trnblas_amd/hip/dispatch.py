@@ -31,6 +31,7 @@ import os
 import warnings
 
 import torch
+from torch.autograd import forward_ad as _fwd
 
 from .._flags import diag_flag, side_flag, trans_flag, uplo_flag
 from . import _lib
@@ -277,7 +278,17 @@ def _mixed_dtypes(*ts) -> bool:
 
 
 def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+    """Whether a result has to carry derivatives: gradients to any of these, or their forward-mode tangents."""
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in ts)) or _has_tangent(*ts)
+
+
+def _forward_mode() -> bool:
+    """Whether a forward-mode level is open (tensors may carry tangents, which `requires_grad` does not tell)."""
+    return _fwd._current_level >= 0
+
+
+def _has_tangent(*ts) -> bool:
+    return _forward_mode() and any(_fwd.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _upload_nbytes(t: torch.Tensor) -> int:
@@ -705,6 +716,7 @@ def gemm_fast(alpha, A, B, beta, C, transA, transB):
         or B.dim() != 2
         or _backend == "pytorch"
         or kern._launch_probe is not None
+        or _forward_mode()
     ):
         return None
     dev = A.get_device()

@@ -13,7 +13,8 @@ in the reference; the products' signatures follow `gemm` and `grouped_gemm`.
 Quantisation of a block: e = floor(log2(max |x|)) - 2 (at least -127), codes
 x / 2^e rounded to nearest even and saturated at 6. A block that holds an
 infinity or a NaN becomes NaN as a whole. There is no gradient through a
-quantised operand: the products refuse operands that require one.
+quantised operand: the products refuse operands that require one or carry
+a forward-mode tangent.
 """
 
 from __future__ import annotations
@@ -190,7 +191,7 @@ def _product(what: str, alpha, A, B, offsets, beta, C, dtype) -> torch.Tensor:
     if (
         beta == 0.0 and type(A) is torch.Tensor and A.is_cuda and type(B) is MXMatrix and len(B.shape) == dims
         and A.dim() == 2 and A.shape[1] == B.shape[-1] and (offsets is None or type(offsets) is torch.Tensor)
-        and not (A.requires_grad and torch.is_grad_enabled()) and _d._use_hip()
+        and not (A.requires_grad and torch.is_grad_enabled()) and not _d._forward_mode() and _d._use_hip()
     ):  # fmt: skip
         try:  # the short way; None: something is out of the ordinary
             D = _gk().mx_gemm_fast(alpha, A, (B.codes, B.scales), offsets, dtype)
