@@ -401,3 +401,23 @@ def test_forward_mode_tangents(dev, dtype):
     a, b = og.grouped_rank_k(1.0, tA, W, off), og.grouped_rank_k(1.0, A, tW, off)
     assert og.excess(P.tangent, a[0] + b[0], a[1] + b[1], 2 * rows) <= 1
     assert M.tangent is not None
+
+
+def test_negated_views(dev):
+    # the imaginary part of a conjugate is a view whose values stand in memory with the other sign
+    for R, K, N in ((150, 64, 128), (150, 1, 1), (150, 33, 1), (4099, 1021, 2043)):  # the last is packed
+        off = _split(R, [17, 33, 1, 64, R - 115])
+        g = torch.Generator(device=dev).manual_seed(K)
+        z = lambda *s: torch.randn(*s, 2, generator=g, device=dev)
+        conj = lambda x: torch.view_as_complex(x).conj().imag
+        a, b, w, c = z(R, K), z(5, K, N), z(R, N), z(R, N)
+        A, B, W, C = (conj(x) for x in (a, b, w, c))
+        assert all(x.is_neg() for x in (A, B, W, C))
+        D = tb.grouped_gemm(1.0, A, B, off.to(dev), 0.5, C)
+        assert og.excess(D, *og.grouped_gemm(1.0, -a[..., 1].cpu(), -b[..., 1].cpu(), off, 0.5, -c[..., 1].cpu()), K) <= 1
+        D = tb.grouped_gemm(1.0, -a[..., 1], B, off.to(dev))
+        assert og.excess(D, *og.grouped_gemm(1.0, -a[..., 1].cpu(), -b[..., 1].cpu(), off), K) <= 1
+        D = tb.grouped_rank_k(1.0, A, W, off.to(dev))
+        assert og.excess(D, *og.grouped_rank_k(1.0, -a[..., 1].cpu(), -w[..., 1].cpu(), off), R) <= 1
+        D = tb.grouped_rank_k(1.0, A, -w[..., 1], off.to(dev))
+        assert og.excess(D, *og.grouped_rank_k(1.0, -a[..., 1].cpu(), -w[..., 1].cpu(), off), R) <= 1

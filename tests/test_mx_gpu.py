@@ -219,3 +219,21 @@ def test_tangents_are_refused(dev):
         with pytest.raises(NotImplementedError, match="no gradient"):
             tb.mx_gemm(1.0, fwd.make_dual(A, A), W)
         assert torch.equal(tb.mx_gemm(1.0, A, W), torch.full((4, 3), 64.0, device=dev))
+
+
+@pytest.mark.parametrize("M,K", [(1, 40), (17, 33), (130, 520)])
+def test_negated_views(dev, M, K):
+    # the imaginary part of a conjugate is a view whose values stand in memory with the other sign
+    g = torch.Generator().manual_seed(M)
+    x, c = torch.randn(M, K, 2, generator=g), torch.randn(M, 24, 2, generator=g)
+    conj = lambda t: torch.view_as_complex(t.to(dev)).conj().imag
+    A, C = conj(x), conj(c)
+    assert A.is_neg() and C.is_neg()
+    _same(tb.mx_quantize(A), -x[..., 1])
+    _same(tb.mx_quantize(A.mT, trans=True), -x[..., 1])
+    _same(tb.mx_quantize(A[None]), -x[None, ..., 1])
+    W = torch.randn(24, K, generator=g)
+    Q = tb.mx_quantize(W.to(dev))
+    a, w = om.quantize(-x[..., 1])[0], om.quantize(W)[0]
+    assert og.excess(tb.mx_gemm(1.0, A, Q), *om.product(1.0, a, w), K) <= 1
+    assert og.excess(tb.mx_gemm(1.0, A, Q, 0.5, C), *om.product(1.0, a, w, None, 0.5, -c[..., 1]), K) <= 1

@@ -32,7 +32,7 @@ def _output_like(C: torch.Tensor | None, beta: float, shape, dtype, dev):
     D = torch.empty(shape, dtype=dtype, device=dev)
     if beta == 0.0 or C is None:
         return D, None
-    c = C.expand(shape)
+    c = C.resolve_neg().expand(shape)
     n = shape[-1]
     return D, c if (c.stride(-1) == 1 or n <= 1) and (c.stride(-2) >= n or shape[-2] <= 1) else c.contiguous()
 
@@ -73,6 +73,7 @@ def grouped_gemm(
 ) -> torch.Tensor:
     """alpha * A[r] @ B[g] + beta * C[r] for the rows r of each group g: A
     (R, K), B (G, K, N) (transposed views are read in place), offsets (G + 1)."""
+    A, B = A.resolve_neg(), B.resolve_neg()
     dev = _require_device(A, B, offsets, *(() if C is None else (C,)))
     R, K = A.shape
     G, _, N = B.shape
@@ -109,6 +110,7 @@ def grouped_rank_k(
 ) -> torch.Tensor:
     """alpha * A_g^T @ B_g + beta * C[g] for each group g of the rows of A
     (R, M) and B (R, N): (G, M, N)."""
+    A, B = A.resolve_neg(), B.resolve_neg()
     dev = _require_device(A, B, offsets, *(() if C is None else (C,)))
     R, M = A.shape
     N = B.shape[1]
@@ -144,6 +146,7 @@ def mx_buffers(shape, dev) -> tuple[torch.Tensor, torch.Tensor]:
 
 def mx_quantize(X: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of X (R, K) or (batch, R, K), any strides."""
+    X = X.resolve_neg()
     dev = _require_device(X)
     codes, scales = mx_buffers(X.shape, dev)
     if any(s < 0 for s in X.stride()):
@@ -177,6 +180,7 @@ def mx_gemm_from(
     C: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """`mx_gemm` of a float A (R, K), quantised on the way (in the same call)."""
+    A = A.resolve_neg()
     dev = _require_device(A, *b, *(() if C is None else (C,)), *(() if offsets is None else (offsets,)))
     if any(s < 0 for s in A.stride()):
         A = A.contiguous()
@@ -261,7 +265,7 @@ def grouped_gemm_fast(alpha, A, B, offsets, transB, out_dtype):
     if (
         k != K or s1 != 1 or lda < K or t1 != 1 or t0 < b1 or sb < 0 or N == 0 or dev < 0
         or B.get_device() != dev or offsets.get_device() != dev or offsets.dtype not in _INTS
-        or offsets.shape != (G + 1,) or offsets.stride() != (1,)
+        or offsets.shape != (G + 1,) or offsets.stride() != (1,) or A.is_neg() or B.is_neg()
     ):  # fmt: skip
         return None
     if out_dtype is not None and out_dtype is not A.dtype and out_dtype is not torch.float32:
@@ -291,7 +295,7 @@ def mx_gemm_fast(alpha, A, b, offsets, out_dtype):
     sr, sk = A.stride()
     dev = A.get_device()
     N = codes.shape[-2]
-    if dev < 0 or codes.get_device() != dev or sr < 0 or sk < 0 or N == 0:
+    if dev < 0 or codes.get_device() != dev or sr < 0 or sk < 0 or N == 0 or A.is_neg():
         return None
     G, o, o64 = 1, None, False
     if offsets is not None:
@@ -324,6 +328,7 @@ def grouped_rank_k_fast(alpha, A, B, offsets, out_dtype):
     if (
         R2 != R or s1 != 1 or lda < M or t1 != 1 or ldb < N or M == 0 or N == 0 or dev < 0 or B.get_device() != dev
         or offsets.get_device() != dev or offsets.dtype not in _INTS or offsets.dim() != 1 or offsets.stride() != (1,)
+        or A.is_neg() or B.is_neg()
     ):  # fmt: skip
         return None
     if out_dtype is not None and out_dtype is not A.dtype and out_dtype is not torch.float32:
@@ -350,7 +355,7 @@ def mx_quantize_fast(X):
         return None
     R, K = X.shape
     sr, sk = X.stride()
-    if sr < 0 or sk < 0:
+    if sr < 0 or sk < 0 or X.is_neg():
         return None
     codes = X.new_empty((R, -(-K // 32) * 16), dtype=torch.uint8)
     scales = X.new_empty((-(-R // 16), -(-K // 512), 256), dtype=torch.uint8)
