@@ -255,12 +255,19 @@ def available() -> bool:
 
 
 def call(name: str, *args) -> int:
-    """Call C-ABI function `name`; raise HipKernelError on a negative return."""
+    """Call C-ABI function `name`; raise HipKernelError on a negative return.
+    A last argument from `stream_of` for a device that is not the current one
+    makes it current for the call: the null stream and the kernels loaded are
+    the current device's."""
     lib = load()
     fn = getattr(lib, name, None)
     if fn is None:
         raise HipLibraryError(f"{LIB_PATH} does not export {name} (rebuild)")
-    rc = fn(*args)
+    if args and type(args[-1]) is _OtherDevice:
+        with torch.cuda.device(args[-1].index):
+            rc = fn(*args)
+    else:
+        rc = fn(*args)
     if rc < 0:
         msg = lib.trnblas_hip_last_error()
         raise HipKernelError(name, rc, msg.decode() if msg else "")
@@ -271,12 +278,27 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+class _OtherDevice(int):
+    """A stream of a device that is not the current one (`index`)."""
+
+    index: int
+
+
+def is_current(index: int) -> bool:
+    """Whether the device is the current one: a call that launches without `call` serves no other."""
+    return torch._C._cuda_getDevice() == index
+
+
 def stream_of(device: torch.device) -> int:
     """hipStream_t of torch's current stream on `device`, as an int (the raw
     lookup: torch.cuda.current_stream builds a Stream object per call, a few
-    microseconds on every launch)."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    return torch._C._cuda_getCurrentRawStream(idx)
+    microseconds on every launch). `call` makes the device current for it."""
+    idx = device.index
+    if idx is None or is_current(idx):
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
+    stream = _OtherDevice(torch._C._cuda_getCurrentRawStream(idx))
+    stream.index = idx
+    return stream
 
 
 def broadcast_shapes(a, b) -> tuple:

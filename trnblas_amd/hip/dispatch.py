@@ -720,7 +720,7 @@ def gemm_fast(alpha, A, B, beta, C, transA, transB):
     ):
         return None
     dev = A.get_device()
-    if B.get_device() != dev or (torch.is_grad_enabled() and (A.requires_grad or B.requires_grad)):
+    if not _lib.is_current(dev) or B.get_device() != dev or (torch.is_grad_enabled() and (A.requires_grad or B.requires_grad)):
         return None
     policy = os.environ.get("TRNBLAS_NATIVE_GEMM")
     if policy is not None and policy.strip().lower() not in ("auto", "hip", "nki"):
