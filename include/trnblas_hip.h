@@ -563,7 +563,9 @@ int trnblas_hip_trsm(int dtype, int64_t n, int64_t nrhs, int upper, int unit, do
  * ones give wrong rows but no access outside the operands.
  * dtype: TRNBLAS_F32, TRNBLAS_BF16 or TRNBLAS_F16, the element type of A and B;
  * C and D have it too, or are fp32 for out_f32 != 0. Sums are fp32, with one
- * rounding at the end. All matrices are row-major with any leading dimension
+ * rounding at the end; those of an fp32 result of 16-bit operands are chains of at
+ * most 4096 values of k (same-sign values: within 2e-6 of |alpha| |A| |B| + |beta C|, whatever
+ * K or the rows of a group). All matrices are row-major with any leading dimension
  * and alignment; 16-byte aligned operands whose leading dimensions, strides and
  * K (N where B is N-contiguous; M and N for grouped_rank_k) are multiples of 16
  * bytes run faster. padded != 0: every row of A and B (16-byte aligned, as
@@ -623,7 +625,7 @@ int trnblas_hip_mx_dequantize(int dtype, int64_t R, int64_t K, const void* codes
 /*
  * D[r] = alpha A[r] B[g]^T + beta C[r] for the rows r of group g (D[r] =
  * beta C[r] for rows of no group): A rows x K, B groups matrices of N x K, both
- * microscaled; products exact, sums fp32. C and D (rows x N) have the type
+ * microscaled; products exact, sums fp32 (one chain, 128 values of K each addition). C and D (rows x N) have the type
  * out_dtype. offsets as in trnblas_hip_grouped_gemm; NULL (groups == 1): one
  * matrix for all rows.
  */

@@ -421,3 +421,59 @@ def test_negated_views(dev):
         assert og.excess(D, *og.grouped_rank_k(1.0, -a[..., 1].cpu(), -w[..., 1].cpu(), off), R) <= 1
         D = tb.grouped_rank_k(1.0, A, -w[..., 1], off.to(dev))
         assert og.excess(D, *og.grouped_rank_k(1.0, -a[..., 1].cpu(), -w[..., 1].cpu(), off), R) <= 1
+
+
+# fp32 results of 16-bit operands: sums in chains of at most 4096 values, of which the largest error on same-sign values was
+# measured as 1.43e-6 |A||B| (a single chain: 2.2e-6 after 8192, 3.9e-6 after 32768); several chains average their errors.
+CHAIN_GATE = 2e-6
+LONG = {  # (op, groups, rows, M, N, K)
+    "ring_kernel 256 x 256": [(1, 3, 36000, 2056, 2312, 0), (0, 3, 5200, 0, 2312, 16392)],
+    "ring_kernel 128 x 128": [(1, 2, 36000, 1032, 1288, 0), (0, 3, 2600, 0, 1288, 16392)],
+    "ring_kernel 64 x 128": [(1, 2, 36000, 264, 520, 0), (0, 1, 600, 0, 520, 33000)],
+    "rows_kernel": [(0, 1, 9, 0, 520, 66000)],
+    "ring_kernel 64 x 128, rows_kernel": [(0, 8, 9, 0, 4104, 33000)],  # by transB
+    "grouped_any_kernel": [(1, 2, 36000, 129, 260, 0), (0, 2, 70, 0, 260, 33001)],
+}
+
+
+def _gemm_ref(A, B, off, transB):
+    """(A B, |A| |B|) in float64 on A's device."""
+    ref, den = torch.zeros(2, A.shape[0], B.shape[1 if transB else 2], dtype=torch.float64, device=A.device)
+    for j, a, b in og.rows_of(off, A.shape[0]):
+        W = (B[j].T if transB else B[j]).double().contiguous()
+        ref[a:b], den[a:b] = A[a:b].double() @ W, A[a:b].double().abs() @ W.abs()
+    return ref, den
+
+
+def _rank_k_ref(A, B, off):
+    ref, den = torch.zeros(2, off.shape[0] - 1, A.shape[1], B.shape[1], dtype=torch.float64, device=A.device)
+    for j, a, b in og.rows_of(off, A.shape[0]):
+        left = A[a:b].double().T.contiguous()
+        ref[j], den[j] = left @ B[a:b].double(), left.abs() @ B[a:b].double().abs()
+    return ref, den
+
+
+def _relative(D, ref, den):
+    return float(((D.double() - ref).abs() / den.clamp_min(2.0**-100)).max())
+
+
+@pytest.mark.parametrize("kernel", list(LONG))
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_fp32_results_of_16_bit_operands_over_long_k(dev, dtype, kernel):
+    for i, (op, G, R, M, N, K) in enumerate(LONG[kernel]):
+        g = torch.Generator(device=dev).manual_seed(i)
+        rand = lambda *s: torch.rand(*s, generator=g, device=dev).to(dtype)
+        off = _uneven(G, R, i)
+        for transB in (False, True) if op == 0 else (False,):
+            assert _plan(op, dtype, transB, G, R, M, N, K) == kernel.split(", ")[-1 if transB else 0]
+            if op == 0:
+                A, B = rand(R, K), rand(G, *((N, K) if transB else (K, N)))
+                ref, den = _gemm_ref(A, B, off, transB)
+                call = lambda *c: tb.grouped_gemm(1.0, A, B, off.to(dev), *c, transB=transB, dtype=F32)
+            else:
+                A, B = rand(R, M), rand(R, N)
+                ref, den = _rank_k_ref(A, B, off)
+                call = lambda *c: tb.grouped_rank_k(1.0, A, B, off.to(dev), *c, dtype=F32)
+            assert _relative(call(), ref, den) <= CHAIN_GATE, (op, G, R, transB)
+            C = 100.0 * torch.rand(ref.shape, generator=g, device=dev)
+            assert _relative(call(0.5, C), ref + 0.5 * C.double(), den + 0.5 * C.double()) <= CHAIN_GATE, (op, G, R, transB)

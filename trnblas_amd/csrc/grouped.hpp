@@ -34,6 +34,22 @@ struct GroupedArgs {
   int vec4;   // D and C take 4-element accesses (aligned, ld % 4 == 0)
 };
 
+// An fp32 result of 16-bit operands is summed in chains of at most so many values of k. One chain
+// is a random walk of its roundings: the largest error of same-sign products over |A||B| was
+// 7.3e-7 after 1024 values, 1.4e-6 after 4096, 2.2e-6 after 8192 and 8.7e-6 after 131072 (bf16 and
+// fp16 alike); chains leave 1.4e-6 at 4096 and less from there on. (A 16-bit result is
+// rounded to 2^-9 or 2^-12 at its end: one chain.) The kernels that restart their sums are CHAINS
+// ones, launched where k is longer: a second set of sums in every one would cost the
+// others' occupancy (rows_kernel of two blocks 126 registers, 135 with them: one workgroup
+// per CU instead of two).
+constexpr int kChain16 = 4096;
+
+// Whether such a product (k: its rows where these are ragged) needs them.
+template <typename T>
+inline bool needs_chains(const GroupedArgs& g, int64_t k) {
+  return sizeof(T) == 2 && g.out32 && k > kChain16;
+}
+
 // Boundaries of the row segments: 0, offsets[0 .. groups], rows. Segment 0
 // (rows before the first group) and segment groups + 1 (rows after the last)
 // belong to no group; segment i is group i - 1. Every boundary is clamped to

@@ -117,9 +117,9 @@ struct Loads {
 
 // Operands of any alignment and any strides: the panels go through registers.
 // 256 threads on a 64 x 64 tile, each wave 32 x 32; the loads of k-tile t + 2 are in
-// flight behind the MFMAs of t. fp32 sums restart every chain_length(K) values of k
-// (gemm.hpp). fp32 gemm takes 32 x 64: its MFMAs are eight times as long, so that the
-// last round's idle CUs cost more than the smaller tile's loads (1501 rows in 6 groups
+// flight behind the MFMAs of t. fp32 and CHAINS (see kChain16): the sums restart every
+// chain_length(K) values of k (gemm.hpp). fp32 gemm takes 32 x 64: its MFMAs are eight
+// times as long, so that the last round's idle CUs cost more than the smaller tile's loads (1501 rows in 6 groups
 // by 515 x 771: 360 tiles 31 us, 720 tiles 27; 4093 by 2047^2 385 and 393). 16-bit:
 // bound by the loads of rows that start anywhere (16 bytes two bytes past a word take
 // several times as long; the five words around them, shifted, longer still): bf16 4093
@@ -128,13 +128,13 @@ struct Loads {
 // merge waited for all loads. Larger products are packed first.
 template <typename T, bool RK>
 constexpr int any_fm = std::is_same_v<T, float> && !RK ? 1 : 2;
-template <typename T, bool BKC, bool RK, bool TINY>
+template <typename T, bool BKC, bool RK, bool TINY, bool CHAINS = false>
 __global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
   constexpr int FM = any_fm<T, RK>, FN = 2, BM = 32 * FM, BN = 32 * FN, AHEAD = 2;
   using PA = Panel<T, BM, !RK>;
   using PB = Panel<T, BN, BKC>;
   constexpr int BK = PA::BK, ES = sizeof(T), HA = PA::BYTES / 4096, HB = PB::BYTES / 4096;
-  constexpr bool FOLD = std::is_same_v<T, float>;
+  constexpr bool F32 = std::is_same_v<T, float>, FOLD = F32 || CHAINS;
   __shared__ __attribute__((aligned(16))) char lds[2][PA::BYTES + PB::BYTES];
   TileJob j;
   if (!tile_job<T, BM, BN, BKC, RK>(g, j)) return;
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256, 3) void grouped_any_kernel(GroupedArgs g) {
       for (int a = 0; a < FM; ++a) fa[a] = PA::frag(qa, a, h);
 #pragma unroll
       for (int b = 0; b < FN; ++b) fb[b] = PB::frag(qb, b, h);
-      if constexpr (FOLD) {  // four products per sum: the sums in turn
+      if constexpr (F32) {  // four products per sum: the sums in turn
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -260,8 +260,12 @@ static int run_any(GroupedArgs g, hipStream_t s) {
   grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
   constexpr int EV = 16 / sizeof(T);
   const bool tiny = (RK ? g.M : g.K) < EV || (BKC ? g.K : g.N) < EV;
-  hipLaunchKernelGGL((tiny ? grouped_any_kernel<T, BKC, RK, true> : grouped_any_kernel<T, BKC, RK, false>), dim3(grid), dim3(256), 0,
-                     s, g);
+  auto kernel = tiny ? grouped_any_kernel<T, BKC, RK, true> : grouped_any_kernel<T, BKC, RK, false>;
+  if constexpr (sizeof(T) == 2) {
+    if (needs_chains<T>(g, RK ? g.rows : g.K))
+      kernel = tiny ? grouped_any_kernel<T, BKC, RK, true, true> : grouped_any_kernel<T, BKC, RK, false, true>;
+  }
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, g);
   return check_launch(what);
 }
 
@@ -289,7 +293,11 @@ static int run_ring(GroupedArgs g, hipStream_t s) {
   unsigned grid;
   const int64_t rows = RK ? (int64_t)g.groups * g.tiles_m : row_tiles(g.rows, g.groups, BM);
   if (int rc = grid_of(ring_grid<FM, FN>(g, rows * g.tiles_n), what, &grid)) return rc;
-  hipLaunchKernelGGL((ring_kernel<T, FM, FN, BKC, RK>), dim3(grid), dim3(256), 0, s, g, MxScales{});
+  auto kernel = ring_kernel<T, FM, FN, BKC, RK>;
+  if constexpr (sizeof(T) == 2) {
+    if (needs_chains<T>(g, RK ? g.rows : g.K)) kernel = ring_kernel<T, FM, FN, BKC, RK, true>;
+  }
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, g, MxScales{});
   return check_launch(what);
 }
 
@@ -300,7 +308,11 @@ static int run_rows(GroupedArgs g, hipStream_t s) {
   unsigned grid;
   if (int rc = grid_of(row_tiles(g.rows, g.groups, 16 * MF) * g.tiles_n, kGemm, &grid)) return rc;
   grid = (grid + kNumXcd - 1) / kNumXcd * kNumXcd;
-  hipLaunchKernelGGL((rows_kernel<T, MF, NF, KS, BKC>), dim3(grid), dim3(512), 0, s, g, MxScales{});
+  auto kernel = rows_kernel<T, MF, NF, KS, BKC>;
+  if constexpr (sizeof(T) == 2) {
+    if (needs_chains<T>(g, g.K / KS)) kernel = rows_kernel<T, MF, NF, KS, BKC, void, true>;  // a wave's share
+  }
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(512), 0, s, g, MxScales{});
   return check_launch(kGemm);
 }
 

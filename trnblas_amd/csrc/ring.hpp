@@ -165,8 +165,8 @@ struct RingLds {
   static constexpr int BYTES = NS * STAGE + SRING * SGROUP;
 };
 
-template <typename T, int FM, int FN, bool BKC, bool RK>
-__device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& x, const TileJob& j, char* lds) {
+template <typename T, int FM, int FN, bool BKC, bool RK, bool CHAINS>
+__device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& x, const TileJob& j, int wave, char* lds) {
   constexpr bool MX = std::is_same_v<T, fp4x2>, FOLD = std::is_same_v<T, float>;
   using L = RingLds<T, FM, FN>;
   constexpr int WAVES = 4, BM = L::BM, BN = L::BN, NS = L::NS, SA = L::SA, SB = L::SB, SGROUP = L::SGROUP, SRING = L::SRING;
@@ -177,8 +177,9 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
   constexpr int STAGE = L::STAGE;
   constexpr int ND = DA::NB + DB::NB;  // DMAs per wave and k-tile, besides scales
   static_assert(STAGE == PA::BYTES + PB::BYTES && SA + SB <= 16, "one scale DMA per wave and step");
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int lane = threadIdx.x & 63;
+  if constexpr (CHAINS)  // anew in each chain: 256 x 256 tiles can keep neither it nor the addresses made of it
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
   const int m0 = (wave & 1) * (16 * FM), n0 = (wave >> 1) * (16 * FN);
   const int nk = (j.K + PA::BK - 1) / PA::BK;
   const uint32_t lds0 = lds_offset(lds);
@@ -378,7 +379,7 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
   static_assert(4 * kStoreLds<FN> <= L::BYTES);
   char* own = lds + wave * kStoreLds<FN>;
   if (!(g.vec4 && (g.N & 3) == 0)) __syncthreads();  // the other waves' reads
-  if (g.out32)
+  if (CHAINS || g.out32)
     store_wave<FM, FN, float>(g, j, acc, m0, n0, lane, own);
   else if (MX && g.out_f16)
     store_wave<FM, FN, _Float16>(g, j, acc, m0, n0, lane, own);
@@ -386,7 +387,39 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
     store_wave<FM, FN, O>(g, j, acc, m0, n0, lane, own);
 }
 
-template <typename T, int FM, int FN, bool BKC, bool RK>
+// An address that all lanes have, as a scalar.
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t a = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)a), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+  return reinterpret_cast<const char*>((uint64_t)hi << 32 | lo);
+}
+
+// CHAINS (see kChain16): 256 x 256 tiles have no registers for a second set of sums, so each
+// chain after the first takes its sum from D. 32768 rows in 2 groups by 4096 x 2048 take 455 us with
+// these round trips, 396 as one chain; where no group has a second chain the kernel costs 3 %.
+template <typename T, int FM, int FN, bool BKC, bool RK, bool CHAINS>
+__device__ __forceinline__ void ring_chains(GroupedArgs g, const MxScales& x, TileJob j, char* lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if constexpr (!CHAINS) {
+    ring_tile<T, FM, FN, BKC, RK, false>(g, x, j, wave, lds);
+  } else {
+    // what the loop carries, in scalar registers
+    j.A = uniform(j.A), j.B = uniform(j.B), j.D = const_cast<char*>(uniform(static_cast<char*>(j.D)));
+    j.C = uniform(static_cast<const char*>(j.C));
+    for (int left = __builtin_amdgcn_readfirstlane(j.K);;) {
+      j.K = min(left, kChain16);
+      ring_tile<T, FM, FN, BKC, RK, true>(g, x, j, wave, lds);
+      left -= j.K;
+      if (left <= 0) return;
+      j.A += j.K * (RK ? g.lda : 1) * (int64_t)sizeof(T);
+      j.B += j.K * (BKC ? 1 : g.ldb) * (int64_t)sizeof(T);
+      j.C = j.D, g.ldc = g.ldd, g.beta = 1.0f;  // each lane reads what it wrote
+      __syncthreads();  // the other waves' LDS reads, before the next chain's DMAs
+    }
+  }
+}
+
+template <typename T, int FM, int FN, bool BKC, bool RK, bool CHAINS = false>
 __global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(GroupedArgs g, MxScales x) {
   constexpr bool SPLIT = FM * FN == 64;  // one workgroup per CU: see tile_of
   __shared__ __attribute__((aligned(16))) char lds[RingLds<T, FM, FN>::BYTES];
@@ -394,11 +427,11 @@ __global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(Groupe
   if (!tile_job<T, 32 * FM, 32 * FN, BKC, RK, SPLIT>(g, j)) return;
   if constexpr (SPLIT) {
     if (j.quarter >= 0) {
-      ring_tile<T, FM / 2, FN / 2, BKC, RK>(g, x, j, lds);
+      ring_chains<T, FM / 2, FN / 2, BKC, RK, CHAINS>(g, x, j, lds);
       return;
     }
   }
-  ring_tile<T, FM, FN, BKC, RK>(g, x, j, lds);
+  ring_chains<T, FM, FN, BKC, RK, CHAINS>(g, x, j, lds);
 }
 
 // Workgroups of such a launch over `tiles` tiles (or at most so many), SPLIT's

@@ -114,14 +114,15 @@ __device__ __forceinline__ void quantize_rows(const GroupedArgs& g, const MxScal
 // bytes along a row lie inside it, or in its padding, or outside as a whole (operands
 // that start anywhere: 8 groups of a row, 4095 x 1535, 69 us here with a branch per
 // load, 33 on grouped_any_kernel). One row of bf16 by 4096 x 1536 9 us, 16 groups of a
-// row by 2048 x 4096 58 us (4.6 TB/s); 4-bit 8192^2 and one row 9.4 (3.8). fp32: the sums restart every 512 values of k per wave.
+// row by 2048 x 4096 58 us (4.6 TB/s); 4-bit 8192^2 and one row 9.4 (3.8). fp32 and CHAINS (see kChain16): the
+// sums restart every 512 values of k per wave.
 //
 // X (4-bit floats only): A comes as values of that type, at most kInPlace in the
 // tile's rows; the workgroup quantises them into LDS behind its first loads of B,
 // which saves a launch of its own (one row of 8192 by 8192^2: 5 us).
-template <typename T, int MF, int NF, int KS, bool BKC, typename X = void>
+template <typename T, int MF, int NF, int KS, bool BKC, typename X = void, bool CHAINS = false>
 __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
-  constexpr bool MX = std::is_same_v<T, fp4x2>, FOLD = std::is_same_v<T, float>;
+  constexpr bool MX = std::is_same_v<T, fp4x2>, FOLD = std::is_same_v<T, float> || CHAINS;
   constexpr int ES = sizeof(T), EV = 16 / ES, BM = 16 * MF, BW = 16 * NF, BN = 8 / KS * BW;
   constexpr int STEPS = rows_steps<T>, CH = 64 * STEPS, CK = CH / ES;  // a chunk: bytes, values of k
   constexpr int U = rows_ahead<T>(MF, NF);
