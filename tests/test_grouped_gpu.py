@@ -477,3 +477,26 @@ def test_fp32_results_of_16_bit_operands_over_long_k(dev, dtype, kernel):
             assert _relative(call(), ref, den) <= CHAIN_GATE, (op, G, R, transB)
             C = 100.0 * torch.rand(ref.shape, generator=g, device=dev)
             assert _relative(call(0.5, C), ref + 0.5 * C.double(), den + 0.5 * C.double()) <= CHAIN_GATE, (op, G, R, transB)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gradient_of_an_fp32_result_is_not_rounded(dev, dtype):
+    # its values pass the range of fp16 and fall below it, and have more bits than a 16-bit type holds
+    rows, sizes, K, N = 60, [9, 21, 0, 25], 24, 40
+    off = _split(rows, sizes)
+    g = torch.Generator().manual_seed(12)
+    A, B = (torch.randn(rows, K, generator=g) * 1e-3).to(dtype), (torch.randn(4, K, N, generator=g) * 2e-3).to(dtype)
+    dD = torch.randn(rows, N, generator=g) * torch.tensor([1e5, 1e-5]).repeat_interleave(rows // 2)[:, None]
+    for transB in (False, True):
+        b0 = B.mT.contiguous() if transB else B
+        a, b = A.to(dev).requires_grad_(), b0.to(dev).requires_grad_()
+        D = tb.grouped_gemm(2.0, a, b, off.to(dev), transB=transB, dtype=torch.float32)
+        dA, dB = torch.autograd.grad(D, (a, b), dD.to(dev))
+        assert dA.dtype == dB.dtype == dtype
+        assert og.excess(dA, *og.grouped_gemm(2.0, dD, b0, off, transB=not transB), N) <= 1
+        assert og.excess(dB, *og.grouped_rank_k(2.0, *((dD, A) if transB else (A, dD)), off), rows) <= 1
+    W, dP = (torch.randn(rows, N, generator=g) * 1e-3).to(dtype), torch.randn(4, K, N, generator=g) * 1e5
+    a, w = A.to(dev).requires_grad_(), W.to(dev).requires_grad_()
+    dA, dW = torch.autograd.grad(tb.grouped_rank_k(1.0, a, w, off.to(dev), dtype=torch.float32), (a, w), dP.to(dev))
+    assert og.excess(dA, *og.grouped_gemm(1.0, W, dP.mT, off), N) <= 1
+    assert og.excess(dW, *og.grouped_gemm(1.0, A, dP, off), K) <= 1

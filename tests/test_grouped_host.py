@@ -47,6 +47,29 @@ def test_gradients_against_differences():
     assert torch.autograd.gradgradcheck(lambda a, b: tb.grouped_gemm(0.7, a, b, off), (A, B))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradient_of_an_fp32_result_is_not_rounded(dtype):
+    # its values pass the range of fp16 and fall below it, and have more bits than a 16-bit type holds
+    rows, K, N = 60, 24, 40
+    off = _offsets(0, 9, 30, 30, 55)
+    g = torch.Generator().manual_seed(12)
+    A, B = (torch.randn(rows, K, generator=g) * 1e-3).to(dtype), (torch.randn(4, K, N, generator=g) * 2e-3).to(dtype)
+    dD = torch.randn(rows, N, generator=g) * torch.tensor([1e5, 1e-5]).repeat_interleave(rows // 2)[:, None]
+    for transB in (False, True):
+        b0 = B.mT.contiguous() if transB else B
+        a, b = A.clone().requires_grad_(), b0.clone().requires_grad_()
+        D = tb.grouped_gemm(2.0, a, b, off, transB=transB, dtype=torch.float32)
+        dA, dB = torch.autograd.grad(D, (a, b), dD)
+        assert dA.dtype == dB.dtype == dtype
+        assert og.excess(dA, *og.grouped_gemm(2.0, dD, b0, off, transB=not transB), N) <= 1
+        assert og.excess(dB, *og.grouped_rank_k(2.0, *((dD, A) if transB else (A, dD)), off), rows) <= 1
+    W, dP = (torch.randn(rows, N, generator=g) * 1e-3).to(dtype), torch.randn(4, K, N, generator=g) * 1e5
+    a, w = A.clone().requires_grad_(), W.clone().requires_grad_()
+    dA, dW = torch.autograd.grad(tb.grouped_rank_k(1.0, a, w, off, dtype=torch.float32), (a, w), dP)
+    assert og.excess(dA, *og.grouped_gemm(1.0, W, dP.mT, off), N) <= 1
+    assert og.excess(dW, *og.grouped_gemm(1.0, A, dP, off), K) <= 1
+
+
 def _products(off):
     return (
         lambda a, b, c, w, s: tb.grouped_gemm(0.7, a, b, off, 0.3, c),

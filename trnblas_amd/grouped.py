@@ -8,7 +8,9 @@ fused). Both are differentiable, and each other's gradients:
     D = grouped_gemm(A, B)     dA = grouped_gemm(dD, B^T)   dB = grouped_rank_k(A, dD)
     D = grouped_rank_k(A, B)   dA = grouped_gemm(B, dD^T)   dB = grouped_gemm(A, dD)
 
-and in forward mode, with tangents tA, tB and tC, tD = alpha (tA B + A tB) + beta tC.
+The gradient of an fp32 result of 16-bit operands meets them in fp32 (those
+products run at the fp32 rate) and is rounded to their type once, at the end. In
+forward mode, with tangents tA, tB and tC: tD = alpha (tA B + A tB) + beta tC.
 
 `offsets` (int32 or int64, groups + 1 entries, nondecreasing) gives group g the
 rows offsets[g] .. offsets[g + 1] - 1; groups may be empty, and rows before
@@ -126,6 +128,15 @@ def _differentiable(function, product, *args):
     return function.apply(*args) if torch.is_grad_enabled() or _d._forward_mode() else product(*args)
 
 
+def _widened(dD, A, B):
+    """The operands of a backward product in one type: an fp32 gradient is not rounded to 16-bit operands' type, whose
+    range (fp16: 65504) it may pass."""
+    if dD.dtype == A.dtype:
+        return dD, A, B
+    wide = torch.promote_types(dD.dtype, A.dtype)
+    return dD.to(wide), A.to(wide), B.to(wide)
+
+
 def _tangent(ctx, product, tA, tB, tC):
     """The tangent of a product, summed in fp32 at least and rounded once."""
     A, B, offsets = ctx.saved_for_forward
@@ -160,15 +171,14 @@ class _GroupedGemm(torch.autograd.Function):
         dA = dB = dC = None
         if ctx.needs_input_grad[5]:
             dC = ctx.beta * dD
-        # an fp32 result of 16-bit operands: its gradient meets them in their type
-        dD = dD.to(A.dtype)
+        dt, (dD, A, B) = A.dtype, _widened(dD, A, B)
         if ctx.needs_input_grad[1]:
-            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, dD, B.mT, offsets, 0.0, None, A.dtype)
+            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, dD, B.mT, offsets, 0.0, None, dD.dtype).to(dt)
         if ctx.needs_input_grad[2]:
             if B.stride(1) == 1 and B.stride(2) > 1:  # B is a transposed view: so is its gradient
-                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, dD, A, offsets, 0.0, None, B.dtype).mT
+                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, dD, A, offsets, 0.0, None, dD.dtype).to(dt).mT
             else:
-                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
+                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, A, dD, offsets, 0.0, None, dD.dtype).to(dt)
         return None, dA, dB, None, None, dC, None
 
 
@@ -188,11 +198,11 @@ class _GroupedRankK(torch.autograd.Function):
         dA = dB = dC = None
         if ctx.needs_input_grad[5]:
             dC = ctx.beta * dD
-        dD = dD.to(A.dtype)
+        dt, (dD, A, B) = A.dtype, _widened(dD, A, B)
         if ctx.needs_input_grad[1]:
-            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, B, dD.mT, offsets, 0.0, None, A.dtype)
+            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, B, dD.mT, offsets, 0.0, None, dD.dtype).to(dt)
         if ctx.needs_input_grad[2]:
-            dB = _differentiable(_GroupedGemm, _gemm, ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
+            dB = _differentiable(_GroupedGemm, _gemm, ctx.alpha, A, dD, offsets, 0.0, None, dD.dtype).to(dt)
         return None, dA, dB, None, None, dC, None
 
 
