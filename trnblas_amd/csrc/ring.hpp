@@ -5,6 +5,7 @@
 
 #include "gemm.hpp"
 #include "grouped.hpp"
+#include "grouped_plan.hpp"
 
 namespace trnblas {
 
@@ -164,6 +165,14 @@ struct RingLds {
   static constexpr int SGROUP = std::is_same_v<T, fp4x2> ? 1024 * (SA + SB) : 0, SRING = 2;
   static constexpr int BYTES = NS * STAGE + SRING * SGROUP;
 };
+
+// Whether the plan's entry is of these tiles, and as many of its workgroups fit into a CU's LDS.
+template <typename T, int FM, int FN>
+constexpr bool fits(const RingCost& c) {
+  return c.fm == FM && c.fn == FN && c.per_cu * RingLds<T, FM, FN>::BYTES <= 160 << 10;
+}
+static_assert(fits<__bf16, 8, 8>(kRing16[0]) && fits<__bf16, 4, 4>(kRing16[1]) && fits<__bf16, 2, 4>(kRing16[2]), "16-bit plan");
+static_assert(fits<fp4x2, 8, 8>(kRing4[0]) && fits<fp4x2, 4, 4>(kRing4[1]) && fits<fp4x2, 2, 4>(kRing4[2]), "4-bit plan");
 
 template <typename T, int FM, int FN, bool BKC, bool RK, bool CHAINS>
 __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& x, const TileJob& j, int wave, char* lds) {
