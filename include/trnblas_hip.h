@@ -656,6 +656,14 @@ int trnblas_hip_mx_gemm_from(int dtype, int out_dtype, int64_t groups, int64_t r
 const char* trnblas_hip_grouped_plan(int op, int dtype, int transB, int64_t groups, int64_t rows,
                                      int64_t M, int64_t N, int64_t K);
 
+/*
+ * How the few-rows kernel serves such a call (op 0 or 2): plan[0] blocks of 16 rows per
+ * workgroup, plan[1] waves of a workgroup along K, plan[2] whether mx_gemm_from
+ * quantises a K-contiguous A (sk == 1) inside it (op 2). Zeros where another kernel serves.
+ */
+int trnblas_hip_grouped_rows_plan(int op, int dtype, int transB, int64_t groups, int64_t rows,
+                                  int64_t N, int64_t K, int32_t plan[3]);
+
 #ifdef __cplusplus
 }
 #endif

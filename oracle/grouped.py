@@ -81,3 +81,14 @@ def uneven(groups, rows, seed):
         w[1] = 0
     sizes = (w / w.sum() * (rows - 3)).long()
     return split(rows, sizes.tolist(), 2)
+
+
+def rows_plan(op, dtype, transB, groups, rows, N, K):
+    """(row blocks, waves along K, A quantised inside) of rows_kernel; zeros for another kernel."""
+    import ctypes
+
+    from trnblas_amd.hip import _lib
+
+    out = (ctypes.c_int32 * 3)()
+    _lib.call("trnblas_hip_grouped_rows_plan", op, _lib.DTYPE_CODES[dtype], transB, groups, rows, N, K, out)
+    return tuple(out)

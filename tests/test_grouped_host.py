@@ -166,3 +166,18 @@ def test_c_abi_refusals():
     assert gemm(rows=0) == 0  # nothing to do
     rc = lib.trnblas_hip_grouped_rank_k(1, 0, 2, 6, 4, 3, 1.0, 4096, 3, 4096, 3, 4096, 0, 0.0, None, 3, 0, 4096, 3, 12, 0, None)
     assert rc == _lib.E_ARG and b"leading" in lib.trnblas_hip_last_error()
+
+
+def test_rows_plan_refusals():
+    import ctypes
+
+    from trnblas_amd.hip import _lib
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    lib = _lib.load()
+    out = (ctypes.c_int32 * 3)(7, 7, 7)
+    for bad in ((1, 1, 0, 2, 6, 4, 3), (3, 1, 0, 2, 6, 4, 3), (0, 3, 0, 2, 6, 4, 3), (0, 1, 0, 0, 6, 4, 3), (0, 1, 0, 2, 6, 0, 3)):
+        assert lib.trnblas_hip_grouped_rows_plan(*bad, out) == _lib.E_ARG and b"bad arguments" in lib.trnblas_hip_last_error()
+    assert lib.trnblas_hip_grouped_rows_plan(0, 1, 0, 2, 6, 64, 64, None) == _lib.E_ARG
+    assert lib.trnblas_hip_grouped_rows_plan(0, 1, 0, 1, 30000, 4096, 4096, out) == 0 and not any(out)

@@ -6,7 +6,7 @@ import torch
 import trnblas_amd as tb
 from oracle import grouped as og
 from oracle import mx as om
-from oracle.grouped import GROUPS, plan, uneven
+from oracle.grouped import GROUPS, plan, rows_plan, uneven
 from oracle.grouped import split as _split
 from oracle.mx import wide as _wide
 
@@ -237,3 +237,44 @@ def test_negated_views(dev, M, K):
     a, w = om.quantize(-x[..., 1])[0], om.quantize(W)[0]
     assert og.excess(tb.mx_gemm(1.0, A, Q), *om.product(1.0, a, w), K) <= 1
     assert og.excess(tb.mx_gemm(1.0, A, Q, 0.5, C), *om.product(1.0, a, w, None, 0.5, -c[..., 1]), K) <= 1
+
+
+# (groups, rows, N, K) by what rows_kernel does with them: (blocks of 16 rows, waves along K, A of values quantised inside).
+# Columns end inside a tile, and where waves split the columns some of them lie past N as a whole.
+ROWS = {
+    (2, 8, 0): [(1, 20, 72, 2056), (2, 30, 200, 1030)],
+    (2, 4, 0): [(13, 801, 520, 64), (5, 200, 2056, 64)],
+    (2, 2, 0): [(57, 1140, 520, 64)],
+    (2, 1, 0): [(64, 3968, 1032, 64)],
+    (1, 8, 0): [(16, 60, 200, 2050), (64, 320, 72, 2056)],
+    (1, 8, 1): [(16, 60, 200, 2048), (2, 9, 520, 1030)],
+    (1, 4, 1): [(41, 287, 520, 520), (5, 5, 4104, 520)],
+    (1, 2, 1): [(9, 18, 4104, 64), (64, 448, 520, 64)],
+    (1, 1, 1): [(57, 399, 1032, 64), (23, 23, 4104, 520), (57, 399, 4104, 1030)],
+}
+
+
+@pytest.mark.parametrize("how", list(ROWS))
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_each_form_of_the_few_rows_kernel(dev, dtype, how):
+    for G, R, N, K in ROWS[how]:
+        assert rows_plan(2, dtype, 1, G, R, N, K) == how
+        g = torch.Generator(device=dev).manual_seed(R)
+        # one group fills a block of 16 rows where there are several groups, the others share what is left unevenly
+        sizes = torch.bincount(torch.arange(R - min(R, 16 * (G > 1))) % max(G - 1, 1) + (G > 1), minlength=G)
+        sizes[0] = R if G == 1 else min(R, 16)
+        off = _split(R, sizes.tolist())
+        A = torch.randn(R, K + 6, generator=g, device=dev) * torch.exp2(torch.arange(R, device=dev) % 7)[:, None]
+        A = A.to(dtype)[:, 3:-3]
+        E = tb.mx_quantize(torch.randn(G, N, K, generator=g, device=dev))
+        q = tb.mx_quantize(A)
+        ref, den = torch.zeros(2, R, N, dtype=torch.float64, device=dev)
+        for j, a, b in og.rows_of(off, R):
+            x, W = q.dequantize().double()[a:b], E[j].dequantize().double().T.contiguous()
+            ref[a:b], den[a:b] = x @ W, x.abs() @ W.abs()
+        ref, den = ref.cpu(), den.cpu()
+        for x in (A, A.contiguous(), q):
+            D = tb.mx_grouped_gemm(1.0, x, E, off.to(dev), dtype=F32)
+            assert og.excess(D.cpu(), ref, den, K) <= 1, (G, R, N, K)
+        if G == 1:
+            assert og.excess(tb.mx_gemm(1.0, A, E[0], dtype=F32).cpu(), ref, den, K) <= 1

@@ -6,6 +6,7 @@
 //    group g (the gradient of the former to B).
 // The group boundaries are read on the device: nothing waits for the host.
 #include <algorithm>
+#include <cstring>
 
 #include "grouped.hpp"
 #include "grouped_plan.hpp"
@@ -98,6 +99,23 @@ extern "C" int trnblas_hip_grouped_rank_k(int dtype, int out_f32, int64_t groups
   }
 }
 
+static GroupedChoice gemm_choice(int op, int64_t es, int transB, int64_t groups, int64_t rows, int64_t N, int64_t K) {
+  return op == 2 ? choose_mx(rows, groups, N, K) : choose_grouped(kRing16, rows, groups, N, K, (double)K * es, es, transB != 0);
+}
+
+extern "C" int trnblas_hip_grouped_rows_plan(int op, int dtype, int transB, int64_t groups, int64_t rows, int64_t N, int64_t K,
+                                             int32_t plan[3]) {
+  TRNBLAS_CHECK_ARG(plan != nullptr && op != 1, "trnblas_hip_grouped_rows_plan: bad arguments");
+  const char* name = trnblas_hip_grouped_plan(op, dtype, transB, groups, rows, 0, N, K);
+  TRNBLAS_CHECK_ARG(name != nullptr, "trnblas_hip_grouped_rows_plan: bad arguments");
+  plan[0] = plan[1] = plan[2] = 0;
+  if (strcmp(name, "rows_kernel") != 0) return TRNBLAS_OK;
+  const GroupedChoice c = gemm_choice(op, dtype == TRNBLAS_F32 ? 4 : 2, transB, groups, rows, N, K);
+  plan[0] = c.mf, plan[1] = c.ks;
+  plan[2] = op == 2 && quantised_in_place(c, rows, K);
+  return TRNBLAS_OK;
+}
+
 extern "C" const char* trnblas_hip_grouped_plan(int op, int dtype, int transB, int64_t groups, int64_t rows, int64_t M, int64_t N,
                                                 int64_t K) {
   static const char* const kRingNames[] = {"ring_kernel 256 x 256", "ring_kernel 128 x 128", "ring_kernel 64 x 128"};
@@ -107,13 +125,8 @@ extern "C" const char* trnblas_hip_grouped_plan(int op, int dtype, int transB, i
     return nullptr;
   }
   if (op < 2 && (first * es % 16 != 0 || second * es % 16 != 0)) return "grouped_any_kernel";
-  int ring;
-  if (op == 1)
-    ring = choose_rank_k(groups, M, N, (double)rows / groups * es / 128.0);
-  else if (op == 2)
-    ring = choose_grouped(kRing4, rows, groups, N, (double)((K + 31) / 32 * 16), (double)((K + 31) / 32 * 16), 17.0 / 16.0, true).ring;
-  else
-    ring = choose_grouped(kRing16, rows, groups, N, K, (double)K * es, es, transB != 0).ring;
+  const int ring = op == 1 ? choose_rank_k(groups, M, N, (double)rows / groups * es / 128.0)
+                           : gemm_choice(op, es, transB, groups, rows, N, K).ring;
   if (ring < 0) return "rows_kernel";
   if (op == 0 && dtype == TRNBLAS_F32 && f32_small_tiles(rows, groups, N)) return "grouped_any_kernel";
   return kRingNames[op < 2 && dtype == TRNBLAS_F32 ? 2 : ring];

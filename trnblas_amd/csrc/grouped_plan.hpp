@@ -80,6 +80,19 @@ inline GroupedChoice choose_grouped(const RingCost (&ring)[3], double rows, doub
   return best;
 }
 
+// mx_gemm: rows_kernel's costs and the rings' over bytes of codes.
+inline GroupedChoice choose_mx(double rows, double groups, double N, double K) {
+  const double bytes = std::ceil(K / 32.0) * 16.0;
+  return choose_grouped(kRing4, rows, groups, N, bytes, bytes, 17.0 / 16.0, true);
+}
+
+// Whether rows_kernel quantises a K-contiguous A of values itself: one block of rows, and no more
+// than kInPlace values in it (its LDS).
+constexpr int kInPlace = 32768;
+inline bool quantised_in_place(const GroupedChoice& c, int64_t rows, int64_t K) {
+  return c.ring < 0 && c.mf == 1 && std::min<int64_t>(rows, 16) * K <= kInPlace;
+}
+
 // fp32 (its MFMAs take eight times as long): below two 64 x 128 tiles per CU the 32 x
 // 64 ones of grouped_any_kernel spread better, aligned or not. 300 rows in 4 groups by
 // 2048 x 1024 35 us, the rings 72; 2000 in 8 by 1024^2 60 and 72; 4096 in 8 by 2048^2

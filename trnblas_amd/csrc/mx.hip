@@ -214,12 +214,7 @@ static int run_rows_split(int ks, const GroupedArgs& g, const MxScales& x, hipSt
                    : run_rows<MF, 1, X>(g, x, s);
 }
 
-static GroupedChoice choose_mx(const GroupedArgs& g) {
-  return choose_grouped(kRing4, g.rows, g.groups, g.N, g.K, g.K, 17.0 / 16.0, true);
-}
-
-static int run_mx(const GroupedArgs& g, const MxScales& x, hipStream_t s) {
-  const GroupedChoice c = choose_mx(g);
+static int run_mx(const GroupedChoice& c, const GroupedArgs& g, const MxScales& x, hipStream_t s) {
   switch (c.ring) {
     case 0: return run_ring<8, 8>(g, x, s);
     case 1: return run_ring<4, 4>(g, x, s);
@@ -364,7 +359,7 @@ extern "C" int trnblas_hip_mx_gemm(int out_dtype, int64_t groups, int64_t rows, 
   TRNBLAS_CHECK_ARG((uintptr_t)A % 16 == 0 && (uintptr_t)A_scales % 16 == 0, "%s: codes and scales must be 16-byte aligned", kMxGemm);
   g.A = A;
   x.a = static_cast<const uint8_t*>(A_scales);
-  return run_mx(g, x, static_cast<hipStream_t>(stream));
+  return run_mx(choose_mx(rows, groups, N, K), g, x, static_cast<hipStream_t>(stream));
 }
 
 extern "C" size_t trnblas_hip_mx_gemm_from_workspace(int64_t rows, int64_t K) {
@@ -384,8 +379,8 @@ extern "C" int trnblas_hip_mx_gemm_from(int dtype, int out_dtype, int64_t groups
   if (rows == 0 || N == 0) return TRNBLAS_OK;
   TRNBLAS_CHECK_ARG(K == 0 || groups == 0 || A, "%s: null operand", kMxGemm);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const GroupedChoice c = choose_mx(g);
-  if (c.ring < 0 && c.mf == 1 && sk == 1 && std::min<int64_t>(rows, 16) * K <= kInPlace) {
+  const GroupedChoice c = choose_mx(rows, groups, N, K);
+  if (sk == 1 && quantised_in_place(c, rows, K)) {
     const int es = dtype == TRNBLAS_F32 ? 4 : 2;
     x.x = A, x.ldx = sr, x.kx = (int)K;
     x.vec = (uintptr_t)A % 16 == 0 && (sr * es % 16 == 0 || rows == 1);
@@ -407,5 +402,5 @@ extern "C" int trnblas_hip_mx_gemm_from(int dtype, int out_dtype, int64_t groups
     g.A = codes;
     x.a = scales;
   }
-  return run_mx(g, x, s);
+  return run_mx(c, g, x, s);
 }

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "gemm.hpp"
+#include "grouped_plan.hpp"
 #include "mx_block.hpp"
 #include "ring.hpp"
 
@@ -55,8 +56,6 @@ struct ColumnStep {
     return v;
   }
 };
-
-constexpr int kInPlace = 32768;
 
 // Quantises nr rows of x.x from row `row` on into LDS, one block of 32 values per
 // thread at a time: rows of g.lda bytes of codes, 16 bytes apart, and scale
