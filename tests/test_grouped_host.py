@@ -181,3 +181,23 @@ def test_rows_plan_refusals():
         assert lib.trnblas_hip_grouped_rows_plan(*bad, out) == _lib.E_ARG and b"bad arguments" in lib.trnblas_hip_last_error()
     assert lib.trnblas_hip_grouped_rows_plan(0, 1, 0, 2, 6, 64, 64, None) == _lib.E_ARG
     assert lib.trnblas_hip_grouped_rows_plan(0, 1, 0, 1, 30000, 4096, 4096, out) == 0 and not any(out)
+
+
+def test_the_plan_asks_for_forms_that_exist():
+    # fewer than eight waves along K: one row block of a K-contiguous 16-bit matrix; wide short matrices of many groups came to
+    # one wave elsewhere, and eight ran
+    from oracle.grouped import rows_plan
+    from trnblas_amd.hip import _lib
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    seen = set()
+    for G in (1, 5, 16, 50, 64):
+        for R in sorted({G, 2 * G + 6, 8 * G, 18 * G + 7, 40 * G}):
+            for N in (72, 520, 2056, 28376, 32160):
+                for K in (40, 96, 520, 2056):
+                    for transB in (0, 1):
+                        blocks, waves, inside = rows_plan(0, torch.bfloat16, transB, G, R, N, K)
+                        assert not inside and (waves in (0, 8) or (blocks == 1 and transB))
+                        seen.add((blocks, waves, transB))
+    assert {(1, 8, 0), (2, 8, 0), (1, 1, 1), (1, 2, 1), (1, 4, 1), (1, 8, 1), (2, 8, 1)} <= seen

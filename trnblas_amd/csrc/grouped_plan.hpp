@@ -63,8 +63,9 @@ inline GroupedChoice choose_grouped(const RingCost (&ring)[3], double rows, doub
     best.mf = rows <= 8.0 * g ? 1 : 2;
     const double again = likely_row_tiles(rows, groups, 16 * best.mf) / g;
     time = 4.5 + row_bytes / 8192.0 + weights * again / (best.mf == 2 && kc ? 3.2e6 : 4.5e6);
-    // the fewest waves along K that leave two workgroups per CU
-    while (best.ks > 1 && again * g * std::ceil(N * (best.ks / 2) / (kc ? 128.0 : 512.0)) >= 2.0 * device_cus()) best.ks /= 2;
+    // the fewest waves along K that leave two workgroups per CU: one block of rows of a K-contiguous
+    // B, and every 4-bit form, have kernels for it (elsewhere the rings mostly have enough tiles before)
+    while (best.ks > 1 && kc && (best.mf == 1 || elem < 2) && again * g * std::ceil(N * (best.ks / 2) / (kc ? 128.0 : 512.0)) >= 2.0 * device_cus()) best.ks /= 2;
   }
   for (int i = 0; i < 3; ++i) {
     const RingCost& c = ring[i];

@@ -316,8 +316,7 @@ static int run_rows(GroupedArgs g, hipStream_t s) {
   return check_launch(kGemm);
 }
 
-// Fewer than eight waves along K only where choose_grouped comes to it: one block of
-// rows, K-contiguous (else the rings have enough tiles before).
+// Fewer than eight waves along K: one block of rows, K-contiguous (choose_grouped asks for no other).
 template <typename T, int MF, bool BKC>
 static int run_rows_split(int ks, const GroupedArgs& g, hipStream_t s) {
   constexpr int NF = BKC ? 1 : 4;
