@@ -201,3 +201,29 @@ def test_the_plan_asks_for_forms_that_exist():
                         assert not inside and (waves in (0, 8) or (blocks == 1 and transB))
                         seen.add((blocks, waves, transB))
     assert {(1, 8, 0), (2, 8, 0), (1, 1, 1), (1, 2, 1), (1, 4, 1), (1, 8, 1), (2, 8, 1)} <= seen
+
+
+def test_the_fp32_plan_follows_fp32_costs():
+    # few rows: the weights straight into registers, not a tile per CU; large products: the ring kernel; between them 32 x 64 tiles
+    from oracle.grouped import plan, rows_plan
+    from trnblas_amd.hip import _lib
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    f32 = torch.float32
+    for transB in (0, 1):
+        for G, R, N, K in ((2, 32, 1536, 4096), (64, 64, 1024, 4096), (1, 1, 8192, 4096)):
+            want = "rows_kernel" if G < 64 or not transB else "grouped_any_kernel"
+            assert plan(0, f32, transB, G, R, 0, N, K) == want, (transB, G, R, N, K)
+        for G, R, N, K in ((16, 512, 4096, 2048), (64, 2048, 1536, 2056), (64, 1024, 2048, 1024)):
+            assert plan(0, f32, transB, G, R, 0, N, K) == "grouped_any_kernel", (transB, G, R, N, K)
+        for G, R, N, K in ((4, 8192, 4096, 2048), (1, 4096, 1024, 4096)):
+            assert plan(0, f32, transB, G, R, 0, N, K) == "ring_kernel 64 x 128", (transB, G, R, N, K)
+    assert plan(1, f32, 0, 8, 4096, 2048, 2048, 0) == "ring_kernel 64 x 128"
+    for G in (1, 6, 12, 20, 33):
+        for R in (G, 8 * G, 24 * G):
+            for N in (520, 856, 3028, 18400):
+                for K in (40, 132, 1412, 3052):
+                    for transB in (0, 1):
+                        blocks, waves, _ = rows_plan(0, f32, transB, G, R, N, K)
+                        assert (blocks, waves) in ((0, 0), (1, 8)) or (transB and (blocks, waves) in ((1, 4), (1, 1)))

@@ -100,7 +100,7 @@ extern "C" int trnblas_hip_grouped_rank_k(int dtype, int out_f32, int64_t groups
 }
 
 static GroupedChoice gemm_choice(int op, int64_t es, int transB, int64_t groups, int64_t rows, int64_t N, int64_t K) {
-  return op == 2 ? choose_mx(rows, groups, N, K) : choose_grouped(kRing16, rows, groups, N, K, (double)K * es, es, transB != 0);
+  return op == 2 ? choose_mx(rows, groups, N, K) : choose_gemm((int)es, rows, groups, N, K, transB != 0);
 }
 
 extern "C" int trnblas_hip_grouped_rows_plan(int op, int dtype, int transB, int64_t groups, int64_t rows, int64_t N, int64_t K,
@@ -125,9 +125,6 @@ extern "C" const char* trnblas_hip_grouped_plan(int op, int dtype, int transB, i
     return nullptr;
   }
   if (op < 2 && (first * es % 16 != 0 || second * es % 16 != 0)) return "grouped_any_kernel";
-  const int ring = op == 1 ? choose_rank_k(groups, M, N, (double)rows / groups * es / 128.0)
-                           : gemm_choice(op, es, transB, groups, rows, N, K).ring;
-  if (ring < 0) return "rows_kernel";
-  if (op == 0 && dtype == TRNBLAS_F32 && f32_small_tiles(rows, groups, N)) return "grouped_any_kernel";
-  return kRingNames[op < 2 && dtype == TRNBLAS_F32 ? 2 : ring];
+  const int ring = op == 1 ? choose_rank_k((int)es, groups, rows, M, N) : gemm_choice(op, es, transB, groups, rows, N, K).ring;
+  return ring < 0 ? "rows_kernel" : ring == kAnyTiles ? "grouped_any_kernel" : kRingNames[ring];
 }

@@ -44,7 +44,7 @@ inline double likely_row_tiles(double rows, double groups, int bm) {
 }
 
 struct GroupedChoice {
-  int ring;    // index into kRing16 / kRing4, or -1: rows_kernel
+  int ring;    // index into kRing16 / kRing4 (fp32: 2 or kAnyTiles), or -1: rows_kernel
   int mf, ks;  // rows_kernel: row blocks, waves along K
 };
 
@@ -94,16 +94,46 @@ inline bool quantised_in_place(const GroupedChoice& c, int64_t rows, int64_t K) 
   return c.ring < 0 && c.mf == 1 && std::min<int64_t>(rows, 16) * K <= kInPlace;
 }
 
-// fp32 (its MFMAs take eight times as long): below two 64 x 128 tiles per CU the 32 x
-// 64 ones of grouped_any_kernel spread better, aligned or not. 300 rows in 4 groups by
-// 2048 x 1024 35 us, the rings 72; 2000 in 8 by 1024^2 60 and 72; 4096 in 8 by 2048^2
-// (1088 tiles) 370 and 310.
-inline bool f32_small_tiles(double rows, double groups, double N) {
-  return likely_row_tiles(rows, groups, 64) * std::ceil(N / 128) < 2.0 * device_cus();
+// fp32: its MFMAs take eight times as long, so its kernels have costs of their own, fitted to 266
+// sizes of 1 .. 64 groups and 1 .. 8192 rows in either layout, each run on all kernels (of 532,
+// the choice is within 10 % of the fastest at all but 62, and 1.9 % slower over all): the
+// rings' 64 x 128 tiles; grouped_any_kernel's 32 x 64, by layout of B (column-, K-contiguous),
+// which spread better below two or three rounds; rows_kernel on one block of rows. 32 rows in 2
+// groups, 4096 x 1536: 138, 66 and 42 us; 128 in 64, 1024 x 2048: 141, 111 and 121; 8192 in 4, 2048 x
+// 4096: 1023 and 1392.
+constexpr RingCost kRing32 = {2, 4, 3, 6.7, 0.86, 2.7};
+constexpr RingCost kAny32[] = {{1, 2, 4, 4.7, 0.43, 1.25}, {1, 2, 4, 4.0, 0.41, 1.1}};
+constexpr int kAnyTiles = 3;  // GroupedChoice::ring: grouped_any_kernel
+
+inline GroupedChoice choose_f32(double rows, double groups, double N, double K, bool kc) {
+  const double g = std::min(groups, rows), weights = 4.0 * g * K * N, nk = std::ceil(K / 32.0);
+  GroupedChoice best{2, 1, 8};
+  double time = std::max(3.0 + weights / 3.2e6, ring_time(kRing32, likely_row_tiles(rows, groups, 64) * std::ceil(N / 128), nk));
+  const double any = std::max(3.0 + weights / (kc ? 4.45e6 : 4.6e6),
+                              ring_time(kAny32[kc], likely_row_tiles(rows, groups, 32) * std::ceil(N / 64), nk));
+  if (any < time) time = any, best.ring = kAnyTiles;
+  if (rows <= 64.0 * g) {
+    const double tiles = likely_row_tiles(rows, groups, 16), again = tiles / g - 1.0;  // weights read again
+    if ((kc ? 6.6 + K * 7.8e-4 + weights * (1.0 / 4.35e6 + again / 4.2e6)
+            : 5.1 + K * 4.8e-3 + weights * (1.0 / 5.6e6 + again / 8.7e6)) < time) {
+      best.ring = -1;
+      for (int ks : {4, 1})  // two: sizes that the 32 x 64 tiles serve
+        if (kc && tiles * std::ceil(N * ks / 128.0) >= 2.0 * device_cus()) best.ks = ks;
+    }
+  }
+  return best;
 }
 
-// grouped_rank_k: groups x (M x N), k_tiles of the average group.
-inline int choose_rank_k(double groups, double M, double N, double k_tiles) {
+// grouped_gemm of aligned operands
+inline GroupedChoice choose_gemm(int elem_bytes, double rows, double groups, double N, double K, bool kc) {
+  return elem_bytes == 4 ? choose_f32(rows, groups, N, K, kc) : choose_grouped(kRing16, rows, groups, N, K, K * elem_bytes, elem_bytes, kc);
+}
+
+// grouped_rank_k of aligned operands: groups x (M x N), over the average group's k-tiles. fp32 has
+// the 64 x 128 tiles alone: three workgroups per CU hide its longer MFMAs' steps.
+inline int choose_rank_k(int elem_bytes, double groups, double rows, double M, double N) {
+  if (elem_bytes == 4) return 2;
+  const double k_tiles = rows / groups * elem_bytes / 128.0;
   int best = 0;
   double time = 1e30;
   for (int i = 0; i < 3; ++i) {

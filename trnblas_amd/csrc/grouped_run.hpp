@@ -316,13 +316,15 @@ static int run_rows(GroupedArgs g, hipStream_t s) {
   return check_launch(kGemm);
 }
 
-// Fewer than eight waves along K: one block of rows, K-contiguous (choose_grouped asks for no other).
+// Fewer than eight waves along K: one block of rows, K-contiguous (the plan asks for no other; fp32: not two).
 template <typename T, int MF, bool BKC>
 static int run_rows_split(int ks, const GroupedArgs& g, hipStream_t s) {
   constexpr int NF = BKC ? 1 : 4;
   if constexpr (MF == 1 && BKC) {
     if (ks == 4) return run_rows<T, MF, NF, 4, BKC>(g, s);
-    if (ks == 2) return run_rows<T, MF, NF, 2, BKC>(g, s);
+    if constexpr (sizeof(T) == 2) {
+      if (ks == 2) return run_rows<T, MF, NF, 2, BKC>(g, s);
+    }
     if (ks == 1) return run_rows<T, MF, NF, 1, BKC>(g, s);
   }
   return run_rows<T, MF, NF, 8, BKC>(g, s);
@@ -330,7 +332,7 @@ static int run_rows_split(int ks, const GroupedArgs& g, hipStream_t s) {
 
 // ring: index of kRing16. fp32 takes the 64 x 128 tiles: three workgroups per CU hide
 // its longer MFMAs' steps best (8 groups of 128 rows, 2048 x 4096: 217 us, 220 on 128 x
-// 128), or 32 x 64 ones (f32_small_tiles).
+// 128).
 template <typename T, bool BKC, bool RK>
 static int run_ring_choice(int ring, const GroupedArgs& g, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
@@ -343,9 +345,13 @@ static int run_ring_choice(int ring, const GroupedArgs& g, hipStream_t s) {
 template <typename T, bool BKC>
 static int run_grouped(const GroupedArgs& g, hipStream_t s) {
   if (!dma_ready<T>(g, BKC, false)) return run_any<T, BKC, false>(g, s);
-  const GroupedChoice c = choose_grouped(kRing16, g.rows, g.groups, g.N, g.K, (double)g.K * sizeof(T), sizeof(T), BKC);
-  if (c.ring < 0) return c.mf == 1 ? run_rows_split<T, 1, BKC>(c.ks, g, s) : run_rows_split<T, 2, BKC>(c.ks, g, s);
-  if (std::is_same_v<T, float> && f32_small_tiles(g.rows, g.groups, g.N)) return run_any<T, BKC, false>(g, s);
+  const GroupedChoice c = choose_gemm(sizeof(T), g.rows, g.groups, g.N, g.K, BKC);
+  if constexpr (sizeof(T) == 2) {
+    if (c.ring < 0 && c.mf == 2) return run_rows_split<T, 2, BKC>(c.ks, g, s);
+  } else {
+    if (c.ring == kAnyTiles) return run_any<T, BKC, false>(g, s);
+  }
+  if (c.ring < 0) return run_rows_split<T, 1, BKC>(c.ks, g, s);
   return run_ring_choice<T, BKC, false>(c.ring, g, s);
 }
 
@@ -357,7 +363,7 @@ int grouped_gemm_run(const GroupedArgs& g, bool bkc, hipStream_t s) {
 template <typename T>
 int grouped_rank_k_run(const GroupedArgs& g, hipStream_t s) {
   if (!dma_ready<T>(g, false, true)) return run_any<T, false, true>(g, s);
-  return run_ring_choice<T, false, true>(choose_rank_k(g.groups, g.M, g.N, (double)g.rows / g.groups * sizeof(T) / 128.0), g, s);
+  return run_ring_choice<T, false, true>(choose_rank_k(sizeof(T), g.groups, g.rows, g.M, g.N), g, s);
 }
 
 }  // namespace trnblas
