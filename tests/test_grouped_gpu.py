@@ -8,6 +8,7 @@ import trnblas_amd as tb
 from oracle import grouped as og
 from oracle.grouped import GROUPS
 from oracle.grouped import plan as _plan
+from oracle.grouped import rows_plan
 from oracle.grouped import split as _split
 from oracle.grouped import uneven as _uneven
 
@@ -500,3 +501,47 @@ def test_gradient_of_an_fp32_result_is_not_rounded(dev, dtype):
     dA, dW = torch.autograd.grad(tb.grouped_rank_k(1.0, a, w, off.to(dev), dtype=torch.float32), (a, w), dP.to(dev))
     assert og.excess(dA, *og.grouped_gemm(1.0, W, dP.mT, off), N) <= 1
     assert og.excess(dW, *og.grouped_gemm(1.0, A, dP, off), K) <= 1
+
+
+# fp32 sums restart every 64 values of k (up to 1024 in long ones), so same-sign products keep `gemm`'s gate on each kernel:
+# (groups, rows, N, K)
+FP32 = {
+    "ring_kernel 64 x 128": [(3, 5200, 2312, 4100), (3, 2600, 1288, 1032)],
+    "rows_kernel": [(8, 8, 520, 4100), (5, 60, 136, 264)],
+    "grouped_any_kernel": [(2, 900, 520, 4104), (16, 32, 2056, 1032)],
+}
+
+
+@pytest.mark.parametrize("kernel", list(FP32))
+@pytest.mark.parametrize("transB", [False, True])
+def test_each_fp32_kernel_keeps_the_fp32_gate(dev, transB, kernel):
+    for i, (G, R, N, K) in enumerate(FP32[kernel]):
+        assert _plan(0, F32, transB, G, R, 0, N, K) == kernel
+        g = torch.Generator(device=dev).manual_seed(i)
+        off = _uneven(G, R, i) if R > 4 * G else torch.arange(G + 1) * (R // G)
+        A = torch.rand(R, K, generator=g, device=dev)
+        B = torch.rand(G, *((N, K) if transB else (K, N)), generator=g, device=dev)
+        C = torch.rand(R, N, generator=g, device=dev)
+        ref, den = _gemm_ref(A, B, off, transB)
+        D = tb.grouped_gemm(1.0, A, B, off.to(dev), transB=transB)
+        assert _relative(D, ref, den) <= 1e-6, (G, R, N, K)
+        D = tb.grouped_gemm(1.0, A, B, off.to(dev), 0.5, C, transB=transB)
+        assert _relative(D, ref + 0.5 * C.double(), den + 0.5 * C.double()) <= 1e-6, (G, R, N, K)
+
+
+@pytest.mark.parametrize("dtype,waves,G,R,N,K", [
+    (F32, 8, 8, 24, 520, 4104), (F32, 4, 23, 184, 752, 1412), (F32, 1, 33, 165, 18400, 132),
+    (BF16, 8, 8, 64, 296, 1832), (BF16, 4, 39, 234, 480, 1504), (F16, 2, 38, 152, 1328, 560), (BF16, 1, 33, 132, 5304, 144),
+])  # fmt: skip
+def test_each_form_of_the_few_rows_kernel(dev, dtype, waves, G, R, N, K):
+    # K-contiguous matrices, one block of 16 rows; one group fills it where it can
+    assert rows_plan(0, dtype, 1, G, R, N, K) == (1, waves, 0)
+    g = torch.Generator(device=dev).manual_seed(R)
+    sizes = torch.bincount(torch.arange(R - min(R, 16)) % (G - 1) + 1, minlength=G)
+    sizes[0] = min(R, 16)
+    off = _split(R, sizes.tolist())
+    A = torch.randn(R, K, generator=g, device=dev).to(dtype)
+    B = torch.randn(G, N, K, generator=g, device=dev).to(dtype)
+    ref, den = _gemm_ref(A, B, off, True)
+    D = tb.grouped_gemm(1.0, A, B, off.to(dev), transB=True)
+    assert _excess_gpu(D, ref, den, K) <= 1
