@@ -40,14 +40,17 @@ def _parse(text):
     return kernels
 
 
-def hazards(text):
-    """(kernel, index, write, MFMA) wherever fewer than WAIT_STATES lie between the two on some path."""
+def hazards(text, needed=WAIT_STATES):
+    """(kernel, index, write, MFMA) wherever fewer than the needed wait states lie between the two on some path."""
     found = []
     for kernel, (code, labels) in _parse(text).items():
         before = [[i - 1] if i and code[i - 1][0] not in ("s_branch", "s_endpgm", "s_setpc_b64") else [] for i in range(len(code))]
         for i, (name, ops) in enumerate(code):
-            if name.startswith(("s_branch", "s_cbranch")) and ops[0] in labels and labels[ops[0]] < len(code):
-                before[labels[ops[0]]].append(i)
+            target = ops[0]
+            if name == "s_setpc_b64":  # a far jump: its target stands in the sum before it
+                target = re.search(r"\((\.\w+)-", code[i - 2][1][2])[1]
+            if name.startswith(("s_branch", "s_cbranch", "s_setpc")) and labels[target] < len(code):
+                before[labels[target]].append(i)
 
         def walk(i, reads, states):
             for p in before[i]:
@@ -55,7 +58,7 @@ def hazards(text):
                 if name.startswith("v_") and not name.startswith("v_mfma") and reads & _registers(ops[0]):
                     yield p
                 passed = states + (int(ops[0], 0) + 1 if name == "s_nop" else 1)
-                if passed < WAIT_STATES:
+                if passed < needed:
                     yield from walk(p, reads, passed)
 
         for i, (name, ops) in enumerate(code):
@@ -77,6 +80,14 @@ def _assembly(source):
 def assembly():
     with ThreadPoolExecutor(len(SOURCES)) as pool:  # a minute each
         return dict(zip(SOURCES, pool.map(_assembly, SOURCES)))
+
+
+def test_the_check_sees_a_far_jump():
+    code = "_Zk:\n.LBB0_1:\n\tv_mfma_f32_16x16x4_f32 a[0:3], v4, v5, a[0:3]\n\tv_lshrrev_b32_e32 v5, 8, v5\n{}"
+    code += "\ts_add_u32 s54, s54, (.LBB0_1-.Lpost_getpc1)&4294967295\n\ts_addc_u32 s55, s55, (.LBB0_1-.Lpost_getpc1)>>32\n"
+    code += "\ts_setpc_b64 s[54:55]\n.Lfunc_end0:\n"
+    assert not hazards(code.format(""))  # the three scalar instructions are states enough
+    assert len(hazards(code.format(""), 4)) == 1 and not hazards(code.format("\ts_nop 0\n"), 4)
 
 
 def test_the_check_sees_a_missing_wait():
