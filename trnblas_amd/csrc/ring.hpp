@@ -174,6 +174,15 @@ constexpr bool fits(const RingCost& c) {
 static_assert(fits<__bf16, 8, 8>(kRing16[0]) && fits<__bf16, 4, 4>(kRing16[1]) && fits<__bf16, 2, 4>(kRing16[2]), "16-bit plan");
 static_assert(fits<fp4x2, 8, 8>(kRing4[0]) && fits<fp4x2, 4, 4>(kRing4[1]) && fits<fp4x2, 2, 4>(kRing4[2]), "4-bit plan");
 
+// The lane's number; ANEW: counted where it is asked for (kernels of chains: 256 x 256 tiles can
+// keep neither it nor the addresses made of it from one chain to the next).
+template <bool ANEW>
+__device__ __forceinline__ int lane_of() {
+  int lane = threadIdx.x & 63;
+  if constexpr (ANEW) asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  return lane;
+}
+
 template <typename T, int FM, int FN, bool BKC, bool RK, bool CHAINS>
 __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& x, const TileJob& j, int wave, char* lds) {
   constexpr bool MX = std::is_same_v<T, fp4x2>, FOLD = std::is_same_v<T, float>;
@@ -186,9 +195,7 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
   constexpr int STAGE = L::STAGE;
   constexpr int ND = DA::NB + DB::NB;  // DMAs per wave and k-tile, besides scales
   static_assert(STAGE == PA::BYTES + PB::BYTES && SA + SB <= 16, "one scale DMA per wave and step");
-  int lane = threadIdx.x & 63;
-  if constexpr (CHAINS)  // anew in each chain: 256 x 256 tiles can keep neither it nor the addresses made of it
-    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  const int lane = lane_of<CHAINS>();
   const int m0 = (wave & 1) * (16 * FM), n0 = (wave >> 1) * (16 * FN);
   const int nk = (j.K + PA::BK - 1) / PA::BK;
   const uint32_t lds0 = lds_offset(lds);
@@ -202,8 +209,8 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
   auto dma_turn = [&](int kt) __attribute__((always_inline)) {
     const int left = j.K - kt * PA::BK;
     if (left > 0 && left < PA::BK) {
-      da.last(left, wave, lane);
-      db.last(left, wave, lane);
+      da.last(left, wave, CHAINS ? lane_of<CHAINS>() : lane);
+      db.last(left, wave, CHAINS ? lane_of<CHAINS>() : lane);
     }
     const uint32_t st = lds0 + (uint32_t)kt % NS * STAGE;
     sta = st + DA::NB * 1024 * wave;
@@ -389,7 +396,7 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
   char* own = lds + wave * kStoreLds<FN>;
   if (!(g.vec4 && (g.N & 3) == 0)) __syncthreads();  // the other waves' reads
   if (CHAINS || g.out32)
-    store_wave<FM, FN, float>(g, j, acc, m0, n0, lane, own);
+    store_wave<FM, FN, float>(g, j, acc, m0, n0, CHAINS ? lane_of<CHAINS>() : lane, own);
   else if (MX && g.out_f16)
     store_wave<FM, FN, _Float16>(g, j, acc, m0, n0, lane, own);
   else
@@ -407,8 +414,7 @@ __device__ __forceinline__ const char* uniform(const char* p) {
 // chain after the first takes its sum from D. 32768 rows in 2 groups by 4096 x 2048 take 455 us with
 // these round trips, 396 as one chain; where no group has a second chain the kernel costs 3 %.
 template <typename T, int FM, int FN, bool BKC, bool RK, bool CHAINS>
-__device__ __forceinline__ void ring_chains(GroupedArgs g, const MxScales& x, TileJob j, char* lds) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ __forceinline__ void ring_chains(GroupedArgs g, const MxScales& x, TileJob j, int wave, char* lds) {
   if constexpr (!CHAINS) {
     ring_tile<T, FM, FN, BKC, RK, false>(g, x, j, wave, lds);
   } else {
@@ -434,13 +440,14 @@ __global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(Groupe
   __shared__ __attribute__((aligned(16))) char lds[RingLds<T, FM, FN>::BYTES];
   TileJob j;
   if (!tile_job<T, 32 * FM, 32 * FN, BKC, RK, SPLIT>(g, j)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if constexpr (SPLIT) {
     if (j.quarter >= 0) {
-      ring_chains<T, FM / 2, FN / 2, BKC, RK, CHAINS>(g, x, j, lds);
+      ring_chains<T, FM / 2, FN / 2, BKC, RK, CHAINS>(g, x, j, wave, lds);
       return;
     }
   }
-  ring_chains<T, FM, FN, BKC, RK, CHAINS>(g, x, j, lds);
+  ring_chains<T, FM, FN, BKC, RK, CHAINS>(g, x, j, wave, lds);
 }
 
 // Workgroups of such a launch over `tiles` tiles (or at most so many), SPLIT's
