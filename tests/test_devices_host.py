@@ -46,6 +46,7 @@ def device(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state["current"], raising=False)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
     monkeypatch.setattr(grouped_kernels, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(grouped_kernels, "_current_device", lambda: state["current"])
     monkeypatch.setattr(torch.cuda, "device", current)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: state["current"])
     monkeypatch.setattr(_lib, "load", Library)

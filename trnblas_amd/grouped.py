@@ -23,6 +23,7 @@ rows (never an access outside the operands).
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad as _fwd
 
 from ._flags import trans_flag
 from .hip import dispatch as _d
@@ -50,7 +51,7 @@ def _fast_call(A, B, offsets) -> bool:
         and type(offsets) is torch.Tensor
         and A.is_cuda
         and not ((A.requires_grad or B.requires_grad) and torch.is_grad_enabled())
-        and not _d._forward_mode()
+        and _fwd._current_level < 0
         and _d._use_hip()
     )
 
@@ -125,16 +126,18 @@ def _rank_k(alpha, A, B, offsets, beta, C, out_dtype):
 
 def _differentiable(function, product, *args):
     """A product of a backward pass, itself differentiable only where that is asked for."""
-    return function.apply(*args) if torch.is_grad_enabled() or _d._forward_mode() else product(*args)
+    return function.apply(*args) if torch.is_grad_enabled() or _fwd._current_level >= 0 else product(*args)
 
 
 def _widened(dD, A, B):
     """The operands of a backward product in one type: an fp32 gradient is not rounded to 16-bit operands' type, whose
     range (fp16: 65504) it may pass."""
-    if dD.dtype == A.dtype:
-        return dD, A, B
     wide = torch.promote_types(dD.dtype, A.dtype)
     return dD.to(wide), A.to(wide), B.to(wide)
+
+
+def _narrowed(dtype, *grads):
+    return (None if g is None else g.to(dtype) for g in grads)
 
 
 def _tangent(ctx, product, tA, tB, tC):
@@ -150,7 +153,7 @@ def _tangent(ctx, product, tA, tB, tC):
 
 def _save(ctx, alpha, A, B, offsets, beta, out_dtype):
     ctx.save_for_backward(A, B, offsets)
-    if _d._forward_mode():
+    if _fwd._current_level >= 0:
         ctx.save_for_forward(A, B, offsets)
     ctx.alpha, ctx.beta, ctx.out_dtype = alpha, beta, out_dtype
 
@@ -171,14 +174,18 @@ class _GroupedGemm(torch.autograd.Function):
         dA = dB = dC = None
         if ctx.needs_input_grad[5]:
             dC = ctx.beta * dD
-        dt, (dD, A, B) = A.dtype, _widened(dD, A, B)
+        dt = A.dtype
+        if dD.dtype != dt:
+            dD, A, B = _widened(dD, A, B)
         if ctx.needs_input_grad[1]:
-            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, dD, B.mT, offsets, 0.0, None, dD.dtype).to(dt)
+            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, dD, B.mT, offsets, 0.0, None, A.dtype)
         if ctx.needs_input_grad[2]:
             if B.stride(1) == 1 and B.stride(2) > 1:  # B is a transposed view: so is its gradient
-                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, dD, A, offsets, 0.0, None, dD.dtype).to(dt).mT
+                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, dD, A, offsets, 0.0, None, B.dtype).mT
             else:
-                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, A, dD, offsets, 0.0, None, dD.dtype).to(dt)
+                dB = _differentiable(_GroupedRankK, _rank_k, ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
+        if A.dtype != dt:
+            dA, dB = _narrowed(dt, dA, dB)
         return None, dA, dB, None, None, dC, None
 
 
@@ -198,11 +205,15 @@ class _GroupedRankK(torch.autograd.Function):
         dA = dB = dC = None
         if ctx.needs_input_grad[5]:
             dC = ctx.beta * dD
-        dt, (dD, A, B) = A.dtype, _widened(dD, A, B)
+        dt = A.dtype
+        if dD.dtype != dt:
+            dD, A, B = _widened(dD, A, B)
         if ctx.needs_input_grad[1]:
-            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, B, dD.mT, offsets, 0.0, None, dD.dtype).to(dt)
+            dA = _differentiable(_GroupedGemm, _gemm, ctx.alpha, B, dD.mT, offsets, 0.0, None, A.dtype)
         if ctx.needs_input_grad[2]:
-            dB = _differentiable(_GroupedGemm, _gemm, ctx.alpha, A, dD, offsets, 0.0, None, dD.dtype).to(dt)
+            dB = _differentiable(_GroupedGemm, _gemm, ctx.alpha, A, dD, offsets, 0.0, None, B.dtype)
+        if A.dtype != dt:
+            dA, dB = _narrowed(dt, dA, dB)
         return None, dA, dB, None, None, dC, None
 
 

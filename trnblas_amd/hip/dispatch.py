@@ -282,13 +282,9 @@ def _wants_grad(*ts) -> bool:
     return (torch.is_grad_enabled() and any(t.requires_grad for t in ts)) or _has_tangent(*ts)
 
 
-def _forward_mode() -> bool:
-    """Whether a forward-mode level is open (tensors may carry tangents, which `requires_grad` does not tell)."""
-    return _fwd._current_level >= 0
-
-
 def _has_tangent(*ts) -> bool:
-    return _forward_mode() and any(_fwd.unpack_dual(t).tangent is not None for t in ts)
+    """Whether one of them carries a forward-mode tangent (`requires_grad` does not tell; none does outside a level)."""
+    return _fwd._current_level >= 0 and any(_fwd.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _upload_nbytes(t: torch.Tensor) -> int:
@@ -716,7 +712,7 @@ def gemm_fast(alpha, A, B, beta, C, transA, transB):
         or B.dim() != 2
         or _backend == "pytorch"
         or kern._launch_probe is not None
-        or _forward_mode()
+        or _fwd._current_level >= 0
     ):
         return None
     dev = A.get_device()

@@ -235,6 +235,7 @@ def mx_gemm(
 
 _PACK_LOOK = 1 << 30  # multiply-adds below which no packing pays
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 _fns: dict = {}
 _INTS = (torch.int32, torch.int64)
 
@@ -263,7 +264,7 @@ def grouped_gemm_fast(alpha, A, B, offsets, transB, out_dtype):
     k, N = (b1, b0) if transB else (b0, b1)
     dev = A.get_device()
     if (
-        k != K or s1 != 1 or lda < K or t1 != 1 or t0 < b1 or sb < 0 or N == 0 or not _lib.is_current(dev)
+        k != K or s1 != 1 or lda < K or t1 != 1 or t0 < b1 or sb < 0 or N == 0 or dev != _current_device()
         or B.get_device() != dev or offsets.get_device() != dev or offsets.dtype not in _INTS
         or offsets.shape != (G + 1,) or offsets.stride() != (1,) or A.is_neg() or B.is_neg()
     ):  # fmt: skip
@@ -295,7 +296,7 @@ def mx_gemm_fast(alpha, A, b, offsets, out_dtype):
     sr, sk = A.stride()
     dev = A.get_device()
     N = codes.shape[-2]
-    if not _lib.is_current(dev) or codes.get_device() != dev or sr < 0 or sk < 0 or N == 0 or A.is_neg():
+    if dev != _current_device() or codes.get_device() != dev or sr < 0 or sk < 0 or N == 0 or A.is_neg():
         return None
     G, o, o64 = 1, None, False
     if offsets is not None:
@@ -326,7 +327,7 @@ def grouped_rank_k_fast(alpha, A, B, offsets, out_dtype):
     ldb, t1 = B.stride()
     dev = A.get_device()
     if (
-        R2 != R or s1 != 1 or lda < M or t1 != 1 or ldb < N or M == 0 or N == 0 or not _lib.is_current(dev) or B.get_device() != dev
+        R2 != R or s1 != 1 or lda < M or t1 != 1 or ldb < N or M == 0 or N == 0 or dev != _current_device() or B.get_device() != dev
         or offsets.get_device() != dev or offsets.dtype not in _INTS or offsets.dim() != 1 or offsets.stride() != (1,)
         or A.is_neg() or B.is_neg()
     ):  # fmt: skip
@@ -351,7 +352,7 @@ def mx_quantize_fast(X):
     """(codes, scales) of X (R, K), or None."""
     code = _lib.DTYPE_CODES.get(X.dtype)
     dev = X.get_device()
-    if code is None or not _lib.is_current(dev) or X.dim() != 2 or _kernels._launch_probe is not None:
+    if code is None or dev != _current_device() or X.dim() != 2 or _kernels._launch_probe is not None:
         return None
     R, K = X.shape
     sr, sk = X.stride()
@@ -369,7 +370,7 @@ def mx_quantize_fast(X):
 def mx_dequantize_fast(codes, scales, K, dtype):
     """The values of one matrix, or None."""
     dev = codes.get_device()
-    if not _lib.is_current(dev) or codes.dim() != 2 or _kernels._launch_probe is not None:
+    if dev != _current_device() or codes.dim() != 2 or _kernels._launch_probe is not None:
         return None
     R = codes.shape[0]
     D = codes.new_empty((R, K), dtype=dtype)

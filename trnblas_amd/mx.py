@@ -20,6 +20,7 @@ a forward-mode tangent.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad as _fwd
 
 from ._flags import trans_flag
 from .grouped import _check_offsets, _check_result, _gk
@@ -191,7 +192,7 @@ def _product(what: str, alpha, A, B, offsets, beta, C, dtype) -> torch.Tensor:
     if (
         beta == 0.0 and type(A) is torch.Tensor and A.is_cuda and type(B) is MXMatrix and len(B.shape) == dims
         and A.dim() == 2 and A.shape[1] == B.shape[-1] and (offsets is None or type(offsets) is torch.Tensor)
-        and not (A.requires_grad and torch.is_grad_enabled()) and not _d._forward_mode() and _d._use_hip()
+        and not (A.requires_grad and torch.is_grad_enabled()) and _fwd._current_level < 0 and _d._use_hip()
     ):  # fmt: skip
         try:  # the short way; None: something is out of the ordinary
             D = _gk().mx_gemm_fast(alpha, A, (B.codes, B.scales), offsets, dtype)
