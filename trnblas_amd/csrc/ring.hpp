@@ -146,7 +146,7 @@ struct PanelDma {
 // and whatever does not fit between two MFMAs (16 cycles) idles the matrix unit.
 //
 // Measured, 256 x 256 tiles: bf16 8192^3 K-contiguous 715 us (1.54 PFLOP/s), 32768 rows
-// in 16 groups by 4096^2 868-905 (1.2-1.27); 4-bit 8192 x 8192 x 32768 5.0 PFLOP/s. The
+// in 16 groups by 4096^2 868-905 (1.2-1.27); 4-bit 8192 x 8192 x 32768 5.1 PFLOP/s. The
 // MFMAs alone run at 2.4 PFLOP/s (4-bit 8.8): with the reads and DMAs between them
 // they take 80 % of the cycles, at the clock that the power limit leaves. A tile costs
 // 10 us besides its k-tiles, most of it the stores of all CUs at once (8192 x 2048 x
