@@ -545,3 +545,18 @@ def test_each_form_of_the_few_rows_kernel(dev, dtype, waves, G, R, N, K):
     ref, den = _gemm_ref(A, B, off, True)
     D = tb.grouped_gemm(1.0, A, B, off.to(dev), transB=True)
     assert _excess_gpu(D, ref, den, K) <= 1
+
+
+@pytest.mark.parametrize("G,R,N,K", [(3, 5200, 2313, 16392), (3, 2600, 1290, 16392), (1, 600, 519, 33000), (1, 300, 37, 8200)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_chains_into_rows_that_start_anywhere(dev, dtype, G, R, N, K):
+    # results whose rows are no multiple of 16 bytes go out through LDS, and each further chain takes them up from there
+    g = torch.Generator(device=dev).manual_seed(N)
+    off = _uneven(G, R, 1)
+    A, B = torch.rand(R, K, generator=g, device=dev).to(dtype), torch.rand(G, N, K, generator=g, device=dev).to(dtype)
+    C = 100.0 * torch.rand(R, N, generator=g, device=dev)
+    ref, den = _gemm_ref(A, B, off, True)
+    D = tb.grouped_gemm(1.0, A, B, off.to(dev), transB=True, dtype=F32)
+    assert _relative(D, ref, den) <= CHAIN_GATE and not D[int(off[-1]) :].any()
+    D = tb.grouped_gemm(-2.0, A, B, off.to(dev), 0.5, C, transB=True, dtype=F32)
+    assert _relative(D, -2.0 * ref + 0.5 * C.double(), 2.0 * den + 0.5 * C.double()) <= CHAIN_GATE
