@@ -560,3 +560,33 @@ def test_chains_into_rows_that_start_anywhere(dev, dtype, G, R, N, K):
     assert _relative(D, ref, den) <= CHAIN_GATE and not D[int(off[-1]) :].any()
     D = tb.grouped_gemm(-2.0, A, B, off.to(dev), 0.5, C, transB=True, dtype=F32)
     assert _relative(D, -2.0 * ref + 0.5 * C.double(), 2.0 * den + 0.5 * C.double()) <= CHAIN_GATE
+
+
+@pytest.mark.parametrize("blocks,waves,transB,G,R,N,K", [
+    (1, 8, 0, 2, 9, 72, 33000), (2, 8, 0, 1, 20, 72, 33000), (1, 8, 1, 2, 9, 72, 33000), (2, 8, 1, 1, 20, 72, 33000),
+    (1, 4, 1, 8, 16, 2056, 16400), (1, 2, 1, 64, 128, 480, 8200), (1, 1, 1, 16, 32, 4104, 4104),
+])  # fmt: skip
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_chains_of_the_few_rows_kernel(dev, dtype, blocks, waves, transB, G, R, N, K):
+    # a wave's share of k is longer than a chain
+    assert rows_plan(0, dtype, transB, G, R, N, K) == (blocks, waves, 0)
+    g = torch.Generator(device=dev).manual_seed(K)
+    off = torch.arange(G + 1) * (R // G)
+    A = torch.rand(R, K, generator=g, device=dev).to(dtype)
+    B = torch.rand(G, *((N, K) if transB else (K, N)), generator=g, device=dev).to(dtype)
+    ref, den = _gemm_ref(A, B, off, transB)
+    assert _relative(tb.grouped_gemm(1.0, A, B, off.to(dev), transB=bool(transB), dtype=F32), ref, den) <= CHAIN_GATE
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_chains_of_rows_shorter_than_16_bytes(dev, dtype):
+    g = torch.Generator(device=dev).manual_seed(13)
+    rand = lambda *s: torch.rand(*s, generator=g, device=dev).to(dtype)
+    off = _split(36000, [20000, 0, 15990], 4)
+    for M, N in ((5, 260), (260, 3), (1, 1)):
+        A, B = rand(36000, M), rand(36000, N)
+        assert _relative(tb.grouped_rank_k(1.0, A, B, off.to(dev), dtype=F32), *_rank_k_ref(A, B, off)) <= CHAIN_GATE, (M, N)
+    off = _split(70, [33, 30], 4)
+    for N in (1, 5):
+        A, B = rand(70, 33001), rand(2, 33001, N)
+        assert _relative(tb.grouped_gemm(1.0, A, B, off.to(dev), dtype=F32), *_gemm_ref(A, B, off, False)) <= CHAIN_GATE, N

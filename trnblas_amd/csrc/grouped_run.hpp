@@ -262,8 +262,12 @@ static int run_any(GroupedArgs g, hipStream_t s) {
   const bool tiny = (RK ? g.M : g.K) < EV || (BKC ? g.K : g.N) < EV;
   auto kernel = tiny ? grouped_any_kernel<T, BKC, RK, true> : grouped_any_kernel<T, BKC, RK, false>;
   if constexpr (sizeof(T) == 2) {
-    if (needs_chains<T>(g, RK ? g.rows : g.K))
-      kernel = tiny ? grouped_any_kernel<T, BKC, RK, true, true> : grouped_any_kernel<T, BKC, RK, false, true>;
+    if (needs_chains<T>(g, RK ? g.rows : g.K)) {
+      kernel = grouped_any_kernel<T, BKC, RK, false, true>;
+      if constexpr (!BKC) {  // a K-contiguous B has long rows then
+        if (tiny) kernel = grouped_any_kernel<T, BKC, RK, true, true>;
+      }
+    }
   }
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, s, g);
   return check_launch(what);
