@@ -65,7 +65,8 @@ inline GroupedChoice choose_grouped(const RingCost (&ring)[3], double rows, doub
     time = 4.5 + row_bytes / 8192.0 + weights * again / (best.mf == 2 && kc ? 3.2e6 : 4.5e6);
     // the fewest waves along K that leave two workgroups per CU: one block of rows of a K-contiguous
     // B, and every 4-bit form, have kernels for it (elsewhere the rings mostly have enough tiles before)
-    while (best.ks > 1 && kc && (best.mf == 1 || elem < 2) && again * g * std::ceil(N * (best.ks / 2) / (kc ? 128.0 : 512.0)) >= 2.0 * device_cus()) best.ks /= 2;
+    if (kc && (best.mf == 1 || elem < 2))
+      while (best.ks > 1 && again * g * std::ceil(N * (best.ks / 2) / 128.0) >= 2.0 * device_cus()) best.ks /= 2;
   }
   for (int i = 0; i < 3; ++i) {
     const RingCost& c = ring[i];
@@ -126,7 +127,8 @@ inline GroupedChoice choose_f32(double rows, double groups, double N, double K, 
 
 // grouped_gemm of aligned operands
 inline GroupedChoice choose_gemm(int elem_bytes, double rows, double groups, double N, double K, bool kc) {
-  return elem_bytes == 4 ? choose_f32(rows, groups, N, K, kc) : choose_grouped(kRing16, rows, groups, N, K, K * elem_bytes, elem_bytes, kc);
+  return elem_bytes == 4 ? choose_f32(rows, groups, N, K, kc)
+                         : choose_grouped(kRing16, rows, groups, N, K, K * elem_bytes, elem_bytes, kc);
 }
 
 // grouped_rank_k of aligned operands: groups x (M x N), over the average group's k-tiles. fp32 has
