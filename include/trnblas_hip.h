@@ -42,6 +42,13 @@ extern "C" {
 #define TRNBLAS_F16 2
 #define TRNBLAS_F64 3 /* trnblas_hip_tri_inv_blocks only (fp64 work has its own entry points) */
 
+/* activations of gated projections */
+#define TRNBLAS_ACT_SILU 0      /* x / (1 + exp(-x)) */
+#define TRNBLAS_ACT_GELU 1      /* x (1 + erf(x / sqrt(2))) / 2 */
+#define TRNBLAS_ACT_GELU_TANH 2 /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+#define TRNBLAS_ACT_RELU 3      /* max(x, 0) */
+#define TRNBLAS_ACT_SIGMOID 4   /* 1 / (1 + exp(-x)) */
+
 /* error codes */
 #define TRNBLAS_OK 0
 #define TRNBLAS_E_ARG (-1)       /* invalid argument (shape, stride, dtype, flag) */
@@ -560,7 +567,8 @@ int trnblas_hip_trsm(int dtype, int64_t n, int64_t nrhs, int upper, int unit, do
  * offsets: device int32 (offsets64 == 0) or int64 [groups + 1], nondecreasing:
  * group g is rows offsets[g] .. offsets[g + 1] - 1. They are read on the device
  * only (the call never waits for them); each is clamped to [0, rows], so bad
- * ones give wrong rows but no access outside the operands.
+ * ones give wrong rows but no access outside the operands. NULL (groups == 1):
+ * all rows are one group.
  * dtype: TRNBLAS_F32, TRNBLAS_BF16 or TRNBLAS_F16, the element type of A and B;
  * C and D have it too, or are fp32 for out_f32 != 0. Sums are fp32, with one
  * rounding at the end; those of an fp32 result of 16-bit operands are chains of at
@@ -626,8 +634,7 @@ int trnblas_hip_mx_dequantize(int dtype, int64_t R, int64_t K, const void* codes
  * D[r] = alpha A[r] B[g]^T + beta C[r] for the rows r of group g (D[r] =
  * beta C[r] for rows of no group): A rows x K, B groups matrices of N x K, both
  * microscaled; products exact, sums fp32 (one chain, 128 values of K each addition). C and D (rows x N) have the type
- * out_dtype. offsets as in trnblas_hip_grouped_gemm; NULL (groups == 1): one
- * matrix for all rows.
+ * out_dtype. offsets as in trnblas_hip_grouped_gemm.
  */
 int trnblas_hip_mx_gemm(int out_dtype, int64_t groups, int64_t rows, int64_t N, int64_t K,
                         double alpha, const void* A, const void* A_scales, const void* B,
@@ -663,6 +670,25 @@ const char* trnblas_hip_grouped_plan(int op, int dtype, int transB, int64_t grou
  */
 int trnblas_hip_grouped_rows_plan(int op, int dtype, int transB, int64_t groups, int64_t rows,
                                   int64_t N, int64_t K, int32_t plan[3]);
+
+/*
+ * Gated projections: H = act(A G) * (A U), elementwise, for weights [G | U] of 2 N
+ * columns. No counterpart in the reference. act: TRNBLAS_ACT_*. Computed in fp32, one
+ * rounding of each result. Matrices are row-major, of any leading dimension and
+ * alignment.
+ *
+ * gate: H (rows x N, out_dtype) = act(P[:, :N]) * P[:, N:] for P (rows x 2 N) of type
+ * `dtype`; out_dtype is that, or with an fp32 P any. S: null, or P rounded to
+ * out_dtype (rows x 2 N).
+ *
+ * gate_backward: for the gradient dH (rows x N) of H, dP[:, :N] = dH * U * act'(G) and
+ * dP[:, N:] = dH * act(G), P = [G | U]; all of type `dtype`. dP may be P itself.
+ */
+int trnblas_hip_gate(int act, int dtype, int out_dtype, int64_t rows, int64_t N, const void* P,
+                     int64_t ldp, void* H, int64_t ldh, void* S, int64_t lds, void* stream);
+int trnblas_hip_gate_backward(int act, int dtype, int64_t rows, int64_t N, const void* P,
+                              int64_t ldp, const void* dH, int64_t ldg, void* dP, int64_t ldd,
+                              void* stream);
 
 #ifdef __cplusplus
 }

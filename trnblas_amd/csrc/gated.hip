@@ -1,0 +1,169 @@
+// Gated projections H = act(A G) * (A U), [G | U] one matrix of 2 N columns: what lies
+// beside the products.
+#include "gate.hpp"
+
+namespace trnblas {
+
+static const char* kGate = "trnblas_hip_gate";
+static const char* kGateBackward = "trnblas_hip_gate_backward";
+
+struct GateArgs {
+  const void* P;  // rows x 2 n: gates, then ups
+  int64_t ldp;
+  const void* dH;  // backward
+  int64_t ldg;
+  void* D;  // H, or dP (backward)
+  int64_t ldd;
+  void* S;  // P in D's type, or null
+  int64_t lds;
+  int64_t rows;
+  int n, act;
+  int vec;  // whole groups of V values, every row's start aligned to them
+};
+
+// V values from p, as floats; only `left` of them where that is fewer.
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T* p, bool vec, int left, float (&v)[V]) {
+  typedef T tv __attribute__((ext_vector_type(V)));
+  if (vec) {
+    const tv w = *reinterpret_cast<const tv*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (float)w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < left ? (float)p[i] : 0.0f;
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_values(T* p, bool vec, int left, const float (&v)[V]) {
+  typedef T tv __attribute__((ext_vector_type(V)));
+  if (vec) {
+    tv w;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = (T)v[i];
+    *reinterpret_cast<tv*>(p) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < left) p[i] = (T)v[i];
+  }
+}
+
+// One thread takes V values of a row: 64 x 4 threads, columns by rows.
+constexpr int kGateV = 8;
+
+template <typename T, typename O>
+__global__ __launch_bounds__(256) void gate_kernel(GateArgs g) {
+  constexpr int V = kGateV;
+  const int c = V * (blockIdx.x * 64 + threadIdx.x);
+  const int left = g.n - c;
+  if (left <= 0) return;
+  for (int64_t r = blockIdx.y * 4 + threadIdx.y; r < g.rows; r += 4 * gridDim.y) {
+    const T* p = static_cast<const T*>(g.P) + r * g.ldp + c;
+    float a[V], u[V], h[V];
+    load_values<T, V>(p, g.vec, left, a);
+    load_values<T, V>(p + g.n, g.vec, left, u);
+#pragma unroll
+    for (int i = 0; i < V; ++i) h[i] = gate(g.act, a[i]) * u[i];
+    store_values<O, V>(static_cast<O*>(g.D) + r * g.ldd + c, g.vec, left, h);
+    if (g.S) {
+      O* s = static_cast<O*>(g.S) + r * g.lds + c;
+      store_values<O, V>(s, g.vec, left, a);
+      store_values<O, V>(s + g.n, g.vec, left, u);
+    }
+  }
+}
+
+// dG = dH * U * act'(G), dU = dH * act(G).
+template <typename T>
+__global__ __launch_bounds__(256) void gate_backward_kernel(GateArgs g) {
+  constexpr int V = kGateV;
+  const int c = V * (blockIdx.x * 64 + threadIdx.x);
+  const int left = g.n - c;
+  if (left <= 0) return;
+  for (int64_t r = blockIdx.y * 4 + threadIdx.y; r < g.rows; r += 4 * gridDim.y) {
+    const T* p = static_cast<const T*>(g.P) + r * g.ldp + c;
+    float a[V], u[V], d[V];
+    load_values<T, V>(p, g.vec, left, a);
+    load_values<T, V>(p + g.n, g.vec, left, u);
+    load_values<T, V>(static_cast<const T*>(g.dH) + r * g.ldg + c, g.vec, left, d);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float y, slope;
+      gate_slope(g.act, a[i], y, slope);
+      a[i] = d[i] * u[i] * slope;
+      u[i] = d[i] * y;
+    }
+    T* o = static_cast<T*>(g.D) + r * g.ldd + c;
+    store_values<T, V>(o, g.vec, left, a);
+    store_values<T, V>(o + g.n, g.vec, left, u);
+  }
+}
+
+static dim3 gate_grid(const GateArgs& g) {
+  const int64_t rows = (g.rows + 3) / 4;
+  return dim3((unsigned)((g.n + 64 * kGateV - 1) / (64 * kGateV)), (unsigned)(rows < 32768 ? rows : 32768));
+}
+
+static bool whole(const void* p, int64_t ld, int64_t n, int es) {
+  const int v = kGateV * es < 16 ? kGateV * es : 16;
+  return p == nullptr || ((uintptr_t)p % v == 0 && ld * es % v == 0 && n * es % v == 0);
+}
+
+static int check_gate(const char* what, int act, int dtype, int64_t rows, int64_t N) {
+  TRNBLAS_CHECK_ARG(act >= TRNBLAS_ACT_SILU && act <= TRNBLAS_ACT_SIGMOID, "%s: bad activation %d", what, act);
+  TRNBLAS_CHECK_ARG(dtype == TRNBLAS_F32 || dtype == TRNBLAS_BF16 || dtype == TRNBLAS_F16, "%s: bad dtype %d", what, dtype);
+  TRNBLAS_CHECK_ARG(rows >= 0 && rows < INT32_MAX - 1024 && N >= 0 && N < (INT32_MAX >> 1) - 1024, "%s: bad sizes (rows %lld, N %lld)",
+                    what, (long long)rows, (long long)N);
+  return TRNBLAS_OK;
+}
+
+}  // namespace trnblas
+
+using namespace trnblas;
+
+extern "C" int trnblas_hip_gate(int act, int dtype, int out_dtype, int64_t rows, int64_t N, const void* P, int64_t ldp, void* H,
+                                int64_t ldh, void* S, int64_t lds, void* stream) {
+  if (int rc = check_gate(kGate, act, dtype, rows, N)) return rc;
+  TRNBLAS_CHECK_ARG(out_dtype == dtype || (dtype == TRNBLAS_F32 && (out_dtype == TRNBLAS_BF16 || out_dtype == TRNBLAS_F16)),
+                    "%s: bad result dtype %d", kGate, out_dtype);
+  TRNBLAS_CHECK_ARG(ldp >= 2 * N && ldh >= N && (S == nullptr || lds >= 2 * N), "%s: bad leading dimension", kGate);
+  if (rows == 0 || N == 0) return TRNBLAS_OK;
+  TRNBLAS_CHECK_ARG(P != nullptr && H != nullptr, "%s: null operand", kGate);
+  const int es = dtype == TRNBLAS_F32 ? 4 : 2, eo = out_dtype == TRNBLAS_F32 ? 4 : 2;
+  GateArgs g{};
+  g.P = P, g.ldp = ldp, g.D = H, g.ldd = ldh, g.S = S, g.lds = lds;
+  g.rows = rows, g.n = (int)N, g.act = act;
+  g.vec = N % kGateV == 0 && whole(P, ldp, N, es) && whole(H, ldh, N, eo) && whole(S, lds, N, eo);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid = gate_grid(g), block(64, 4);
+  switch (dtype == TRNBLAS_F32 ? 3 + out_dtype : dtype) {
+    case TRNBLAS_BF16: hipLaunchKernelGGL((gate_kernel<__bf16, __bf16>), grid, block, 0, s, g); break;
+    case TRNBLAS_F16: hipLaunchKernelGGL((gate_kernel<_Float16, _Float16>), grid, block, 0, s, g); break;
+    case 3 + TRNBLAS_BF16: hipLaunchKernelGGL((gate_kernel<float, __bf16>), grid, block, 0, s, g); break;
+    case 3 + TRNBLAS_F16: hipLaunchKernelGGL((gate_kernel<float, _Float16>), grid, block, 0, s, g); break;
+    default: hipLaunchKernelGGL((gate_kernel<float, float>), grid, block, 0, s, g); break;
+  }
+  return check_launch(kGate);
+}
+
+extern "C" int trnblas_hip_gate_backward(int act, int dtype, int64_t rows, int64_t N, const void* P, int64_t ldp, const void* dH,
+                                         int64_t ldg, void* dP, int64_t ldd, void* stream) {
+  if (int rc = check_gate(kGateBackward, act, dtype, rows, N)) return rc;
+  TRNBLAS_CHECK_ARG(ldp >= 2 * N && ldg >= N && ldd >= 2 * N, "%s: bad leading dimension", kGateBackward);
+  if (rows == 0 || N == 0) return TRNBLAS_OK;
+  TRNBLAS_CHECK_ARG(P != nullptr && dH != nullptr && dP != nullptr, "%s: null operand", kGateBackward);
+  const int es = dtype == TRNBLAS_F32 ? 4 : 2;
+  GateArgs g{};
+  g.P = P, g.ldp = ldp, g.dH = dH, g.ldg = ldg, g.D = dP, g.ldd = ldd;
+  g.rows = rows, g.n = (int)N, g.act = act;
+  g.vec = N % kGateV == 0 && whole(P, ldp, N, es) && whole(dH, ldg, N, es) && whole(dP, ldd, N, es);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid = gate_grid(g), block(64, 4);
+  switch (dtype) {
+    case TRNBLAS_F32: hipLaunchKernelGGL(gate_backward_kernel<float>, grid, block, 0, s, g); break;
+    case TRNBLAS_BF16: hipLaunchKernelGGL(gate_backward_kernel<__bf16>, grid, block, 0, s, g); break;
+    default: hipLaunchKernelGGL(gate_backward_kernel<_Float16>, grid, block, 0, s, g); break;
+  }
+  return check_launch(kGateBackward);
+}

@@ -30,7 +30,8 @@ static int common_args(const char* what, GroupedArgs& g, int dtype, int out_f32,
   TRNBLAS_CHECK_ARG(dtype == TRNBLAS_F32 || dtype == TRNBLAS_BF16 || dtype == TRNBLAS_F16, "%s: bad dtype %d", what, dtype);
   TRNBLAS_CHECK_ARG(groups >= 0 && groups < (1 << 24) && rows >= 0 && rows < INT32_MAX - 1024,
                     "%s: bad sizes (groups %lld, rows %lld)", what, (long long)groups, (long long)rows);
-  TRNBLAS_CHECK_ARG(offsets != nullptr && (uintptr_t)offsets % (offsets64 ? 8 : 4) == 0, "%s: offsets missing or misaligned", what);
+  TRNBLAS_CHECK_ARG(offsets != nullptr ? (uintptr_t)offsets % (offsets64 ? 8 : 4) == 0 : groups == 1,
+                    "%s: offsets missing or misaligned", what);
   TRNBLAS_CHECK_ARG(beta == 0.0 || C != nullptr, "%s: beta != 0 without C", what);
   g.padded = padded != 0;
   g.offsets = offsets;

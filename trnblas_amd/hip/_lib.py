@@ -19,7 +19,7 @@ import torch  # noqa: F401  (loads torch's HIP runtime before the library)
 _PKG = Path(__file__).resolve().parent.parent
 LIB_PATH = Path(os.environ.get("TRNBLAS_HIP_LIB", _PKG / "lib" / "libtrnblas_hip.so"))
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 F32, BF16, F16, F64 = 0, 1, 2, 3
 DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
@@ -186,6 +186,14 @@ SIGNATURES = {
     "trnblas_hip_grouped_rows_plan": (
         _c_int,
         [_c_int, _c_int, _c_int] + [_c_i64] * 4 + [ctypes.POINTER(ctypes.c_int32)],
+    ),
+    "trnblas_hip_gate": (
+        _c_int,
+        [_c_int, _c_int, _c_int, _c_i64, _c_i64] + [_c_ptr, _c_i64] * 3 + [_c_ptr],
+    ),
+    "trnblas_hip_gate_backward": (
+        _c_int,
+        [_c_int, _c_int, _c_i64, _c_i64] + [_c_ptr, _c_i64] * 3 + [_c_ptr],
     ),
     "trnblas_hip_dgemm": (
         _c_int,

@@ -1320,9 +1320,9 @@ def get_native_ops() -> dict:
 # reads the offsets on the host).
 
 
-def _group_rows(offsets: torch.Tensor, rows: int):
-    """(group, first row, row after the last) of each group that has rows."""
-    o = [min(max(int(x), 0), rows) for x in offsets.tolist()]
+def _group_rows(offsets: torch.Tensor | None, rows: int):
+    """(group, first row, row after the last) of each group that has rows (no offsets: one group of all)."""
+    o = [0, rows] if offsets is None else [min(max(int(x), 0), rows) for x in offsets.tolist()]
     for g, (a, b) in enumerate(zip(o, o[1:])):
         if b > a:
             yield g, a, b
@@ -1374,7 +1374,8 @@ def grouped_rank_k(alpha, A, B, offsets, beta, C, out_dtype) -> torch.Tensor:
         except Exception as exc:  # noqa: BLE001
             _kernel_failed(exc)
     dt = _sum_dtype(A.dtype)
-    P = torch.zeros((offsets.shape[0] - 1, A.shape[1], B.shape[1]), dtype=dt, device=A.device)
+    groups = 1 if offsets is None else offsets.shape[0] - 1
+    P = torch.zeros((groups, A.shape[1], B.shape[1]), dtype=dt, device=A.device)
     for g, a, b in _group_rows(offsets, A.shape[0]):
         P[g] = A[a:b].to(dt).mT @ B[a:b].to(dt)
     return _scaled_sum(P, alpha, beta, C, out_dtype)

@@ -23,8 +23,9 @@ def row_major(X: torch.Tensor) -> tuple[torch.Tensor, int]:
     return X, max(c, 1)
 
 
-def offsets_of(offsets: torch.Tensor) -> tuple[torch.Tensor, int]:
-    return offsets.contiguous(), int(offsets.dtype == torch.int64)
+def offsets_of(offsets: torch.Tensor | None) -> tuple[torch.Tensor | None, int]:
+    """None: all rows are one group."""
+    return (None, 0) if offsets is None else (offsets.contiguous(), int(offsets.dtype == torch.int64))
 
 
 def _output_like(C: torch.Tensor | None, beta: float, shape, dtype, dev):
@@ -65,14 +66,15 @@ def _up(n: int, ev: int) -> int:
 def grouped_gemm(
     A: torch.Tensor,
     B: torch.Tensor,
-    offsets: torch.Tensor,
+    offsets: torch.Tensor | None,
     alpha: float = 1.0,
     beta: float = 0.0,
     C: torch.Tensor | None = None,
     out_dtype: torch.dtype | None = None,
 ) -> torch.Tensor:
     """alpha * A[r] @ B[g] + beta * C[r] for the rows r of each group g: A
-    (R, K), B (G, K, N) (transposed views are read in place), offsets (G + 1)."""
+    (R, K), B (G, K, N) (transposed views are read in place), offsets (G + 1), or
+    None for one group of all rows."""
     A, B = A.resolve_neg(), B.resolve_neg()
     dev = _require_device(A, B, offsets, *(() if C is None else (C,)))
     R, K = A.shape
@@ -102,7 +104,7 @@ def grouped_gemm(
 def grouped_rank_k(
     A: torch.Tensor,
     B: torch.Tensor,
-    offsets: torch.Tensor,
+    offsets: torch.Tensor | None,
     alpha: float = 1.0,
     beta: float = 0.0,
     C: torch.Tensor | None = None,
@@ -114,7 +116,7 @@ def grouped_rank_k(
     dev = _require_device(A, B, offsets, *(() if C is None else (C,)))
     R, M = A.shape
     N = B.shape[1]
-    G = offsets.shape[0] - 1
+    G = 1 if offsets is None else offsets.shape[0] - 1
     a, lda = row_major(A)
     b, ldb = row_major(B)
     ev, padded = 16 // A.element_size(), False
@@ -186,7 +188,7 @@ def mx_gemm_from(
         A = A.contiguous()
     R, K = A.shape
     N = b[0].shape[-2]
-    o, o64 = (None, 0) if offsets is None else offsets_of(offsets)
+    o, o64 = offsets_of(offsets)
     D, c = _output_like(C, beta, (R, N), out_dtype, dev)
     ws = torch.empty(_from_workspace(R, K), dtype=torch.uint8, device=dev)
     _probed_call(
@@ -217,7 +219,7 @@ def mx_gemm(
     B (N, K), or (G, N, K) with offsets (G + 1)."""
     dev = _require_device(*a, *b, *(() if C is None else (C,)), *(() if offsets is None else (offsets,)))
     R, N = a[0].shape[0], b[0].shape[-2]
-    o, o64 = (None, 0) if offsets is None else offsets_of(offsets)
+    o, o64 = offsets_of(offsets)
     D, c = _output_like(C, beta, (R, N), out_dtype, dev)
     _probed_call(
         "mx_gemm", "trnblas_hip_mx_gemm", _lib.DTYPE_CODES[out_dtype], 1 if offsets is None else b[0].shape[0], R, N, K,
@@ -265,10 +267,16 @@ def grouped_gemm_fast(alpha, A, B, offsets, transB, out_dtype):
     dev = A.get_device()
     if (
         k != K or s1 != 1 or lda < K or t1 != 1 or t0 < b1 or sb < 0 or N == 0 or dev != _current_device()
-        or B.get_device() != dev or offsets.get_device() != dev or offsets.dtype not in _INTS
-        or offsets.shape != (G + 1,) or offsets.stride() != (1,) or A.is_neg() or B.is_neg()
+        or B.get_device() != dev or A.is_neg() or B.is_neg()
     ):  # fmt: skip
         return None
+    o, o64 = None, False
+    if offsets is not None:
+        if (
+            offsets.get_device() != dev or offsets.dtype not in _INTS or offsets.shape != (G + 1,) or offsets.stride() != (1,)
+        ):  # fmt: skip
+            return None
+        o, o64 = offsets.data_ptr(), offsets.dtype is torch.int64
     if out_dtype is not None and out_dtype is not A.dtype and out_dtype is not torch.float32:
         return None
     pa, pb = A.data_ptr(), B.data_ptr()
@@ -278,8 +286,8 @@ def grouped_gemm_fast(alpha, A, B, offsets, transB, out_dtype):
             return None  # the general path may pack
     D = A.new_empty((R, N), dtype=out_dtype)
     rc = _fn("trnblas_hip_grouped_gemm")(
-        code, D.dtype is torch.float32, transB, G, R, N, K, alpha, pa, lda, pb, t0, sb,
-        offsets.data_ptr(), offsets.dtype is torch.int64, 0.0, None, N, D.data_ptr(), N, 0, _raw_stream(dev),
+        code, D.dtype is torch.float32, transB, G, R, N, K, alpha, pa, lda, pb, t0, sb, o, o64, 0.0, None, N,
+        D.data_ptr(), N, 0, _raw_stream(dev),
     )  # fmt: skip
     _checked("trnblas_hip_grouped_gemm", rc)
     return D
@@ -328,21 +336,24 @@ def grouped_rank_k_fast(alpha, A, B, offsets, out_dtype):
     dev = A.get_device()
     if (
         R2 != R or s1 != 1 or lda < M or t1 != 1 or ldb < N or M == 0 or N == 0 or dev != _current_device() or B.get_device() != dev
-        or offsets.get_device() != dev or offsets.dtype not in _INTS or offsets.dim() != 1 or offsets.stride() != (1,)
         or A.is_neg() or B.is_neg()
     ):  # fmt: skip
         return None
+    G, o, o64 = 1, None, False
+    if offsets is not None:
+        if offsets.get_device() != dev or offsets.dtype not in _INTS or offsets.dim() != 1 or offsets.stride() != (1,):
+            return None
+        G, o, o64 = offsets.shape[0] - 1, offsets.data_ptr(), offsets.dtype is torch.int64
     if out_dtype is not None and out_dtype is not A.dtype and out_dtype is not torch.float32:
         return None
     ev = 4 if code == 0 else 8
     if (A.data_ptr() | B.data_ptr()) % 16 or (lda | ldb | M | N) % ev:
         if R * M * N > _PACK_LOOK:
             return None
-    G = offsets.shape[0] - 1
     D = A.new_empty((G, M, N), dtype=out_dtype)
     rc = _fn("trnblas_hip_grouped_rank_k")(
-        code, D.dtype is torch.float32, G, R, M, N, alpha, A.data_ptr(), lda, B.data_ptr(), ldb, offsets.data_ptr(),
-        offsets.dtype is torch.int64, 0.0, None, N, 0, D.data_ptr(), N, M * N, 0, _raw_stream(dev),
+        code, D.dtype is torch.float32, G, R, M, N, alpha, A.data_ptr(), lda, B.data_ptr(), ldb, o, o64, 0.0, None, N, 0,
+        D.data_ptr(), N, M * N, 0, _raw_stream(dev),
     )  # fmt: skip
     _checked("trnblas_hip_grouped_rank_k", rc)
     return D
