@@ -672,10 +672,23 @@ int trnblas_hip_grouped_rows_plan(int op, int dtype, int transB, int64_t groups,
                                   int64_t N, int64_t K, int32_t plan[3]);
 
 /*
- * Gated projections: H = act(A G) * (A U), elementwise, for weights [G | U] of 2 N
- * columns. No counterpart in the reference. act: TRNBLAS_ACT_*. Computed in fp32, one
- * rounding of each result. Matrices are row-major, of any leading dimension and
- * alignment.
+ * Gated projections: H = act(A G) * (A U), the second product elementwise, for weights
+ * [G | U] of 2 N columns. No counterpart in the reference. act: TRNBLAS_ACT_*. Computed in
+ * fp32, one rounding of each result. Matrices are row-major.
+ *
+ * gated_gemm: H (rows x N) from A (rows x K), for the rows of group g with the gates at B +
+ * g * strideB (K x N, or N x K for transB != 0; leading dimension ldb) and the ups strideU
+ * elements after them. groups, offsets, dtype and padded as in
+ * trnblas_hip_grouped_gemm; rows of no group come out as act(0) * 0. P: null, or the sums
+ * [A G | A U] (rows x 2 N), as gate_backward takes them. H and P have the type of A and B.
+ * A, B, lda, ldb, both strides and K (N where B is N-contiguous) are multiples of 16 bytes,
+ * but for extents of padded operands: other calls are errors (use grouped_gemm into fp32,
+ * and gate, there and for fp32 results of 16-bit operands).
+ *
+ * gated_plan: the name of the kernel that such a call runs on (for rows_kernel: rows of a
+ * tile, waves along K), or NULL with the last error set. Launches nothing.
+ *
+ * gate and gate_backward, of any leading dimension and alignment:
  *
  * gate: H (rows x N, out_dtype) = act(P[:, :N]) * P[:, N:] for P (rows x 2 N) of type
  * `dtype`; out_dtype is that, or with an fp32 P any. S: null, or P rounded to
@@ -684,6 +697,13 @@ int trnblas_hip_grouped_rows_plan(int op, int dtype, int transB, int64_t groups,
  * gate_backward: for the gradient dH (rows x N) of H, dP[:, :N] = dH * U * act'(G) and
  * dP[:, N:] = dH * act(G), P = [G | U]; all of type `dtype`. dP may be P itself.
  */
+int trnblas_hip_gated_gemm(int act, int dtype, int transB, int64_t groups, int64_t rows,
+                           int64_t N, int64_t K, const void* A, int64_t lda,
+                           const void* B, int64_t ldb, int64_t strideB, int64_t strideU,
+                           const void* offsets, int offsets64, void* H, int64_t ldh, void* P,
+                           int64_t ldp, int padded, void* stream);
+const char* trnblas_hip_gated_plan(int dtype, int transB, int64_t groups, int64_t rows, int64_t N,
+                                   int64_t K);
 int trnblas_hip_gate(int act, int dtype, int out_dtype, int64_t rows, int64_t N, const void* P,
                      int64_t ldp, void* H, int64_t ldh, void* S, int64_t lds, void* stream);
 int trnblas_hip_gate_backward(int act, int dtype, int64_t rows, int64_t N, const void* P,

@@ -29,6 +29,65 @@ def _holds(H, A, B, off, transB, act):
     return og.ratio(H, *og.forward(act, P, den, A.shape[1], H.dtype)) <= 1
 
 
+def _plan(dtype, transB, groups, rows, N, K):
+    from trnblas_amd.hip import _lib
+
+    return _lib.load().trnblas_hip_gated_plan(_lib.DTYPE_CODES[dtype], transB, groups, rows, N, K).decode()
+
+
+# (dtype, transB, groups, rows, N, K) that each kernel serves: results that end inside a tile
+REACH = {
+    "gated_ring_kernel 256 x 128": [(BF16, 0, 8, 2600, 2056, 264), (F16, 1, 8, 2600, 2056, 520), (BF16, 1, 8, 5200, 1032, 264)],
+    "gated_ring_kernel 128 x 64": [(F16, 0, 40, 9000, 264, 72), (BF16, 1, 1, 900, 4104, 136)],
+    "gated_ring_kernel 64 x 64": [(BF16, 0, 3, 300, 520, 264), (F16, 1, 3, 300, 520, 1032), (F32, 0, 3, 300, 520, 260), (F32, 1, 1, 900, 260, 516)],
+    "rows_kernel 16 1": [(BF16, 1, 64, 64, 2056, 72), (F16, 1, 40, 40, 4104, 72), (F32, 1, 64, 64, 1032, 68)],
+    "rows_kernel 16 2": [(BF16, 1, 8, 8, 4104, 1032), (F16, 1, 64, 64, 520, 1040)],
+    "rows_kernel 16 4": [(BF16, 1, 8, 8, 2056, 1032), (F16, 1, 64, 64, 264, 1040)],
+    "rows_kernel 16 8": [(BF16, 0, 1, 3, 72, 264), (F16, 1, 3, 3, 72, 1032), (F32, 0, 3, 3, 72, 260), (F32, 1, 1, 1, 72, 4100)],
+    "rows_kernel 32 8": [(BF16, 0, 1, 20, 72, 264), (F16, 1, 3, 27, 72, 520)],
+}
+
+
+@pytest.mark.parametrize("kernel", list(REACH))
+def test_each_kernel(dev, kernel):
+    for i, (dtype, transB, G, R, N, K) in enumerate(REACH[kernel]):
+        assert _plan(dtype, transB, G, R, N, K) == kernel, (dtype, transB, G, R, N, K)
+        A, B = _operands(i, dtype, R, K, N, G, transB, dev)
+        off = _uneven(G, R, i) if R > 4 * G else torch.arange(G + 1) * (R // G)
+        act = og.ACTS[i % 5]
+        H = tb.grouped_gated_gemm(A, B, off.to(dev), act, transB=bool(transB))
+        assert _holds(H, A, B, off, transB, act), (dtype, transB, G, R, N, K)
+        # with what a backward pass needs of it beside it: the same values, and both sums
+        P, den = og.products(A, B, off, transB)
+        from trnblas_amd.hip import gated_kernels
+
+        H2, S = gated_kernels.gated_gemm(A, B.mT if transB else B, off.to(dev), act, dtype, True)
+        assert torch.equal(H2, H)
+        e = (K + 2) * 2.0**-23 * den
+        assert og.ratio(S, P, e + og.EPS[dtype] * (P.abs() + e) + og.TINY[dtype]) <= 1
+        if K % 8 == 0 and transB:  # columns that are no multiple of four: results go out value by value
+            b = B[:, : 2 * (N - 3)].contiguous()
+            H = tb.grouped_gated_gemm(A, b, off.to(dev), act, transB=True)
+            assert _holds(H, A, b, off, True, act)
+            H2, S = gated_kernels.gated_gemm(A, b.mT, off.to(dev), act, dtype, True)
+            P, den = og.products(A, b, off, True)
+            e = (K + 2) * 2.0**-23 * den
+            assert torch.equal(H2, H) and og.ratio(S, P, e + og.EPS[dtype] * (P.abs() + e) + og.TINY[dtype]) <= 1
+
+
+def test_packed_operands(dev):
+    # large ones that LDS DMA cannot read in place
+    for dtype, R, K, N, transB in ((BF16, 1100, 1021, 515, False), (F16, 1100, 1021, 515, True), (BF16, 1100, 1024, 515, False), (F32, 1100, 1021, 515, False)):
+        A, B = _operands(R, dtype, R, K, N, 1, transB, dev)
+        off = torch.tensor([0, R])
+        for a in (A, torch.nn.functional.pad(A, (1, 2))[:, 1 : K + 1]):
+            assert _holds(tb.gated_gemm(a, B[0], transB=transB), A, B, off, transB, "silu"), (dtype, K, transB)
+        a, b = A.requires_grad_(), B[0].requires_grad_()
+        dH = torch.randn(R, N, generator=torch.Generator(device=dev).manual_seed(1), device=dev).to(dtype)
+        grads = torch.autograd.grad(tb.gated_gemm(a, b, transB=transB), (a, b), dH)
+        assert _gradients_hold([grads[0], grads[1][None]], A.detach(), B.detach(), off, transB, "silu", dH, dtype)
+
+
 # (K, N): below and across the tiles of 16, 32, 64 and 128 columns, multiples of 16 bytes and not
 SIZES = [(1, 1), (7, 5), (33, 70), (64, 128), (100, 61), (136, 264), (264, 136), (512, 520), (515, 257), (1032, 384)]
 

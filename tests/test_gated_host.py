@@ -145,3 +145,27 @@ def test_c_abi_refusals():
                       (dict(ldd=15), b"leading"), (dict(d=None), b"null")):  # fmt: skip
         assert back(**bad) == _lib.E_ARG and word in lib.trnblas_hip_last_error(), bad
     assert back(rows=0) == 0
+
+    def product(act=0, dtype=1, groups=2, rows=6, n=8, k=16, a=4096, lda=16, b=4096, ldb=16, sb=128, su=8, off=4096, h=4096, ldh=8,
+                p=None, ldp=16):  # fmt: skip
+        return lib.trnblas_hip_gated_gemm(act, dtype, 0, groups, rows, n, k, a, lda, b, ldb, sb, su, off, 0, h, ldh, p, ldp, 0, None)
+
+    for bad, word in ((dict(act=5), b"activation"), (dict(dtype=3), b"dtype"), (dict(groups=-1), b"sizes"), (dict(rows=1 << 31), b"sizes"),
+                      (dict(k=1 << 31), b"sizes"), (dict(lda=15), b"leading"), (dict(ldb=7), b"leading"), (dict(su=-8), b"leading"),
+                      (dict(ldh=7), b"leading"), (dict(p=4096, ldp=15), b"leading"), (dict(off=None), b"offsets"),
+                      (dict(off=4098), b"offsets"), (dict(a=None), b"null"), (dict(h=None), b"null"), (dict(a=4098), b"16 bytes"),
+                      (dict(lda=17), b"16 bytes"), (dict(su=9), b"16 bytes"), (dict(sb=129), b"16 bytes"), (dict(k=15), b"16 bytes"),
+                      (dict(n=7), b"16 bytes")):  # fmt: skip
+        assert product(**bad) == _lib.E_ARG and word in lib.trnblas_hip_last_error(), bad
+    assert product(rows=0) == 0 and product(n=0) == 0
+    for bad in ((3, 0, 1, 6, 8, 8), (1, 0, 0, 6, 8, 8), (1, 0, 1, 0, 8, 8), (1, 0, 1, 6, 0, 8), (1, 0, 1, 6, 8, -1)):
+        assert lib.trnblas_hip_gated_plan(*bad) is None and b"bad arguments" in lib.trnblas_hip_last_error()
+
+
+@pytest.mark.parametrize("source", ["gated_bf16.hip", "gated_f16.hip"])
+def test_wait_states_before_matrix_instructions(source):
+    from test_wait_states_host import _assembly, hazards
+
+    r = _assembly(source)
+    assert r.returncode == 0, r.stderr
+    assert "v_mfma" in r.stdout and not hazards(r.stdout)

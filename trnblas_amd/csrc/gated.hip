@@ -1,11 +1,14 @@
-// Gated projections H = act(A G) * (A U), [G | U] one matrix of 2 N columns: what lies
-// beside the products.
+// Gated projections H = act(A G) * (A U), [G | U] one matrix of 2 N columns: the C entry of the
+// products (ring.hpp, rows.hpp) and the elementwise kernels beside them.
 #include "gate.hpp"
+#include "grouped.hpp"
+#include "grouped_plan.hpp"
 
 namespace trnblas {
 
-static const char* kGate = "trnblas_hip_gate";
-static const char* kGateBackward = "trnblas_hip_gate_backward";
+static const char* const kGated = "trnblas_hip_gated_gemm";
+static const char* const kGate = "trnblas_hip_gate";
+static const char* const kGateBackward = "trnblas_hip_gate_backward";
 
 struct GateArgs {
   const void* P;  // rows x 2 n: gates, then ups
@@ -166,4 +169,51 @@ extern "C" int trnblas_hip_gate_backward(int act, int dtype, int64_t rows, int64
     default: hipLaunchKernelGGL(gate_backward_kernel<_Float16>, grid, block, 0, s, g); break;
   }
   return check_launch(kGateBackward);
+}
+
+extern "C" int trnblas_hip_gated_gemm(int act, int dtype, int transB, int64_t groups, int64_t rows, int64_t N, int64_t K,
+                                      const void* A, int64_t lda, const void* B, int64_t ldb, int64_t strideB, int64_t strideU,
+                                      const void* offsets, int offsets64, void* H, int64_t ldh, void* P, int64_t ldp, int padded,
+                                      void* stream) {
+  if (int rc = check_gate(kGated, act, dtype, rows, N)) return rc;
+  TRNBLAS_CHECK_ARG(groups >= 0 && groups < (1 << 24) && K >= 0 && K < INT32_MAX - 1024, "%s: bad sizes (groups %lld, K %lld)", kGated,
+                    (long long)groups, (long long)K);
+  TRNBLAS_CHECK_ARG(offsets != nullptr ? (uintptr_t)offsets % (offsets64 ? 8 : 4) == 0 : groups == 1,
+                    "%s: offsets missing or misaligned", kGated);
+  TRNBLAS_CHECK_ARG(lda >= K && ldb >= (transB ? K : N) && strideB >= 0 && strideU >= 0 && ldh >= N && (P == nullptr || ldp >= 2 * N),
+                    "%s: bad leading dimension", kGated);
+  if (rows == 0 || N == 0) return TRNBLAS_OK;
+  TRNBLAS_CHECK_ARG(H != nullptr && ((A != nullptr && B != nullptr) || K == 0 || groups == 0), "%s: null operand", kGated);
+  GroupedArgs g{};
+  g.A = A, g.lda = lda;
+  g.B = B, g.ldb = ldb, g.sB = strideB, g.sU = strideU;
+  g.D = H, g.ldd = ldh;
+  g.P = P, g.ldp = ldp;
+  g.offsets = offsets, g.offsets64 = offsets64 != 0;
+  g.groups = (int)groups, g.rows = (int)rows, g.N = (int)N, g.K = (int)K;
+  g.alpha = 1.0f;
+  g.act = act;
+  g.out32 = dtype == TRNBLAS_F32;
+  g.padded = padded != 0;
+  const int64_t eo = g.out32 ? 4 : 2;
+  g.vec4 = (uintptr_t)H % (4 * eo) == 0 && ldh % 4 == 0 &&
+           (P == nullptr || ((uintptr_t)P % (4 * eo) == 0 && ldp % 4 == 0 && N % 4 == 0));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case TRNBLAS_F32: return gated_gemm_run<float>(g, transB != 0, s);
+    case TRNBLAS_BF16: return gated_gemm_run<__bf16>(g, transB != 0, s);
+    default: return gated_gemm_run<_Float16>(g, transB != 0, s);
+  }
+}
+
+extern "C" const char* trnblas_hip_gated_plan(int dtype, int transB, int64_t groups, int64_t rows, int64_t N, int64_t K) {
+  static const char* const kRing[] = {"gated_ring_kernel 256 x 128", "gated_ring_kernel 128 x 64", "gated_ring_kernel 64 x 64"};
+  static const char* const kRows[] = {"rows_kernel 16 1", "rows_kernel 16 2", "rows_kernel 16 4", "rows_kernel 16 8", "rows_kernel 32 8"};
+  if (dtype < 0 || dtype > 2 || groups < 1 || rows < 1 || N < 1 || K < 0) {
+    set_error("trnblas_hip_gated_plan: bad arguments");
+    return nullptr;
+  }
+  const GroupedChoice c = choose_gated(dtype == TRNBLAS_F32 ? 4 : 2, rows, groups, N, K, transB != 0);
+  if (c.ring >= 0) return kRing[c.ring];
+  return kRows[c.mf == 2 ? 4 : c.ks == 8 ? 3 : c.ks / 2];
 }

@@ -32,6 +32,11 @@ struct GroupedArgs {
   int out32;  // D and C are fp32 whatever the operands are
   int padded; // operands end in zeros up to 16 bytes (host only)
   int vec4;   // D and C take 4-element accesses (aligned, ld % 4 == 0)
+  // gated projections: B holds the gates' columns (g.N of them), the ups' stand sU elements further on
+  int64_t sU;
+  void* P;  // sums of both as [gates | ups] in D's type, or null
+  int64_t ldp;
+  int act;
 };
 
 // An fp32 result of 16-bit operands is summed in chains of at most so many values of k. One chain
@@ -383,7 +388,8 @@ __device__ __forceinline__ bool tile_job(const GroupedArgs& g, TileJob& j) {
 // stores of each lane's quad: 16383 x 4095 bf16 took 120 us longer).
 template <int FN>
 constexpr int kStoreLds = 16 * (16 * FN + 4) * 4;
-template <int FM, int FN, typename O>
+// BETA: g.beta may be other than zero.
+template <int FM, int FN, typename O, bool BETA = true>
 __device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& j, const f32x4 (&acc)[FM][FN], int m0,
                                            int n0, int lane, char* lds) {
   typedef O o4 __attribute__((ext_vector_type(4)));
@@ -411,7 +417,7 @@ __device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& 
     // blocks, so that a lane stores 16 bytes and a row 64 at a time (8 and 32: 8192 x
     // 2048 x 8192 237 us, now 223; 8191 x 2056 x 4104 of 4-bit values 88, now 82)
     if constexpr (sizeof(O) == 2) {
-      if (g.beta == 0.0f && (((uint64_t)D / 2 | (uint64_t)g.ldd | (uint64_t)g.N) & 7) == 0) {
+      if ((!BETA || g.beta == 0.0f) && (((uint64_t)D / 2 | (uint64_t)g.ldd | (uint64_t)g.N) & 7) == 0) {
         typedef int i32x2 __attribute__((ext_vector_type(2)));
         auto pack = [&](int a, int b) __attribute__((always_inline)) {
           const f32x4 v = take(a, b) * g.alpha;
@@ -435,7 +441,7 @@ __device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& 
         return;
       }
     }
-    if (g.beta == 0.0f) {
+    if (!BETA || g.beta == 0.0f) {
 #pragma unroll
       for (int a = 0; a < FM; ++a) store(a, [&](int p, int b) __attribute__((always_inline)) { return take(p, b) * g.alpha; });
     } else {
@@ -471,7 +477,7 @@ __device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& 
       const int e = 64 * h + lane, r = e / W, c = e % W, m = m0 + 16 * a + r, col = j.n + n0 + c;
       float v = buf[r * LD + c];
       if (m < j.rows_a && col < g.N) {
-        if (g.beta != 0.0f) v = __builtin_fmaf(g.beta, (float)C[(j.m + m) * g.ldc + col], v);
+        if (BETA && g.beta != 0.0f) v = __builtin_fmaf(g.beta, (float)C[(j.m + m) * g.ldc + col], v);
         D[(j.m + m) * g.ldd + col] = (O)v;
       }
     }
@@ -485,5 +491,8 @@ template <typename T>
 int grouped_gemm_run(const GroupedArgs& g, bool bkc, hipStream_t s);
 template <typename T>
 int grouped_rank_k_run(const GroupedArgs& g, hipStream_t s);
+// gated_run.hpp
+template <typename T>
+int gated_gemm_run(const GroupedArgs& g, bool bkc, hipStream_t s);
 
 }  // namespace trnblas

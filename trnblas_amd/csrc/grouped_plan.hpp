@@ -131,6 +131,20 @@ inline GroupedChoice choose_gemm(int elem_bytes, double rows, double groups, dou
                          : choose_grouped(kRing16, rows, groups, N, K, K * elem_bytes, elem_bytes, kc);
 }
 
+// gated_gemm: by the costs of a product of all 2 N columns. rows_kernel: a workgroup takes half
+// as many columns of H, hence the fewest waves along K that leave two workgroups per CU of
+// these (fp32: eight or one, the sizes between run on the ring).
+inline GroupedChoice choose_gated(int elem_bytes, double rows, double groups, double N, double K, bool kc) {
+  GroupedChoice c = choose_gemm(elem_bytes, rows, groups, 2.0 * N, K, kc);
+  if (c.ring == kAnyTiles) c.ring = 2;
+  c.ks = 8;
+  if (c.ring < 0 && kc && c.mf == 1)
+    for (const int step = elem_bytes == 4 ? 8 : 2;
+         c.ks > 1 && likely_row_tiles(rows, groups, 16) * std::ceil(N * (c.ks / step) / 128.0) >= 2.0 * device_cus();)
+      c.ks /= step;
+  return c;
+}
+
 // grouped_rank_k of aligned operands: groups x (M x N), over the average group's k-tiles. fp32 has
 // the 64 x 128 tiles alone: three workgroups per CU hide its longer MFMAs' steps.
 inline int choose_rank_k(int elem_bytes, double groups, double rows, double M, double N) {

@@ -3,6 +3,7 @@
 // k-tiles of 128 bytes per row in two LDS stages.
 #pragma once
 
+#include "gate.hpp"
 #include "gemm.hpp"
 #include "grouped.hpp"
 #include "grouped_plan.hpp"
@@ -183,20 +184,59 @@ __device__ __forceinline__ int lane_of() {
   return lane;
 }
 
-template <typename T, int FM, int FN, bool BKC, bool RK, bool CHAINS>
+// The outputs of a wave of gated projections: both sums to P, where it is asked for, and H.
+template <int FM, int FH, typename O>
+__device__ __forceinline__ void store_gated(const GroupedArgs& g, TileJob j, f32x4 (&acc)[2][FM][FH], int m0, int n0, int lane,
+                                            char* lds) {
+  if (g.P) {
+    GroupedArgs p = g;
+    p.ldd = g.ldp;
+    void* h = j.D;
+    j.D = g.P;
+    store_wave<FM, FH, O, false>(p, j, acc[0], m0, n0, lane, lds);
+    j.D = static_cast<O*>(g.P) + g.N;
+    store_wave<FM, FH, O, false>(p, j, acc[1], m0, n0, lane, lds);
+    j.D = h;
+  }
+  // one kind of activation at a time: a switch in each value's path costs registers and branches
+  auto apply = [&](auto actc) __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < FM; ++a) {
+#pragma unroll
+      for (int b = 0; b < FH; ++b)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[0][a][b][u] = gate(decltype(actc)::value, acc[0][a][b][u]) * acc[1][a][b][u];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  switch (g.act) {
+    case TRNBLAS_ACT_SILU: apply(std::integral_constant<int, TRNBLAS_ACT_SILU>{}); break;
+    case TRNBLAS_ACT_GELU: apply(std::integral_constant<int, TRNBLAS_ACT_GELU>{}); break;
+    case TRNBLAS_ACT_GELU_TANH: apply(std::integral_constant<int, TRNBLAS_ACT_GELU_TANH>{}); break;
+    case TRNBLAS_ACT_RELU: apply(std::integral_constant<int, TRNBLAS_ACT_RELU>{}); break;
+    default: apply(std::integral_constant<int, TRNBLAS_ACT_SIGMOID>{}); break;
+  }
+  store_wave<FM, FH, O, false>(g, j, acc[0], m0, n0, lane, lds);
+}
+
+// GATED (see trnblas_hip_gated_gemm): B's panel is two of half the columns, gates and ups, and a wave has
+// FN / 2 blocks of each at the same columns of H, so that gate and up of a value meet in
+// a lane.
+template <typename T, int FM, int FN, bool BKC, bool RK, bool CHAINS, bool GATED = false>
 __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& x, const TileJob& j, int wave, char* lds) {
   constexpr bool MX = std::is_same_v<T, fp4x2>, FOLD = std::is_same_v<T, float>;
   using L = RingLds<T, FM, FN>;
   constexpr int WAVES = 4, BM = L::BM, BN = L::BN, NS = L::NS, SA = L::SA, SB = L::SB, SGROUP = L::SGROUP, SRING = L::SRING;
+  constexpr int HALVES = GATED ? 2 : 1, FH = FN / HALVES;  // of B's panel; a wave's blocks in each
   using DA = PanelDma<T, BM, !RK, WAVES>;
-  using DB = PanelDma<T, BN, BKC, WAVES>;
+  using DB = PanelDma<T, BN / HALVES, BKC, WAVES>;
   using PA = typename DA::P;
   using PB = typename DB::P;
   constexpr int STAGE = L::STAGE;
-  constexpr int ND = DA::NB + DB::NB;  // DMAs per wave and k-tile, besides scales
-  static_assert(STAGE == PA::BYTES + PB::BYTES && SA + SB <= 16, "one scale DMA per wave and step");
+  constexpr int ND = DA::NB + HALVES * DB::NB;  // DMAs per wave and k-tile, besides scales
+  static_assert(STAGE == PA::BYTES + HALVES * PB::BYTES && SA + SB <= 16, "one scale DMA per wave and step");
   const int lane = lane_of<CHAINS>();
-  const int m0 = (wave & 1) * (16 * FM), n0 = (wave >> 1) * (16 * FN);
+  const int m0 = (wave & 1) * (16 * FM), n0 = (wave >> 1) * (16 * FH);
   const int nk = (j.K + PA::BK - 1) / PA::BK;
   const uint32_t lds0 = lds_offset(lds);
   DA da;
@@ -204,6 +244,7 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
   da.init(j.A, g.lda, j.rows_a, wave, lane);
   db.init(j.B, g.ldb, j.rows_b, wave, lane);
   i32x4 ra, rb;
+  [[maybe_unused]] i32x4 ru;
   uint32_t sta, stb;  // LDS offsets of the wave's blocks in the stage that takes the DMA
   // k-tile kt is the next to move, into stage kt % NS
   auto dma_turn = [&](int kt) __attribute__((always_inline)) {
@@ -217,6 +258,7 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
     stb = st + PA::BYTES + DB::NB * 1024 * wave;
     ra = dma_rsrc(da.base, left > 0 ? kRecords : 0);
     rb = dma_rsrc(db.base, left > 0 ? kRecords : 0);
+    if constexpr (GATED) ru = dma_rsrc(db.base + g.sU * (int64_t)sizeof(T), left > 0 ? kRecords : 0);
     da.base += da.step;
     db.base += db.step;
   };
@@ -224,8 +266,10 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
     constexpr int u = decltype(uc)::value;
     if constexpr (u < DA::NB)
       lds_dma<1024 * u>(ra, sta, da.off[u]);
-    else if constexpr (u < ND)
+    else if constexpr (u < DA::NB + DB::NB)
       lds_dma<1024 * (u - DA::NB)>(rb, stb, db.off[u - DA::NB]);
+    else if constexpr (u < ND)
+      lds_dma<1024 * (u - DA::NB - DB::NB) + PB::BYTES>(ru, stb, db.off[u - DA::NB - DB::NB]);
   };
 
   // DMA i of a scale group: chunks 4 i .. 4 i + 3 of A's rows, then of B's. In
@@ -249,14 +293,14 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
     }
   };
 
-  f32x4 acc[FM][FN];
+  f32x4 acc[HALVES][FM][FH];
   [[maybe_unused]] f32x4 sum[FOLD ? FM : 1][FOLD ? FN : 1];
 #pragma unroll
   for (int a = 0; a < FM; ++a)
 #pragma unroll
     for (int b = 0; b < FN; ++b) {
-      acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (FOLD) sum[a][b] = acc[a][b];
+      acc[b / FH][a][b % FH] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (FOLD) sum[a][b] = acc[b / FH][a][b % FH];
     }
   [[maybe_unused]] int qa[FM], qb[FN];
   auto read_scales = [&](int grp) __attribute__((always_inline)) {
@@ -291,9 +335,14 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
     for (int i = 0; i < PB::NV; ++i) pb[i] += d;
   };
   auto read = [&](int i, int set) __attribute__((always_inline)) {
-    if (i < FN)
+    if (i < FH) {
       fb[set][i] = PB::frag(pb, i, set);
-    else if (i < FN + FM)
+    } else if (i < FN) {
+      const char* pu[PB::NV];
+#pragma unroll
+      for (int v = 0; v < PB::NV; ++v) pu[v] = pb[v] + PB::BYTES;
+      fb[set][i] = PB::frag(pu, i - FH, set);
+    } else if (i < FN + FM)
       fa[set][i - FN] = PA::frag(pa, i - FN, set);
   };
   [[maybe_unused]] int span = 0, chain = 0;
@@ -318,7 +367,7 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
           read_from(kt + 1);
         }
       }
-      mma_block<T, 2 * ODD + s>(acc[a][b], fb[s][b], fa[s][a], MX ? qb[b] : 0, MX ? qa[a] : 0);
+      mma_block<T, 2 * ODD + s>(acc[b / FH][a][b % FH], fb[s][b], fa[s][a], MX ? qb[b] : 0, MX ? qa[a] : 0);
       each<ND>([&](auto uc) __attribute__((always_inline)) {
         if constexpr (t >= 0 && decltype(uc)::value * DW / ND == t) dma(uc);
       });
@@ -338,8 +387,8 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
         for (int a = 0; a < FM; ++a)
 #pragma unroll
           for (int b = 0; b < FN; ++b) {
-            sum[a][b] += acc[a][b];
-            acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            sum[a][b] += acc[b / FH][a][b % FH];
+            acc[b / FH][a][b % FH] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
           }
         chain = span;
       }
@@ -383,24 +432,30 @@ __device__ __forceinline__ void ring_tile(const GroupedArgs& g, const MxScales& 
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA into the LDS of the next workgroup
-    if constexpr (!FOLD) settle(acc);
+    if constexpr (!FOLD) {
+      settle(acc[0]);
+      if constexpr (GATED) settle(acc[1]);
+    }
   }
   if constexpr (FOLD) {
 #pragma unroll
     for (int a = 0; a < FM; ++a)
 #pragma unroll
-      for (int b = 0; b < FN; ++b) acc[a][b] += sum[a][b];
+      for (int b = 0; b < FN; ++b) acc[b / FH][a][b % FH] += sum[a][b];
   }
   using O = std::conditional_t<MX, __bf16, T>;
-  static_assert(4 * kStoreLds<FN> <= L::BYTES);
-  char* own = lds + wave * kStoreLds<FN>;
+  static_assert(4 * kStoreLds<FH> <= L::BYTES);
+  char* own = lds + wave * kStoreLds<FH>;
   if (!(g.vec4 && (g.N & 3) == 0)) __syncthreads();  // the other waves' reads
-  if (CHAINS || g.out32)
-    store_wave<FM, FN, float>(g, j, acc, m0, n0, CHAINS ? lane_of<CHAINS>() : lane, own);
-  else if (MX && g.out_f16)
-    store_wave<FM, FN, _Float16>(g, j, acc, m0, n0, lane, own);
-  else
-    store_wave<FM, FN, O>(g, j, acc, m0, n0, lane, own);
+  if constexpr (GATED) {
+    store_gated<FM, FH, O>(g, j, acc, m0, n0, lane, own);
+  } else if (CHAINS || g.out32) {
+    store_wave<FM, FN, float>(g, j, acc[0], m0, n0, CHAINS ? lane_of<CHAINS>() : lane, own);
+  } else if (MX && g.out_f16) {
+    store_wave<FM, FN, _Float16>(g, j, acc[0], m0, n0, lane, own);
+  } else {
+    store_wave<FM, FN, O>(g, j, acc[0], m0, n0, lane, own);
+  }
 }
 
 // An address that all lanes have, as a scalar.
@@ -448,6 +503,23 @@ __global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void ring_kernel(Groupe
     }
   }
   ring_chains<T, FM, FN, BKC, RK, CHAINS>(g, x, j, wave, lds);
+}
+
+// The same tiles of gated projections: 32 FM rows by 16 FN columns of H.
+template <typename T, int FM, int FN, bool BKC>
+__global__ __launch_bounds__(256, FM * FN <= 16 ? 2 : 1) void gated_ring_kernel(GroupedArgs g) {
+  constexpr bool SPLIT = FM * FN == 64;
+  __shared__ __attribute__((aligned(16))) char lds[RingLds<T, FM, FN>::BYTES];
+  TileJob j;
+  if (!tile_job<T, 32 * FM, 16 * FN, BKC, false, SPLIT>(g, j)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if constexpr (SPLIT) {
+    if (j.quarter >= 0) {
+      ring_tile<T, FM / 2, FN / 2, BKC, false, false, true>(g, MxScales{}, j, wave, lds);
+      return;
+    }
+  }
+  ring_tile<T, FM, FN, BKC, false, false, true>(g, MxScales{}, j, wave, lds);
 }
 
 // Workgroups of such a launch over `tiles` tiles (or at most so many), SPLIT's

@@ -2,6 +2,7 @@
 // once, straight into registers.
 #pragma once
 
+#include "gate.hpp"
 #include "gemm.hpp"
 #include "grouped_plan.hpp"
 #include "mx_block.hpp"
@@ -24,7 +25,7 @@ template <typename T>
 constexpr int rows_steps = sizeof(T) == 1 ? 4 : 2;
 template <typename T>
 constexpr int rows_ahead(int mf, int nf) {
-  return (mf + nf <= 3 ? 8 : 4) / rows_steps<T>;
+  return (mf + nf <= 3 ? 8 : nf <= 4 ? 4 : 2) / rows_steps<T>;
 }
 
 // NF MFMA operands of 16 columns over one step of 64 bytes of k, as loaded from
@@ -101,6 +102,21 @@ __device__ __forceinline__ void quantize_rows(const GroupedArgs& g, const MxScal
   }
 }
 
+// Four outputs of gated projections, of their sums, and the sums to P where it is asked for.
+template <typename O>
+__device__ __forceinline__ void store_gated_quad(const GroupedArgs& g, int64_t m, int n, const f32x4& gates, const f32x4& ups) {
+  if (g.P) {
+    GroupedArgs p = g;
+    p.ldd = g.ldp;
+    store_quad<O>(p, nullptr, static_cast<O*>(g.P), m, n, gates);
+    store_quad<O>(p, nullptr, static_cast<O*>(g.P) + g.N, m, n, ups);
+  }
+  f32x4 h;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) h[u] = gate(g.act, gates[u]) * ups[u];
+  store_quad<O>(g, nullptr, static_cast<O*>(g.D), m, n, h);
+}
+
 // Tiles of 16 MF rows by BN columns. KS of the eight waves split K between them
 // (chunks of CH bytes per row, chunk c to wave c % KS) and add their sums through
 // LDS in wave order; 8 / KS such sets take 16 NF columns each. What bounds it is
@@ -119,15 +135,18 @@ __device__ __forceinline__ void quantize_rows(const GroupedArgs& g, const MxScal
 // X (4-bit floats only): A comes as values of that type, at most kInPlace in the
 // tile's rows; the workgroup quantises them into LDS behind its first loads of B,
 // which saves a launch of its own (one row of 8192 by 8192^2: 5 us).
-template <typename T, int MF, int NF, int KS, bool BKC, typename X = void, bool CHAINS = false>
+//
+// GATED (see trnblas_hip_gated_gemm): a wave has NF blocks of gate columns and the same of ups.
+template <typename T, int MF, int NF, int KS, bool BKC, typename X = void, bool CHAINS = false, bool GATED = false>
 __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
   constexpr bool MX = std::is_same_v<T, fp4x2>, FOLD = std::is_same_v<T, float> || CHAINS;
   constexpr int ES = sizeof(T), EV = 16 / ES, BM = 16 * MF, BW = 16 * NF, BN = 8 / KS * BW;
   constexpr int STEPS = rows_steps<T>, CH = 64 * STEPS, CK = CH / ES;  // a chunk: bytes, values of k
-  constexpr int U = rows_ahead<T>(MF, NF);
+  constexpr int HALVES = GATED ? 2 : 1, NB = HALVES * NF, NC = BKC ? 1 : HALVES;
+  constexpr int U = rows_ahead<T>(MF, NB);
   static_assert(BKC || NF == 4, "four columns of a lane");
   constexpr bool QUANT = !std::is_void_v<X>;
-  __shared__ __attribute__((aligned(16))) f32x4 part[8][BM * BW / 4];
+  __shared__ __attribute__((aligned(16))) f32x4 part[HALVES][8][BM * BW / 4];
   Segment s;
   if (!ragged_tile<BM>(g, blockIdx.x, 8, s)) return;
   const bool of_group = s.group >= 0 && s.group < g.groups;
@@ -140,8 +159,8 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
   __shared__ __attribute__((aligned(16))) char qlds[QUANT ? kInPlace / 2 + kInPlace / 32 + 64 * BM : 16];
   [[maybe_unused]] const int nr = min(s.end - s.row, BM);
   const char* pa[MF];
-  const char* pb[BKC ? NF : 1];
-  [[maybe_unused]] const uint8_t *qa[MF], *qb[NF];
+  const char* pb[BKC ? NB : NC];
+  [[maybe_unused]] const uint8_t *qa[MF], *qb[NB];
 #pragma unroll
   for (int a = 0; a < MF; ++a) {
     if constexpr (QUANT) {
@@ -156,26 +175,29 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
   }
   if constexpr (BKC) {
 #pragma unroll
-    for (int b = 0; b < NF; ++b) {
-      const int64_t n = min(n0 + 16 * b + li, g.N - 1);
-      pb[b] = static_cast<const char*>(g.B) + (grp * g.sB + n * g.ldb) * ES + 16 * lg;
+    for (int b = 0; b < NB; ++b) {
+      const int64_t n = min(n0 + 16 * (b % NF) + li, g.N - 1);
+      pb[b] = static_cast<const char*>(g.B) + (grp * g.sB + n * g.ldb + (b < NF ? 0 : g.sU)) * ES + 16 * lg;
       if constexpr (MX) qb[b] = x.b + grp * x.b_step + (n >> 4) * x.chunks * kChunk + 64 * lg + 4 * (n & 15);
     }
   } else {
-    pb[0] = static_cast<const char*>(g.B) + (grp * g.sB + (int64_t)(EV * lg) * g.ldb + min(n0 + 4 * li, ((g.N + 3) & ~3) - 4)) * ES;
+#pragma unroll
+    for (int h = 0; h < NC; ++h)
+      pb[h] = static_cast<const char*>(g.B) +
+              (grp * g.sB + (int64_t)(EV * lg) * g.ldb + min(n0 + 4 * li, ((g.N + 3) & ~3) - 4) + (h ? g.sU : 0)) * ES;
   }
   const int64_t kstep = (BKC ? 64 : 64 / ES * g.ldb * ES);  // bytes of B per step
   struct Chunk {
     i32x4 a[MF][STEPS];
-    i32x4 b[BKC ? NF : 1][STEPS];
-    ColumnStep<std::conditional_t<MX, __bf16, T>> c[BKC ? 1 : STEPS];
-    int sa[MF], sb[NF];
+    i32x4 b[BKC ? NB : 1][STEPS];
+    ColumnStep<std::conditional_t<MX, __bf16, T>> c[NC][BKC ? 1 : STEPS];
+    int sa[MF], sb[NB];
   } w[U];
-  f32x4 acc[MF][NF], sum[FOLD ? MF : 1][FOLD ? NF : 1];
+  f32x4 acc[MF][NB], sum[FOLD ? MF : 1][FOLD ? NB : 1];
 #pragma unroll
   for (int a = 0; a < MF; ++a)
 #pragma unroll
-    for (int b = 0; b < NF; ++b) {
+    for (int b = 0; b < NB; ++b) {
       acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if constexpr (FOLD) sum[a][b] = acc[a][b];
     }
@@ -192,14 +214,15 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
     for (int h = 0; h < STEPS; ++h) {
       if constexpr (BKC) {
 #pragma unroll
-        for (int b = 0; b < NF; ++b) v.b[b][h] = load16<T>(pb[b] + (int64_t)c * CH + 64 * h);
+        for (int b = 0; b < NB; ++b) v.b[b][h] = load16<T>(pb[b] + (int64_t)c * CH + 64 * h);
       } else {
-        v.c[h].load(pb[0] + (int64_t)(STEPS * c + h) * kstep, g.ldb);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) v.c[i][h].load(pb[i] + (int64_t)(STEPS * c + h) * kstep, g.ldb);
       }
     }
     if constexpr (MX) {
 #pragma unroll
-      for (int b = 0; b < NF; ++b) v.sb[b] = *reinterpret_cast<const int*>(qb[b] + (int64_t)c * kChunk);
+      for (int b = 0; b < NB; ++b) v.sb[b] = *reinterpret_cast<const int*>(qb[b] + (int64_t)c * kChunk);
     }
   };
   // the last, partial chunk
@@ -211,28 +234,29 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
       for (int a = 0; a < MF; ++a) v.a[a][h] = left > 0 ? load16<T>(pa[a] + (int64_t)c * CH + 64 * h) : i32x4{0, 0, 0, 0};
       if constexpr (BKC) {
 #pragma unroll
-        for (int b = 0; b < NF; ++b) v.b[b][h] = left > 0 ? load16<T>(pb[b] + (int64_t)c * CH + 64 * h) : i32x4{0, 0, 0, 0};
+        for (int b = 0; b < NB; ++b) v.b[b][h] = left > 0 ? load16<T>(pb[b] + (int64_t)c * CH + 64 * h) : i32x4{0, 0, 0, 0};
       } else {
-        v.c[h].load_last(pb[0] + (int64_t)(STEPS * c + h) * kstep, g.ldb, left);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) v.c[i][h].load_last(pb[i] + (int64_t)(STEPS * c + h) * kstep, g.ldb, left);
       }
     }
     if constexpr (MX) {
 #pragma unroll
       for (int a = 0; a < MF; ++a) v.sa[a] = *reinterpret_cast<const int*>(qa[a] + (int64_t)c * (QUANT ? 16 : kChunk));
 #pragma unroll
-      for (int b = 0; b < NF; ++b) v.sb[b] = *reinterpret_cast<const int*>(qb[b] + (int64_t)c * kChunk);
+      for (int b = 0; b < NB; ++b) v.sb[b] = *reinterpret_cast<const int*>(qb[b] + (int64_t)c * kChunk);
     }
   };
   auto multiply = [&](const Chunk& v) __attribute__((always_inline)) {
     each<STEPS>([&](auto hc) __attribute__((always_inline)) {
       constexpr int h = decltype(hc)::value;
 #pragma unroll
-      for (int b = 0; b < NF; ++b) {
+      for (int b = 0; b < NB; ++b) {
         i32x4 fb;
         if constexpr (BKC)
           fb = v.b[b][h];
         else
-          fb = v.c[h].operand(b);
+          fb = v.c[b / NF][h].operand(b % NF);
 #pragma unroll
         for (int a = 0; a < MF; ++a) {
           if constexpr (MX) {
@@ -268,7 +292,7 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
 #pragma unroll
         for (int a = 0; a < MF; ++a)
 #pragma unroll
-          for (int b = 0; b < NF; ++b) {
+          for (int b = 0; b < NB; ++b) {
             sum[a][b] += acc[a][b];
             acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
           }
@@ -283,32 +307,38 @@ __global__ __launch_bounds__(512) void rows_kernel(GroupedArgs g, MxScales x) {
 #pragma unroll
   for (int a = 0; a < MF; ++a)
 #pragma unroll
-    for (int b = 0; b < NF; ++b) {
+    for (int b = 0; b < NB; ++b) {
       if constexpr (FOLD) acc[a][b] += sum[a][b];
       if constexpr (BKC) {
-        part[wave][(16 * a + li) * (BW / 4) + 4 * b + lg] = acc[a][b];
+        part[b / NF][wave][(16 * a + li) * (BW / 4) + 4 * (b % NF) + lg] = acc[a][b];
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          reinterpret_cast<float*>(&part[wave][(16 * a + li) * (BW / 4) + 4 * lg + r])[b] = acc[a][b][r];
+          reinterpret_cast<float*>(&part[b / NF][wave][(16 * a + li) * (BW / 4) + 4 * lg + r])[b % NF] = acc[a][b][r];
       }
     }
   __syncthreads();
   constexpr int PER = BM * BW / 4;
+  using O = std::conditional_t<MX, __bf16, T>;
   for (int i = threadIdx.x; i < 8 / KS * PER; i += 512) {
     const int q = i / PER, e = i % PER;
-    f32x4 v = part[q * KS][e];
+    f32x4 v = part[0][q * KS][e];
 #pragma unroll
-    for (int p = 1; p < KS; ++p) v += part[q * KS + p][e];
+    for (int p = 1; p < KS; ++p) v += part[0][q * KS + p][e];
     const int m = s.row + e / (BW / 4), n = s.tn * BN + q * BW + 4 * (e % (BW / 4));
     if (m >= s.end) continue;
-    if (g.out32)
+    if constexpr (GATED) {
+      f32x4 w = part[1][q * KS][e];
+#pragma unroll
+      for (int p = 1; p < KS; ++p) w += part[1][q * KS + p][e];
+      store_gated_quad<O>(g, m, n, v, w);
+    } else if (g.out32) {
       store_quad<float>(g, static_cast<const float*>(g.C), static_cast<float*>(g.D), m, n, v);
-    else if (MX && g.out_f16)
+    } else if (MX && g.out_f16) {
       store_quad<_Float16>(g, static_cast<const _Float16*>(g.C), static_cast<_Float16*>(g.D), m, n, v);
-    else
-      store_quad<std::conditional_t<MX, __bf16, T>>(g, static_cast<const std::conditional_t<MX, __bf16, T>*>(g.C),
-                                                    static_cast<std::conditional_t<MX, __bf16, T>*>(g.D), m, n, v);
+    } else {
+      store_quad<O>(g, static_cast<const O*>(g.C), static_cast<O*>(g.D), m, n, v);
+    }
   }
 }
 

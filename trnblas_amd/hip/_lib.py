@@ -187,6 +187,12 @@ SIGNATURES = {
         _c_int,
         [_c_int, _c_int, _c_int] + [_c_i64] * 4 + [ctypes.POINTER(ctypes.c_int32)],
     ),
+    "trnblas_hip_gated_gemm": (
+        _c_int,
+        [_c_int] * 3 + [_c_i64] * 4 + [_c_ptr, _c_i64] + [_c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int]
+        + [_c_ptr, _c_i64] * 2 + [_c_int, _c_ptr],
+    ),
+    "trnblas_hip_gated_plan": (ctypes.c_char_p, [_c_int, _c_int] + [_c_i64] * 4),
     "trnblas_hip_gate": (
         _c_int,
         [_c_int, _c_int, _c_int, _c_i64, _c_i64] + [_c_ptr, _c_i64] * 3 + [_c_ptr],
