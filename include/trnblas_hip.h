@@ -672,6 +672,53 @@ int trnblas_hip_grouped_rows_plan(int op, int dtype, int transB, int64_t groups,
                                   int64_t N, int64_t K, int32_t plan[3]);
 
 /*
+ * 4-bit integer weights with scales of groups along K. No counterpart in the reference.
+ *
+ * A weight is (q - z) s, q of 4 bits; a scale s (scale_dtype: TRNBLAS_BF16 or TRNBLAS_F16) and a
+ * zero point z (a byte; 8 where zeros is NULL) serve `group` (32, 64 or 128) values along K of a row.
+ * A matrix of R rows by K is two or three buffers, 16-byte aligned, a stack of them back to back:
+ *  - codes: 1 KiB per 16 rows x 128 values, ceil(K / 128) of them along K, then the next 16
+ *    rows. The 16 bytes at 16 (16 p + r), p = 0 .. 3, are of row r; dword h of these holds the values
+ *    k = 32 h + 8 p + e, e = 0 .. 7: nibble e / 2 (e even) or 4 + e / 2 (odd) is q - 8 as a signed
+ *    number. Nibbles outside the matrix are zero.
+ *  - scales and zeros: per 16 rows, for each of ceil(K / 128) * 128 / group groups along K the rows' 16.
+ *    Those outside the matrix are zero.
+ *
+ * int4_quantize: s = max|x| / 7, q = 8 + x / s; with zeros s = (hi - lo) / 15, z = -lo / s, q = z + x / s,
+ * where lo and hi are the least and largest value and zero. Scales are rounded to fp32, then to
+ * their type, quotients by them to fp32, then to the nearest whole number (even at ties), within 4 bits. A
+ * scale of zero gives zeros; one that is not finite (a NaN, an infinity or a range past the scale's
+ * type) makes its group NaN. X as in trnblas_hip_mx_quantize.
+ */
+int trnblas_hip_int4_quantize(int dtype, int scale_dtype, int64_t R, int64_t K, int64_t group,
+                              const void* X, int64_t sr, int64_t sk, int64_t sx, void* codes,
+                              void* scales, void* zeros, int64_t batch, void* stream);
+
+/* The weights of such a matrix, in D's type `dtype` (rounded to nearest even). */
+int trnblas_hip_int4_dequantize(int dtype, int scale_dtype, int64_t R, int64_t K, int64_t group,
+                                const void* codes, const void* scales, const void* zeros, void* D,
+                                int64_t ldd, int64_t strideD, int64_t batch, void* stream);
+
+/*
+ * D[r] = alpha A[r] W[g]^T + beta C[r] for the rows r of group g (D[r] = beta C[r] for rows of no
+ * group), W groups matrices of N rows by K; gated != 0: H[r] = act(A[r] G^T) * (A[r] U^T) for matrices of 2
+ * N rows, gates first (alpha 1, beta 0). A is rows x K values of `dtype` (fp32, bf16 or fp16), element
+ * (r, k) at r * sr + k * sk; C and D (rows x N) have the type out_dtype. Weights enter as they
+ * are: products of q - z and A are exact, their fp32 sums over a group enter the fp32 sum
+ * times the scale. offsets as in trnblas_hip_grouped_gemm. workspace: as many bytes as int4_gemm_workspace says,
+ * 16-byte aligned, not shared by calls that can overlap; bf16 and fp16 rows that start
+ * on 16 bytes (K a multiple of 8, sk 1) do not use it.
+ */
+size_t trnblas_hip_int4_gemm_workspace(int dtype, int64_t rows, int64_t K);
+int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int act, int64_t groups,
+                          int64_t rows, int64_t N, int64_t K, int64_t group, double alpha,
+                          const void* A, int64_t sr, int64_t sk, const void* codes,
+                          const void* scales, const void* zeros, int scale_dtype,
+                          const void* offsets, int offsets64, double beta, const void* C,
+                          int64_t ldc, void* D, int64_t ldd, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
  * Gated projections: H = act(A G) * (A U), the second product elementwise, for weights
  * [G | U] of 2 N columns. No counterpart in the reference. act: TRNBLAS_ACT_*. Computed in
  * fp32, one rounding of each result. Matrices are row-major.

@@ -16,6 +16,7 @@ from . import ozaki  # noqa: F401
 from .gated import gated_gemm, grouped_gated_gemm
 from .grouped import grouped_gemm, grouped_rank_k
 from .hip import get_autotune, get_backend, get_cores, set_autotune, set_backend, set_cores
+from .int4 import Int4Matrix, int4_dequantize, int4_gemm, int4_grouped_gemm, int4_quantize
 from .level3 import batched_gemm, gemm, gemm_fp64, metric_inv_half, syrk, trsm
 from .mx import MXMatrix, mx_dequantize, mx_gemm, mx_grouped_gemm, mx_quantize
 
@@ -39,6 +40,11 @@ __all__ = [
     "grouped_rank_k",
     "gated_gemm",
     "grouped_gated_gemm",
+    "Int4Matrix",
+    "int4_quantize",
+    "int4_dequantize",
+    "int4_gemm",
+    "int4_grouped_gemm",
     "MXMatrix",
     "mx_quantize",
     "mx_dequantize",

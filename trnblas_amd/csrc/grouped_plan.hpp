@@ -145,6 +145,18 @@ inline GroupedChoice choose_gated(int elem_bytes, double rows, double groups, do
   return c;
 }
 
+// int4_gemm: row blocks of a tile and waves along K of the few-rows kernel.
+struct Int4Choice {
+  int mf, ks;
+};
+inline Int4Choice choose_int4(double rows, double groups, double N, double K, int pieces) {
+  const double g = std::max(1.0, std::min(groups, rows));
+  Int4Choice c{rows <= 16.0 * g ? 1 : rows <= 32.0 * g || pieces == 3 ? 2 : 4, 8};
+  const double tiles = likely_row_tiles(rows, groups, 16 * c.mf);
+  while (c.ks > 1 && tiles * std::ceil(N * (c.ks / 2) / 128.0) >= 2.0 * device_cus()) c.ks /= 2;
+  return c;
+}
+
 // grouped_rank_k of aligned operands: groups x (M x N), over the average group's k-tiles. fp32 has
 // the 64 x 128 tiles alone: three workgroups per CU hide its longer MFMAs' steps.
 inline int choose_rank_k(int elem_bytes, double groups, double rows, double M, double N) {

@@ -9,6 +9,7 @@ operands as in `gemm` and `grouped_gemm`. Activations: "silu", "gelu" (by erf),
 
     H = gated_gemm(x, W, "silu", transB=True)           # x (R, K), W (2 N, K): gate rows, then up rows
     H = grouped_gated_gemm(x, E, offsets)               # rows sorted by expert, E (G, K, 2 N)
+    H = gated_gemm(x, int4_quantize(W))                 # served from 4-bit weights
 
 Differentiable: where a gradient is asked for, the forward pass keeps P = [A G | A U] in
 the result's type, the backward pass forms
@@ -28,6 +29,8 @@ from torch.autograd import forward_ad as _fwd
 from ._flags import trans_flag
 from .grouped import _check_offsets, _check_operands, _check_result, _gemm, _GroupedGemm, _narrowed, _rank_k, _widened
 from .hip import dispatch as _d
+from .int4 import Int4Matrix
+from .int4 import _product as _int4_product
 
 __all__ = ["gated_gemm", "grouped_gated_gemm"]
 
@@ -142,9 +145,15 @@ def _gated(what, A, b, offsets, activation, dtype):
     return _forward(A, b, offsets, act, out, False)[0]
 
 
+def _int4_gated(what, A, B, offsets, activation, transB, dtype, grouped):
+    act = _check_activation(what, activation)
+    trans_flag(transB, "transB")
+    return _int4_product(what, 1.0, A, B, offsets, 0.0, None, dtype, (act, lambda P: _gate_torch(P, act)), grouped)
+
+
 def gated_gemm(
     A: torch.Tensor,
-    B: torch.Tensor,
+    B: torch.Tensor | Int4Matrix,
     activation: str = "silu",
     transB: bool = False,
     dtype: torch.dtype | None = None,
@@ -152,8 +161,11 @@ def gated_gemm(
     """act(A @ G) * (A @ U) for op(B) = [G | U].
 
     A (R, K), B (K, 2 N), or (2 N, K) with transB: gate rows first. The result (R, N)
-    has the operands' dtype, or `dtype` float32.
+    has the operands' dtype, or `dtype` float32. B may be an Int4Matrix (2 N, K) (`transB` then says nothing
+    new): rows of any float type, results in any, no gradient.
     """
+    if isinstance(B, Int4Matrix):
+        return _int4_gated("gated_gemm", A, B, None, activation, transB, dtype, False)
     _check_operands("gated_gemm", A, B, (2, 2))
     b = B.mT if trans_flag(transB, "transB") else B
     return _gated("gated_gemm", A, b[None], None, activation, dtype)
@@ -161,7 +173,7 @@ def gated_gemm(
 
 def grouped_gated_gemm(
     A: torch.Tensor,
-    B: torch.Tensor,
+    B: torch.Tensor | Int4Matrix,
     offsets: torch.Tensor,
     activation: str = "silu",
     transB: bool = False,
@@ -169,7 +181,9 @@ def grouped_gated_gemm(
 ) -> torch.Tensor:
     """H[r] = act(A[r] @ G[g]) * (A[r] @ U[g]) for the rows r of group g, op(B[g]) = [G[g] | U[g]]:
     `grouped_gemm` with `gated_gemm`'s products, B (groups, K, 2 N), or (groups, 2 N, K) with transB.
-    Rows of no group come out as zeros (sigmoid: too)."""
+    Rows of no group come out as zeros. B may be an Int4Matrix (groups, 2 N, K) as in `gated_gemm`."""
+    if isinstance(B, Int4Matrix):
+        return _int4_gated("grouped_gated_gemm", A, B, offsets, activation, transB, dtype, True)
     _check_operands("grouped_gated_gemm", A, B, (2, 3))
     b = B.mT if trans_flag(transB, "transB") else B
     _check_offsets("grouped_gated_gemm", offsets, A, b.shape[0])
