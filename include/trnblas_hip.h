@@ -681,8 +681,8 @@ int trnblas_hip_grouped_rows_plan(int op, int dtype, int transB, int64_t groups,
  *    rows. The 16 bytes at 16 (16 p + r), p = 0 .. 3, are of row r; dword h of these holds the values
  *    k = 32 h + 8 p + e, e = 0 .. 7: nibble e / 2 (e even) or 4 + e / 2 (odd) is q - 8 as a signed
  *    number. Nibbles outside the matrix are zero.
- *  - scales and zeros: per 16 rows, for each of ceil(K / 128) * 128 / group groups along K the rows' 16.
- *    Those outside the matrix are zero.
+ *  - scales and zeros: per 16 rows x 128 values (in the order of the codes) the rows' 128 / group one
+ *    after the other. Those outside the matrix are zero.
  *
  * int4_quantize: s = max|x| / 7, q = 8 + x / s; with zeros s = (hi - lo) / 15, z = -lo / s, q = z + x / s,
  * where lo and hi are the least and largest value and zero. Scales are rounded to fp32, then to

@@ -45,21 +45,35 @@ __device__ __forceinline__ Int4Group int4_group(float lo, float hi, uint32_t top
   return q;
 }
 
-// q - 8 as a nibble.
-__device__ __forceinline__ uint32_t int4_code(float x, const Int4Group& q, bool zeros) {
-  float v;
-  if (q.s > 0.0f)
-    v = zeros ? fminf(fmaxf(rintf(x / q.s) + q.z, 0.0f), 15.0f) - 8.0f : fminf(fmaxf(rintf(x / q.s), -8.0f), 7.0f);
-  else
-    v = q.z - 8.0f;
-  return (uint32_t)(int)v & 15u;
+// round(x / s) by the reciprocal of s, as a float: |x / s| < 23 (15 times a scale of few bits, rounded down), so
+// that the product is within 2^-18 of the quotient, and only where it lies within 2^-16 of halfway between two whole numbers may the two round apart (or
+// the quotient's own rounding to fp32 decide): `close` says that.
+__device__ __forceinline__ float int4_near(float x, float inverse, bool& close) {
+  const float y = x * inverse, v = rintf(y);
+  close |= __builtin_fabsf(y - v) > 0.5f - 0x1p-16f;
+  return v;
 }
 
-// The first `left` of eight values, zeros behind them.
-__device__ __forceinline__ uint32_t int4_dword(const float (&x)[8], const Int4Group& q, bool zeros, int left) {
+// The first `left` of eight values as nibbles q - 8, zeros behind them. (A division for each value: 8192 x 8192 bf16 took
+// 61 us.)
+__device__ __forceinline__ uint32_t int4_dword(const float (&x)[8], const Int4Group& q, int left) {
+  float v[8];
+  // a scale at the ends of the range has no reciprocal that is near enough
+  bool close = q.s < 0x1p-120f || q.s > 0x1p120f;
+  const float inverse = __builtin_amdgcn_rcpf(q.s);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = int4_near(x[e], inverse, close);
+  if (close) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = q.s > 0.0f ? rintf(x[e] / q.s) : 0.0f;
+  }
+  const float lo = -q.z, hi = 15.0f - q.z;
   uint32_t w = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w |= (e < left ? int4_code(x[e], q, zeros) : 0u) << 4 * (e / 2 + 4 * (e & 1));
+  for (int e = 0; e < 8; ++e) {
+    const int c = (int)(fminf(fmaxf(v[e], lo), hi) + (q.z - 8.0f));
+    w |= ((uint32_t)c & (e < left ? 15u : 0u)) << 4 * (e / 2 + 4 * (e & 1));
+  }
   return w;
 }
 
@@ -119,10 +133,9 @@ __global__ __launch_bounds__(256) void int4_quantize_kernel(Int4QuantArgs g) {
       top[h] = max(top[h], (uint32_t)__shfl_xor((int)top[h], d));
     }
     const Int4Group q = int4_group(lo[h], hi[h], top[h], zeros, g.scale_f16);
-    w[h] = (int)int4_dword(v[h], q, zeros, row < g.R ? g.K - (128 * chunk + 32 * h + 8 * p) : 0);
+    w[h] = (int)int4_dword(v[h], q, row < g.R ? g.K - (128 * chunk + 32 * h + 8 * p) : 0);
     if (p == 0 && (h & (g.steps - 1)) == 0) {
-      const int64_t groups = (int64_t)g.chunks * (4 / g.steps);
-      const int64_t at = ((blockIdx.y * (int64_t)blocks + block) * groups + (int64_t)chunk * (4 / g.steps) + h / g.steps) * 16 + r;
+      const int64_t at = (((blockIdx.y * (int64_t)blocks + block) * g.chunks + chunk) * 16 + r) * (4 / g.steps) + h / g.steps;
       const bool inside = row < g.R && 128 * chunk + 32 * h < g.K;
       g.scales[at] = inside ? q.bits : 0;
       if (zeros) g.zeros[at] = inside ? (uint8_t)q.z : 0;
@@ -154,8 +167,7 @@ __global__ __launch_bounds__(256) void int4_dequantize_kernel(Int4DequantArgs g)
   T* D = static_cast<T*>(g.D) + blockIdx.y * g.sD + row * g.ldd;
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
-    const int64_t groups = (int64_t)g.chunks * (4 / g.steps);
-    const int64_t at = ((blockIdx.y * (int64_t)blocks + block) * groups + (int64_t)chunk * (4 / g.steps) + h / g.steps) * 16 + r;
+    const int64_t at = (((blockIdx.y * (int64_t)blocks + block) * g.chunks + chunk) * 16 + r) * (4 / g.steps) + h / g.steps;
     const float s = int4_scale(g.scales[at], g.scale_f16), z = g.zeros ? (float)g.zeros[at] : 8.0f;
     const int k = 128 * chunk + 32 * h + 8 * p, left = row < g.R ? g.K - k : 0;
     union {
@@ -304,6 +316,8 @@ extern "C" int trnblas_hip_int4_dequantize(int dtype, int scale_dtype, int64_t R
   return check_launch(kDequantize);
 }
 
+constexpr int64_t kInt4Far = (int64_t)1 << 22;  // elements between rows that are read in place
+
 static int64_t up128(int64_t k) { return (k + 127) / 128 * 128; }
 
 extern "C" size_t trnblas_hip_int4_gemm_workspace(int dtype, int64_t rows, int64_t K) {
@@ -322,8 +336,11 @@ extern "C" int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int ac
   TRNBLAS_CHECK_ARG(!gated || (act >= TRNBLAS_ACT_SILU && act <= TRNBLAS_ACT_SIGMOID && alpha == 1.0 && beta == 0.0),
                     "%s: bad activation %d (and alpha 1, beta 0 with one)", kGemm, act);
   if (int rc = check_int4(kGemm, N, K, group, scale_dtype, 0)) return rc;
-  TRNBLAS_CHECK_ARG(groups >= 0 && groups < (1 << 24) && rows >= 0 && rows < INT32_MAX - 1024 && N < (INT32_MAX >> 1) - 1024,
-                    "%s: bad sizes (groups %lld, rows %lld, N %lld)", kGemm, (long long)groups, (long long)rows, (long long)N);
+  // K: two row blocks' codes lie within 32-bit offsets
+  TRNBLAS_CHECK_ARG(groups >= 0 && groups < (1 << 24) && rows >= 0 && rows < INT32_MAX - 1024 && N < (INT32_MAX >> 1) - 1024 &&
+                        K < 1 << 24,
+                    "%s: bad sizes (groups %lld, rows %lld, N %lld, K %lld)", kGemm, (long long)groups, (long long)rows, (long long)N,
+                    (long long)K);
   TRNBLAS_CHECK_ARG(offsets != nullptr ? (uintptr_t)offsets % (offsets64 ? 8 : 4) == 0 : groups == 1,
                     "%s: offsets missing or misaligned", kGemm);
   TRNBLAS_CHECK_ARG(beta == 0.0 || C != nullptr, "%s: beta != 0 without C", kGemm);
@@ -338,7 +355,8 @@ extern "C" int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int ac
   Int4Args q{};
   g.A = A, g.lda = sr;
   g.K = (int)K;
-  if (sums && (dtype == TRNBLAS_F32 || sk != 1 || K % 8 != 0 || (uintptr_t)A % 16 != 0 || (sr % 8 != 0 && rows > 1))) {
+  // (rows far apart: a tile's lie within 32-bit offsets)
+  if (sums && (dtype == TRNBLAS_F32 || sk != 1 || K % 8 != 0 || (uintptr_t)A % 16 != 0 || (rows > 1 && (sr % 8 != 0 || sr > kInt4Far)))) {
     const size_t need = trnblas_hip_int4_gemm_workspace(dtype, rows, K);
     if (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0) {
       set_error("%s: workspace of %zu bytes, 16-byte aligned, needed (got %zu)", kGemm, need, workspace_bytes);

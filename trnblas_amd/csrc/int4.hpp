@@ -7,8 +7,8 @@
 //    16 (16 p + r), p = 0 .. 3, are of row r; dword h of them holds k = 32 h + 8 p + e, e = 0 .. 7: what lane 16
 //    p + r of a 16 x 16 x 32 matrix instruction takes in step h. Nibble e / 2 of it (e even) or 4 + e / 2
 //    (odd) is q - 8 as a signed number. Values outside the matrix are zero.
-//  * scales, zero points: per 16 rows, for each group along K (of whole chunks) the rows' 16. Those
-//    outside the matrix are zero.
+//  * scales, zero points: per 16 rows x 128 values the rows' one after the other, 4, 2 or 1 each, so that a
+//    lane loads those of its row and chunk at once. Those outside the matrix are zero.
 #pragma once
 
 #include "gate.hpp"
@@ -32,6 +32,11 @@ struct Int4Args {
 
 constexpr int kInt4Chunk = 1024;  // bytes of codes
 
+// A buffer at a (uniform) address; reads at or past kRecords bytes from it give zeros with no memory access.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(uniform(static_cast<const char*>(p))), 0, kRecords, 0x00020000);
+}
+
 __device__ __forceinline__ float int4_scale(uint16_t bits, int f16) {
   return f16 ? (float)__builtin_bit_cast(_Float16, bits) : __builtin_bit_cast(float, (uint32_t)bits << 16);
 }
@@ -49,13 +54,25 @@ __device__ __forceinline__ i32x4 int4_values(uint32_t w, uint32_t zc) {
       v[i] = __builtin_bit_cast(
           int, __builtin_bit_cast(f16x2, ((w >> 4 * i) & 0x000f000fu) ^ 0x64086408u) + __builtin_bit_cast(f16x2, zc));
   } else {
-    auto value = [&](int byte, int high) __attribute__((always_inline)) {
-      float f = __builtin_amdgcn_cvt_off_f32_i4((int)((high ? w >> 4 : w) >> 8 * byte));
-      if constexpr (ZERO) f += __builtin_bit_cast(float, zc);
-      return __builtin_bit_cast(uint32_t, f);
-    };
+    // by asm: the compiler shifts bytes down that the instruction can pick, and waits between each conversion
+    // and what takes it (17 instructions and 8 waits for eight values; 13)
+    float f[8];
+    asm("v_lshrrev_b32 %8, 4, %9\n\t"
+        "v_cvt_off_f32_i4 %0, %9\n\t"
+        "v_cvt_off_f32_i4_sdwa %1, %9 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+        "v_cvt_off_f32_i4_sdwa %4, %9 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
+        "v_cvt_off_f32_i4_sdwa %5, %9 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3\n\t"
+        "v_cvt_off_f32_i4 %2, %8\n\t"
+        "v_cvt_off_f32_i4_sdwa %3, %8 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+        "v_cvt_off_f32_i4_sdwa %6, %8 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
+        "v_cvt_off_f32_i4_sdwa %7, %8 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3"
+        : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7]), "=&v"(v[0])
+        : "v"(w));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (int)__builtin_amdgcn_perm(value(2 + i / 2, i & 1), value(i / 2, i & 1), 0x07060302u);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (ZERO) f[2 * i] += __builtin_bit_cast(float, zc), f[2 * i + 1] += __builtin_bit_cast(float, zc);
+      v[i] = (int)__builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f[2 * i + 1]), __builtin_bit_cast(uint32_t, f[2 * i]), 0x07060302u);
+    }
   }
   return v;
 }

@@ -27,7 +27,7 @@ import torch
 from torch.autograd import forward_ad as _fwd
 
 from ._flags import trans_flag
-from .grouped import _check_offsets, _check_operands, _check_result, _gemm, _GroupedGemm, _narrowed, _rank_k, _widened
+from .grouped import _check_offsets, _check_operands, _check_result, _fast_call, _gemm, _GroupedGemm, _narrowed, _rank_k, _widened
 from .hip import dispatch as _d
 from .int4 import Int4Matrix
 from .int4 import _product as _int4_product
@@ -77,6 +77,11 @@ def _forward(A, b, offsets, act, out, save):
     """(H, P in H's type where `save` says so)."""
     if _d._grouped_on_hip("gated_gemm", A, b):
         try:
+            if save:
+                kc = b.stride(2) != 1 and b.stride(1) == 1
+                HP = _gk().gated_gemm_fast(A, b.mT if kc else b, offsets, act, kc, out, True)
+                if HP is not None:
+                    return HP
             return _gk().gated_gemm(A, b, offsets, act, out, save)
         except Exception as exc:  # noqa: BLE001
             _d._kernel_failed(exc)
@@ -130,6 +135,16 @@ class _GatedGemm(torch.autograd.Function):
         return dA, dB, None, None, None
 
 
+def _fast(A, B, offsets, activation, transB, dtype):
+    """The short way; None: something is out of the ordinary."""
+    if type(activation) is str and type(transB) is bool and _fast_call(A, B, offsets, True):
+        try:
+            return _gk().gated_gemm_fast(A, B, offsets, activation, transB, dtype)
+        except _d.HipKernelError as exc:
+            _d._kernel_failed(exc)
+    return None
+
+
 def _gated(what, A, b, offsets, activation, dtype):
     """b: op(B) (G, K, 2 N)."""
     act = _check_activation(what, activation)
@@ -166,6 +181,9 @@ def gated_gemm(
     """
     if isinstance(B, Int4Matrix):
         return _int4_gated("gated_gemm", A, B, None, activation, transB, dtype, False)
+    H = _fast(A, B, None, activation, transB, dtype)
+    if H is not None:
+        return H
     _check_operands("gated_gemm", A, B, (2, 2))
     b = B.mT if trans_flag(transB, "transB") else B
     return _gated("gated_gemm", A, b[None], None, activation, dtype)
@@ -184,6 +202,10 @@ def grouped_gated_gemm(
     Rows of no group come out as zeros. B may be an Int4Matrix (groups, 2 N, K) as in `gated_gemm`."""
     if isinstance(B, Int4Matrix):
         return _int4_gated("grouped_gated_gemm", A, B, offsets, activation, transB, dtype, True)
+    if isinstance(offsets, torch.Tensor):
+        H = _fast(A, B, offsets, activation, transB, dtype)
+        if H is not None:
+            return H
     _check_operands("grouped_gated_gemm", A, B, (2, 3))
     b = B.mT if trans_flag(transB, "transB") else B
     _check_offsets("grouped_gated_gemm", offsets, A, b.shape[0])

@@ -43,12 +43,12 @@ def _gk():
     return _kernels
 
 
-def _fast_call(A, B, offsets) -> bool:
-    """Tensors on the GPU, no gradient, and the kernels serve: the call may take the short way."""
+def _fast_call(A, B, offsets, none=False) -> bool:
+    """Tensors on the GPU, no gradient, and the kernels serve: the call may take the short way. none: so it may without offsets."""
     return (
         type(A) in _PLAIN
         and type(B) in _PLAIN
-        and type(offsets) is torch.Tensor
+        and (type(offsets) is torch.Tensor or (none and offsets is None))
         and A.is_cuda
         and not ((A.requires_grad or B.requires_grad) and torch.is_grad_enabled())
         and _fwd._current_level < 0

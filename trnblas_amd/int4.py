@@ -19,6 +19,7 @@ forward-mode tangent.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad as _fwd
 
 from ._flags import trans_flag
 from .grouped import _check_offsets, _check_result
@@ -53,7 +54,7 @@ class Int4Matrix:
     """A matrix (R, K), or a stack (G, R, K), of 4-bit integer weights.
 
     codes: uint8 (..., ceil(R / 16), ceil(K / 128), 1024); scales: bfloat16 or float16 (..., ceil(R / 16),
-    groups, 16), groups = ceil(K / 128) * 128 / group; zeros: uint8 like the scales, or None: in the order the
+    ceil(K / 128), 16, 128 / group); zeros: uint8 like the scales, or None: in the order the
     matrix instructions take them (include/trnblas_hip.h). `from_parts` and `parts` go from and to plain rows.
     """
 
@@ -66,7 +67,7 @@ class Int4Matrix:
         _check_group("Int4Matrix", group)
         *lead, R, K = shape
         blocks, chunks = -(-R // 16), -(-K // 128)
-        of_groups = (*lead, blocks, chunks * (128 // group), 16)
+        of_groups = (*lead, blocks, chunks, 16, 128 // group)
         for name, t, want, types in (("codes", codes, (*lead, blocks, chunks, 1024), (torch.uint8,)),
                                      ("scales", scales, of_groups, _SCALES), ("zeros", zeros, of_groups, (torch.uint8,))):  # fmt: skip
             if t is None and name == "zeros":
@@ -118,7 +119,7 @@ class Int4Matrix:
 
     def _rows(self, t):
         """Scales or zero points as rows (..., R, ceil(K / group))."""
-        return t.mT.flatten(-3, -2)[..., : self.shape[-2], : -(-self.shape[-1] // self.group)]
+        return t.transpose(-3, -2).flatten(-2).flatten(-3, -2)[..., : self.shape[-2], : -(-self.shape[-1] // self.group)]
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         return int4_dequantize(self, dtype)
@@ -169,7 +170,7 @@ def _blocked(t: torch.Tensor, K: int, group: int) -> torch.Tensor:
     """Scales or zero points (..., R, ceil(K / group)) as an Int4Matrix's."""
     *lead, R, n = t.shape
     t = torch.nn.functional.pad(t, (0, -(-K // 128) * (128 // group) - n, 0, -R % 16))
-    return t.reshape(*lead, -(-R // 16), 16, t.shape[-1]).mT.contiguous()
+    return t.reshape(*lead, -(-R // 16), 16, -(-K // 128), 128 // group).transpose(-3, -2).contiguous()
 
 
 def _quantize_torch(X, group, zeros, scale_dtype) -> Int4Matrix:
@@ -229,7 +230,8 @@ def int4_quantize(
     _check_group("int4_quantize", group)
     if scale_dtype not in _SCALES:
         raise TypeError(f"int4_quantize: scale_dtype {scale_dtype} (bfloat16 or float16)")
-    X = X.detach()
+    if X.requires_grad:
+        X = X.detach()
     if X.dtype not in _FLOATS:
         X = X.float()
     if trans_flag(trans):
@@ -237,7 +239,8 @@ def int4_quantize(
     zeros = bool(zeros)
     if _d.mx_on_hip(X):
         try:
-            return Int4Matrix._of(_gk().quantize(X, group, zeros, scale_dtype), X.shape, group)
+            parts = _gk().quantize_fast(X, group, zeros, scale_dtype)
+            return Int4Matrix._of(parts or _gk().quantize(X, group, zeros, scale_dtype), X.shape, group)
         except Exception as exc:  # noqa: BLE001
             _d._kernel_failed(exc)
     return _quantize_torch(X, group, zeros, scale_dtype)
@@ -251,15 +254,35 @@ def int4_dequantize(Q: Int4Matrix, dtype: torch.dtype = torch.float32) -> torch.
         raise TypeError(f"int4_dequantize: dtype {dtype} (float32, bfloat16 or float16)")
     if _d.mx_on_hip(Q.codes):
         try:
-            return _gk().dequantize((Q.codes, Q.scales, Q.zeros), Q.shape, Q.group, dtype)
+            q = Q.codes, Q.scales, Q.zeros
+            D = _gk().dequantize_fast(q, Q.shape, Q.group, dtype)
+            return _gk().dequantize(q, Q.shape, Q.group, dtype) if D is None else D
         except Exception as exc:  # noqa: BLE001
             _d._kernel_failed(exc)
     return _dequantize_torch(Q, dtype)
 
 
+def _fast_product(alpha, A, B, offsets, dtype, dims, act=None):
+    """The short way (`int4_gemm_fast`); None: something is out of the ordinary."""
+    if (
+        type(A) is torch.Tensor and A.is_cuda and type(B) is Int4Matrix and len(B.shape) == dims
+        and (offsets is None if dims == 2 else type(offsets) is torch.Tensor)
+        and not (A.requires_grad and torch.is_grad_enabled()) and _fwd._current_level < 0 and _d._use_hip()
+    ):  # fmt: skip
+        try:
+            return _gk().int4_gemm_fast(alpha, A, B, offsets, dtype, act)
+        except _d.HipKernelError as exc:
+            _d._kernel_failed(exc)
+    return None
+
+
 def _product(what: str, alpha, A, B, offsets, beta, C, dtype, gate=None, grouped=False) -> torch.Tensor:
     """gate: None, or (activation, its function of [G | U]) for B of 2 N rows."""
     dims = 3 if grouped else 2
+    if beta == 0.0:
+        D = _fast_product(alpha, A, B, offsets, dtype, dims, gate and gate[0])
+        if D is not None:
+            return D
     if not isinstance(B, Int4Matrix) or len(B.shape) != dims:
         raise ValueError(f"{what}: B must be an Int4Matrix of {dims} dimensions (see int4_quantize)")
     if not isinstance(A, torch.Tensor) or A.dim() != 2:
