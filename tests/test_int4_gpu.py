@@ -126,6 +126,31 @@ def test_gated(dev, dtype, act):
         assert oa.ratio(H, *oa.forward(act, P, den, K, dtype)) <= 1, (shape, K, N)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_many_rows(dev, group, dtype):
+    # tiles of 128 rows that end inside, columns that end inside a tile and a block, chunks of 128 values cut short
+    for i, (G, R, K, N) in enumerate([(1, 65, 128, 16), (1, 300, 1160, 400), (1, 513, 72, 1000), (2, 390, 2056, 264), (3, 1200, 515, 333), (1, 129, 4100, 48)]):
+        g = torch.Generator(device=dev).manual_seed(i)
+        off = torch.tensor([0, R]) if G == 1 else og.uneven(G, R, i)
+        A = torch.randn(R, K, generator=g, device=dev).to(dtype)
+        E, W = oi.random_matrix(g, G, N, K, group=group, zeros=bool(i % 2), scale_dtype=(BF16, F16)[i % 2], device=dev)
+        ref, den = torch.zeros(2, R, N, dtype=torch.float64, device=dev)
+        for j, a, b in og.rows_of(off, R):
+            V = W[j].T.contiguous()
+            ref[a:b], den[a:b] = A[a:b].double() @ V, A[a:b].double().abs() @ V.abs()
+        for out in {dtype, F32}:
+            D = tb.int4_grouped_gemm(1.0, A, E, off.to(dev), dtype=out)
+            assert og.excess(D.cpu(), ref.cpu(), den.cpu(), K) <= 1, (G, R, K, N, out)
+        # the same matrix as gates and ups, where their rows start on a block of sixteen and where they do not
+        if N % 2 == 0:
+            P, d = oa.products(A, W, off, True)
+            act = oa.ACTS[i % 3]
+            for out in {dtype, F32}:
+                H = tb.grouped_gated_gemm(A, E, off.to(dev), act, dtype=out)
+                assert oa.ratio(H, *oa.forward(act, P, d, K, out)) <= 1, (G, R, K, N, out)
+
+
 @pytest.mark.parametrize("out", DTYPES)
 def test_alpha_beta_and_result_type(dev, out):
     rows, sizes, lead = GROUPS["gaps"]

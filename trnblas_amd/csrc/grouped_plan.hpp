@@ -145,14 +145,17 @@ inline GroupedChoice choose_gated(int elem_bytes, double rows, double groups, do
   return c;
 }
 
-// int4_gemm: blocks of 16 rows and of 16 columns of a wave, and waves along K, of the few-rows kernel.
+// int4_gemm: the tile kernel, or blocks of 16 rows and of 16 columns of a wave, and waves along K, of the
+// few-rows kernel.
 struct Int4Choice {
   int mf, nf, ks;
+  bool tile;
 };
 inline Int4Choice choose_int4(double rows, double groups, double N, double K, int pieces, bool gated) {
   const double g = std::max(1.0, std::min(groups, rows));
   Int4Choice c{rows <= 16.0 * g ? 1 : rows <= 32.0 * g || pieces == 3 ? 2 : 4, rows <= 4.0 * g ? 1 : 2, 8};
   if (gated || c.mf > 1) c.nf = 2;
+  c.tile = rows > 64.0 * g && (!gated || std::fmod(N, 16.0) == 0.0);
   const double tiles = likely_row_tiles(rows, groups, 16 * c.mf), columns = gated ? 16 : 16 * c.nf;
   while (c.ks > 1 && tiles * std::ceil(N * (c.ks / 2) / (8.0 * columns)) >= 2.0 * device_cus()) c.ks /= 2;
   return c;

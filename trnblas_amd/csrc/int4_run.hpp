@@ -3,7 +3,7 @@
 
 #include <algorithm>
 
-#include "int4_rows.hpp"
+#include "int4_tile.hpp"
 
 namespace trnblas {
 
@@ -28,9 +28,21 @@ static int run_int4_rows(GroupedArgs g, const Int4Args& q, int ks, hipStream_t s
   return check_launch(kInt4Gemm);
 }
 
+template <typename T, int STEPS, bool GATED>
+static int run_int4_tile(GroupedArgs g, const Int4Args& q, int pieces, hipStream_t s) {
+  constexpr int BN = GATED ? 128 : 256;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  unsigned grid;
+  if (int rc = int4_grid(g, 128, &grid)) return rc;
+  auto kernel = q.zeros ? int4_tile_kernel<T, STEPS, true, GATED> : int4_tile_kernel<T, STEPS, false, GATED>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(512), 0, s, g, q, pieces);
+  return check_launch(kInt4Gemm);
+}
+
 template <typename T, int P, int STEPS, bool GATED>
 static int run_int4(const GroupedArgs& g, const Int4Args& q, hipStream_t s) {
   const Int4Choice c = choose_int4(g.rows, g.groups, g.N, g.K, P, GATED);
+  if (c.tile) return run_int4_tile<T, STEPS, GATED>(g, q, P, s);
   if constexpr (P == 1) {
     if (c.mf == 4) return run_int4_rows<T, P, 4, 2, STEPS, GATED>(g, q, c.ks, s);
   }
