@@ -706,10 +706,12 @@ int trnblas_hip_int4_dequantize(int dtype, int scale_dtype, int64_t R, int64_t K
  * (r, k) at r * sr + k * sk; C and D (rows x N) have the type out_dtype. Weights enter as they
  * are: products of q - z and A are exact, their fp32 sums over a group enter the fp32 sum
  * times the scale. offsets as in trnblas_hip_grouped_gemm. workspace: as many bytes as int4_gemm_workspace says,
- * 16-byte aligned, not shared by calls that can overlap; bf16 and fp16 rows that start
- * on 16 bytes (K a multiple of 8, sk 1) do not use it.
+ * 16-byte aligned, not shared by calls that can overlap (it holds the rows as the kernels read them, but for
+ * bf16 and fp16 rows that start on 16 bytes, no more than 2^22 values apart, K a multiple of 8, sk 1; and the
+ * sums of parts of K, which those need too).
  */
-size_t trnblas_hip_int4_gemm_workspace(int dtype, int64_t rows, int64_t K);
+size_t trnblas_hip_int4_gemm_workspace(int dtype, int gated, int64_t groups, int64_t rows,
+                                       int64_t N, int64_t K);
 int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int act, int64_t groups,
                           int64_t rows, int64_t N, int64_t K, int64_t group, double alpha,
                           const void* A, int64_t sr, int64_t sk, const void* codes,
@@ -717,6 +719,14 @@ int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int act, int64_t 
                           const void* offsets, int offsets64, double beta, const void* C,
                           int64_t ldc, void* D, int64_t ldd, void* workspace,
                           size_t workspace_bytes, void* stream);
+
+/*
+ * How int4_gemm serves such a call: plan[0] rows of a tile (0: the few-rows kernel), plan[1]
+ * parts of K; of the few-rows kernel plan[2] and [3] blocks of 16 rows and columns of a wave, plan[4] waves along K.
+ * Launches nothing and needs no GPU.
+ */
+int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, int64_t N, int64_t K,
+                          int32_t plan[5]);
 
 /*
  * Gated projections: H = act(A G) * (A U), the second product elementwise, for weights

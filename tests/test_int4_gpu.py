@@ -151,6 +151,60 @@ def test_many_rows(dev, group, dtype):
                 assert oa.ratio(H, *oa.forward(act, P, d, K, out)) <= 1, (G, R, K, N, out)
 
 
+def _plan(dtype, gated, groups, rows, N, K):
+    """(rows of a tile, parts of K, blocks of rows, blocks of columns, waves along K)"""
+    import ctypes
+
+    from trnblas_amd.hip import _lib
+
+    out = (ctypes.c_int32 * 5)()
+    _lib.call("trnblas_hip_int4_plan", _lib.DTYPE_CODES[dtype], gated, groups, rows, N, K, out)
+    return tuple(out)
+
+
+# (dtype, gated, groups, rows, N, K) that each form of the kernels serves
+FORMS = {
+    (0, 1, 1, 1, 1): [(BF16, 0, 64, 68, 264, 275), (F32, 0, 2, 2, 9200, 16)],
+    (0, 1, 1, 1, 2): [(F16, 0, 16, 14, 593, 134), (F32, 0, 33, 34, 244, 16)],
+    (0, 1, 1, 1, 4): [(BF16, 0, 1, 1, 4416, 132), (F32, 0, 1, 1, 4606, 16)],
+    (0, 1, 1, 1, 8): [(F16, 0, 1, 1, 16, 140), (F32, 0, 1, 41, 31, 491)],
+    (0, 1, 1, 2, 1): [(F16, 0, 16, 22, 3875, 17), (BF16, 1, 64, 84, 480, 17), (F32, 1, 2, 2, 8688, 16)],
+    (0, 1, 1, 2, 2): [(BF16, 0, 16, 16, 1392, 129), (F16, 1, 64, 52, 160, 134), (F32, 0, 64, 55, 339, 136)],
+    (0, 1, 1, 2, 4): [(F16, 0, 33, 960, 194, 288), (BF16, 1, 8, 7, 592, 148), (F32, 0, 16, 14, 782, 257)],
+    (0, 1, 1, 2, 8): [(BF16, 0, 64, 65, 66, 545), (F16, 1, 8, 9, 128, 857), (F32, 1, 1, 1, 16, 131)],
+    (0, 1, 2, 2, 1): [(BF16, 0, 16, 251, 4203, 17), (F16, 1, 33, 421, 1056, 16), (F32, 0, 8, 124, 9412, 16)],
+    (0, 1, 2, 2, 4): [(F16, 0, 33, 581, 407, 472), (BF16, 1, 1, 64, 3360, 337), (F32, 1, 2, 3334, 48, 474)],
+    (0, 1, 2, 2, 8): [(BF16, 0, 1, 2624, 109, 543), (F16, 1, 4, 99, 848, 1019), (F32, 1, 1, 1136, 96, 733)],
+    (0, 1, 4, 2, 8): [(F16, 0, 1, 575, 671, 889), (BF16, 1, 1, 34, 3824, 795)],
+    (64, 1, 0, 0, 0): [(BF16, 0, 4, 983, 17, 41), (F16, 1, 8, 2516, 16, 16), (F32, 1, 1, 3, 4160, 31)],
+    (64, 2, 0, 0, 0): [(F16, 0, 2, 126, 4501, 2175), (BF16, 1, 16, 687, 336, 1609), (F32, 1, 2, 5427, 96, 990)],
+    (64, 4, 0, 0, 0): [(BF16, 0, 64, 5648, 67, 2995), (F16, 1, 1, 39, 4304, 1565), (F32, 0, 4, 89, 2762, 2092)],
+    (64, 8, 0, 0, 0): [(F16, 0, 1, 2337, 105, 4165), (BF16, 1, 1, 64, 128, 11171), (F32, 0, 1, 2326, 35, 1274)],
+    (128, 1, 0, 0, 0): [(BF16, 0, 8, 335, 7043, 17), (F16, 1, 33, 1713, 768, 17), (BF16, 0, 2, 5000, 2051, 1000), (F32, 0, 8, 1636, 3278, 66)],
+}
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_each_form(dev, form):
+    for i, (dtype, gated, G, R, N, K) in enumerate(FORMS[form]):
+        assert _plan(dtype, gated, G, R, N, K) == form, (dtype, gated, G, R, N, K)
+        g = torch.Generator(device=dev).manual_seed(i)
+        off = og.uneven(G, R, i) if R > 4 * G else torch.arange(G + 1) * (R // G)
+        A = torch.randn(R, K, generator=g, device=dev).to(dtype)
+        for group, zeros in ((128, False), (32, True), (64, False)):
+            E, W = oi.random_matrix(g, G, 2 * N if gated else N, K, group=group, zeros=zeros, scale_dtype=BF16 if zeros else F16, device=dev)
+            if gated:
+                P, d = oa.products(A, W, off, True)
+                H = tb.grouped_gated_gemm(A, E, off.to(dev), "gelu")
+                assert oa.ratio(H, *oa.forward("gelu", P, d, K, dtype)) <= 1, (G, R, N, K, group)
+            else:
+                C = torch.randn(N, generator=g, device=dev).to(dtype)
+                P, d = oa.products(A, W, off, True)
+                D = tb.int4_grouped_gemm(2.0, A, E, off.to(dev), 0.5, C)
+                ref, den = 2.0 * P + 0.5 * C.double(), 2.0 * d + 0.5 * C.double().abs()
+                assert og.excess(D.cpu(), ref.cpu(), den.cpu(), K) <= 1, (G, R, N, K, group)
+
+
 @pytest.mark.parametrize("out", DTYPES)
 def test_alpha_beta_and_result_type(dev, out):
     rows, sizes, lead = GROUPS["gaps"]

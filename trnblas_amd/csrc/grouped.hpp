@@ -416,7 +416,7 @@ __device__ __forceinline__ void store_wave(const GroupedArgs& g, const TileJob& 
     // 16-bit rows that start on 16 bytes: lanes 16 apart exchange halves of two
     // blocks, so that a lane stores 16 bytes and a row 64 at a time (8 and 32: 8192 x
     // 2048 x 8192 237 us, now 223; 8191 x 2056 x 4104 of 4-bit values 88, now 82)
-    if constexpr (sizeof(O) == 2) {
+    if constexpr (sizeof(O) == 2 && FN % 2 == 0) {
       if ((!BETA || g.beta == 0.0f) && (((uint64_t)D / 2 | (uint64_t)g.ldd | (uint64_t)g.N) & 7) == 0) {
         typedef int i32x2 __attribute__((ext_vector_type(2)));
         auto pack = [&](int a, int b) __attribute__((always_inline)) {

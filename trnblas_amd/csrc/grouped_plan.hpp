@@ -145,20 +145,50 @@ inline GroupedChoice choose_gated(int elem_bytes, double rows, double groups, do
   return c;
 }
 
-// int4_gemm: the tile kernel, or blocks of 16 rows and of 16 columns of a wave, and waves along K, of the
-// few-rows kernel.
+// int4_gemm: the tile kernel's rows (0: the few-rows kernel) and parts of K, or blocks of 16 rows and of 16 columns
+// of a wave, and waves along K, of the few-rows kernel.
 struct Int4Choice {
-  int mf, nf, ks;
-  bool tile;
+  int mf, nf, ks, tile, splits;
 };
+
+// Times (us) fitted to sweeps of 1 .. 2048 rows over matrices of 2048 .. 8192 squared, bf16, groups of 128 (others
+// scale all kernels alike; over 70 random sizes the choice took 5.6 % longer than the fastest of 15 forms). The few-rows kernel: 2.6 for each round of a workgroup per CU, and for
+// each chunk of a wave by its blocks of rows and columns; the tile kernel's tiles as in ring_time; parts of K: what
+// writes and reads their sums. 64 rows, 8192 x 8192: few rows 36, tiles of 64 in four parts 28, in one 52, of 128 106;
+// 2048 rows: 1025, 376, 285, 237.
 inline Int4Choice choose_int4(double rows, double groups, double N, double K, int pieces, bool gated) {
-  const double g = std::max(1.0, std::min(groups, rows));
-  Int4Choice c{rows <= 16.0 * g ? 1 : rows <= 32.0 * g || pieces == 3 ? 2 : 4, rows <= 4.0 * g ? 1 : 2, 8};
-  if (gated || c.mf > 1) c.nf = 2;
-  c.tile = rows > 64.0 * g && (!gated || std::fmod(N, 16.0) == 0.0);
-  const double tiles = likely_row_tiles(rows, groups, 16 * c.mf), columns = gated ? 16 : 16 * c.nf;
-  while (c.ks > 1 && tiles * std::ceil(N * (c.ks / 2) / (8.0 * columns)) >= 2.0 * device_cus()) c.ks /= 2;
-  return c;
+  const double cus = device_cus(), chunks = std::ceil(K / 128.0), columns = gated ? 2.0 * N : N, chain = chunks * pieces;
+  // of a block's sixteen rows those that are there: the others are read from the first level's cache
+  const double filled = std::min(1.0, rows / std::max(1.0, std::min(groups, rows)) / 16.0);
+  Int4Choice best{1, 2, 8, 0, 1};
+  double time = 1e30;
+  for (int mf : {1, 2, 4}) {
+    if (mf == 4 && pieces == 3) break;
+    for (int nf : {2, 1}) {
+      if (nf == 1 && (mf > 1 || gated)) continue;
+      const double each = (mf == 1 ? (nf == 1 ? 0.35 + 0.45 * filled : 0.72 + 0.33 * filled) : mf == 2 ? 1.85 : 3.6) * (pieces == 3 ? 2.5 : 1.0);
+      for (int ks : {8, 4, 2, 1}) {
+        const double groups_of = likely_row_tiles(rows, groups, 16 * mf) * std::ceil(columns * ks / (128.0 * nf));
+        const double t = 2.0 + std::max(1.0, groups_of / cus) * (2.6 + std::ceil(chunks / ks) * each);
+        if (t < time) time = t, best = {mf, nf, ks, 0, 1};
+      }
+    }
+  }
+  // (gates and ups: from one to the other within 32-bit offsets of the scales)
+  if (gated && (std::fmod(N, 16.0) != 0.0 || N * K >= 16.0 * INT32_MAX)) return best;
+  for (int tile : {64, 128})
+    for (int splits : {1, 2, 4, 8}) {
+      const double sums = splits * rows * columns * 4.0;
+      if (splits > 1 && (tile == 128 || chain < 2.0 * splits || sums > 256e6)) break;
+      const double slots = tile == 64 ? 2.0 * cus : cus;
+      const double r = likely_row_tiles(rows, groups, tile) * std::ceil(columns / (2.0 * tile)) * splits / slots;
+      const double busy = tile == 64 ? std::min(1.0, std::max(0.0, 2.0 * r - 1.0)) : std::min(1.0, r);
+      const double each = tile == 64 ? 0.75 + 0.43 * busy : 1.58 + 0.3 * busy;
+      const double rounds = r <= 1.0 ? 1.0 : tile == 64 ? r + 0.3 : std::ceil(r);
+      const double t = rounds * (4.2 + std::ceil(chain / splits) * each) + (splits > 1 ? 2.5 + sums / 2.7e6 : 0.0);
+      if (t < time) time = t, best = {1, 2, 8, tile, splits};
+    }
+  return best;
 }
 
 // grouped_rank_k of aligned operands: groups x (M x N), over the average group's k-tiles. fp32 has

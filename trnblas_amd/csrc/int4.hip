@@ -8,7 +8,7 @@ namespace trnblas {
 
 static const char* const kQuantize = "trnblas_hip_int4_quantize";
 static const char* const kDequantize = "trnblas_hip_int4_dequantize";
-static const char* const kGemm = "trnblas_hip_int4_gemm";
+static const char* const kGemm = kInt4Gemm;
 
 struct Int4QuantArgs {
   const void* X;
@@ -235,6 +235,25 @@ __global__ __launch_bounds__(256) void int4_rows_of_kernel(Int4RowsArgs g) {
   }
 }
 
+// The parts' sums of int4_tile_kernel to results, four columns per thread, in the order of the parts.
+template <bool GATED>
+__global__ __launch_bounds__(256) void int4_join_kernel(GroupedArgs g, Int4Args q) {
+  const int quads = (g.N + 3) / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / quads;
+  if (m >= g.rows) return;
+  const int n = 4 * (int)(i - m * quads);
+  const int64_t step = g.rows * q.ldp;
+  const float* p = q.partial + m * q.ldp + n;
+  f32x4 v = *reinterpret_cast<const f32x4*>(p), w = v;
+  if constexpr (GATED) w = *reinterpret_cast<const f32x4*>(p + g.N);
+  for (int part = 1; part < q.splits; ++part) {
+    p += step;
+    v += *reinterpret_cast<const f32x4*>(p);
+    if constexpr (GATED) w += *reinterpret_cast<const f32x4*>(p + g.N);
+  }
+  int4_store<GATED>(g, m, n, v, w);
+}
+
 static int check_int4(const char* what, int64_t R, int64_t K, int64_t group, int scale_dtype, int64_t batch) {
   TRNBLAS_CHECK_ARG(R >= 0 && R < INT32_MAX - 1024 && K >= 0 && K < INT32_MAX - 1024 && batch >= 0 && batch < 65536,
                     "%s: bad sizes (rows %lld, K %lld, batch %lld)", what, (long long)R, (long long)K, (long long)batch);
@@ -320,9 +339,14 @@ constexpr int64_t kInt4Far = (int64_t)1 << 22;  // elements between rows that ar
 
 static int64_t up128(int64_t k) { return (k + 127) / 128 * 128; }
 
-extern "C" size_t trnblas_hip_int4_gemm_workspace(int dtype, int64_t rows, int64_t K) {
-  if (rows <= 0 || K <= 0) return 0;
-  return (size_t)(rows * up128(K)) * 2 * (dtype == TRNBLAS_F32 ? 3 : 1);
+// Rows as the kernels read them, and the parts' sums behind them.
+static size_t rows_bytes(int dtype, int64_t rows, int64_t K) { return (size_t)(rows * up128(K)) * 2 * (dtype == TRNBLAS_F32 ? 3 : 1); }
+static int64_t partial_ld(bool gated, int64_t N) { return ((gated ? 2 * N : N) + 3) / 4 * 4; }
+
+extern "C" size_t trnblas_hip_int4_gemm_workspace(int dtype, int gated, int64_t groups, int64_t rows, int64_t N, int64_t K) {
+  if (rows <= 0 || K <= 0 || N <= 0 || groups <= 0) return 0;
+  const Int4Choice c = choose_int4(rows, groups, N, K, dtype == TRNBLAS_F32 ? 3 : 1, gated != 0);
+  return rows_bytes(dtype, rows, K) + (c.splits > 1 ? (size_t)c.splits * rows * partial_ld(gated != 0, N) * 4 : 0);
 }
 
 extern "C" int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int act, int64_t groups, int64_t rows, int64_t N, int64_t K,
@@ -356,12 +380,17 @@ extern "C" int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int ac
   g.A = A, g.lda = sr;
   g.K = (int)K;
   // (rows far apart: a tile's lie within 32-bit offsets)
-  if (sums && (dtype == TRNBLAS_F32 || sk != 1 || K % 8 != 0 || (uintptr_t)A % 16 != 0 || (rows > 1 && (sr % 8 != 0 || sr > kInt4Far)))) {
-    const size_t need = trnblas_hip_int4_gemm_workspace(dtype, rows, K);
+  Int4Choice c = choose_int4(rows, groups, N, K, dtype == TRNBLAS_F32 ? 3 : 1, gated != 0);
+  const bool lay = sums && (dtype == TRNBLAS_F32 || sk != 1 || K % 8 != 0 || (uintptr_t)A % 16 != 0 || (rows > 1 && (sr % 8 != 0 || sr > kInt4Far)));
+  if (!sums || c.tile == 0) c.splits = 1;
+  if (lay || c.splits > 1) {
+    const size_t need = (lay ? rows_bytes(dtype, rows, K) : 0) + (c.splits > 1 ? (size_t)c.splits * rows * partial_ld(gated != 0, N) * 4 : 0);
     if (workspace == nullptr || workspace_bytes < need || (uintptr_t)workspace % 16 != 0) {
       set_error("%s: workspace of %zu bytes, 16-byte aligned, needed (got %zu)", kGemm, need, workspace_bytes);
       return TRNBLAS_E_WORKSPACE;
     }
+  }
+  if (lay) {
     Int4RowsArgs r{A, sr, sk, rows, (int)K, (int)up128(K), workspace, rows * up128(K)};
     const int64_t grid = (rows * (r.kp / 8) + 255) / 256;
     TRNBLAS_CHECK_ARG(grid < (int64_t)1 << 31, "%s: too many rows", kGemm);
@@ -389,6 +418,32 @@ extern "C" int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int ac
   g.out32 = out_dtype == TRNBLAS_F32, g.out_f16 = out_dtype == TRNBLAS_F16;
   const int eo = g.out32 ? 4 : 2;
   g.vec4 = (uintptr_t)D % (4 * eo) == 0 && ldd % 4 == 0 && (g.C == nullptr || ((uintptr_t)C % (4 * eo) == 0 && ldc % 4 == 0));
-  if (dtype == TRNBLAS_F16) return int4_gemm_run<_Float16>(g, q, 1, gated != 0, s);
-  return int4_gemm_run<__bf16>(g, q, dtype == TRNBLAS_F32 ? 3 : 1, gated != 0, s);
+  q.splits = c.splits;
+  q.ldp = partial_ld(gated != 0, N);
+  q.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + (lay ? rows_bytes(dtype, rows, K) : 0));
+  const int pieces = dtype == TRNBLAS_F32 ? 3 : 1;
+  if (c.tile == 0)
+    return dtype == TRNBLAS_F16 ? int4_gemm_run<_Float16>(g, q, 1, gated != 0, s) : int4_gemm_run<__bf16>(g, q, pieces, gated != 0, s);
+  if (int rc = dtype == TRNBLAS_F16 ? int4_tile_run<_Float16>(g, q, 1, gated != 0, c.tile, s)
+                                    : int4_tile_run<__bf16>(g, q, pieces, gated != 0, c.tile, s))
+    return rc;
+  if (q.splits > 1) {
+    const int64_t grid = (rows * ((N + 3) / 4) + 255) / 256;
+    TRNBLAS_CHECK_ARG(grid < (int64_t)1 << 31, "%s: too many rows", kGemm);
+    if (gated)
+      hipLaunchKernelGGL(int4_join_kernel<true>, dim3((unsigned)grid), dim3(256), 0, s, g, q);
+    else
+      hipLaunchKernelGGL(int4_join_kernel<false>, dim3((unsigned)grid), dim3(256), 0, s, g, q);
+    return check_launch(kGemm);
+  }
+  return TRNBLAS_OK;
+}
+
+extern "C" int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, int64_t N, int64_t K, int32_t plan[5]) {
+  TRNBLAS_CHECK_ARG(plan != nullptr && dtype >= 0 && dtype <= 2 && groups >= 1 && rows >= 1 && N >= 1 && K >= 1,
+                    "trnblas_hip_int4_plan: bad arguments");
+  const Int4Choice c = choose_int4(rows, groups, N, K, dtype == TRNBLAS_F32 ? 3 : 1, gated != 0);
+  const bool few = c.tile == 0;
+  plan[0] = c.tile, plan[1] = c.splits, plan[2] = few ? c.mf : 0, plan[3] = few ? c.nf : 0, plan[4] = few ? c.ks : 0;
+  return TRNBLAS_OK;
 }

@@ -11,6 +11,8 @@
 //    lane loads those of its row and chunk at once. Those outside the matrix are zero.
 #pragma once
 
+#include <algorithm>
+
 #include "gate.hpp"
 #include "gemm.hpp"
 #include "grouped.hpp"
@@ -28,6 +30,9 @@ struct Int4Args {
   int scale_f16;
   int64_t codes_step, groups_step;  // from one matrix of a stack to the next: bytes of codes; scales
   int64_t a_step;                   // elements from one piece of A to the next (fp32)
+  int splits;                       // parts of K (int4_tile_kernel)
+  float* partial;                   // their sums, rows of ldp values
+  int64_t ldp;
 };
 
 constexpr int kInt4Chunk = 1024;  // bytes of codes
@@ -114,9 +119,22 @@ __device__ __forceinline__ void int4_store(const GroupedArgs& g, int64_t m, int 
     store_quad<__bf16>(g, static_cast<const __bf16*>(g.C), static_cast<__bf16*>(g.D), m, n, v);
 }
 
+static const char* const kInt4Gemm = "trnblas_hip_int4_gemm";
+
+// Bound on the tiles of bm rows (see ragged_tile), in whole rounds of the XCDs.
+static int int4_grid(const GroupedArgs& g, int bm, unsigned* grid) {
+  const int64_t tiles = (g.rows / bm + std::min<int64_t>(g.groups + 2, g.rows)) * g.tiles_n;
+  TRNBLAS_CHECK_ARG(tiles < ((int64_t)1 << 31) - 4096, "%s: too many tiles", kInt4Gemm);
+  *grid = (unsigned)((tiles + kNumXcd - 1) / kNumXcd * kNumXcd);
+  return TRNBLAS_OK;
+}
+
 // The launches for operands as the kernels read them (rows 16-byte aligned, K a multiple of 8): T
 // fp16 or bf16, `pieces` 1, or 3 bf16 pieces of fp32 rows. int4_f16.hip, int4_bf16.hip.
 template <typename T>
 int int4_gemm_run(const GroupedArgs& g, const Int4Args& q, int pieces, bool gated, hipStream_t s);
+// The tile kernel; `rows` of a tile 64 or 128. int4_tile_f16.hip, int4_tile_bf16.hip.
+template <typename T>
+int int4_tile_run(const GroupedArgs& g, const Int4Args& q, int pieces, bool gated, int rows, hipStream_t s);
 
 }  // namespace trnblas

@@ -3,19 +3,9 @@
 
 #include <algorithm>
 
-#include "int4_tile.hpp"
+#include "int4_rows.hpp"
 
 namespace trnblas {
-
-static const char* const kInt4Gemm = "trnblas_hip_int4_gemm";
-
-// Bound on the tiles of bm rows (see ragged_tile), in whole rounds of the XCDs.
-static int int4_grid(const GroupedArgs& g, int bm, unsigned* grid) {
-  const int64_t tiles = (g.rows / bm + std::min<int64_t>(g.groups + 2, g.rows)) * g.tiles_n;
-  TRNBLAS_CHECK_ARG(tiles < ((int64_t)1 << 31) - 4096, "%s: too many tiles", kInt4Gemm);
-  *grid = (unsigned)((tiles + kNumXcd - 1) / kNumXcd * kNumXcd);
-  return TRNBLAS_OK;
-}
 
 template <typename T, int P, int MF, int NF, int STEPS, bool GATED>
 static int run_int4_rows(GroupedArgs g, const Int4Args& q, int ks, hipStream_t s) {
@@ -28,21 +18,9 @@ static int run_int4_rows(GroupedArgs g, const Int4Args& q, int ks, hipStream_t s
   return check_launch(kInt4Gemm);
 }
 
-template <typename T, int STEPS, bool GATED>
-static int run_int4_tile(GroupedArgs g, const Int4Args& q, int pieces, hipStream_t s) {
-  constexpr int BN = GATED ? 128 : 256;
-  g.tiles_n = (g.N + BN - 1) / BN;
-  unsigned grid;
-  if (int rc = int4_grid(g, 128, &grid)) return rc;
-  auto kernel = q.zeros ? int4_tile_kernel<T, STEPS, true, GATED> : int4_tile_kernel<T, STEPS, false, GATED>;
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(512), 0, s, g, q, pieces);
-  return check_launch(kInt4Gemm);
-}
-
 template <typename T, int P, int STEPS, bool GATED>
 static int run_int4(const GroupedArgs& g, const Int4Args& q, hipStream_t s) {
   const Int4Choice c = choose_int4(g.rows, g.groups, g.N, g.K, P, GATED);
-  if (c.tile) return run_int4_tile<T, STEPS, GATED>(g, q, P, s);
   if constexpr (P == 1) {
     if (c.mf == 4) return run_int4_rows<T, P, 4, 2, STEPS, GATED>(g, q, c.ks, s);
   }

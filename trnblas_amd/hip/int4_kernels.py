@@ -4,6 +4,8 @@
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -55,13 +57,24 @@ def dequantize(q, shape, group: int, dtype: torch.dtype) -> torch.Tensor:
 FAR = 1 << 22  # elements between rows that are read in place (int4.hip)
 
 
-def _workspace(A: torch.Tensor) -> int:
-    """trnblas_hip_int4_gemm_workspace (the same formula; a library call costs more), 0 where the rows are read in place."""
+@functools.lru_cache(maxsize=4096)
+def _partial_bytes(code: int, gated: int, groups: int, R: int, N: int, K: int) -> int:
+    """Bytes of the parts' sums, by the sizes alone: trnblas_hip_int4_gemm_workspace without the rows'."""
+    total = _fn("trnblas_hip_int4_gemm_workspace")(code, gated, groups, R, N, K)
+    return total - _rows_bytes(code, R, K) if total else 0
+
+
+def _rows_bytes(code: int, R: int, K: int) -> int:
+    return R * (-(-K // 128) * 128) * 2 * (3 if code == 0 else 1)
+
+
+def _in_place(A: torch.Tensor) -> bool:
+    """Whether the kernels read these rows as they are."""
     R, K = A.shape
-    es = A.element_size()
-    if es == 2 and A.stride(1) == 1 and K % 8 == 0 and A.data_ptr() % 16 == 0 and (R <= 1 or (A.stride(0) % 8 == 0 and A.stride(0) <= FAR)):
-        return 0
-    return R * (-(-K // 128) * 128) * 2 * (3 if es == 4 else 1)
+    return (
+        A.element_size() == 2 and A.stride(1) == 1 and K % 8 == 0 and A.data_ptr() % 16 == 0
+        and (R <= 1 or (A.stride(0) % 8 == 0 and A.stride(0) <= FAR))
+    )  # fmt: skip
 
 
 def int4_gemm(
@@ -86,10 +99,12 @@ def int4_gemm(
     R, K = A.shape
     o, o64 = offsets_of(offsets)
     D, c = _output_like(C, beta, (R, N), out_dtype, dev)
-    ws = torch.empty(_workspace(A), dtype=torch.uint8, device=dev)
+    code, G, gated = _lib.DTYPE_CODES[A.dtype], 1 if offsets is None else codes.shape[0], int(act is not None)
+    with torch.cuda.device(dev):  # the plan goes by its compute units
+        n = _partial_bytes(code, gated, G, R, N, K)
+    ws = torch.empty(n + (0 if _in_place(A) else _rows_bytes(code, R, K)), dtype=torch.uint8, device=dev)
     _probed_call(
-        "int4_gemm", "trnblas_hip_int4_gemm", _lib.DTYPE_CODES[A.dtype], _lib.DTYPE_CODES[out_dtype], int(act is not None),
-        ACTS.get(act, 0), 1 if offsets is None else codes.shape[0], R, N, K, group, float(alpha), ptr(A), A.stride(0),
+        "int4_gemm", "trnblas_hip_int4_gemm", code, _lib.DTYPE_CODES[out_dtype], gated, ACTS.get(act, 0), G, R, N, K, group, float(alpha), ptr(A), A.stride(0),
         A.stride(1), ptr(codes), ptr(scales), ptr(zeros), _lib.DTYPE_CODES[scales.dtype], ptr(o), o64,
         float(beta) if c is not None else 0.0, ptr(c), max(c.stride(0), N) if c is not None else N, ptr(D), max(N, 1), ptr(ws),
         ws.numel(), stream_of(dev),
@@ -134,10 +149,12 @@ def int4_gemm_fast(alpha, A, B, offsets, out_dtype, act=None):
             return None
         o, o64 = offsets.data_ptr(), offsets.dtype is torch.int64
     D = A.new_empty((R, N), dtype=out_dtype)
+    n = _partial_bytes(code, gated, G, R, N, K)
+    ws = codes.new_empty(n) if n else None
     rc = _fn("trnblas_hip_int4_gemm")(
         code, out, gated, act or 0, G, R, N, K, B.group, alpha, pa, sr, 1, codes.data_ptr(), scales.data_ptr(),
-        None if zeros is None else zeros.data_ptr(), _SCALE_CODES[scales.dtype], o, o64, 0.0, None, N, D.data_ptr(), N, None, 0,
-        _grouped._raw_stream(dev),
+        None if zeros is None else zeros.data_ptr(), _SCALE_CODES[scales.dtype], o, o64, 0.0, None, N, D.data_ptr(), N,
+        ws.data_ptr() if n else None, n, _grouped._raw_stream(dev),
     )  # fmt: skip
     _checked("trnblas_hip_int4_gemm", rc)
     return D
