@@ -711,7 +711,7 @@ int trnblas_hip_int4_dequantize(int dtype, int scale_dtype, int64_t R, int64_t K
  * sums of parts of K, which those need too).
  */
 size_t trnblas_hip_int4_gemm_workspace(int dtype, int gated, int64_t groups, int64_t rows,
-                                       int64_t N, int64_t K);
+                                       int64_t N, int64_t K, int64_t group);
 int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int act, int64_t groups,
                           int64_t rows, int64_t N, int64_t K, int64_t group, double alpha,
                           const void* A, int64_t sr, int64_t sk, const void* codes,
@@ -726,7 +726,7 @@ int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int act, int64_t 
  * Launches nothing and needs no GPU.
  */
 int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, int64_t N, int64_t K,
-                          int32_t plan[5]);
+                          int64_t group, int32_t plan[5]);
 
 /*
  * Gated projections: H = act(A G) * (A U), the second product elementwise, for weights

@@ -61,6 +61,28 @@ def test_values_at_the_ends(dev, dtype, trans, zeros):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quotients_near_halfway(dev, zeros, dtype):
+    # a group per leading value with each of a type's significands; the rest nearest to (n + 1/2) scales, and one step each way
+    bits = {F32: 10, BF16: 7, F16: 10}[dtype]
+    for scale_dtype in (BF16, F16):
+        for exponent in (-14, -3, 0, 11) if F16 in (dtype, scale_dtype) else (-100, -3, 0, 100):
+            top = ((1 + torch.arange(2**bits) * 2.0**-bits) * 2.0**exponent).to(dtype)
+            low = torch.where(torch.arange(2**bits) % 3 == 0, top.float() * 0, -top.float() / 4).to(dtype)
+            s = (((top.float() - low.float()) / 15 if zeros else top.float() / 7).to(scale_dtype)).double()
+            half = torch.arange(-8, 16) + 0.5
+            mid = (s[:, None] * half).to(dtype)
+            mid = torch.maximum(torch.minimum(mid, top[:, None]), low[:, None] if zeros else -top[:, None])
+            x = torch.stack([mid, torch.nextafter(mid, low[:, None]), torch.nextafter(mid, top[:, None])], -1).flatten(1)
+            x = torch.where(x.float().abs() <= top.float()[:, None], x, top[:, None])
+            x = torch.where(x < low[:, None], low[:, None], x) if zeros else x
+            X = torch.cat([top[:, None], low[:, None], x, x[:, :54]], 1)
+            assert X.shape[1] == 128
+            _same(tb.int4_quantize(X.to(dev), 128, zeros, scale_dtype=scale_dtype), X, 128, zeros, scale_dtype)
+            _same(tb.int4_quantize(X.to(dev), 32, zeros, scale_dtype=scale_dtype), X, 32, zeros, scale_dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_dequantize_and_layout(dev, dtype):
     g = torch.Generator().manual_seed(0)
     for group in (32, 64, 128):
@@ -151,47 +173,51 @@ def test_many_rows(dev, group, dtype):
                 assert oa.ratio(H, *oa.forward(act, P, d, K, out)) <= 1, (G, R, K, N, out)
 
 
-def _plan(dtype, gated, groups, rows, N, K):
+def _plan(dtype, gated, groups, rows, N, K, group):
     """(rows of a tile, parts of K, blocks of rows, blocks of columns, waves along K)"""
     import ctypes
 
     from trnblas_amd.hip import _lib
 
     out = (ctypes.c_int32 * 5)()
-    _lib.call("trnblas_hip_int4_plan", _lib.DTYPE_CODES[dtype], gated, groups, rows, N, K, out)
+    _lib.call("trnblas_hip_int4_plan", _lib.DTYPE_CODES[dtype], gated, groups, rows, N, K, group, out)
     return tuple(out)
 
 
-# (dtype, gated, groups, rows, N, K) that each form of the kernels serves
+# (dtype, gated, groups, rows, N, K) that each form of the kernels serves with each length of group
 FORMS = {
-    (0, 1, 1, 1, 1): [(BF16, 0, 64, 68, 264, 275), (F32, 0, 2, 2, 9200, 16)],
-    (0, 1, 1, 1, 2): [(F16, 0, 16, 14, 593, 134), (F32, 0, 33, 34, 244, 16)],
-    (0, 1, 1, 1, 4): [(BF16, 0, 1, 1, 4416, 132), (F32, 0, 1, 1, 4606, 16)],
-    (0, 1, 1, 1, 8): [(F16, 0, 1, 1, 16, 140), (F32, 0, 1, 41, 31, 491)],
-    (0, 1, 1, 2, 1): [(F16, 0, 16, 22, 3875, 17), (BF16, 1, 64, 84, 480, 17), (F32, 1, 2, 2, 8688, 16)],
-    (0, 1, 1, 2, 2): [(BF16, 0, 16, 16, 1392, 129), (F16, 1, 64, 52, 160, 134), (F32, 0, 64, 55, 339, 136)],
-    (0, 1, 1, 2, 4): [(F16, 0, 33, 960, 194, 288), (BF16, 1, 8, 7, 592, 148), (F32, 0, 16, 14, 782, 257)],
-    (0, 1, 1, 2, 8): [(BF16, 0, 64, 65, 66, 545), (F16, 1, 8, 9, 128, 857), (F32, 1, 1, 1, 16, 131)],
-    (0, 1, 2, 2, 1): [(BF16, 0, 16, 251, 4203, 17), (F16, 1, 33, 421, 1056, 16), (F32, 0, 8, 124, 9412, 16)],
-    (0, 1, 2, 2, 4): [(F16, 0, 33, 581, 407, 472), (BF16, 1, 1, 64, 3360, 337), (F32, 1, 2, 3334, 48, 474)],
-    (0, 1, 2, 2, 8): [(BF16, 0, 1, 2624, 109, 543), (F16, 1, 4, 99, 848, 1019), (F32, 1, 1, 1136, 96, 733)],
-    (0, 1, 4, 2, 8): [(F16, 0, 1, 575, 671, 889), (BF16, 1, 1, 34, 3824, 795)],
-    (64, 1, 0, 0, 0): [(BF16, 0, 4, 983, 17, 41), (F16, 1, 8, 2516, 16, 16), (F32, 1, 1, 3, 4160, 31)],
-    (64, 2, 0, 0, 0): [(F16, 0, 2, 126, 4501, 2175), (BF16, 1, 16, 687, 336, 1609), (F32, 1, 2, 5427, 96, 990)],
-    (64, 4, 0, 0, 0): [(BF16, 0, 64, 5648, 67, 2995), (F16, 1, 1, 39, 4304, 1565), (F32, 0, 4, 89, 2762, 2092)],
-    (64, 8, 0, 0, 0): [(F16, 0, 1, 2337, 105, 4165), (BF16, 1, 1, 64, 128, 11171), (F32, 0, 1, 2326, 35, 1274)],
-    (128, 1, 0, 0, 0): [(BF16, 0, 8, 335, 7043, 17), (F16, 1, 33, 1713, 768, 17), (BF16, 0, 2, 5000, 2051, 1000), (F32, 0, 8, 1636, 3278, 66)],
+    (0, 1, 1, 1, 1): [(F32, 0, 8, 8, 2158, 17)],
+    (0, 1, 1, 1, 2): [(BF16, 0, 1, 1, 9316, 135), (F32, 0, 2, 2, 4179, 17)],
+    (0, 1, 1, 1, 4): [(BF16, 0, 2, 2, 2077, 133), (F32, 0, 1, 1, 4138, 16)],
+    (0, 1, 1, 1, 8): [(F16, 0, 1, 1, 16, 141), (F32, 0, 1, 1, 19, 17)],
+    (0, 1, 1, 2, 1): [(F16, 0, 33, 44, 1942, 16), (F32, 0, 16, 87, 2319, 16), (F16, 1, 2, 2126, 67, 17), (F32, 1, 4, 2021, 66, 19)],
+    (0, 1, 1, 2, 2): [(F16, 0, 8, 2193, 67, 135), (F32, 0, 33, 71, 1853, 20), (F16, 1, 64, 1605, 40, 20), (F32, 1, 2, 2197, 35, 18)],
+    (0, 1, 1, 2, 4): [(F16, 0, 1, 2076, 33, 278), (F32, 0, 64, 1652, 34, 278), (F16, 1, 2, 9, 2179, 17), (F32, 1, 1, 2151, 17, 17)],
+    (0, 1, 1, 2, 8): [(F16, 0, 1, 1, 4105, 540), (F32, 0, 1, 1, 4492, 525), (BF16, 1, 1, 1, 18, 16), (F32, 1, 1, 2, 18, 16)],
+    (0, 1, 2, 2, 1): [(F16, 0, 64, 908, 1344, 16), (F32, 0, 16, 138, 3852, 21), (BF16, 1, 64, 1993, 132, 18), (F32, 1, 64, 2004, 132, 19)],
+    (0, 1, 2, 2, 2): [(BF16, 0, 64, 974, 335, 701), (F32, 0, 64, 872, 293, 169), (BF16, 1, 16, 4254, 33, 17), (F32, 1, 64, 4487, 43, 17)],
+    (0, 1, 2, 2, 4): [(BF16, 0, 64, 3763, 38, 257), (F32, 0, 64, 1595, 152, 133), (BF16, 1, 64, 3763, 18, 17), (F32, 1, 64, 3604, 25, 17)],
+    (0, 1, 2, 2, 8): [(BF16, 0, 4, 4246, 18, 259), (F32, 0, 2, 4508, 17, 287), (F16, 1, 33, 3879, 16, 277), (F32, 1, 8, 4119, 16, 268)],
+    (0, 1, 4, 2, 1): [(F16, 0, 64, 1259, 2032, 16), (BF16, 1, 64, 3859, 156, 16)],
+    (0, 1, 4, 2, 2): [(BF16, 1, 8, 4809, 141, 19)],
+    (0, 1, 4, 2, 4): [(F16, 0, 8, 203, 1935, 427), (F16, 1, 8, 215, 945, 323)],
+    (0, 1, 4, 2, 8): [(BF16, 0, 64, 2424, 80, 548), (F16, 1, 64, 3742, 27, 540)],
+    (64, 1, 0, 0, 0): [(F16, 0, 1, 4, 16, 17), (F32, 0, 1, 4285, 16, 17), (BF16, 1, 1, 1, 16, 16), (F32, 1, 1, 10, 16, 16)],
+    (64, 2, 0, 0, 0): [(F16, 0, 64, 1938, 207, 1243), (F32, 0, 33, 805, 407, 564), (BF16, 1, 64, 1547, 112, 1223), (F32, 1, 64, 2863, 80, 416)],
+    (64, 4, 0, 0, 0): [(BF16, 0, 16, 4157, 33, 1030), (F32, 0, 1, 4100, 65, 268), (F16, 1, 1, 4167, 32, 1577), (F32, 1, 1, 18, 4448, 561)],
+    (64, 8, 0, 0, 0): [(F16, 0, 8, 2347, 34, 3389), (F32, 0, 4, 2270, 33, 1037), (BF16, 1, 1, 16, 16, 10816), (F32, 1, 1, 18, 2320, 1064)],
+    (128, 1, 0, 0, 0): [(F16, 0, 64, 2971, 786, 17), (F32, 0, 64, 2617, 1015, 17), (F16, 1, 64, 3743, 336, 17), (F32, 1, 4, 145, 7984, 16)],
 }
 
 
 @pytest.mark.parametrize("form", list(FORMS))
 def test_each_form(dev, form):
     for i, (dtype, gated, G, R, N, K) in enumerate(FORMS[form]):
-        assert _plan(dtype, gated, G, R, N, K) == form, (dtype, gated, G, R, N, K)
         g = torch.Generator(device=dev).manual_seed(i)
         off = og.uneven(G, R, i) if R > 4 * G else torch.arange(G + 1) * (R // G)
         A = torch.randn(R, K, generator=g, device=dev).to(dtype)
         for group, zeros in ((128, False), (32, True), (64, False)):
+            assert _plan(dtype, gated, G, R, N, K, group) == form, (dtype, gated, G, R, N, K, group)
             E, W = oi.random_matrix(g, G, 2 * N if gated else N, K, group=group, zeros=zeros, scale_dtype=BF16 if zeros else F16, device=dev)
             if gated:
                 P, d = oa.products(A, W, off, True)

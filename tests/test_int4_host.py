@@ -194,9 +194,9 @@ def test_c_abi_refusals():
                       (dict(sk=-1), b"stride"), (dict(ldd=7), b"leading"), (dict(a=None), b"null"), (dict(codes=8), b"aligned")):  # fmt: skip
         assert gemm(**bad) == _lib.E_ARG and word in lib.trnblas_hip_last_error(), bad
     # rows that are not read in place need a workspace
-    need = lib.trnblas_hip_int4_gemm_workspace(0, 0, 1, 3, 8, 64)
-    assert need == 3 * 128 * 2 * 3 and lib.trnblas_hip_int4_gemm_workspace(1, 0, 1, 3, 8, 130) == 3 * 256 * 2
-    assert lib.trnblas_hip_int4_gemm_workspace(1, 0, 1, 0, 8, 130) == 0
+    need = lib.trnblas_hip_int4_gemm_workspace(0, 0, 1, 3, 8, 64, 32)
+    assert need == 3 * 128 * 2 * 3 and lib.trnblas_hip_int4_gemm_workspace(1, 0, 1, 3, 8, 130, 64) == 3 * 256 * 2
+    assert lib.trnblas_hip_int4_gemm_workspace(1, 0, 1, 0, 8, 130, 64) == 0
     for how in (dict(dtype=0), dict(sk=2), dict(a=4098), dict(sr=65)):
         assert gemm(**how) == _lib.E_WORKSPACE and b"workspace" in lib.trnblas_hip_last_error(), how
     assert gemm(dtype=0, ws=4096, size=need - 1) == _lib.E_WORKSPACE and gemm(dtype=0, ws=4104, size=need) == _lib.E_WORKSPACE

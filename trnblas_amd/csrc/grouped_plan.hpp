@@ -151,39 +151,44 @@ struct Int4Choice {
   int mf, nf, ks, tile, splits;
 };
 
-// Times (us) fitted to sweeps of 1 .. 2048 rows over matrices of 2048 .. 8192 squared, bf16, groups of 128 (others
-// scale all kernels alike; over 70 random sizes the choice took 5.6 % longer than the fastest of 15 forms). The few-rows kernel: 2.6 for each round of a workgroup per CU, and for
-// each chunk of a wave by its blocks of rows and columns; the tile kernel's tiles as in ring_time; parts of K: what
-// writes and reads their sums. 64 rows, 8192 x 8192: few rows 36, tiles of 64 in four parts 28, in one 52, of 128 106;
-// 2048 rows: 1025, 376, 285, 237.
-inline Int4Choice choose_int4(double rows, double groups, double N, double K, int pieces, bool gated) {
+// Times (us) fitted to sweeps of 1 .. 2048 rows over matrices of 2048 .. 8192 squared and of 130 random sizes, dense and
+// of up to 64 groups, where the choice took 1.05 times what the best of all forms did. The few-rows kernel: a workgroup
+// alone on its CU takes `alone` for each chunk of a wave, several take `busy`; of a block's sixteen rows those count
+// that are there, the others are read from the first level's cache. The tile kernel's tiles as in ring_time; parts of K:
+// what writes and reads their sums. steps: of 32 values per group: a group's sums are taken at its end. 64 rows,
+// 8192 x 8192: few rows 36, tiles of 64 in four parts 28, in one 52, of 128 106; 2048 rows: 1025, 376, 285, 237.
+inline Int4Choice choose_int4(double rows, double groups, double N, double K, int steps, int pieces, bool gated) {
   const double cus = device_cus(), chunks = std::ceil(K / 128.0), columns = gated ? 2.0 * N : N, chain = chunks * pieces;
-  // of a block's sixteen rows those that are there: the others are read from the first level's cache
-  const double filled = std::min(1.0, rows / std::max(1.0, std::min(groups, rows)) / 16.0);
+  const double per = rows / std::max(1.0, std::min(groups, rows)), folds = steps == 4 ? 0.0 : steps == 2 ? 0.15 : 0.45;
   Int4Choice best{1, 2, 8, 0, 1};
   double time = 1e30;
   for (int mf : {1, 2, 4}) {
     if (mf == 4 && pieces == 3) break;
+    const double filled = std::min(1.0, per / (16.0 * mf));
     for (int nf : {2, 1}) {
       if (nf == 1 && (mf > 1 || gated)) continue;
-      const double each = (mf == 1 ? (nf == 1 ? 0.35 + 0.45 * filled : 0.72 + 0.33 * filled) : mf == 2 ? 1.85 : 3.6) * (pieces == 3 ? 2.5 : 1.0);
+      double alone = nf == 1 ? 0.35 + 0.45 * filled : 0.72 + 0.33 * filled, busy = nf == 1 ? 0.42 + 0.58 * filled : 0.15 + 0.95 * filled;
+      if (mf > 1) alone = 0.45 * mf + 0.45 * mf * filled, busy = 0.15 * mf + 0.85 * mf * filled;
+      alone += 0.3 * folds * mf, busy += folds * mf;
+      if (pieces == 3) alone *= 2.5, busy *= 2.5;
       for (int ks : {8, 4, 2, 1}) {
-        const double groups_of = likely_row_tiles(rows, groups, 16 * mf) * std::ceil(columns * ks / (128.0 * nf));
-        const double t = 2.0 + std::max(1.0, groups_of / cus) * (2.6 + std::ceil(chunks / ks) * each);
+        const double r = likely_row_tiles(rows, groups, 16 * mf) * std::ceil(columns * ks / (128.0 * nf)) / cus, n = std::ceil(chunks / ks);
+        const double rounds = r <= 1.0 ? 0.0 : r < 4.0 ? std::ceil(r) : r + 0.5;
+        const double t = 2.0 + std::max(2.6 + n * alone, rounds * (1.3 + n * busy));
         if (t < time) time = t, best = {mf, nf, ks, 0, 1};
       }
     }
   }
   // (gates and ups: from one to the other within 32-bit offsets of the scales)
-  if (gated && (std::fmod(N, 16.0) != 0.0 || N * K >= 16.0 * INT32_MAX)) return best;
+  const bool tiles = !gated || (std::fmod(N, 16.0) == 0.0 && N * K < 16.0 * INT32_MAX);
   for (int tile : {64, 128})
     for (int splits : {1, 2, 4, 8}) {
       const double sums = splits * rows * columns * 4.0;
-      if (splits > 1 && (tile == 128 || chain < 2.0 * splits || sums > 256e6)) break;
+      if (!tiles || (splits > 1 && (tile == 128 || chain < 2.0 * splits || sums > 256e6))) break;
       const double slots = tile == 64 ? 2.0 * cus : cus;
       const double r = likely_row_tiles(rows, groups, tile) * std::ceil(columns / (2.0 * tile)) * splits / slots;
       const double busy = tile == 64 ? std::min(1.0, std::max(0.0, 2.0 * r - 1.0)) : std::min(1.0, r);
-      const double each = tile == 64 ? 0.75 + 0.43 * busy : 1.58 + 0.3 * busy;
+      const double each = (tile == 64 ? 0.75 + 0.43 * busy : 1.58 + 0.3 * busy) * (1.0 + 0.7 * folds);
       const double rounds = r <= 1.0 ? 1.0 : tile == 64 ? r + 0.3 : std::ceil(r);
       const double t = rounds * (4.2 + std::ceil(chain / splits) * each) + (splits > 1 ? 2.5 + sums / 2.7e6 : 0.0);
       if (t < time) time = t, best = {1, 2, 8, tile, splits};

@@ -33,53 +33,112 @@ __device__ __forceinline__ uint16_t int4_scale_bits(float s, int f16) {
 }
 
 // lo, hi: the least and largest value, and zero; top: bits of the largest magnitude.
-__device__ __forceinline__ Int4Group int4_group(float lo, float hi, uint32_t top, bool zeros, int f16) {
+template <bool ZEROS>
+__device__ __forceinline__ Int4Group int4_group(float lo, float hi, uint32_t top, int f16) {
   Int4Group q;
-  q.bits = int4_scale_bits(zeros ? (hi - lo) / 15.0f : __builtin_bit_cast(float, top) / 7.0f, f16);
+  q.bits = int4_scale_bits(ZEROS ? (hi - lo) / 15.0f : __builtin_bit_cast(float, top) / 7.0f, f16);
   q.s = int4_scale(q.bits, f16);
   if (top >= 0x7f800000u || !(__builtin_fabsf(q.s) <= 3.4028235e38f)) {
     q.bits = int4_scale_bits(__builtin_nanf(""), f16);
     q.s = 0.0f;  // codes of zero
   }
-  q.z = zeros ? (q.s > 0.0f ? fminf(fmaxf(rintf(-lo / q.s), 0.0f), 15.0f) : 0.0f) : 8.0f;
+  q.z = ZEROS ? (q.s > 0.0f ? fminf(fmaxf(rintf(-lo / q.s), 0.0f), 15.0f) : 0.0f) : 8.0f;
   return q;
 }
 
-// round(x / s) by the reciprocal of s, as a float: |x / s| < 23 (15 times a scale of few bits, rounded down), so
-// that the product is within 2^-18 of the quotient, and only where it lies within 2^-16 of halfway between two whole numbers may the two round apart (or
-// the quotient's own rounding to fp32 decide): `close` says that.
-__device__ __forceinline__ float int4_near(float x, float inverse, bool& close) {
-  const float y = x * inverse, v = rintf(y);
-  close |= __builtin_fabsf(y - v) > 0.5f - 0x1p-16f;
-  return v;
-}
-
-// The first `left` of eight values as nibbles q - 8, zeros behind them. (A division for each value: 8192 x 8192 bf16 took
-// 61 us.)
-__device__ __forceinline__ uint32_t int4_dword(const float (&x)[8], const Int4Group& q, int left) {
-  float v[8];
-  // a scale at the ends of the range has no reciprocal that is near enough
-  bool close = q.s < 0x1p-120f || q.s > 0x1p120f;
-  const float inverse = __builtin_amdgcn_rcpf(q.s);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = int4_near(x[e], inverse, close);
-  if (close) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = q.s > 0.0f ? rintf(x[e] / q.s) : 0.0f;
-  }
-  const float lo = -q.z, hi = 15.0f - q.z;
-  uint32_t w = 0;
+// Eight values as nibbles q - 8. round(x / s) is taken from the product with the reciprocal of s: |x / s| < 23 (15
+// times what rounding the scale takes away, a third of it at most), so that the product is within 2^-18 of
+// the quotient, and adding 1.5 * 2^23 rounds it to a whole number, whose low bits are the code's.
+// Values of 16 bits: a quotient of two numbers of 11 bits is halfway between two whole numbers or 2^-13 from that at
+// least. In steps of 2^-13 or 2^-14, where 1024 is added, the product of a quotient halfway is exactly that, and another's
+// on its side. Values of 32 bits: where the product is within 2^-16 of halfway, they are divided, as where the scale has
+// no reciprocal.
+template <bool NARROW, bool ZEROS>
+__device__ __forceinline__ uint32_t int4_dword(const float (&x)[8], const Int4Group& q) {
+  constexpr float kWhole = 0x1.8p23f;
+  const float inverse = __builtin_amdgcn_rcpf(q.s), lo = kWhole - q.z, hi = kWhole + 15.0f - q.z;
+  float v[8], off = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int c = (int)(fminf(fmaxf(v[e], lo), hi) + (q.z - 8.0f));
-    w |= ((uint32_t)c & (e < left ? 15u : 0u)) << 4 * (e / 2 + 4 * (e & 1));
+    if constexpr (NARROW) {
+      v[e] = __builtin_fmaf(x[e], inverse, 1024.0f) + (kWhole - 1024.0f);
+    } else {
+      v[e] = __builtin_fmaf(x[e], inverse, kWhole);
+      off = fmaxf(off, __builtin_fabsf(__builtin_fmaf(x[e], inverse, kWhole - v[e])));
+    }
+  }
+  if (off > 0.5f - 0x1p-16f || q.s < 0x1p-120f || q.s > 0x1p120f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = kWhole + (q.s > 0.0f ? rintf(x[e] / q.s) : 0.0f);
+  }
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int e = 2 * (i & 3) + i / 4;  // the nibbles from the lowest
+    const float c = __builtin_amdgcn_fmed3f(v[e], lo, hi) + (ZEROS ? q.z - 8.0f : 0.0f);
+    w = __builtin_amdgcn_alignbit(__builtin_bit_cast(uint32_t, c), w, 4);
   }
   return w;
 }
 
+// The least, the largest and the largest magnitude of values: of 16 bits in pairs, as whole numbers in their order.
+template <typename T, bool ZEROS>
+struct Int4Range;
+
+template <bool ZEROS>
+struct Int4Range<float, ZEROS> {
+  float lo = 0.0f, hi = 0.0f;
+  uint32_t top = 0;
+  __device__ __forceinline__ void take(const float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (ZEROS) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
+      top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
+    }
+  }
+  __device__ __forceinline__ void join(int lanes) {
+    if constexpr (ZEROS) lo = fminf(lo, __shfl_xor(lo, lanes)), hi = fmaxf(hi, __shfl_xor(hi, lanes));
+    top = max(top, (uint32_t)__shfl_xor((int)top, lanes));
+  }
+  __device__ __forceinline__ Int4Group group(int f16) const { return int4_group<ZEROS>(lo, hi, top, f16); }
+};
+
+template <typename T, bool ZEROS>
+struct Int4Range {
+  using i16x2 = __attribute__((ext_vector_type(2))) int16_t;
+  i16x2 lo = 0, hi = 0;  // symmetric: hi alone, of magnitudes
+  __device__ __forceinline__ void take(const T (&x)[8]) {
+    i16x2 v[4];
+    __builtin_memcpy(v, x, 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (ZEROS) {
+        v[e] ^= (v[e] >> 15) & 0x7fff;
+        lo = __builtin_elementwise_min(lo, v[e]);
+      } else {
+        v[e] &= 0x7fff;
+      }
+      hi = __builtin_elementwise_max(hi, v[e]);
+    }
+  }
+  __device__ __forceinline__ void join(int lanes) {
+    if constexpr (ZEROS) lo = __builtin_elementwise_min(lo, __builtin_bit_cast(i16x2, __shfl_xor(__builtin_bit_cast(int, lo), lanes)));
+    hi = __builtin_elementwise_max(hi, __builtin_bit_cast(i16x2, __shfl_xor(__builtin_bit_cast(int, hi), lanes)));
+  }
+  __device__ __forceinline__ Int4Group group(int f16) const {
+    const int16_t l = min(lo.x, lo.y), h = max(hi.x, hi.y);
+    const float least = (float)__builtin_bit_cast(T, (int16_t)(l ^ (l >> 15 & 0x7fff))), most = (float)__builtin_bit_cast(T, h);
+    // (a NaN's bits are past an infinity's on its side)
+    const uint32_t top = max(__builtin_bit_cast(uint32_t, least) & 0x7fffffffu, __builtin_bit_cast(uint32_t, most));
+    return int4_group<ZEROS>(least, most, top, f16);
+  }
+};
+
 // 16 rows x 128 values per wave, four waves per workgroup: lane 16 p + r takes row r, k = 32 h + 8 p .. + 7
 // for h = 0 .. 3, which are its 16 bytes of codes; a group's values lie in the four lanes of a row.
-template <typename T>
+// 8192 x 8192 bf16 in groups of 128: 34 us, 168 MB at 4.9 TB/s. With a division for each value, extremes as floats and a scale
+// for each h it was 63 us, bound by the vector unit. A transposed 487 x 1283 fp32: 5.5 us, 6.8 with loads behind branches.
+template <typename T, int STEPS, bool ZEROS>
 __global__ __launch_bounds__(256) void int4_quantize_kernel(Int4QuantArgs g) {
   const int lane = threadIdx.x & 63, r = lane & 15, p = lane >> 4;
   const int blocks = (g.R + 15) / 16;
@@ -87,61 +146,77 @@ __global__ __launch_bounds__(256) void int4_quantize_kernel(Int4QuantArgs g) {
   if (item >= (int64_t)blocks * g.chunks) return;
   const int block = (int)(item / g.chunks), chunk = (int)(item - (int64_t)block * g.chunks);
   const int row = 16 * block + r;
-  const T* X = static_cast<const T*>(g.X) + blockIdx.y * g.sx + row * g.sr;
-  float v[4][8];
+  T v[4][8];
+  if (g.vec && (chunk + 1) * 128 <= g.K && row < g.R) {
+    const T* x = static_cast<const T*>(g.X) + blockIdx.y * g.sx + row * g.sr + 128 * chunk + 8 * p;
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    const int k = 128 * chunk + 32 * h + 8 * p, left = row < g.R ? g.K - k : 0;
-    const T* x = X + k * g.sk;
-    if (g.vec && left >= 8) {
-      union {
-        i32x4 w[sizeof(T) / 2];
-        T e[8];
-      } u;
+    for (int h = 0; h < 4; ++h)
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.w[i] = reinterpret_cast<const i32x4*>(x)[i];
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        const i32x4 w = *reinterpret_cast<const i32x4*>(x + 32 * h + 16 / sizeof(T) * i);
+        __builtin_memcpy(&v[h][16 / sizeof(T) * i], &w, 16);
+      }
+  } else {
+    // values past the matrix: its last one instead, then zero, so that no load waits for a branch
+    const T* x = static_cast<const T*>(g.X) + blockIdx.y * g.sx + (row < g.R ? row : g.R - 1) * g.sr;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[h][e] = (float)u.e[e];
-    } else {
+    for (int h = 0; h < 4; ++h)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[h][e] = e < left ? (float)x[e * g.sk] : 0.0f;
-    }
+      for (int e = 0; e < 8; ++e) v[h][e] = x[min(128 * chunk + 32 * h + 8 * p + e, g.K - 1) * g.sk];
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (row >= g.R || 128 * chunk + 32 * h + 8 * p + e >= g.K) v[h][e] = (T)0.0f;
   }
-  float lo[4], hi[4];
-  uint32_t top[4];
-#pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    lo[h] = hi[h] = 0.0f, top[h] = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      lo[h] = fminf(lo[h], v[h][e]), hi[h] = fmaxf(hi[h], v[h][e]);
-      top[h] = max(top[h], __builtin_bit_cast(uint32_t, v[h][e]) & 0x7fffffffu);
-    }
-  }
-  auto join = [&](int a, int b) __attribute__((always_inline)) {
-    lo[a] = lo[b] = fminf(lo[a], lo[b]), hi[a] = hi[b] = fmaxf(hi[a], hi[b]), top[a] = top[b] = max(top[a], top[b]);
-  };
-  if (g.steps >= 2) join(0, 1), join(2, 3);
-  if (g.steps == 4) join(0, 2), join(1, 3);
-  const bool zeros = g.zeros != nullptr;
+  const int64_t at = ((blockIdx.y * (int64_t)blocks + block) * g.chunks + chunk);
   i32x4 w;
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
+  for (int h = 0; h < 4; h += STEPS) {
+    Int4Range<T, ZEROS> range;
 #pragma unroll
-    for (int d = 16; d <= 32; d *= 2) {
-      lo[h] = fminf(lo[h], __shfl_xor(lo[h], d)), hi[h] = fmaxf(hi[h], __shfl_xor(hi[h], d));
-      top[h] = max(top[h], (uint32_t)__shfl_xor((int)top[h], d));
+    for (int i = 0; i < STEPS; ++i) range.take(v[h + i]);
+    range.join(16), range.join(32);
+    const Int4Group q = range.group(g.scale_f16);
+#pragma unroll
+    for (int i = h; i < h + STEPS; ++i) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)v[i][e];
+      w[i] = (int)int4_dword<sizeof(T) == 2, ZEROS>(x, q);
+      const int left = row < g.R ? g.K - (128 * chunk + 32 * i + 8 * p) : 0;
+      if (left < 8) {
+        uint32_t keep = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) keep |= (e < left ? 15u : 0u) << 4 * (e / 2 + 4 * (e & 1));
+        w[i] &= (int)keep;
+      }
     }
-    const Int4Group q = int4_group(lo[h], hi[h], top[h], zeros, g.scale_f16);
-    w[h] = (int)int4_dword(v[h], q, row < g.R ? g.K - (128 * chunk + 32 * h + 8 * p) : 0);
-    if (p == 0 && (h & (g.steps - 1)) == 0) {
-      const int64_t at = (((blockIdx.y * (int64_t)blocks + block) * g.chunks + chunk) * 16 + r) * (4 / g.steps) + h / g.steps;
+    if (p == 0) {
+      const int64_t to = (at * 16 + r) * (4 / STEPS) + h / STEPS;
       const bool inside = row < g.R && 128 * chunk + 32 * h < g.K;
-      g.scales[at] = inside ? q.bits : 0;
-      if (zeros) g.zeros[at] = inside ? (uint8_t)q.z : 0;
+      g.scales[to] = inside ? q.bits : 0;
+      if constexpr (ZEROS) g.zeros[to] = inside ? (uint8_t)q.z : 0;
     }
   }
-  *reinterpret_cast<i32x4*>(g.codes + ((blockIdx.y * (int64_t)blocks + block) * g.chunks + chunk) * kInt4Chunk + 16 * lane) = w;
+  *reinterpret_cast<i32x4*>(g.codes + at * kInt4Chunk + 16 * lane) = w;
+}
+
+template <typename T, int STEPS>
+static void launch_quantize(const Int4QuantArgs& g, dim3 grid, hipStream_t s) {
+  if (g.zeros != nullptr)
+    hipLaunchKernelGGL((int4_quantize_kernel<T, STEPS, true>), grid, dim3(256), 0, s, g);
+  else
+    hipLaunchKernelGGL((int4_quantize_kernel<T, STEPS, false>), grid, dim3(256), 0, s, g);
+}
+
+template <typename T>
+static void launch_quantize(const Int4QuantArgs& g, dim3 grid, hipStream_t s) {
+  switch (g.steps) {
+    case 1: return launch_quantize<T, 1>(g, grid, s);
+    case 2: return launch_quantize<T, 2>(g, grid, s);
+    default: return launch_quantize<T, 4>(g, grid, s);
+  }
 }
 
 struct Int4DequantArgs {
@@ -300,9 +375,9 @@ extern "C" int trnblas_hip_int4_quantize(int dtype, int scale_dtype, int64_t R, 
   g.vec = sk == 1 && (uintptr_t)X % 16 == 0 && sr * es % 16 == 0 && sx * es % 16 == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case TRNBLAS_F32: hipLaunchKernelGGL(int4_quantize_kernel<float>, grid, dim3(256), 0, s, g); break;
-    case TRNBLAS_BF16: hipLaunchKernelGGL(int4_quantize_kernel<__bf16>, grid, dim3(256), 0, s, g); break;
-    default: hipLaunchKernelGGL(int4_quantize_kernel<_Float16>, grid, dim3(256), 0, s, g); break;
+    case TRNBLAS_F32: launch_quantize<float>(g, grid, s); break;
+    case TRNBLAS_BF16: launch_quantize<__bf16>(g, grid, s); break;
+    default: launch_quantize<_Float16>(g, grid, s); break;
   }
   return check_launch(kQuantize);
 }
@@ -343,9 +418,10 @@ static int64_t up128(int64_t k) { return (k + 127) / 128 * 128; }
 static size_t rows_bytes(int dtype, int64_t rows, int64_t K) { return (size_t)(rows * up128(K)) * 2 * (dtype == TRNBLAS_F32 ? 3 : 1); }
 static int64_t partial_ld(bool gated, int64_t N) { return ((gated ? 2 * N : N) + 3) / 4 * 4; }
 
-extern "C" size_t trnblas_hip_int4_gemm_workspace(int dtype, int gated, int64_t groups, int64_t rows, int64_t N, int64_t K) {
+extern "C" size_t trnblas_hip_int4_gemm_workspace(int dtype, int gated, int64_t groups, int64_t rows, int64_t N, int64_t K,
+                                                  int64_t group) {
   if (rows <= 0 || K <= 0 || N <= 0 || groups <= 0) return 0;
-  const Int4Choice c = choose_int4(rows, groups, N, K, dtype == TRNBLAS_F32 ? 3 : 1, gated != 0);
+  const Int4Choice c = choose_int4(rows, groups, N, K, (int)(group / 32), dtype == TRNBLAS_F32 ? 3 : 1, gated != 0);
   return rows_bytes(dtype, rows, K) + (c.splits > 1 ? (size_t)c.splits * rows * partial_ld(gated != 0, N) * 4 : 0);
 }
 
@@ -380,7 +456,7 @@ extern "C" int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int ac
   g.A = A, g.lda = sr;
   g.K = (int)K;
   // (rows far apart: a tile's lie within 32-bit offsets)
-  Int4Choice c = choose_int4(rows, groups, N, K, dtype == TRNBLAS_F32 ? 3 : 1, gated != 0);
+  Int4Choice c = choose_int4(rows, groups, N, K, (int)(group / 32), dtype == TRNBLAS_F32 ? 3 : 1, gated != 0);
   const bool lay = sums && (dtype == TRNBLAS_F32 || sk != 1 || K % 8 != 0 || (uintptr_t)A % 16 != 0 || (rows > 1 && (sr % 8 != 0 || sr > kInt4Far)));
   if (!sums || c.tile == 0) c.splits = 1;
   if (lay || c.splits > 1) {
@@ -439,10 +515,12 @@ extern "C" int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int ac
   return TRNBLAS_OK;
 }
 
-extern "C" int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, int64_t N, int64_t K, int32_t plan[5]) {
-  TRNBLAS_CHECK_ARG(plan != nullptr && dtype >= 0 && dtype <= 2 && groups >= 1 && rows >= 1 && N >= 1 && K >= 1,
+extern "C" int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, int64_t N, int64_t K, int64_t group,
+                                     int32_t plan[5]) {
+  TRNBLAS_CHECK_ARG(plan != nullptr && dtype >= 0 && dtype <= 2 && groups >= 1 && rows >= 1 && N >= 1 && K >= 1 &&
+                        (group == 32 || group == 64 || group == 128),
                     "trnblas_hip_int4_plan: bad arguments");
-  const Int4Choice c = choose_int4(rows, groups, N, K, dtype == TRNBLAS_F32 ? 3 : 1, gated != 0);
+  const Int4Choice c = choose_int4(rows, groups, N, K, (int)(group / 32), dtype == TRNBLAS_F32 ? 3 : 1, gated != 0);
   const bool few = c.tile == 0;
   plan[0] = c.tile, plan[1] = c.splits, plan[2] = few ? c.mf : 0, plan[3] = few ? c.nf : 0, plan[4] = few ? c.ks : 0;
   return TRNBLAS_OK;

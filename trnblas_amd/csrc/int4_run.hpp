@@ -20,7 +20,7 @@ static int run_int4_rows(GroupedArgs g, const Int4Args& q, int ks, hipStream_t s
 
 template <typename T, int P, int STEPS, bool GATED>
 static int run_int4(const GroupedArgs& g, const Int4Args& q, hipStream_t s) {
-  const Int4Choice c = choose_int4(g.rows, g.groups, g.N, g.K, P, GATED);
+  const Int4Choice c = choose_int4(g.rows, g.groups, g.N, 128.0 * q.chunks, STEPS, P, GATED);
   if constexpr (P == 1) {
     if (c.mf == 4) return run_int4_rows<T, P, 4, 2, STEPS, GATED>(g, q, c.ks, s);
   }

@@ -195,8 +195,8 @@ SIGNATURES = {
         _c_int,
         [_c_int, _c_int, _c_i64, _c_i64, _c_i64] + [_c_ptr] * 4 + [_c_i64, _c_i64, _c_i64, _c_ptr],
     ),
-    "trnblas_hip_int4_gemm_workspace": (_c_size, [_c_int, _c_int] + [_c_i64] * 4),
-    "trnblas_hip_int4_plan": (_c_int, [_c_int, _c_int] + [_c_i64] * 4 + [ctypes.POINTER(ctypes.c_int32)]),
+    "trnblas_hip_int4_gemm_workspace": (_c_size, [_c_int, _c_int] + [_c_i64] * 5),
+    "trnblas_hip_int4_plan": (_c_int, [_c_int, _c_int] + [_c_i64] * 5 + [ctypes.POINTER(ctypes.c_int32)]),
     "trnblas_hip_int4_gemm": (
         _c_int,
         [_c_int] * 4 + [_c_i64] * 5 + [_c_dbl, _c_ptr, _c_i64, _c_i64] + [_c_ptr] * 3 + [_c_int, _c_ptr, _c_int]
