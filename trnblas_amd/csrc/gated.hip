@@ -24,72 +24,58 @@ struct GateArgs {
   int vec;  // whole groups of V values, every row's start aligned to them
 };
 
-// V values from p, as floats; only `left` of them where that is fewer.
-template <typename T, int V>
-__device__ __forceinline__ void load_values(const T* p, bool vec, int left, float (&v)[V]) {
+// V values from p, as floats.
+template <int V, typename T>
+__device__ __forceinline__ void load_values(const T* p, float (&v)[V]) {
   typedef T tv __attribute__((ext_vector_type(V)));
-  if (vec) {
-    const tv w = *reinterpret_cast<const tv*>(p);
+  const tv w = *reinterpret_cast<const tv*>(p);
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (float)w[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = i < left ? (float)p[i] : 0.0f;
-  }
+  for (int i = 0; i < V; ++i) v[i] = (float)w[i];
 }
-template <typename T, int V>
-__device__ __forceinline__ void store_values(T* p, bool vec, int left, const float (&v)[V]) {
+template <int V, typename T>
+__device__ __forceinline__ void store_values(T* p, const float (&v)[V]) {
   typedef T tv __attribute__((ext_vector_type(V)));
-  if (vec) {
-    tv w;
+  tv w;
 #pragma unroll
-    for (int i = 0; i < V; ++i) w[i] = (T)v[i];
-    *reinterpret_cast<tv*>(p) = w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < left) p[i] = (T)v[i];
-  }
+  for (int i = 0; i < V; ++i) w[i] = (T)v[i];
+  *reinterpret_cast<tv*>(p) = w;
 }
 
-// One thread takes V values of a row: 64 x 4 threads, columns by rows.
+// One thread takes V values of a row: 64 x 4 threads, columns by rows. Rows that start anywhere, or end inside eight
+// values: one each, side by side (301 x 771 fp32: 3.0 us, with eight each 6.3).
 constexpr int kGateV = 8;
 
-template <typename T, typename O>
+template <typename T, typename O, int V>
 __global__ __launch_bounds__(256) void gate_kernel(GateArgs g) {
-  constexpr int V = kGateV;
   const int c = V * (blockIdx.x * 64 + threadIdx.x);
-  const int left = g.n - c;
-  if (left <= 0) return;
+  if (c >= g.n) return;
   for (int64_t r = blockIdx.y * 4 + threadIdx.y; r < g.rows; r += 4 * gridDim.y) {
     const T* p = static_cast<const T*>(g.P) + r * g.ldp + c;
     float a[V], u[V], h[V];
-    load_values<T, V>(p, g.vec, left, a);
-    load_values<T, V>(p + g.n, g.vec, left, u);
+    load_values<V>(p, a);
+    load_values<V>(p + g.n, u);
 #pragma unroll
     for (int i = 0; i < V; ++i) h[i] = gate(g.act, a[i]) * u[i];
-    store_values<O, V>(static_cast<O*>(g.D) + r * g.ldd + c, g.vec, left, h);
+    store_values<V>(static_cast<O*>(g.D) + r * g.ldd + c, h);
     if (g.S) {
       O* s = static_cast<O*>(g.S) + r * g.lds + c;
-      store_values<O, V>(s, g.vec, left, a);
-      store_values<O, V>(s + g.n, g.vec, left, u);
+      store_values<V>(s, a);
+      store_values<V>(s + g.n, u);
     }
   }
 }
 
 // dG = dH * U * act'(G), dU = dH * act(G).
-template <typename T>
+template <typename T, int V>
 __global__ __launch_bounds__(256) void gate_backward_kernel(GateArgs g) {
-  constexpr int V = kGateV;
   const int c = V * (blockIdx.x * 64 + threadIdx.x);
-  const int left = g.n - c;
-  if (left <= 0) return;
+  if (c >= g.n) return;
   for (int64_t r = blockIdx.y * 4 + threadIdx.y; r < g.rows; r += 4 * gridDim.y) {
     const T* p = static_cast<const T*>(g.P) + r * g.ldp + c;
     float a[V], u[V], d[V];
-    load_values<T, V>(p, g.vec, left, a);
-    load_values<T, V>(p + g.n, g.vec, left, u);
-    load_values<T, V>(static_cast<const T*>(g.dH) + r * g.ldg + c, g.vec, left, d);
+    load_values<V>(p, a);
+    load_values<V>(p + g.n, u);
+    load_values<V>(static_cast<const T*>(g.dH) + r * g.ldg + c, d);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float y, slope;
@@ -98,14 +84,31 @@ __global__ __launch_bounds__(256) void gate_backward_kernel(GateArgs g) {
       u[i] = d[i] * y;
     }
     T* o = static_cast<T*>(g.D) + r * g.ldd + c;
-    store_values<T, V>(o, g.vec, left, a);
-    store_values<T, V>(o + g.n, g.vec, left, u);
+    store_values<V>(o, a);
+    store_values<V>(o + g.n, u);
   }
 }
 
 static dim3 gate_grid(const GateArgs& g) {
   const int64_t rows = (g.rows + 3) / 4;
-  return dim3((unsigned)((g.n + 64 * kGateV - 1) / (64 * kGateV)), (unsigned)(rows < 32768 ? rows : 32768));
+  const int columns = 64 * (g.vec ? kGateV : 1);
+  return dim3((unsigned)((g.n + columns - 1) / columns), (unsigned)(rows < 32768 ? rows : 32768));
+}
+
+template <typename T, typename O>
+static void launch_gate(const GateArgs& g, hipStream_t s) {
+  if (g.vec)
+    hipLaunchKernelGGL((gate_kernel<T, O, kGateV>), gate_grid(g), dim3(64, 4), 0, s, g);
+  else
+    hipLaunchKernelGGL((gate_kernel<T, O, 1>), gate_grid(g), dim3(64, 4), 0, s, g);
+}
+
+template <typename T>
+static void launch_gate_backward(const GateArgs& g, hipStream_t s) {
+  if (g.vec)
+    hipLaunchKernelGGL((gate_backward_kernel<T, kGateV>), gate_grid(g), dim3(64, 4), 0, s, g);
+  else
+    hipLaunchKernelGGL((gate_backward_kernel<T, 1>), gate_grid(g), dim3(64, 4), 0, s, g);
 }
 
 static bool whole(const void* p, int64_t ld, int64_t n, int es) {
@@ -139,13 +142,12 @@ extern "C" int trnblas_hip_gate(int act, int dtype, int out_dtype, int64_t rows,
   g.rows = rows, g.n = (int)N, g.act = act;
   g.vec = N % kGateV == 0 && whole(P, ldp, N, es) && whole(H, ldh, N, eo) && whole(S, lds, N, eo);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid = gate_grid(g), block(64, 4);
   switch (dtype == TRNBLAS_F32 ? 3 + out_dtype : dtype) {
-    case TRNBLAS_BF16: hipLaunchKernelGGL((gate_kernel<__bf16, __bf16>), grid, block, 0, s, g); break;
-    case TRNBLAS_F16: hipLaunchKernelGGL((gate_kernel<_Float16, _Float16>), grid, block, 0, s, g); break;
-    case 3 + TRNBLAS_BF16: hipLaunchKernelGGL((gate_kernel<float, __bf16>), grid, block, 0, s, g); break;
-    case 3 + TRNBLAS_F16: hipLaunchKernelGGL((gate_kernel<float, _Float16>), grid, block, 0, s, g); break;
-    default: hipLaunchKernelGGL((gate_kernel<float, float>), grid, block, 0, s, g); break;
+    case TRNBLAS_BF16: launch_gate<__bf16, __bf16>(g, s); break;
+    case TRNBLAS_F16: launch_gate<_Float16, _Float16>(g, s); break;
+    case 3 + TRNBLAS_BF16: launch_gate<float, __bf16>(g, s); break;
+    case 3 + TRNBLAS_F16: launch_gate<float, _Float16>(g, s); break;
+    default: launch_gate<float, float>(g, s); break;
   }
   return check_launch(kGate);
 }
@@ -162,11 +164,10 @@ extern "C" int trnblas_hip_gate_backward(int act, int dtype, int64_t rows, int64
   g.rows = rows, g.n = (int)N, g.act = act;
   g.vec = N % kGateV == 0 && whole(P, ldp, N, es) && whole(dH, ldg, N, es) && whole(dP, ldd, N, es);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid = gate_grid(g), block(64, 4);
   switch (dtype) {
-    case TRNBLAS_F32: hipLaunchKernelGGL(gate_backward_kernel<float>, grid, block, 0, s, g); break;
-    case TRNBLAS_BF16: hipLaunchKernelGGL(gate_backward_kernel<__bf16>, grid, block, 0, s, g); break;
-    default: hipLaunchKernelGGL(gate_backward_kernel<_Float16>, grid, block, 0, s, g); break;
+    case TRNBLAS_F32: launch_gate_backward<float>(g, s); break;
+    case TRNBLAS_BF16: launch_gate_backward<__bf16>(g, s); break;
+    default: launch_gate_backward<_Float16>(g, s); break;
   }
   return check_launch(kGateBackward);
 }

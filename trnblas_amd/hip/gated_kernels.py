@@ -16,14 +16,23 @@ from .kernels import _batched_layout, _pack_k, _probed_call, _require_device
 ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}  # TRNBLAS_ACT_*
 
 
+def _call(kernel: str, dev: int, *args) -> None:
+    """The C entry of `kernel` on `dev`'s current stream: the short way where `dev` is the current device and nothing is probed."""
+    name = "trnblas_hip_" + kernel
+    if dev == _grouped._current_device() and _kernels._launch_probe is None:
+        _checked(name, _fn(name)(*args, _grouped._raw_stream(dev)))
+    else:
+        _probed_call(kernel, name, *args, stream_of(torch.device("cuda", dev)))
+
+
 def gate(P: torch.Tensor, act: str, out_dtype: torch.dtype, save: bool):
-    """(H, S): act(P[:, :N]) * P[:, N:] in out_dtype, and where `save` says so P in that type."""
+    """(H, S): act(P[:, :N]) * P[:, N:] in out_dtype, and where `save` says so P (contiguous) in that type."""
     R, N = P.shape[0], P.shape[1] // 2
-    H = torch.empty((R, N), dtype=out_dtype, device=P.device)
-    S = torch.empty((R, 2 * N), dtype=out_dtype, device=P.device) if save and out_dtype != P.dtype else None
-    _probed_call(
-        "gate", "trnblas_hip_gate", ACTS[act], _lib.DTYPE_CODES[P.dtype], _lib.DTYPE_CODES[out_dtype], R, N, ptr(P),
-        max(2 * N, 1), ptr(H), max(N, 1), ptr(S), max(2 * N, 1), stream_of(P.device),
+    H = P.new_empty((R, N), dtype=out_dtype)
+    S = P.new_empty((R, 2 * N), dtype=out_dtype) if save and out_dtype != P.dtype else None
+    _call(
+        "gate", P.get_device(), ACTS[act], _lib.DTYPE_CODES[P.dtype], _lib.DTYPE_CODES[out_dtype], R, N, P.data_ptr(),
+        max(2 * N, 1), H.data_ptr(), max(N, 1), ptr(S), max(2 * N, 1),
     )  # fmt: skip
     return H, (P if S is None else S) if save else None
 
@@ -31,11 +40,13 @@ def gate(P: torch.Tensor, act: str, out_dtype: torch.dtype, save: bool):
 def gate_backward(P: torch.Tensor, dH: torch.Tensor, act: str) -> torch.Tensor:
     """dP of H = act(P[:, :N]) * P[:, N:] for the gradient dH of H (P's type)."""
     R, N = dH.shape
-    dH, ldg = row_major(dH.resolve_neg())
-    D = torch.empty_like(P)
-    _probed_call(
-        "gate_backward", "trnblas_hip_gate_backward", ACTS[act], _lib.DTYPE_CODES[P.dtype], R, N, ptr(P), max(2 * N, 1),
-        ptr(dH), max(ldg, N), ptr(D), max(2 * N, 1), stream_of(P.device),
+    ldg = N
+    if dH.stride() != (N, 1) or dH.is_neg():
+        dH, ldg = row_major(dH.resolve_neg())
+    D = P.new_empty((R, 2 * N))
+    _call(
+        "gate_backward", P.get_device(), ACTS[act], _lib.DTYPE_CODES[P.dtype], R, N, P.data_ptr(), max(2 * N, 1), dH.data_ptr(),
+        max(ldg, N), D.data_ptr(), max(2 * N, 1),
     )  # fmt: skip
     return D
 
@@ -83,12 +94,14 @@ def gated_gemm(A: torch.Tensor, B: torch.Tensor, offsets, act: str, out_dtype: t
 
 
 def gated_gemm_fast(A, B, offsets, act, transB, out_dtype, save=False):
-    """The common calls without the general path's checks, one by one, as in `grouped_kernels.py` (15 us on the host, these 9): B as
-    given (without offsets 2-D or a stack of one), aligned. None where anything is out of the ordinary; (H, P) where `save` says so, else H."""
-    code, act = _lib.DTYPE_CODES.get(A.dtype), ACTS.get(act)
-    if code is None or act is None or B.dtype is not A.dtype or _kernels._launch_probe is not None or A.dim() != 2:
+    """The common calls without the general path's checks, one by one, as in `grouped_kernels.py` (15 us on the host, these 9; two
+    launches 29 and 16): B as given (without offsets 2-D or a stack of one). None where anything is out of the ordinary; (H, P)
+    where `save` says so, else H."""
+    code, a = _lib.DTYPE_CODES.get(A.dtype), ACTS.get(act)
+    if code is None or a is None or B.dtype is not A.dtype or _kernels._launch_probe is not None or A.dim() != 2:
         return None
-    if (out_dtype is not None and out_dtype is not A.dtype) or (B.dim() != 3 and (B.dim() != 2 or offsets is not None)):
+    same = out_dtype is None or out_dtype is A.dtype
+    if (not same and out_dtype is not torch.float32) or (B.dim() != 3 and (B.dim() != 2 or offsets is not None)):
         return None
     R, K = A.shape
     lda, s1 = A.stride()
@@ -112,14 +125,21 @@ def gated_gemm_fast(A, B, offsets, act, transB, out_dtype, save=False):
     su = N * t0 if transB else N
     if (
         k != K or n2 % 2 or s1 != 1 or lda < K or t1 != 1 or t0 < b1 or N == 0 or dev != _grouped._current_device()
-        or B.get_device() != dev or A.is_neg() or B.is_neg() or (pa | pb) % 16
-        or (lda | t0 | sb | su | K | b1) % (4 if code == 0 else 8)
+        or B.get_device() != dev or A.is_neg() or B.is_neg()
     ):  # fmt: skip
         return None
+    if not same or (pa | pb) % 16 or (lda | t0 | sb | su | K | b1) % (4 if code == 0 else 8):
+        if same and R * K * n2 >= _PACK_MACS:
+            return None
+        P = _grouped.grouped_gemm_fast(1.0, A, B if B.dim() == 3 else B.unsqueeze(0), offsets, transB, torch.float32)
+        if P is None:
+            return None
+        HP = gate(P, act, out_dtype or A.dtype, save)
+        return HP if save else HP[0]
     H = A.new_empty((R, N))
     P = A.new_empty((R, n2)) if save else None
     rc = _fn("trnblas_hip_gated_gemm")(
-        act, code, transB, G, R, N, K, pa, lda, pb, t0, sb, su, o, o64, H.data_ptr(), N, P.data_ptr() if save else None, n2, 0,
+        a, code, transB, G, R, N, K, pa, lda, pb, t0, sb, su, o, o64, H.data_ptr(), N, P.data_ptr() if save else None, n2, 0,
         _grouped._raw_stream(dev),
     )  # fmt: skip
     _checked("trnblas_hip_gated_gemm", rc)
