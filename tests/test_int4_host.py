@@ -190,7 +190,7 @@ def test_c_abi_refusals():
 
     for bad, word in ((dict(dtype=3), b"dtype"), (dict(out=3), b"result dtype"), (dict(gated=1, act=5), b"activation"),
                       (dict(gated=1, alpha=2.0), b"alpha"), (dict(gated=1, beta=1.0, c=4096), b"beta"), (dict(group=48), b"group"),
-                      (dict(n=1 << 31), b"sizes"), (dict(groups=2), b"offsets"), (dict(off=4098), b"offsets"), (dict(beta=1.0), b"without C"),
+                      (dict(n=1 << 31), b"sizes"), (dict(k=(1 << 22) + 1, sr=1 << 23), b"sizes"), (dict(groups=2), b"offsets"), (dict(off=4098), b"offsets"), (dict(beta=1.0), b"without C"),
                       (dict(sk=-1), b"stride"), (dict(ldd=7), b"leading"), (dict(a=None), b"null"), (dict(codes=8), b"aligned")):  # fmt: skip
         assert gemm(**bad) == _lib.E_ARG and word in lib.trnblas_hip_last_error(), bad
     # rows that are not read in place need a workspace

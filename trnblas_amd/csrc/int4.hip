@@ -436,9 +436,9 @@ extern "C" int trnblas_hip_int4_gemm(int dtype, int out_dtype, int gated, int ac
   TRNBLAS_CHECK_ARG(!gated || (act >= TRNBLAS_ACT_SILU && act <= TRNBLAS_ACT_SIGMOID && alpha == 1.0 && beta == 0.0),
                     "%s: bad activation %d (and alpha 1, beta 0 with one)", kGemm, act);
   if (int rc = check_int4(kGemm, N, K, group, scale_dtype, 0)) return rc;
-  // K: two row blocks' codes lie within 32-bit offsets
+  // K: a tile's rows, and two row blocks' codes, lie within 32-bit offsets
   TRNBLAS_CHECK_ARG(groups >= 0 && groups < (1 << 24) && rows >= 0 && rows < INT32_MAX - 1024 && N < (INT32_MAX >> 1) - 1024 &&
-                        K < 1 << 24,
+                        K <= kInt4Far,
                     "%s: bad sizes (groups %lld, rows %lld, N %lld, K %lld)", kGemm, (long long)groups, (long long)rows, (long long)N,
                     (long long)K);
   TRNBLAS_CHECK_ARG(offsets != nullptr ? (uintptr_t)offsets % (offsets64 ? 8 : 4) == 0 : groups == 1,

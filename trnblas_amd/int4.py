@@ -328,7 +328,7 @@ def int4_gemm(
 ) -> torch.Tensor:
     """alpha * A @ B^T + beta * C for A (M, K) and an Int4Matrix B (N, K).
 
-    The result (M, N) has `dtype` (float32, bfloat16 or float16), A's by default.
+    The result (M, N) has `dtype` (float32, bfloat16 or float16), A's by default. K is at most 2^22 on a GPU.
     """
     return _product("int4_gemm", alpha, A, B, None, beta, C, dtype)
 
