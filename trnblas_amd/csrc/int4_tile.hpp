@@ -33,8 +33,8 @@ struct Int4Stage {
 // waves of all rows by 32 columns, so that each code becomes an operand once. All operands come by LDS DMA, chunk c + 2 behind the barrier that says that
 // every wave has read chunk c - 1 and that c has landed. A group's sums are in one set of registers, those of all
 // groups in another. What bounds it is the vector unit: a matrix instruction of 16 cycles keeps it out for 8 of them, and
-// eight values of codes take 13 instructions (fp16: 11) of 4 cycles, a group's 64 sums of a lane one each. (Waves of 64 x
-// 64, which make each operand twice: 2048 rows by 8192^2 286 us.)
+// eight values of codes take 13 instructions (fp16: 11) of 4 cycles, a group's 64 sums of a lane one each: 2048 rows by
+// 8192^2 in groups of 128 237 us, 1.16 PFLOP/s. (Waves of 64 x 64, which make each operand twice: 286.)
 // pieces: K is walked so many times, each time with another piece of A. q.splits > 1: the grid's y takes so many parts
 // of that walk; their sums go to q.partial (g.rows rows of q.ldp values each), for int4_join_kernel.
 template <typename T, int FM, int WAVES, int STEPS, bool ZERO, bool SF16, bool GATED>

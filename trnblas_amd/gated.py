@@ -17,7 +17,10 @@ the result's type, the backward pass forms
     dP = [dH * U * act'(G) | dH * act(G)]     dA = dP op(B)^T     dB = A^T dP
 
 with dP in that type too (the operand type of its products; an fp32 result's is
-fp32, and its products are). Second derivatives and forward-mode tangents go through a
+fp32, and its products are). With 16-bit operands that rounds P and dP besides the gradients: bf16
+ones come out 0.0030 of their norm from the 64-bit ones, one rounding alone leaves 0.0017. (P in fp32
+would leave 0.0024 for twice its memory; dP as two pieces doubles the work of both products.) Where
+that matters, `dtype=torch.float32` keeps both in fp32. Second derivatives and forward-mode tangents go through a
 product in fp32 and elementary operations.
 """
 
