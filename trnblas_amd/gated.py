@@ -118,6 +118,9 @@ class _GatedGemm(torch.autograd.Function):
     def backward(ctx, dH):
         A, b, offsets, P = ctx.saved_tensors
         if torch.is_grad_enabled() or _d._has_tangent(dH):  # a derivative of this one may be asked for
+            # by views of their own: where one operand depends on the other, the gradient to it ends at
+            # the operand, and what leads on from there is counted by whoever asked
+            A, b = A.view_as(A), b.view_as(b)
             H = _composed(A, b, offsets, ctx.act, ctx.out)
             wanted = [x for x, need in zip((A, b), ctx.needs_input_grad) if need]
             grads = iter(torch.autograd.grad(H, wanted, dH, create_graph=True))
