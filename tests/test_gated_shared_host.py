@@ -91,3 +91,20 @@ def test_gradient_penalty_of_one_operand():
         of = [t for t in (x, w) if torch.autograd.grad(plain.sum(), t, retain_graph=True, allow_unused=True)[0] is not None]
         got, want = (torch.autograd.grad(torch.autograd.grad(h.square().sum(), of, create_graph=True)[0].square().sum(), of) for h in (own, plain))
         assert torch.allclose(got[0], want[0], rtol=1e-10, atol=1e-10)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu", "sigmoid"])
+def test_tangent_of_the_result_s_gradient(act):
+    # without create_graph: the gradients are linear in it, and so are their tangents
+    from torch.autograd import forward_ad as fwd
+
+    dH, t = _random(7, 6, seed=3), _random(7, 6, seed=4)
+    x, e = X.clone().requires_grad_(), E.clone().requires_grad_()
+    for a, b in ((x, e), (x, E), (X, e)):
+        of = [leaf for leaf in (a, b) if leaf.requires_grad]
+        h = tb.grouped_gated_gemm(a, b, OFF, act)
+        want = torch.autograd.grad(h, of, dH, retain_graph=True), torch.autograd.grad(h, of, t, retain_graph=True)
+        with fwd.dual_level():
+            got = [fwd.unpack_dual(g) for g in torch.autograd.grad(h, of, fwd.make_dual(dH, t))]
+        for g, value, tangent in zip(got, *want):
+            assert torch.equal(g.primal, value) and torch.equal(g.tangent, tangent)

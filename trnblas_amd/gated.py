@@ -116,15 +116,27 @@ class _GatedGemm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dH):
-        A, b, offsets, P = ctx.saved_tensors
-        if torch.is_grad_enabled() or _d._has_tangent(dH):  # a derivative of this one may be asked for
+        if torch.is_grad_enabled():  # a derivative of this one may be asked for
             # by views of their own: where one operand depends on the other, the gradient to it ends at
             # the operand, and what leads on from there is counted by whoever asked
+            A, b, offsets, _ = ctx.saved_tensors
             A, b = A.view_as(A), b.view_as(b)
             H = _composed(A, b, offsets, ctx.act, ctx.out)
             wanted = [x for x, need in zip((A, b), ctx.needs_input_grad) if need]
             grads = iter(torch.autograd.grad(H, wanted, dH, create_graph=True))
             return *(next(grads) if need else None for need in ctx.needs_input_grad[:2]), None, None, None
+        if _d._has_tangent(dH):  # the gradients are linear in it
+            dH, t = _fwd.unpack_dual(dH)
+            both = zip(_GatedGemm._gradients(ctx, dH), _GatedGemm._gradients(ctx, t))
+            dA, dB = (None if g is None else _fwd.make_dual(g, tangent) for g, tangent in both)
+        else:
+            dA, dB = _GatedGemm._gradients(ctx, dH)
+        return dA, dB, None, None, None
+
+    @staticmethod
+    def _gradients(ctx, dH):
+        """(dA, dB), None what no gradient is asked for."""
+        A, b, offsets, P = ctx.saved_tensors
         dP, dt = _backward(P, dH, ctx.act), A.dtype
         if dP.dtype != dt:
             dP, A, b = _widened(dP, A, b)
@@ -138,7 +150,7 @@ class _GatedGemm(torch.autograd.Function):
                 dB = _rank_k(1.0, A, dP, offsets, 0.0, None, A.dtype)
         if A.dtype != dt:
             dA, dB = _narrowed(dt, dA, dB)
-        return dA, dB, None, None, None
+        return dA, dB
 
 
 def _fast(A, B, offsets, activation, transB, dtype):
