@@ -737,7 +737,8 @@ int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, in
  * g * strideB (K x N, or N x K for transB != 0; leading dimension ldb) and the ups strideU
  * elements after them. groups, offsets, dtype and padded as in
  * trnblas_hip_grouped_gemm; rows of no group come out as act(0) * 0. P: null, or the sums
- * [A G | A U] (rows x 2 N), as gate_backward takes them. H and P have the type of A and B.
+ * [A G | A U] (rows x 2 N), as gate_backward takes them: fp32, with bf16 operands bf16. H has the type
+ * of A and B.
  * A, B, lda, ldb, both strides and K (N where B is N-contiguous) are multiples of 16 bytes,
  * but for extents of padded operands: other calls are errors (use grouped_gemm into fp32,
  * and gate, there and for fp32 results of 16-bit operands).
@@ -752,7 +753,8 @@ int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, in
  * out_dtype (rows x 2 N).
  *
  * gate_backward: for the gradient dH (rows x N) of H, dP[:, :N] = dH * U * act'(G) and
- * dP[:, N:] = dH * act(G), P = [G | U]; all of type `dtype`. dP may be P itself.
+ * dP[:, N:] = dH * act(G), P = [G | U]; dH and dP have the type `dtype`, P is fp32, for bf16 ones
+ * bf16. A dP of P's type may be P itself.
  */
 int trnblas_hip_gated_gemm(int act, int dtype, int transB, int64_t groups, int64_t rows,
                            int64_t N, int64_t K, const void* A, int64_t lda,

@@ -11,13 +11,13 @@ static const char* const kGate = "trnblas_hip_gate";
 static const char* const kGateBackward = "trnblas_hip_gate_backward";
 
 struct GateArgs {
-  const void* P;  // rows x 2 n: gates, then ups
+  const void* P;  // rows x 2 n: gates, then ups; GateSums (backward)
   int64_t ldp;
   const void* dH;  // backward
   int64_t ldg;
   void* D;  // H, or dP (backward)
   int64_t ldd;
-  void* S;  // P in D's type, or null
+  void* S;  // P in D's type, or null (forward)
   int64_t lds;
   int64_t rows;
   int n, act;
@@ -65,13 +65,13 @@ __global__ __launch_bounds__(256) void gate_kernel(GateArgs g) {
   }
 }
 
-// dG = dH * U * act'(G), dU = dH * act(G).
+// dG = dH * U * act'(G), dU = dH * act(G), rounded once, to dH's type.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gate_backward_kernel(GateArgs g) {
   const int c = V * (blockIdx.x * 64 + threadIdx.x);
   if (c >= g.n) return;
   for (int64_t r = blockIdx.y * 4 + threadIdx.y; r < g.rows; r += 4 * gridDim.y) {
-    const T* p = static_cast<const T*>(g.P) + r * g.ldp + c;
+    const GateSums<T>* p = static_cast<const GateSums<T>*>(g.P) + r * g.ldp + c;
     float a[V], u[V], d[V];
     load_values<V>(p, a);
     load_values<V>(p + g.n, u);
@@ -162,7 +162,7 @@ extern "C" int trnblas_hip_gate_backward(int act, int dtype, int64_t rows, int64
   GateArgs g{};
   g.P = P, g.ldp = ldp, g.dH = dH, g.ldg = ldg, g.D = dP, g.ldd = ldd;
   g.rows = rows, g.n = (int)N, g.act = act;
-  g.vec = N % kGateV == 0 && whole(P, ldp, N, es) && whole(dH, ldg, N, es) && whole(dP, ldd, N, es);
+  g.vec = N % kGateV == 0 && whole(P, ldp, N, dtype == TRNBLAS_BF16 ? 2 : 4) && whole(dH, ldg, N, es) && whole(dP, ldd, N, es);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case TRNBLAS_F32: launch_gate_backward<float>(g, s); break;
@@ -196,9 +196,9 @@ extern "C" int trnblas_hip_gated_gemm(int act, int dtype, int transB, int64_t gr
   g.act = act;
   g.out32 = dtype == TRNBLAS_F32;
   g.padded = padded != 0;
-  const int64_t eo = g.out32 ? 4 : 2;
+  const int64_t eo = g.out32 ? 4 : 2, ep = dtype == TRNBLAS_BF16 ? 2 : 4;
   g.vec4 = (uintptr_t)H % (4 * eo) == 0 && ldh % 4 == 0 &&
-           (P == nullptr || ((uintptr_t)P % (4 * eo) == 0 && ldp % 4 == 0 && N % 4 == 0));
+           (P == nullptr || ((uintptr_t)P % (4 * ep) == 0 && ldp % 4 == 0 && N % 4 == 0));
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case TRNBLAS_F32: return gated_gemm_run<float>(g, transB != 0, s);

@@ -34,7 +34,7 @@ struct GroupedArgs {
   int vec4;   // D and C take 4-element accesses (aligned, ld % 4 == 0)
   // gated projections: B holds the gates' columns (g.N of them), the ups' stand sU elements further on
   int64_t sU;
-  void* P;  // sums of both as [gates | ups] in D's type, or null
+  void* P;  // sums of both as [gates | ups], bf16 with bf16 operands, else fp32, or null
   int64_t ldp;
   int act;
 };

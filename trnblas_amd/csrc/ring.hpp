@@ -193,9 +193,9 @@ __device__ __forceinline__ void store_gated(const GroupedArgs& g, TileJob j, f32
     p.ldd = g.ldp;
     void* h = j.D;
     j.D = g.P;
-    store_wave<FM, FH, O, false>(p, j, acc[0], m0, n0, lane, lds);
-    j.D = static_cast<O*>(g.P) + g.N;
-    store_wave<FM, FH, O, false>(p, j, acc[1], m0, n0, lane, lds);
+    store_wave<FM, FH, GateSums<O>, false>(p, j, acc[0], m0, n0, lane, lds);
+    j.D = static_cast<GateSums<O>*>(g.P) + g.N;
+    store_wave<FM, FH, GateSums<O>, false>(p, j, acc[1], m0, n0, lane, lds);
     j.D = h;
   }
   // one kind of activation at a time: a switch in each value's path costs registers and branches

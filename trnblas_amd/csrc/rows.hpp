@@ -108,8 +108,8 @@ __device__ __forceinline__ void store_gated_quad(const GroupedArgs& g, int64_t m
   if (g.P) {
     GroupedArgs p = g;
     p.ldd = g.ldp;
-    store_quad<O>(p, nullptr, static_cast<O*>(g.P), m, n, gates);
-    store_quad<O>(p, nullptr, static_cast<O*>(g.P) + g.N, m, n, ups);
+    store_quad<GateSums<O>>(p, nullptr, static_cast<GateSums<O>*>(g.P), m, n, gates);
+    store_quad<GateSums<O>>(p, nullptr, static_cast<GateSums<O>*>(g.P) + g.N, m, n, ups);
   }
   f32x4 h;
 #pragma unroll

@@ -11,17 +11,17 @@ operands as in `gemm` and `grouped_gemm`. Activations: "silu", "gelu" (by erf),
     H = grouped_gated_gemm(x, E, offsets)               # rows sorted by expert, E (G, K, 2 N)
     H = gated_gemm(x, int4_quantize(W))                 # served from 4-bit weights
 
-Differentiable: where a gradient is asked for, the forward pass keeps P = [A G | A U] in
-the result's type, the backward pass forms
+Differentiable: where a gradient is asked for, the forward pass keeps P = [A G | A U], the backward pass forms
 
     dP = [dH * U * act'(G) | dH * act(G)]     dA = dP op(B)^T     dB = A^T dP
 
-with dP in that type too (the operand type of its products; an fp32 result's is
-fp32, and its products are). With 16-bit operands that rounds P and dP besides the gradients: bf16
-ones come out 0.0030 of their norm from the 64-bit ones, one rounding alone leaves 0.0017. (P in fp32
-would leave 0.0024 for twice its memory; dP as two pieces doubles the work of both products.) Where
-that matters, `dtype=torch.float32` keeps both in fp32. Second derivatives and forward-mode tangents go through a
-product in fp32 and elementary operations.
+with dP in the result's type (the operand type of its products; an fp32 result's is
+fp32, and its products are). P is kept in fp32, but for bf16 results, whose type has its range, in bf16: in fp16 a gate below
+-65504 would be infinite and its gradients NaN. 16-bit gradients come out further from the 64-bit ones than one rounding
+leaves them: fp16 0.00029 of their norm (0.00021), by dP's rounding, bf16 0.0030 (0.0017), by P's too. (An fp32 P
+would leave 0.0024 for twice its memory and 1.15 times the step's time at 8192 rows, 2048 by 2 x 4096; dP as two pieces doubles the
+work of both products.) Where that matters, `dtype=torch.float32` keeps both in fp32. Second derivatives and
+forward-mode tangents go through a product in fp32 and elementary operations.
 """
 
 from __future__ import annotations
@@ -77,7 +77,7 @@ def _composed(A, b, offsets, act, out):
 
 
 def _forward(A, b, offsets, act, out, save):
-    """(H, P in H's type where `save` says so)."""
+    """(H, P as `_backward` takes it where `save` says so)."""
     if _d._grouped_on_hip("gated_gemm", A, b):
         try:
             if save:
@@ -90,12 +90,13 @@ def _forward(A, b, offsets, act, out, save):
             _d._kernel_failed(exc)
     wide = torch.promote_types(A.dtype, torch.float32)
     P = _d.grouped_gemm(1.0, A, b, offsets, 0.0, None, wide)
-    return _gate_torch(P, act).to(out), P.to(out) if save else None
+    # bf16 has fp32's range, fp16 does not: see GateSums in csrc/gate.hpp
+    return _gate_torch(P, act).to(out), (P.to(out) if out == torch.bfloat16 else P) if save else None
 
 
 def _backward(P, dH, act):
-    """dP in P's type."""
-    if _d._grouped_on_hip("gated_gemm", P, dH):
+    """dP in dH's type."""
+    if _d._grouped_on_hip("gated_gemm", dH, P):
         try:
             return _gk().gate_backward(P, dH, act)
         except Exception as exc:  # noqa: BLE001
@@ -103,7 +104,7 @@ def _backward(P, dH, act):
     with torch.enable_grad():
         p = P.detach().to(_d._sum_dtype(P.dtype)).requires_grad_()
         (dP,) = torch.autograd.grad(_gate_torch(p, act), p, dH.to(p.dtype))
-    return dP.to(P.dtype)
+    return dP.to(dH.dtype)
 
 
 class _GatedGemm(torch.autograd.Function):

@@ -25,11 +25,16 @@ def _call(kernel: str, dev: int, *args) -> None:
         _probed_call(kernel, name, *args, stream_of(torch.device("cuda", dev)))
 
 
+def sums_dtype(out_dtype: torch.dtype) -> torch.dtype:
+    """The type of the sums P that a gradient is taken from, for results of out_dtype: fp16 ends where P does not (`GateSums`, csrc/gate.hpp)."""
+    return torch.bfloat16 if out_dtype is torch.bfloat16 else torch.float32
+
+
 def gate(P: torch.Tensor, act: str, out_dtype: torch.dtype, save: bool):
-    """(H, S): act(P[:, :N]) * P[:, N:] in out_dtype, and where `save` says so P (contiguous) in that type."""
+    """(H, S): act(P[:, :N]) * P[:, N:] in out_dtype, and where `save` says so P (contiguous) as gate_backward takes it."""
     R, N = P.shape[0], P.shape[1] // 2
     H = P.new_empty((R, N), dtype=out_dtype)
-    S = P.new_empty((R, 2 * N), dtype=out_dtype) if save and out_dtype != P.dtype else None
+    S = P.new_empty((R, 2 * N), dtype=sums_dtype(out_dtype)) if save and sums_dtype(out_dtype) != P.dtype else None
     _call(
         "gate", P.get_device(), ACTS[act], _lib.DTYPE_CODES[P.dtype], _lib.DTYPE_CODES[out_dtype], R, N, P.data_ptr(),
         max(2 * N, 1), H.data_ptr(), max(N, 1), ptr(S), max(2 * N, 1),
@@ -38,14 +43,14 @@ def gate(P: torch.Tensor, act: str, out_dtype: torch.dtype, save: bool):
 
 
 def gate_backward(P: torch.Tensor, dH: torch.Tensor, act: str) -> torch.Tensor:
-    """dP of H = act(P[:, :N]) * P[:, N:] for the gradient dH of H (P's type)."""
+    """dP, in dH's type, of H = act(P[:, :N]) * P[:, N:] for the gradient dH of H; P of sums_dtype."""
     R, N = dH.shape
     ldg = N
     if dH.stride() != (N, 1) or dH.is_neg():
         dH, ldg = row_major(dH.resolve_neg())
-    D = P.new_empty((R, 2 * N))
+    D = P.new_empty((R, 2 * N), dtype=dH.dtype)
     _call(
-        "gate_backward", P.get_device(), ACTS[act], _lib.DTYPE_CODES[P.dtype], R, N, P.data_ptr(), max(2 * N, 1), dH.data_ptr(),
+        "gate_backward", P.get_device(), ACTS[act], _lib.DTYPE_CODES[dH.dtype], R, N, P.data_ptr(), max(2 * N, 1), dH.data_ptr(),
         max(ldg, N), D.data_ptr(), max(2 * N, 1),
     )  # fmt: skip
     return D
@@ -58,8 +63,8 @@ _PACK_MACS = 1 << 30
 
 
 def gated_gemm(A: torch.Tensor, B: torch.Tensor, offsets, act: str, out_dtype: torch.dtype, save: bool):
-    """(H, P) for A (R, K) and B (G, K, 2 N): H = act(G) * U of P = [G | U] = A[r] @ B[g]; P (in
-    out_dtype) only where `save` says so, else None. Rows of no group are zeros."""
+    """(H, P) for A (R, K) and B (G, K, 2 N): H = act(G) * U of P = [G | U] = A[r] @ B[g]; P (sums_dtype)
+    only where `save` says so, else None. Rows of no group are zeros."""
     A, B = A.resolve_neg(), B.resolve_neg()
     dev = _require_device(A, B, offsets)
     R, K = A.shape
@@ -85,7 +90,7 @@ def gated_gemm(A: torch.Tensor, B: torch.Tensor, offsets, act: str, out_dtype: t
         padded = True
     o, o64 = offsets_of(offsets)
     H = torch.empty((R, N), dtype=out_dtype, device=dev)
-    P = torch.empty((R, 2 * N), dtype=out_dtype, device=dev) if save else None
+    P = torch.empty((R, 2 * N), dtype=sums_dtype(out_dtype), device=dev) if save else None
     _probed_call(
         "gated_gemm", "trnblas_hip_gated_gemm", ACTS[act], _lib.DTYPE_CODES[A.dtype], int(tb), G, R, N, K, ptr(a), lda, ptr(b), ldb, sb, su, ptr(o), o64, ptr(H), max(N, 1), ptr(P), max(2 * N, 1),
         int(padded), stream_of(dev),
@@ -137,7 +142,7 @@ def gated_gemm_fast(A, B, offsets, act, transB, out_dtype, save=False):
         HP = gate(P, act, out_dtype or A.dtype, save)
         return HP if save else HP[0]
     H = A.new_empty((R, N))
-    P = A.new_empty((R, n2)) if save else None
+    P = A.new_empty((R, n2), dtype=sums_dtype(A.dtype)) if save else None
     rc = _fn("trnblas_hip_gated_gemm")(
         a, code, transB, G, R, N, K, pa, lda, pb, t0, sb, su, o, o64, H.data_ptr(), N, P.data_ptr() if save else None, n2, 0,
         _grouped._raw_stream(dev),
