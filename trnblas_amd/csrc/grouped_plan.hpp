@@ -150,6 +150,7 @@ inline GroupedChoice choose_gated(int elem_bytes, double rows, double groups, do
 struct Int4Choice {
   int mf, nf, ks, tile, splits;
 };
+constexpr int kInt4Reach = 0x7ffffff0;  // bytes of scales that the tile kernel reads from one address
 
 // Times (us) fitted to sweeps of 1 .. 2048 rows over matrices of 2048 .. 8192 squared and of 130 random sizes, dense and
 // of up to 64 groups, where the choice took 1.05 times what the best of all forms did. The few-rows kernel: a workgroup
@@ -179,8 +180,8 @@ inline Int4Choice choose_int4(double rows, double groups, double N, double K, in
       }
     }
   }
-  // (gates and ups: from one to the other within 32-bit offsets of the scales)
-  const bool tiles = !gated || (std::fmod(N, 16.0) == 0.0 && N * K < 16.0 * INT32_MAX);
+  // (gates and ups: whole row blocks of each, and the ups' scales within the one buffer that starts at the gates')
+  const bool tiles = !gated || (std::fmod(N, 16.0) == 0.0 && (N / 16.0 * chunks + 1.0) * (128 / steps) <= kInt4Reach);
   for (int tile : {64, 128})
     for (int splits : {1, 2, 4, 8}) {
       const double sums = splits * rows * columns * 4.0;

@@ -69,6 +69,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void int4_tile_kernel(GroupedArgs g,
   const uint8_t* scales = reinterpret_cast<const uint8_t*>(q.scales + grp * q.groups_step + block * q.chunks * (64 / STEPS));
   const uint8_t* zeros = ZERO ? q.zeros + grp * q.groups_step + block * q.chunks * (64 / STEPS) : nullptr;
   constexpr int SP = 8 / STEPS, ZP = 4 / STEPS;  // 16-byte pieces of a block's scales, zero points
+  static_assert(kInt4Reach <= kRecords);         // (choose_int4)
   const uint32_t os = lane / SP < have ? (uint32_t)(lane / SP) * apart * q.chunks * (128 / STEPS) + 16 * (lane % SP) : kPastEnd;
   const uint32_t oz = lane / ZP < have ? (uint32_t)(lane / ZP) * apart * q.chunks * (64 / STEPS) + 16 * (lane % ZP) : kPastEnd;
   const char* corner = static_cast<const char*>(g.A) + s.row * g.lda * (int64_t)sizeof(T);
