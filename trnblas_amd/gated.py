@@ -156,7 +156,7 @@ class _GatedGemm(torch.autograd.Function):
 
 def _fast(A, B, offsets, activation, transB, dtype):
     """The short way; None: something is out of the ordinary."""
-    if type(activation) is str and type(transB) is bool and _fast_call(A, B, offsets, True):
+    if type(activation) is str and type(transB) is bool and _fast_call(A, B, offsets, True) and B.dim() == (2 if offsets is None else 3):
         try:
             return _gk().gated_gemm_fast(A, B, offsets, activation, transB, dtype)
         except _d.HipKernelError as exc:
