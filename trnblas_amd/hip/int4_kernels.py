@@ -58,8 +58,9 @@ FAR = 1 << 22  # elements between rows that are read in place (int4.hip)
 
 
 @functools.lru_cache(maxsize=4096)
-def _partial_bytes(code: int, gated: int, groups: int, R: int, N: int, K: int, group: int) -> int:
-    """Bytes of the parts' sums, by the sizes alone: trnblas_hip_int4_gemm_workspace without the rows'."""
+def _partial_bytes(dev: int, code: int, gated: int, groups: int, R: int, N: int, K: int, group: int) -> int:
+    """Bytes of the parts' sums: trnblas_hip_int4_gemm_workspace without the rows'. dev: the current device, by whose compute
+    units the plan goes."""
     total = _fn("trnblas_hip_int4_gemm_workspace")(code, gated, groups, R, N, K, group)
     return total - _rows_bytes(code, R, K) if total else 0
 
@@ -100,8 +101,8 @@ def int4_gemm(
     o, o64 = offsets_of(offsets)
     D, c = _output_like(C, beta, (R, N), out_dtype, dev)
     code, G, gated = _lib.DTYPE_CODES[A.dtype], 1 if offsets is None else codes.shape[0], int(act is not None)
-    with torch.cuda.device(dev):  # the plan goes by its compute units
-        n = _partial_bytes(code, gated, G, R, N, K, group)
+    with torch.cuda.device(dev):
+        n = _partial_bytes(dev.index, code, gated, G, R, N, K, group)
     ws = torch.empty(n + (0 if _in_place(A) else _rows_bytes(code, R, K)), dtype=torch.uint8, device=dev)
     _probed_call(
         "int4_gemm", "trnblas_hip_int4_gemm", code, _lib.DTYPE_CODES[out_dtype], gated, ACTS.get(act, 0), G, R, N, K, group, float(alpha), ptr(A), A.stride(0),
@@ -149,7 +150,7 @@ def int4_gemm_fast(alpha, A, B, offsets, out_dtype, act=None):
             return None
         o, o64 = offsets.data_ptr(), offsets.dtype is torch.int64
     D = A.new_empty((R, N), dtype=out_dtype)
-    n = _partial_bytes(code, gated, G, R, N, K, B.group)
+    n = _partial_bytes(dev, code, gated, G, R, N, K, B.group)
     ws = codes.new_empty(n) if n else None
     rc = _fn("trnblas_hip_int4_gemm")(
         code, out, gated, act or 0, G, R, N, K, B.group, alpha, pa, sr, 1, codes.data_ptr(), scales.data_ptr(),
