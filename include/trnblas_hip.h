@@ -740,8 +740,9 @@ int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, in
  * [A G | A U] (rows x 2 N), as gate_backward takes them: fp32, with bf16 operands bf16. H has the type
  * of A and B.
  * A, B, lda, ldb, both strides and K (N where B is N-contiguous) are multiples of 16 bytes,
- * but for extents of padded operands: other calls are errors (use grouped_gemm into fp32,
- * and gate, there and for fp32 results of 16-bit operands).
+ * but for extents of padded operands, and 256 rows of A and of a K-contiguous B, 128 bytes of k of
+ * another, span less than 2^31 - 1024 bytes: other calls are errors (use grouped_gemm into
+ * fp32, and gate, there and for fp32 results of 16-bit operands).
  *
  * gated_plan: the name of the kernel that such a call runs on (for rows_kernel: rows of a
  * tile, waves along K), or NULL with the last error set. Launches nothing.

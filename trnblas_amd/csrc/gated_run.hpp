@@ -58,7 +58,7 @@ static int run_gated(const GroupedArgs& g, hipStream_t s) {
 template <typename T>
 int gated_gemm_run(const GroupedArgs& g, bool bkc, hipStream_t s) {
   TRNBLAS_CHECK_ARG(bkc ? gated_ready<T>(g, true) : gated_ready<T>(g, false),
-                    "%s: operands must start and continue on 16 bytes (or be padded)", kGated);
+                    "%s: operands must start and continue on 16 bytes (or be padded), a tile's rows within 2^31 bytes", kGated);
   return bkc ? run_gated<T, true>(g, s) : run_gated<T, false>(g, s);
 }
 

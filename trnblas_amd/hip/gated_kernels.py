@@ -60,6 +60,13 @@ def gate_backward(P: torch.Tensor, dH: torch.Tensor, act: str) -> torch.Tensor:
 # Operands that the fused kernels cannot read in place are copied first, rows padded with zeros, from so many
 # multiply-adds on; below it the product goes to fp32 by `grouped_gemm`'s kernels, and the gate is a launch of its own.
 _PACK_MACS = 1 << 30
+# So do operands whose rows lie too far apart: a tile's rows (128 bytes of k, of a B whose columns are contiguous) have 32-bit
+# offsets (dma_ready, csrc/grouped_run.hpp). The last tokens of sequences, x[:, -1] of (batch, tokens, width), are such rows.
+_REACH = (1 << 31) - 1025
+
+
+def _far(lda: int, ldb: int, kc: bool, es: int) -> bool:
+    return 256 * lda * es >= _REACH or (256 * es if kc else 128) * ldb >= _REACH
 
 
 def gated_gemm(A: torch.Tensor, B: torch.Tensor, offsets, act: str, out_dtype: torch.dtype, save: bool):
@@ -74,12 +81,16 @@ def gated_gemm(A: torch.Tensor, B: torch.Tensor, offsets, act: str, out_dtype: t
     a, lda = row_major(A)
     b, tb, ldb, sb = _batched_layout(B)
     su = N * ldb if tb else N
-    a_ok = _ready(a.data_ptr(), lda, 0, K, ev)
-    b_ok = _ready(b.data_ptr(), ldb, sb, K if tb else N, ev) and su % ev == 0
-    if out_dtype != A.dtype or (not (a_ok and b_ok) and 2 * R * K * N < _PACK_MACS):
+    if R == 1:
+        lda = max(K, 1)
+    ka, kb = _up(K, ev), _up(K, ev) if tb else 2 * _up(N, ev)  # leading dimensions of copies
+    a_ok = _ready(a.data_ptr(), lda, 0, K, ev) and not _far(lda, 0, tb, es)
+    b_ok = _ready(b.data_ptr(), ldb, sb, K if tb else N, ev) and su % ev == 0 and not _far(0, ldb, tb, es)
+    beyond = (not a_ok and _far(ka, 0, tb, es)) or (not b_ok and _far(0, kb, tb, es))
+    if out_dtype != A.dtype or beyond or (not (a_ok and b_ok) and 2 * R * K * N < _PACK_MACS):
         return gate(grouped_gemm(A, B, offsets, out_dtype=torch.float32), act, out_dtype, save)
     if not a_ok:
-        a, lda, padded = _pack_k(A, _up(K, ev)), _up(K, ev), True
+        a, lda, padded = _pack_k(A, ka), ka, True
     if not b_ok:
         if tb:
             b = _pack_k(B.mT, _up(K, ev))
@@ -128,12 +139,14 @@ def gated_gemm_fast(A, B, offsets, act, transB, out_dtype, save=False):
     N = n2 // 2
     pa, pb = A.data_ptr(), B.data_ptr()
     su = N * t0 if transB else N
+    if R == 1:
+        lda = K
     if (
         k != K or n2 % 2 or s1 != 1 or lda < K or t1 != 1 or t0 < b1 or N == 0 or dev != _grouped._current_device()
         or B.get_device() != dev or A.is_neg() or B.is_neg()
     ):  # fmt: skip
         return None
-    if not same or (pa | pb) % 16 or (lda | t0 | sb | su | K | b1) % (4 if code == 0 else 8):
+    if not same or (pa | pb) % 16 or (lda | t0 | sb | su | K | b1) % (4 if code == 0 else 8) or _far(lda, t0, transB, 4 if code == 0 else 2):
         if same and R * K * n2 >= _PACK_MACS:
             return None
         P = _grouped.grouped_gemm_fast(1.0, A, B if B.dim() == 3 else B.unsqueeze(0), offsets, transB, torch.float32)
