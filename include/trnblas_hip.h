@@ -705,7 +705,8 @@ int trnblas_hip_int4_dequantize(int dtype, int scale_dtype, int64_t R, int64_t K
  * N rows, gates first (alpha 1, beta 0). A is rows x K values of `dtype` (fp32, bf16 or fp16), element
  * (r, k) at r * sr + k * sk; C and D (rows x N) have the type out_dtype. Weights enter as they
  * are: products of q - z and A are exact, their fp32 sums over a group enter the fp32 sum
- * times the scale. K is at most 2^22. offsets as in trnblas_hip_grouped_gemm. workspace: as many bytes as int4_gemm_workspace says,
+ * times the scale. (Those of |A| up to 2^116 are finite whatever the weights: 128 * 255 / 16 * 2^116 < 2^128.)
+ * Scales are finite, or NaN. K is at most 2^22. offsets as in trnblas_hip_grouped_gemm. workspace: as many bytes as int4_gemm_workspace says,
  * 16-byte aligned, not shared by calls that can overlap (it holds the rows as the kernels read them, but for
  * bf16 and fp16 rows that start on 16 bytes, no more than 2^22 values apart, K a multiple of 8, sk 1; and the
  * sums of parts of K, which those need too).

@@ -95,7 +95,7 @@ class Int4Matrix:
     @classmethod
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, K: int, group: int, zeros: torch.Tensor | None = None) -> Int4Matrix:
         """From plain rows, as checkpoints store them: codes uint8 (..., R, ceil(K / 2)), two values q to a byte, the even one
-        low; scales (..., R, ceil(K / group)); zeros (whole numbers 0 .. 255) like the scales, or None for 8."""
+        low; scales (..., R, ceil(K / group)), finite or NaN; zeros (whole numbers 0 .. 255) like the scales, or None for 8."""
         _check_group("Int4Matrix", group)
         if type(K) is not int or K < 0:
             raise ValueError(f"Int4Matrix: K must be a whole number, got {K!r}")
@@ -328,7 +328,8 @@ def int4_gemm(
 ) -> torch.Tensor:
     """alpha * A @ B^T + beta * C for A (M, K) and an Int4Matrix B (N, K).
 
-    The result (M, N) has `dtype` (float32, bfloat16 or float16), A's by default. K is at most 2^22 on a GPU.
+    The result (M, N) has `dtype` (float32, bfloat16 or float16), A's by default. K is at most 2^22 on a GPU, where
+    a group's products are summed before its scale: values of A beyond 2^116 (8e34) may make infinite sums there.
     """
     return _product("int4_gemm", alpha, A, B, None, beta, C, dtype)
 
