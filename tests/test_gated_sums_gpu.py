@@ -8,7 +8,7 @@ from test_gated_sums_host import FAR, check
 
 from oracle import gated as og
 from oracle.grouped import uneven as _uneven
-from trnblas_amd.hip import gated_kernels
+from trnblas_amd.hip import _lib, gated_kernels
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,27 @@ def test_gate_backward(dev, dtype, act):
         e = e + 2.0**-22 * (want.abs() + e)
         for got in dP:
             assert got.dtype == dtype and og.ratio(got.cpu(), want, e + og.EPS[dtype] * (want.abs() + e) + og.TINY[dtype]) <= 1, (R, N)
+
+
+@pytest.mark.parametrize("act", og.ACTS)
+@pytest.mark.parametrize("dtype, out", [(BF16, BF16), (F16, F16), (F32, BF16), (F32, F16), (F32, F32)])
+def test_gate_of_every_type(dev, dtype, out, act):
+    # the C entry, of P in 16 bits too: alone, and with P as it goes into the result's type; rows that start anywhere
+    g = torch.Generator().manual_seed(7)
+    codes = _lib.DTYPE_CODES
+    for R, N, gap in ((1, 8, 0), (130, 520, 0), (7, 61, 0), (5, 64, 3), (33, 72, 8)):
+        P = torch.full((R, 2 * N + gap), float("nan"), dtype=dtype)
+        P[:, : 2 * N] = (torch.randn(R, 2 * N, generator=g) * 3).to(dtype)
+        G, U = P[:, : 2 * N].double().chunk(2, -1)
+        want = og.gate(act, G)[0] * U
+        e = U.abs() * og.FN * (1.0 + G.abs()) + 2.0**-23 * want.abs()
+        for keep in (False, True):
+            p = P.to(dev)
+            H = torch.full((R, N + gap), 7.0, dtype=out, device=dev)
+            S = torch.full((R, 2 * N + gap), 7.0, dtype=out, device=dev)
+            stream = torch.cuda.current_stream().cuda_stream
+            _lib.call("trnblas_hip_gate", gated_kernels.ACTS[act], codes[dtype], codes[out], R, N, p.data_ptr(), 2 * N + gap, H.data_ptr(),
+                      N + gap, S.data_ptr() if keep else None, 2 * N + gap, stream)  # fmt: skip
+            assert og.ratio(H[:, :N].cpu(), want, e + og.EPS[out] * (want.abs() + e) + og.TINY[out]) <= 1, (R, N)
+            assert (H[:, N:] == 7.0).all() and (S[:, 2 * N :] == 7.0).all()
+            assert torch.equal(S[:, : 2 * N], p[:, : 2 * N].to(out)) if keep else (S == 7.0).all()
