@@ -737,9 +737,8 @@ int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, in
  * gated_gemm: H (rows x N) from A (rows x K), for the rows of group g with the gates at B +
  * g * strideB (K x N, or N x K for transB != 0; leading dimension ldb) and the ups strideU
  * elements after them. groups, offsets, dtype and padded as in
- * trnblas_hip_grouped_gemm; rows of no group come out as act(0) * 0. P: null, or the sums
- * [A G | A U] (rows x 2 N), as gate_backward takes them: fp32, with bf16 operands bf16. H has the type
- * of A and B.
+ * trnblas_hip_grouped_gemm; rows of no group come out as act(0) * 0. P: null, or the fp32 sums
+ * [A G | A U] (rows x 2 N), as gate_backward takes them. H has the type of A and B.
  * A, B, lda, ldb, both strides and K (N where B is N-contiguous) are multiples of 16 bytes,
  * but for extents of padded operands, and 256 rows of A and of a K-contiguous B, 128 bytes of k of
  * another, span less than 2^31 - 1024 bytes: other calls are errors (use grouped_gemm into
@@ -755,19 +754,19 @@ int trnblas_hip_int4_plan(int dtype, int gated, int64_t groups, int64_t rows, in
  * out_dtype (rows x 2 N).
  *
  * gate_backward: for the gradient dH (rows x N) of H, dP[:, :N] = dH * U * act'(G) and
- * dP[:, N:] = dH * act(G), P = [G | U]; dH and dP have the type `dtype`, P is fp32, for bf16 ones
- * bf16. A dP of P's type may be P itself.
+ * dP[:, N:] = dH * act(G), P = [G | U] in fp32; dH and dP have the type `dtype`. An fp32 dP may be P
+ * itself.
  */
 int trnblas_hip_gated_gemm(int act, int dtype, int transB, int64_t groups, int64_t rows,
                            int64_t N, int64_t K, const void* A, int64_t lda,
                            const void* B, int64_t ldb, int64_t strideB, int64_t strideU,
-                           const void* offsets, int offsets64, void* H, int64_t ldh, void* P,
+                           const void* offsets, int offsets64, void* H, int64_t ldh, float* P,
                            int64_t ldp, int padded, void* stream);
 const char* trnblas_hip_gated_plan(int dtype, int transB, int64_t groups, int64_t rows, int64_t N,
                                    int64_t K);
 int trnblas_hip_gate(int act, int dtype, int out_dtype, int64_t rows, int64_t N, const void* P,
                      int64_t ldp, void* H, int64_t ldh, void* S, int64_t lds, void* stream);
-int trnblas_hip_gate_backward(int act, int dtype, int64_t rows, int64_t N, const void* P,
+int trnblas_hip_gate_backward(int act, int dtype, int64_t rows, int64_t N, const float* P,
                               int64_t ldp, const void* dH, int64_t ldg, void* dP, int64_t ldd,
                               void* stream);
 

@@ -48,12 +48,12 @@ def test_gradients_of_far_sums(name, act):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16, torch.float64])
-def test_sums_are_kept_in_a_type_of_their_range(dtype):
+def test_sums_are_kept_in_32_bits_or_more(dtype):
     from trnblas_amd import gated
 
     A = torch.tensor([[1.0, 2.0**-12]], dtype=dtype)
     B = torch.tensor([[1.0, 1.0], [0.0, 1.0]], dtype=dtype)  # G = 1, U = 1 + 2^-12, which has more than 16 bits
     H, P = gated._forward(A, B[None], None, "relu", dtype, True)
-    want = torch.tensor([[1.0, 1.0 + 2.0**-12]], dtype=torch.bfloat16 if dtype == torch.bfloat16 else torch.promote_types(dtype, torch.float32))
+    want = torch.tensor([[1.0, 1.0 + 2.0**-12]], dtype=torch.promote_types(dtype, torch.float32))
     assert H.dtype == dtype and P.dtype == want.dtype and torch.equal(P, want)
     assert gated._backward(P, torch.ones(1, 1, dtype=dtype), "relu").dtype == dtype

@@ -1,18 +1,9 @@
 // The activations of gated projections and their derivatives, in fp32.
 #pragma once
 
-#include <type_traits>
-
 #include "common.hpp"
 
 namespace trnblas {
-
-// The type of the sums [G | U] that a gradient is taken from, for results of type O. fp16 ends at 65504: a gate far below
-// zero, or an up that a small gate leaves within range in H, would be infinite and the gradients 0 x infinity. bf16
-// has fp32's range and half its bytes (8192 rows, 2048 by 2 x 4096: a training step took 657 us with bf16 sums, 755
-// with fp32 ones); what their rounding costs is said in trnblas_amd/gated.py.
-template <typename O>
-using GateSums = std::conditional_t<std::is_same_v<O, __bf16>, __bf16, float>;
 
 constexpr float kLog2e = 1.44269504f, kInvSqrt2Pi = 0.39894228f, kTanhScale = 1.5957691f;  // 2 sqrt(2 / pi)
 

@@ -184,7 +184,7 @@ __device__ __forceinline__ int lane_of() {
   return lane;
 }
 
-// The outputs of a wave of gated projections: both sums to P, where it is asked for, and H.
+// The outputs of a wave of gated projections: both sums to P, in fp32, where it is asked for, and H.
 template <int FM, int FH, typename O>
 __device__ __forceinline__ void store_gated(const GroupedArgs& g, TileJob j, f32x4 (&acc)[2][FM][FH], int m0, int n0, int lane,
                                             char* lds) {
@@ -193,9 +193,9 @@ __device__ __forceinline__ void store_gated(const GroupedArgs& g, TileJob j, f32
     p.ldd = g.ldp;
     void* h = j.D;
     j.D = g.P;
-    store_wave<FM, FH, GateSums<O>, false>(p, j, acc[0], m0, n0, lane, lds);
-    j.D = static_cast<GateSums<O>*>(g.P) + g.N;
-    store_wave<FM, FH, GateSums<O>, false>(p, j, acc[1], m0, n0, lane, lds);
+    store_wave<FM, FH, float, false>(p, j, acc[0], m0, n0, lane, lds);
+    j.D = g.P + g.N;
+    store_wave<FM, FH, float, false>(p, j, acc[1], m0, n0, lane, lds);
     j.D = h;
   }
   // one kind of activation at a time: a switch in each value's path costs registers and branches

@@ -102,14 +102,14 @@ __device__ __forceinline__ void quantize_rows(const GroupedArgs& g, const MxScal
   }
 }
 
-// Four outputs of gated projections, of their sums, and the sums to P where it is asked for.
+// Four outputs of gated projections, of their sums, and the sums to P, in fp32, where it is asked for.
 template <typename O>
 __device__ __forceinline__ void store_gated_quad(const GroupedArgs& g, int64_t m, int n, const f32x4& gates, const f32x4& ups) {
   if (g.P) {
     GroupedArgs p = g;
     p.ldd = g.ldp;
-    store_quad<GateSums<O>>(p, nullptr, static_cast<GateSums<O>*>(g.P), m, n, gates);
-    store_quad<GateSums<O>>(p, nullptr, static_cast<GateSums<O>*>(g.P) + g.N, m, n, ups);
+    store_quad<float>(p, nullptr, g.P, m, n, gates);
+    store_quad<float>(p, nullptr, g.P + g.N, m, n, ups);
   }
   f32x4 h;
 #pragma unroll

@@ -16,11 +16,10 @@ Differentiable: where a gradient is asked for, the forward pass keeps P = [A G |
     dP = [dH * U * act'(G) | dH * act(G)]     dA = dP op(B)^T     dB = A^T dP
 
 with dP in the result's type (the operand type of its products; an fp32 result's is
-fp32, and its products are). P is kept in fp32, but for bf16 results, whose type has its range, in bf16: in fp16 a gate below
--65504 would be infinite and its gradients NaN. 16-bit gradients come out further from the 64-bit ones than one rounding
-leaves them: fp16 0.00029 of their norm (0.00021), by dP's rounding, bf16 0.0030 (0.0017), by P's too. (An fp32 P
-would leave 0.0024 for twice its memory and 1.15 times the step's time at 8192 rows, 2048 by 2 x 4096; dP as two pieces doubles the
-work of both products.) Where that matters, `dtype=torch.float32` keeps both in fp32. Second derivatives and
+fp32, and its products are). P is kept in fp32: in fp16 a gate below -65504 would be infinite and its gradients NaN, and in
+bf16 the gradients would be 0.0030 of their norm from the 64-bit ones. 16-bit ones come out 0.0023 (bf16) and 0.00029 (fp16)
+from them, by dP's rounding and their own, which alone leaves 0.0017 and 0.00021 (dP as two pieces would double the work of both
+products). Where that matters, `dtype=torch.float32` has dP in fp32. Second derivatives and
 forward-mode tangents go through a product in fp32 and elementary operations.
 """
 
@@ -77,7 +76,7 @@ def _composed(A, b, offsets, act, out):
 
 
 def _forward(A, b, offsets, act, out, save):
-    """(H, P as `_backward` takes it where `save` says so)."""
+    """(H, P in fp32 at least where `save` says so)."""
     if _d._grouped_on_hip("gated_gemm", A, b):
         try:
             if save:
@@ -90,8 +89,7 @@ def _forward(A, b, offsets, act, out, save):
             _d._kernel_failed(exc)
     wide = torch.promote_types(A.dtype, torch.float32)
     P = _d.grouped_gemm(1.0, A, b, offsets, 0.0, None, wide)
-    # bf16 has fp32's range, fp16 does not: see GateSums in csrc/gate.hpp
-    return _gate_torch(P, act).to(out), (P.to(out) if out == torch.bfloat16 else P) if save else None
+    return _gate_torch(P, act).to(out), P if save else None
 
 
 def _backward(P, dH, act):
@@ -102,7 +100,7 @@ def _backward(P, dH, act):
         except Exception as exc:  # noqa: BLE001
             _d._kernel_failed(exc)
     with torch.enable_grad():
-        p = P.detach().to(_d._sum_dtype(P.dtype)).requires_grad_()
+        p = P.detach().requires_grad_()
         (dP,) = torch.autograd.grad(_gate_torch(p, act), p, dH.to(p.dtype))
     return dP.to(dH.dtype)
 

@@ -25,16 +25,11 @@ def _call(kernel: str, dev: int, *args) -> None:
         _probed_call(kernel, name, *args, stream_of(torch.device("cuda", dev)))
 
 
-def sums_dtype(out_dtype: torch.dtype) -> torch.dtype:
-    """The type of the sums P that a gradient is taken from, for results of out_dtype: fp16 ends where P does not (`GateSums`, csrc/gate.hpp)."""
-    return torch.bfloat16 if out_dtype is torch.bfloat16 else torch.float32
-
-
 def gate(P: torch.Tensor, act: str, out_dtype: torch.dtype, save: bool):
-    """(H, S): act(P[:, :N]) * P[:, N:] in out_dtype, and where `save` says so P (contiguous) as gate_backward takes it."""
+    """(H, S): act(P[:, :N]) * P[:, N:] in out_dtype, and where `save` says so P (contiguous) in that type."""
     R, N = P.shape[0], P.shape[1] // 2
     H = P.new_empty((R, N), dtype=out_dtype)
-    S = P.new_empty((R, 2 * N), dtype=sums_dtype(out_dtype)) if save and sums_dtype(out_dtype) != P.dtype else None
+    S = P.new_empty((R, 2 * N), dtype=out_dtype) if save and out_dtype != P.dtype else None
     _call(
         "gate", P.get_device(), ACTS[act], _lib.DTYPE_CODES[P.dtype], _lib.DTYPE_CODES[out_dtype], R, N, P.data_ptr(),
         max(2 * N, 1), H.data_ptr(), max(N, 1), ptr(S), max(2 * N, 1),
@@ -43,7 +38,7 @@ def gate(P: torch.Tensor, act: str, out_dtype: torch.dtype, save: bool):
 
 
 def gate_backward(P: torch.Tensor, dH: torch.Tensor, act: str) -> torch.Tensor:
-    """dP, in dH's type, of H = act(P[:, :N]) * P[:, N:] for the gradient dH of H; P of sums_dtype."""
+    """dP, in dH's type, of H = act(P[:, :N]) * P[:, N:] for the gradient dH of H; P fp32."""
     R, N = dH.shape
     ldg = N
     if dH.stride() != (N, 1) or dH.is_neg():
@@ -70,7 +65,7 @@ def _far(lda: int, ldb: int, kc: bool, es: int) -> bool:
 
 
 def gated_gemm(A: torch.Tensor, B: torch.Tensor, offsets, act: str, out_dtype: torch.dtype, save: bool):
-    """(H, P) for A (R, K) and B (G, K, 2 N): H = act(G) * U of P = [G | U] = A[r] @ B[g]; P (sums_dtype)
+    """(H, P) for A (R, K) and B (G, K, 2 N): H = act(G) * U of P = [G | U] = A[r] @ B[g]; P (fp32)
     only where `save` says so, else None. Rows of no group are zeros."""
     A, B = A.resolve_neg(), B.resolve_neg()
     dev = _require_device(A, B, offsets)
@@ -88,7 +83,8 @@ def gated_gemm(A: torch.Tensor, B: torch.Tensor, offsets, act: str, out_dtype: t
     b_ok = _ready(b.data_ptr(), ldb, sb, K if tb else N, ev) and su % ev == 0 and not _far(0, ldb, tb, es)
     beyond = (not a_ok and _far(ka, 0, tb, es)) or (not b_ok and _far(0, kb, tb, es))
     if out_dtype != A.dtype or beyond or (not (a_ok and b_ok) and 2 * R * K * N < _PACK_MACS):
-        return gate(grouped_gemm(A, B, offsets, out_dtype=torch.float32), act, out_dtype, save)
+        P = grouped_gemm(A, B, offsets, out_dtype=torch.float32)
+        return gate(P, act, out_dtype, False)[0], P if save else None
     if not a_ok:
         a, lda, padded = _pack_k(A, ka), ka, True
     if not b_ok:
@@ -101,7 +97,7 @@ def gated_gemm(A: torch.Tensor, B: torch.Tensor, offsets, act: str, out_dtype: t
         padded = True
     o, o64 = offsets_of(offsets)
     H = torch.empty((R, N), dtype=out_dtype, device=dev)
-    P = torch.empty((R, 2 * N), dtype=sums_dtype(out_dtype), device=dev) if save else None
+    P = torch.empty((R, 2 * N), dtype=torch.float32, device=dev) if save else None
     _probed_call(
         "gated_gemm", "trnblas_hip_gated_gemm", ACTS[act], _lib.DTYPE_CODES[A.dtype], int(tb), G, R, N, K, ptr(a), lda, ptr(b), ldb, sb, su, ptr(o), o64, ptr(H), max(N, 1), ptr(P), max(2 * N, 1),
         int(padded), stream_of(dev),
@@ -152,10 +148,10 @@ def gated_gemm_fast(A, B, offsets, act, transB, out_dtype, save=False):
         P = _grouped.grouped_gemm_fast(1.0, A, B if B.dim() == 3 else B.unsqueeze(0), offsets, transB, torch.float32)
         if P is None:
             return None
-        HP = gate(P, act, out_dtype or A.dtype, save)
-        return HP if save else HP[0]
+        H = gate(P, act, out_dtype or A.dtype, False)[0]
+        return (H, P) if save else H
     H = A.new_empty((R, N))
-    P = A.new_empty((R, n2), dtype=sums_dtype(A.dtype)) if save else None
+    P = A.new_empty((R, n2), dtype=torch.float32) if save else None
     rc = _fn("trnblas_hip_gated_gemm")(
         a, code, transB, G, R, N, K, pa, lda, pb, t0, sb, su, o, o64, H.data_ptr(), N, P.data_ptr() if save else None, n2, 0,
         _grouped._raw_stream(dev),
