@@ -88,3 +88,10 @@ def test_the_last_tokens_of_sequences(dev):
     assert last.stride(0) > 1 << 22
     H = tb.gated_gemm(last, W.to(dev), transB=True)
     assert _holds(H, last.cpu(), W, True, BF16)
+
+
+def test_one_row_of_no_values(dev):
+    for dtype in (F32, BF16, F16):
+        for N in (16, 5):
+            H = tb.gated_gemm(torch.ones(1, 0, dtype=dtype, device=dev), torch.zeros(0, 2 * N, dtype=dtype, device=dev))
+            assert H.shape == (1, N) and not H.any()

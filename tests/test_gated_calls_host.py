@@ -90,6 +90,12 @@ class TestFarRows:
             ((name, args),) = self._call(device, dtype, (1 << 40, 1), (32, 1), False, rows=1)
             assert name == "gated_gemm" and args[8] == 64
 
+    def test_one_row_without_values(self, device):  # noqa: F811
+        # no operand to read: not the fused kernels
+        A, B, off = _Tensor((1, 0), torch.bfloat16, 0), _Tensor((1, 0, 32), torch.bfloat16, 0), _Tensor(2, torch.int32, 0)
+        assert gated_kernels.gated_gemm_fast(A, B, off, "silu", False, None) is not None
+        assert [name.removeprefix("trnblas_hip_") for name, _, _ in device["calls"]] == ["grouped_gemm", "gate"]
+
     def test_the_library_refuses_them(self):
         # so none may reach it
         if not _lib.LIB_PATH.exists():

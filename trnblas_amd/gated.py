@@ -19,7 +19,7 @@ with dP in the result's type (the operand type of its products; an fp32 result's
 fp32, and its products are). P is kept in fp32: in fp16 a gate below -65504 would be infinite and its gradients NaN, and in
 bf16 the gradients would be 0.0030 of their norm from the 64-bit ones. 16-bit ones come out 0.0023 (bf16) and 0.00029 (fp16)
 from them, by dP's rounding and their own, which alone leaves 0.0017 and 0.00021 (dP as two pieces would double the work of both
-products). Where that matters, `dtype=torch.float32` has dP in fp32. Second derivatives and
+products); a dP past 65504 is infinite in fp16. Where that matters, `dtype=torch.float32` has dP in fp32. Second derivatives and
 forward-mode tangents go through a product in fp32 and elementary operations.
 """
 

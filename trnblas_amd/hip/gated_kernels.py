@@ -136,7 +136,7 @@ def gated_gemm_fast(A, B, offsets, act, transB, out_dtype, save=False):
     pa, pb = A.data_ptr(), B.data_ptr()
     su = N * t0 if transB else N
     if R == 1:
-        lda = K
+        lda = max(K, 1)
     if (
         k != K or n2 % 2 or s1 != 1 or lda < K or t1 != 1 or t0 < b1 or N == 0 or dev != _grouped._current_device()
         or B.get_device() != dev or A.is_neg() or B.is_neg()
