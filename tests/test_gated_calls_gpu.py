@@ -1,7 +1,9 @@
 """Calls of the gated projections that the short paths leave to the others."""
 
 import pytest
+import test_gated_shared_host
 import torch
+from test_gated_shared_host import CASES
 
 import trnblas_amd as tb
 from oracle import gated as og
@@ -95,3 +97,38 @@ def test_one_row_of_no_values(dev):
         for N in (16, 5):
             H = tb.gated_gemm(torch.ones(1, 0, dtype=dtype, device=dev), torch.zeros(0, 2 * N, dtype=dtype, device=dev))
             assert H.shape == (1, N) and not H.any()
+
+
+@pytest.mark.parametrize("name", list(CASES))
+def test_operands_that_depend_on_each_other(dev, name, monkeypatch):
+    # first and second derivatives, fp32 on the GPU against 64 bits on the host
+    leaves, own, plain = CASES[name]
+
+    def second(f, device, dtype):
+        x = [(t / 4).to(device, dtype).requires_grad_() for t in leaves]
+        first = torch.autograd.grad(f(*x).square().sum(), x, create_graph=True)
+        return [t.detach() for t in first] + list(torch.autograd.grad(sum(g.square().sum() for g in first), x))
+
+    want = second(plain, "cpu", torch.float64)
+    monkeypatch.setattr(test_gated_shared_host, "OFF", test_gated_shared_host.OFF.to(dev))
+    for got, ref in zip(second(own, dev, F32), want):
+        # some hundred fp32 operations
+        assert torch.allclose(got.double().cpu(), ref, rtol=1e-4, atol=1e-4 * float(ref.abs().max())), name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_a_step_repeats_itself(dev, dtype):
+    g = torch.Generator(device=dev).manual_seed(8)
+    off = torch.tensor([0, 300, 300, 1100], device=dev)
+    for K, N in ((264, 520), (261, 515)):
+        a = torch.randn(1100, K, generator=g, device=dev).to(dtype).requires_grad_()
+        b = (torch.randn(3, K, 2 * N, generator=g, device=dev) / 16).to(dtype).requires_grad_()
+        dH = torch.randn(1100, N, generator=g, device=dev).to(dtype)
+
+        def step():
+            H = tb.grouped_gated_gemm(a, b, off)
+            return (H.detach(), *torch.autograd.grad(H, (a, b), dH))
+
+        first = step()
+        for _ in range(4):
+            assert all(torch.equal(x, y) for x, y in zip(first, step()))
